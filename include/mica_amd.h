@@ -194,6 +194,24 @@ int mica_gather_logits(const void *h, int ldh, int n_rows, const int *rows, int 
                        mica_stream_t stream);
 
 /*
+ * Log probabilities of given tokens, the entropy and the top alternatives of T rows of V logits, in one pass:
+ *   M = max_v x[t, v],  S = sum_v e^(x[t, v] - M),  lp(v) = (x[t, v] - M) - ln S
+ *   logprobs[t, c] = lp(tokens[t, c])  (NaN for an id outside 0 .. V - 1),  entropy[t] = -sum_v e^lp(v) lp(v)
+ *   top_ids[t, i], top_logprobs[t, i]: the i-th largest logit's id and lp, equal logits by the lower id (-0 equals 0)
+ * logits: bf16 / fp16 / fp32, rows ldx elements apart (ldx >= V), of any alignment of their type.  -inf logits have
+ * probability 0.  A row of which a logit is NaN or +inf, or every one -inf, has no distribution: NaN in every logprob and
+ * the entropy; its ids stay ordered, NaN as the largest.  tokens: [T][C] contiguous int32, or int64 with tokens_64.
+ * logprobs fp32 [T][C], entropy fp32 [T], top_ids int64 [T][top], top_logprobs fp32 [T][top], contiguous.  C >= 0;
+ * 0 <= top <= 32 and top <= V <= 2^30.  fp32 sums, in an order that depends on the sizes and alignment only.
+ * workspace: mica_token_logprobs_workspace_bytes(T, V, dtype, top) bytes (0: none), 16-byte aligned, no initialisation
+ * needed.  No counterpart in the reference, which reads the label rows only (mica_gather_logits).
+ */
+int mica_token_logprobs(const void *logits, int dtype, long long ldx, int T, int V, const void *tokens, int tokens_64,
+                        int C, int top, float *logprobs, float *entropy, long long *top_ids, float *top_logprobs,
+                        void *workspace, long long workspace_bytes, mica_stream_t stream);
+long long mica_token_logprobs_workspace_bytes(int T, int V, int dtype, int top);
+
+/*
  * Rotary position embedding in place on the first n_heads heads of each token row (the q and k heads
  * of a fused QKV projection output), in bf16 arithmetic as transformers' apply_rotary_pos_emb
  * computes it for the attention layers: for i < h = head_dim / 2,
@@ -347,6 +365,45 @@ int mica_attention_fwd_rope(const void *q, long long sbq, long long shq, long lo
                             const void *q_norm_w, const void *k_norm_w, float norm_offset, float norm_eps, int rot_dim,
                             const void *cos_tab, const void *sin_tab, int n_pos, const int *pos, void *workspace,
                             long long workspace_bytes, mica_stream_t stream);
+
+/*
+ * Attention of a tree of candidate tokens over a cache, head dim 256, HQ = 4 HK.  Sequence b has N new nodes (queries q,
+ * keys k and values v) and cache_len[b] cached keys (int32 [B], device memory, clamped to 0 .. cache_cap; NULL: cache_cap):
+ *   o[b, i, h] = sum_{u in S} softmax_u(scale q[b, i, h] . key_u[h / 4]) value_u[h / 4],
+ *   S = the sequence's cached keys and the nodes j with bit j % 64 of word tree[b sbt + i W + j / 64] set, W = ceil(N / 64).
+ * A node whose words hold no bit below N is absent (a padded batch): it sees nothing, the cache neither, and its output is
+ * zeros.  No order of the nodes is assumed.  q / k / v / o: bf16; head j of node t of sequence b at ptr + b sb + j sh + t ld
+ * (elements, all % 8); k_cache / v_cache: [cache_cap] rows likewise, a batch stride of 0 shares them.  tree: device memory,
+ * 8-byte aligned; sbt words between sequences (0: one tree for all).  N <= 512; scale positive.  Keys past cache_len are
+ * never read; a key or value that is not finite reaches only the nodes that see it.  fp32 softmax and sums, the weights
+ * rounded to bf16 for the product with v.  workspace: mica_attention_tree_workspace_bytes(B, N, HK, cache_cap) bytes (0:
+ * none), 16-byte aligned, no initialisation needed.  No counterpart in the reference, which runs every candidate as a
+ * request of its own.
+ */
+int mica_attention_tree(const void *q, long long sbq, long long shq, long long ldq, const void *k, long long sbk,
+                        long long shk, long long ldk, const void *v, long long sbv, long long shv, long long ldv,
+                        const void *k_cache, long long sbkc, long long shkc, long long ldkc, const void *v_cache,
+                        long long sbvc, long long shvc, long long ldvc, int cache_cap, const int *cache_len,
+                        const unsigned long long *tree, long long sbt, void *o, long long sbo, long long sho, long long ldo,
+                        int B, int N, int HQ, int HK, int head_dim, float scale, void *workspace, long long workspace_bytes,
+                        mica_stream_t stream);
+long long mica_attention_tree_workspace_bytes(int B, int N, int HK, int cache_cap);
+
+/*
+ * Causal attention within a sliding window and over a few first tokens, head dim 256, HQ = 4 HK.  Sequence b has
+ * kv_len[b] keys (int32 [B], device memory, clamped to 0 .. Sk; NULL: Sk); its Sq queries are its last Sq positions:
+ * query i is at position p = kv_len[b] - Sq + i and sees the keys u <= p with u > p - window or u < sinks.
+ *   o[b, i, h] = sum_u softmax_u(scale q[b, i, h] . k[b, u, h / 4]) v[b, u, h / 4];  zeros where p < 0.
+ * window >= 1, sinks >= 0; Sk may be less than Sq.  Layouts, types and values that are not finite as in
+ * mica_attention_tree.  workspace: mica_attention_window_workspace_bytes(B, Sq, Sk, HK, window, sinks) bytes (0: none),
+ * 16-byte aligned, no initialisation needed.  No counterpart in the reference (its attention sees every key).
+ */
+int mica_attention_window(const void *q, long long sbq, long long shq, long long ldq, const void *k, long long sbk,
+                          long long shk, long long ldk, const void *v, long long sbv, long long shv, long long ldv, void *o,
+                          long long sbo, long long sho, long long ldo, int B, int Sq, int Sk, int HQ, int HK, int head_dim,
+                          float scale, int window, int sinks, const int *kv_len, void *workspace, long long workspace_bytes,
+                          mica_stream_t stream);
+long long mica_attention_window_workspace_bytes(int B, int Sq, int Sk, int HK, int window, int sinks);
 
 /* ---- gated delta net (GDN) token mixer ------------------------------------------------------- */
 

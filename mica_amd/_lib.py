@@ -51,6 +51,8 @@ SIGNATURES = {
     "mica_swiglu": (_I, [_P, _P, _P, _LL, _I, _P]),
     "mica_gather_logits": (_I, [_P, _I, _I, _P, _I, _P, _I, _F, _F, _P, _I, _I, _I, _P, _I, _I, _P, _P, _P, _P, _I,
                                 _P]),
+    "mica_token_logprobs": (_I, [_P, _I, _LL, _I, _I, _P, _I, _I, _I, _P, _P, _P, _P, _P, _LL, _P]),
+    "mica_token_logprobs_workspace_bytes": (_LL, [_I, _I, _I, _I]),
     "mica_rope_inplace": (_I, [_P, _LL, _I, _I, _P, _P, _I, _P, _I, _I, _P]),
     "mica_head_norm_rope": (_I, [_P, _LL, _I, _I, _I, _I, _I, _I, _P, _P, _F, _F, _I, _P, _P, _I, _P, _I, _P]),
     "mica_gate_quant": (_I, [_P, _LL, _P, _LL, _P, _LL, _P, _P, _LL, _I, _I, _I, _P]),
@@ -70,6 +72,11 @@ SIGNATURES = {
     "mica_attention_fwd_rope": (_I, [_P, _LL, _LL, _LL, _P, _LL, _LL, _LL, _P, _LL, _LL, _LL, _P, _LL, _LL, _P, _LL,
                                      _LL, _I, _P, _LL, _LL, _LL, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P, _P, _F, _F,
                                      _I, _P, _P, _I, _P, _P, _LL, _P]),
+    "mica_attention_tree": (_I, [*[_P, _LL, _LL, _LL] * 5, _I, _P, _P, _LL, _P, _LL, _LL, _LL, _I, _I, _I, _I, _I, _F, _P,
+                                 _LL, _P]),
+    "mica_attention_tree_workspace_bytes": (_LL, [_I, _I, _I, _I]),
+    "mica_attention_window": (_I, [*[_P, _LL, _LL, _LL] * 4, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P, _P, _LL, _P]),
+    "mica_attention_window_workspace_bytes": (_LL, [_I, _I, _I, _I, _I, _I]),
     "mica_causal_conv1d": (_I, [_P, _LL, _I, _P, _P, _I, _I, _P, _P, _P, _LL, _I, _I, _I, _I, _I, _I, _F, _P]),
     "mica_gdn_chunk": (_I, [_P, _LL, _I, _P, _LL, _I, _P, _LL, _I, _P, _P, _I, _P, _P, _P, _F, _I, _I, _I, _I, _P,
                             _LL, _P]),

@@ -182,3 +182,142 @@ def causal_gqa_attention(q, k, v, scale: float | None = None, key_splits: int = 
     With Sk > Sq the queries are the last Sq positions; key_splits, kv_len, prefix, rope and head_norm as
     in attention_fwd."""
     return attention_fwd(q, k, v, "bshd", scale, key_splits, kv_len, prefix, rope, head_norm)
+
+
+MAX_TREE_NODES = 512
+
+
+def tree_masks(parents, device=None):
+    """The node masks that tree_attention takes, of trees given by their nodes' parents.
+
+    parents: int [N], or [B, N] for a tree per sequence (host values; a device tensor is copied to the host): an earlier
+    node of the same tree, -1 for a node that follows the cached tokens directly, -2 for none (padding).  Returns int64
+    [N, W] or [B, N, W], W = ceil(N / 64): bit j % 64 of word j / 64 of node i is set when i sees node j, itself and its
+    ancestors.  Made once per tree shape and kept by the caller."""
+    par = torch.as_tensor(parents)
+    if par.dtype.is_floating_point or par.dtype in (torch.bool, torch.complex64, torch.complex128) or par.dim() not in (1, 2):
+        raise ValueError("parents must be whole numbers [N] or [B, N]")
+    n = par.shape[-1]
+    if n > MAX_TREE_NODES:
+        raise ValueError(f"a tree has at most {MAX_TREE_NODES} nodes")
+    words = -(-n // 64)
+    rows = []
+    for tree in par.reshape(-1, n).tolist() if par.numel() else []:
+        sees = []
+        for i, p in enumerate(tree):
+            if not -2 <= p < i or (p >= 0 and tree[p] == -2):
+                raise ValueError(f"node {i} has the parent {p}: an earlier node, -1 (follows the cache) or -2 (no node)")
+            sees.append(0 if p == -2 else (sees[p] if p >= 0 else 0) | 1 << i)
+        rows += [[(s >> 64 * w & 0xffffffffffffffff) - (1 << 64 if s >> 64 * w + 63 & 1 else 0) for w in range(words)]
+                 for s in sees]
+    masks = torch.tensor(rows, dtype=torch.int64).reshape(*par.shape, words)
+    return masks if device is None else masks.to(device)
+
+
+def _heads(t, what, dev=None):
+    """Checks a bf16 [B, S, heads, 256] view; its (batch, head, row) strides, those of axes of one element as 0."""
+    if not t.is_cuda:
+        raise ValueError("mica_amd attention runs on the GPU only (got a CPU tensor)")
+    if t.dim() != 4 or t.dtype != torch.bfloat16 or t.shape[3] != HEAD_DIM or t.stride(3) != 1:
+        raise ValueError(f"{what} must be a bf16 4-D tensor with head dim 256 and unit feature stride")
+    if dev is not None and t.device != dev:
+        raise ValueError(f"{what} is on another device than q")
+    return tuple(t.stride(i) if t.shape[i] > 1 else 0 for i in (0, 2, 1))
+
+
+def _scale(scale):
+    scale = 1.0 / math.sqrt(HEAD_DIM) if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError("the softmax scale must be positive and finite")
+    return scale
+
+
+def _counts(t, B, dev, what):
+    if t is not None and (t.dtype != torch.int32 or t.device != dev or t.shape != (B,) or not t.is_contiguous()):
+        raise ValueError(f"{what} must be a contiguous int32 [B] tensor on q's device")
+    return None if t is None else t.data_ptr()
+
+
+def _cache_call(name, q, nbytes, call):
+    """Allocates o [B, Sq, HQ, 256] and a workspace and launches call(o, o's strides, workspace, stream)."""
+    dev = q.device
+    if nbytes < 0:
+        raise ValueError("attention: invalid sizes")
+    o = torch.empty(q.shape, dtype=torch.bfloat16, device=dev)
+    ws = torch.empty((max(nbytes, 16),), dtype=torch.uint8, device=dev)
+    rc = _lib.check(_on(dev, lambda: call(o.data_ptr(), (o.stride(0), o.stride(2), o.stride(1)), ws.data_ptr(),
+                                          _stream(dev))), name)
+    if rc:
+        raise ValueError(f"attention: unsupported input ({_lib.status_name(rc)})")
+    _launched()
+    return o
+
+
+def tree_attention(q, k, v, tree, cache=None, cache_len=None, scale: float | None = None):
+    """Attention of a tree of candidate tokens over cached keys (mica_attention_tree): every node attends to its
+    sequence's cached keys, its ancestors and itself, in one call instead of one continuation per branch.
+
+    q [B, N, HQ, 256], k / v [B, N, HK, 256]: the new nodes' heads, bf16 views (e.g. of the fused QKV output), with their
+    positions already applied, HQ = 4 HK, N <= 512.  tree: int64 masks [N, W] for every sequence or [B, N, W]
+    (tree_masks(parents)); a node without a bit is padding: it sees nothing and its output is zeros.  cache: (keys, values),
+    [B, C, HK, 256] or one for all sequences, [1, C, HK, 256] or [C, HK, 256] (a PrefixState's layer), of any strides;
+    cache_len: int32 [B] on the device, how many of them sequence b has (None: C; clamped to 0 .. C).  Rows past it are
+    never read.  Returns o [B, N, HQ, 256] bf16."""
+    sq, sk, sv = _heads(q, "q"), _heads(k, "k", q.device), _heads(v, "v", q.device)
+    dev = q.device
+    B, N, HQ, _ = q.shape
+    HK = k.shape[2]
+    if k.shape != v.shape or k.shape[:2] != (B, N) or HQ != GROUP * HK:
+        raise ValueError("q / k / v shapes do not match (4 query heads per key/value head, one key per node)")
+    if N > MAX_TREE_NODES:
+        raise ValueError(f"a tree has at most {MAX_TREE_NODES} nodes")
+    W = -(-N // 64)
+    if (tree.dtype != torch.int64 or tree.device != dev or not tree.is_contiguous()
+            or tuple(tree.shape) not in ((N, W), (B, N, W))):
+        raise ValueError("tree must be a contiguous int64 [N, ceil(N / 64)] or [B, N, ceil(N / 64)] tensor on q's device")
+    C, skc, svc, pk, pv = 0, (0, 0, 0), (0, 0, 0), None, None
+    if cache is not None:
+        kc, vc = (t.unsqueeze(0) if t.dim() == 3 else t for t in cache)
+        skc, svc = _heads(kc, "cached keys", dev), _heads(vc, "cached values", dev)
+        C = kc.shape[1]
+        if kc.shape != vc.shape or kc.shape[2] != HK or kc.shape[0] not in (1, B):
+            raise ValueError("cached keys and values must both be [B, C, HK, 256] or [1, C, HK, 256]")
+        pk, pv = kc.data_ptr(), vc.data_ptr()
+    n_len = _counts(cache_len, B, dev, "cache_len")
+    scale = _scale(scale)
+    if not _gpu_ok(dev):
+        raise RuntimeError(f"mica_amd kernels need a gfx950 GPU (device {dev})")
+    L = _lib.load()
+    nbytes = int(L.mica_attention_tree_workspace_bytes(B, N, HK, C))
+    return _cache_call("mica_attention_tree", q, nbytes, lambda o, so, ws, st: L.mica_attention_tree(
+        q.data_ptr(), *sq, k.data_ptr(), *sk, v.data_ptr(), *sv, pk, *skc, pv, *svc, C, n_len, tree.data_ptr(),
+        N * W if tree.dim() == 3 else 0, o, *so, B, N, HQ, HK, HEAD_DIM, scale, ws, nbytes, st))
+
+
+def window_attention(q, k, v, window: int, sinks: int = 0, scale: float | None = None, kv_len=None):
+    """Causal attention within a sliding window and over the sequence's first tokens (mica_attention_window): the query
+    at position p sees the keys u <= p with u > p - window or u < sinks.
+
+    q [B, Sq, HQ, 256], k / v [B, Sk, HK, 256] bf16 views, HQ = 4 HK.  Sequence b has kv_len[b] keys (int32 [B] on the
+    device, clamped to 0 .. Sk; None: Sk) and its queries are the last Sq of those positions; a query before the first
+    key sees nothing, and its output is zeros.  window >= 1, sinks >= 0.  Keys past kv_len or outside every query's
+    reach are not read.  Returns o [B, Sq, HQ, 256] bf16."""
+    sq, sk, sv = _heads(q, "q"), _heads(k, "k", q.device), _heads(v, "v", q.device)
+    dev = q.device
+    B, Sq, HQ, _ = q.shape
+    Sk, HK = k.shape[1:3]
+    if k.shape != v.shape or k.shape[0] != B or HQ != GROUP * HK:
+        raise ValueError("q / k / v shapes do not match (4 query heads per key/value head)")
+    window, sinks = int(window), int(sinks)
+    if window < 1 or sinks < 0:
+        raise ValueError("window must be at least 1 and sinks at least 0")
+    window, sinks = min(window, max(Sk, 1)), min(sinks, Sk)
+    n_len = _counts(kv_len, B, dev, "kv_len")
+    scale = _scale(scale)
+    if not _gpu_ok(dev):
+        raise RuntimeError(f"mica_amd kernels need a gfx950 GPU (device {dev})")
+    L = _lib.load()
+    nbytes = int(L.mica_attention_window_workspace_bytes(B, Sq, Sk, HK, window, sinks))
+    return _cache_call("mica_attention_window", q, nbytes, lambda o, so, ws, st: L.mica_attention_window(
+        q.data_ptr(), *sq, k.data_ptr(), *sk, v.data_ptr(), *sv, o, *so, B, Sq, Sk, HQ, HK, HEAD_DIM, scale, window,
+        sinks, n_len, ws, nbytes, st))

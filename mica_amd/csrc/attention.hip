@@ -34,21 +34,9 @@
 
 #include <type_traits>
 
-#include "common.h"
+#include "attn_common.h"
 
 namespace {
-
-// Combine a value with the one held by lane l ^ 32 (v_permlane32_swap: no LDS round trip).  With the
-// same register as both operands, the swap leaves (own, other) in lanes 0-31 and (other, own) in lanes
-// 32-63, so max and sum come out bit-identical in every lane.
-__device__ __forceinline__ float half_swap_max(float v) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __builtin_fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float half_swap_sum(float v) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
 
 constexpr int kD = 256;              // head dim
 constexpr int kBQ = 32;              // query positions per workgroup
@@ -64,20 +52,6 @@ constexpr int kPSt = 4;                  // the pipelined schedule's: one read, 
 template <bool PIPE>
 constexpr int kFaSmem = (PIPE ? kPSt : kNSt) * kStage;
 constexpr int kMaxKeySplits = 64;
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef __attribute__((address_space(3))) void lds_void;
-
-constexpr int kBufferFlags = 0x00020000;   // raw buffer, 32-bit data format (gfx9)
-
-MICA_DEVICE f32x16 mfma_bf16(const bf16x8 &a, const bf16x8 &b, const f32x16 &c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-}
-template <int N>
-MICA_DEVICE void fa_wait_vmcnt() {
-    static_assert(N >= 0 && N < 64, "vmcnt range");
-    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
-}
 
 // V^T tile image: dim d's 32 keys are a 64-byte row of four 16-byte chunks.  Chunk c = 2 s + h holds
 // key units (4 keys each) 4 s + h and 4 s + 2 + h: the 8 keys that a lane in half h of the wave feeds
@@ -427,7 +401,7 @@ __global__ __launch_bounds__(kFaThreads, PIPE ? 1 : 2) void fa_fwd_kernel(FaPara
         const int st = (j - first) & 1;
         // this wave's DMA of tile j landed; after the barrier every wave's has, and nobody reads
         // stage st ^ 1 (tile j - 1) any more
-        fa_wait_vmcnt<0>();
+        wait_vmcnt<0>();
         __syncthreads();
         if (j + 1 <= last_own) dma_tile(j + 1, st ^ 1);
         const int8_t *ks = smem + st * kStage;
@@ -535,7 +509,7 @@ __global__ __launch_bounds__(kFaThreads, PIPE ? 1 : 2) void fa_fwd_kernel(FaPara
         dma_v(first, 0, 0, 4);
         dma_k(first + 3, 3, 0, 4);
         dma_v(first + 1, 1, 0, 4);
-        fa_wait_vmcnt<16>();   // K of the first two tiles, the zeros
+        wait_vmcnt<16>();   // K of the first two tiles, the zeros
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -573,7 +547,7 @@ __global__ __launch_bounds__(kFaThreads, PIPE ? 1 : 2) void fa_fwd_kernel(FaPara
         // this wave's DMA of K(j + 2) and V(j) landed (those of the last step, 8, may still be out); after the barrier
         // every wave's has, and nobody reads K(j) or V(j - 2) any more: K(j + 4) and V(j + 2) go there.  K(j + 1) and
         // V(j - 1) were there a barrier earlier, so their first fragments are in registers already.
-        fa_wait_vmcnt<8>();
+        wait_vmcnt<8>();
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
         mask(j, sc);
@@ -638,7 +612,7 @@ __global__ __launch_bounds__(kFaThreads, PIPE ? 1 : 2) void fa_fwd_kernel(FaPara
     }
     if (first <= last_own) {   // the last tile: O += V P of the tile before, its softmax, O += V P
         const int t = last_own - first, sv = t % kPSt, svp = (t + 3) % kPSt;
-        fa_wait_vmcnt<0>();
+        wait_vmcnt<0>();
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
         auto product = [&](int stage) {

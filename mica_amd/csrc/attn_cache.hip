@@ -1,0 +1,566 @@
+// Attention of new tokens over kept keys on gfx950, head dim 256, 4 query heads per key/value head: a tree of
+// candidate tokens over a cache (mica_attention_tree) and causal attention within a sliding window and over a few
+// first tokens (mica_attention_window).
+//
+//   o[i, h] = sum_{u in S(i)} softmax_u(scale q[i, h] . k[u, h / 4]) v[u, h / 4];   zeros where S(i) is empty
+//   tree:    S(i) = the sequence's first cache_len cached keys and the new keys j whose bit is set in node i's words
+//            (a node without any bit is absent and sees nothing)
+//   window:  S(i) = { u : u <= p and (u > p - window or u < sinks) },  p = position of query i
+//
+// Work split: a workgroup takes one (sequence, key/value head), a block of 8 R query positions, i.e. 32 R rows (position,
+// head), and a run of 32-key tiles.  Each of its R x D waves holds 32 rows: it computes S^T = K Q^T (32 keys x 32 rows,
+// v_mfma_f32_32x32x16_bf16), the online softmax of its rows (a lane holds 16 of a row's 32 scores, its partner l ^ 32
+// the others) and 256 / D dims of O^T += V^T P^T.  With few rows, D > 1 waves share a row block: they repeat its scores
+// (cheap beside the tile's memory time) and divide the dims of O.
+//
+// Data movement: K and V tiles of 32 rows come by LDS DMA into a ring of ST stages, 16-byte chunks XOR-swizzled by row,
+// rows past the last key as zeros (the buffer's range check).  K fragments are 16-byte reads; V is kept as it lies in
+// memory and its V^T fragments are transposing reads (ds_read_b64_tr_b16: 16 lanes fetch 4 keys x 16 dims and each gets
+// the 4 keys of one dim), so no pass over V comes before.
+//
+// When there are few workgroups, the key tiles are divided into chunks and ca_merge_kernel joins the partial softmax
+// states (fp32).
+#include "attn_common.h"
+
+namespace {
+
+constexpr int kD = 256;                    // head dim
+constexpr int kGroup = 4;                  // query heads per key/value head
+constexpr int kBK = 32;                    // keys per tile
+constexpr int kTile = kBK * kD * 2;        // 16 KB of K or V
+constexpr int kStage = 2 * kTile;
+constexpr int kMaxNodes = 512;             // nodes of a tree
+constexpr int kSlots = 256;                // CUs of the chip
+
+struct CaParams {
+    const uint16_t *q; long long sbq, shq, ldq;     // head h of row t of sequence b: q + b sbq + h shq + t ldq
+    const uint16_t *k; long long sbk, shk, ldk;     // the new keys (tree), all keys (window)
+    const uint16_t *v; long long sbv, shv, ldv;
+    const uint16_t *kc; long long sbkc, shkc, ldkc; // the cache (tree)
+    const uint16_t *vc; long long sbvc, shvc, ldvc;
+    uint16_t *o; long long sbo, sho, ldo;
+    const int *len;                                 // [B] cached keys (tree) or keys (window), or null: cap
+    const uint32_t *tree; long long sbt;            // words [N][tw] of a sequence, sbt words apart (0: one tree for all)
+    int tw;
+    int B, Sq, cap, HK;
+    int window, sinks;
+    float scale_log2;                               // softmax scale x log2(e)
+    int nqb, gq, chunk, nchunk;                     // query blocks, in groups of gq; tiles a workgroup, chunks a sequence
+    float *part_o;                                  // partial O, a wave's accumulators 64 lanes x 16 bytes at a time
+    float2 *part_ml;                                // partial (m, l) of each row
+};
+
+// a sequence's key count
+MICA_DEVICE int key_count(const CaParams &p, int b) { return p.len ? min(max(p.len[b], 0), p.cap) : p.cap; }
+
+// The key tiles of a query block, in the order they are walked.  tree: the cache's, then the new keys'.  window: the
+// sinks' tiles below the window, then the window's.
+template <bool TREE>
+struct Tiles {
+    int n, n0, skip; // tiles; of them cached (tree) or before the window (window); tiles skipped after those (window)
+    MICA_DEVICE Tiles(const CaParams &p, int keys, int q0, int rows) {
+        if constexpr (TREE) {
+            n0 = (keys + kBK - 1) / kBK;
+            n = n0 + (p.Sq + kBK - 1) / kBK;
+            skip = 0;
+        } else {
+            const int first = keys - p.Sq + q0, last = first + rows - 1; // positions of the block's queries
+            if (last < 0) {
+                n = n0 = skip = 0;
+                return;
+            }
+            const int w0 = max(max(first, 0) - (p.window - 1), 0) / kBK;
+            n0 = min((min(p.sinks, last + 1) + kBK - 1) / kBK, w0);
+            skip = w0 - n0;
+            n = n0 + last / kBK - w0 + 1;
+        }
+    }
+    MICA_DEVICE int tile(int i) const { return i < n0 ? i : i + skip; } // window: the key tile's index
+};
+
+// A V value (bf16 code) that is not finite as the largest finite value of its sign, NaN with the given sign (0 or 0x8000);
+// 0 for a finite one.  Times 2^127 and summed by the matrix cores these give +-inf, and, with both signs, NaN.
+MICA_DEVICE uint32_t odd_value(uint32_t h, uint32_t nan_sign) {
+    if ((h & 0x7f80u) != 0x7f80u) return 0u;
+    return 0x7f7fu | ((h & 0x7fu) ? nan_sign : (h & 0x8000u));
+}
+
+template <int R, int D, int ST, bool TREE>
+__global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca_fwd_kernel(CaParams p) {
+    constexpr int kWaves = R * D, kThreads = 64 * kWaves;
+    constexpr int NB = 8 * R;                 // query positions of the workgroup
+    constexpr int NDT = kD / 32 / D;          // 32-dim tiles of O a wave holds
+    constexpr int kBlk = 16 / kWaves;         // 1 KB DMA blocks of K, and of V, a wave issues for a tile
+    constexpr int kWords = TREE ? NB * (kMaxNodes / 32) : 1;
+    static_assert(R * 32 * kD * 2 <= ST * kStage, "the output is staged where the tiles were");
+    __shared__ __attribute__((aligned(1024))) int8_t smem[ST * kStage];
+    __shared__ uint32_t words[kWords];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int l32 = lane & 31, hi = lane >> 5;
+    const int rb = wave / D, dt0 = (wave % D) * NDT;
+    // Workgroup -> (sequence, chunk, key/value head, query block).  Consecutive workgroups go to the 8 XCDs in turn; the
+    // gq query blocks of a group, which read the same keys, stay on one XCD, one after the other.
+    const int id = blockIdx.x, ngq = (p.nqb + p.gq - 1) / p.gq;
+    const int grp = id / (8 * p.gq) * 8 + id % 8, unit = grp / ngq, qb = grp % ngq * p.gq + id / 8 % p.gq;
+    if (unit >= p.B * p.nchunk * p.HK || qb >= p.nqb) return;
+    const int hk = unit % p.HK, c = unit / p.HK % p.nchunk, b = unit / p.HK / p.nchunk;
+    const int q0 = qb * NB, keys = key_count(p, b);
+    const Tiles<TREE> tl(p, keys, q0, min(NB, p.Sq - q0));
+    const int i0 = c * p.chunk, i1 = min(i0 + p.chunk, tl.n);
+    if (i0 >= tl.n && p.nchunk > 1) return; // (a block without tiles writes its zeros when it is alone)
+
+    // this lane's row: a position and a query head
+    const int row = rb * 32 + l32, head = hk * kGroup + row / NB, t = q0 + row % NB;
+    bool absent = false; // a tree node without a bit
+    if constexpr (TREE) {
+#pragma unroll 1
+        for (int i = tid; i < NB * p.tw; i += kThreads) {
+            const int node = q0 + i / p.tw, w = i % p.tw;
+            uint32_t x = node < p.Sq ? p.tree[b * p.sbt + (long long)node * p.tw + w] : 0u;
+            const int left = p.Sq - 32 * w; // bits past the last node do not count
+            x = left >= 32 ? x : left <= 0 ? 0u : x & ((1u << left) - 1u);
+            words[i] = x;
+        }
+        __syncthreads();
+        uint32_t any = 0;
+#pragma unroll 1
+        for (int w = 0; w < p.tw; ++w) any |= words[row % NB * p.tw + w];
+        absent = any == 0;
+    }
+
+    // DMA of tile i into stage st; past i1 from a zero-sized buffer, so that every step issues as many instructions
+    auto issue = [&](int i, int st) {
+        const uint16_t *kb, *vb;
+        long long ldk = p.ldk, ldv = p.ldv;
+        int rows;
+        if (TREE && i < tl.n0) {
+            ldk = p.ldkc, ldv = p.ldvc;
+            kb = p.kc + b * p.sbkc + hk * p.shkc + (long long)i * kBK * ldk;
+            vb = p.vc + b * p.sbvc + hk * p.shvc + (long long)i * kBK * ldv;
+            rows = keys - i * kBK;
+        } else {
+            const int j = TREE ? i - tl.n0 : tl.tile(i);
+            kb = p.k + b * p.sbk + hk * p.shk + (long long)j * kBK * ldk;
+            vb = p.v + b * p.sbv + hk * p.shv + (long long)j * kBK * ldv;
+            rows = (TREE ? p.Sq : keys) - j * kBK;
+        }
+        rows = i < i1 ? min(rows, kBK) : 0;
+        const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
+            (void *)kb, 0, rows > 0 ? (int)((rows - 1) * ldk * 2) + kD * 2 : 0, kBufferFlags);
+        const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
+            (void *)vb, 0, rows > 0 ? (int)((rows - 1) * ldv * 2) + kD * 2 : 0, kBufferFlags);
+        int8_t *s = smem + st * kStage;
+#pragma unroll
+        for (int x = 0; x < kBlk; ++x) {
+            const int blk = wave * kBlk + x, r = 2 * blk + hi; // 1 KB = key rows 2 blk and 2 blk + 1
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void *)(s + blk * 1024), 16,
+                                                     r * (int)(ldk * 2) + ((l32 ^ r) << 4), 0, 0, 0);
+        }
+#pragma unroll
+        for (int x = 0; x < kBlk; ++x) {
+            const int blk = wave * kBlk + x, r = 2 * blk + hi;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void *)(s + kTile + blk * 1024), 16,
+                                                     r * (int)(ldv * 2) + ((l32 ^ ((r & 7) << 1)) << 4), 0, 0, 0);
+        }
+    };
+#pragma unroll
+    for (int s = 0; s < ST - 1; ++s) issue(i0 + s, s);
+
+    // Q fragments (B operand of S^T): dims 16 s + 8 hi .. + 7 of this lane's row
+    bf16x8 qf[kD / 16];
+    {
+        const uint16_t *qr = p.q + b * p.sbq + head * p.shq + (long long)t * p.ldq + hi * 8;
+#pragma unroll
+        for (int s = 0; s < kD / 16; ++s) {
+            u32x4 x = {0u, 0u, 0u, 0u};
+            if (t < p.Sq) x = *(const u32x4 *)(qr + s * 16);
+            qf[s] = __builtin_bit_cast(bf16x8, x);
+        }
+    }
+    f32x16 O[NDT];
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) O[dt] = f32x16{};
+    float m = -__builtin_inff(), lsum = 0.0f;
+    const int pos = keys - p.Sq + t; // window: this row's position
+
+    // V^T fragment of 32-dim tile dt, step s: keys 16 s + 4 hi .. + 3 and 16 s + 8 + 4 hi .. + 3 (the keys of P^T's
+    // accumulator rows 8 s .. 8 s + 7) of dim 32 dt + l % 32.  The lane's address: key row 4 hi + (l % 16) / 4, dims
+    // 16 ((l / 16) % 2) + 4 (l % 4); chunk c of row r lies at c ^ 2 (r % 8), which spreads the 8 rows x 64 bytes of a
+    // read over all banks twice, the least 512 bytes can take.
+    const int vrow = 4 * hi + ((l32 & 15) >> 2);
+    const int vc0 = (2 * (l32 >> 4) + ((l32 & 3) >> 1)) ^ (vrow << 1);
+    int vaddr[NDT < 4 ? NDT : 4];
+#pragma unroll
+    for (int j = 0; j < (NDT < 4 ? NDT : 4); ++j)
+        vaddr[j] = kTile + vrow * (kD * 2) + (((4 * (dt0 + j)) ^ vc0) << 4) + (l32 & 1) * 8;
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    auto vfrag = [&](const int8_t *stage, int s, int dt) {
+        const int8_t *a = stage + vaddr[dt & 3] + (dt >> 2) * 256 + s * 16 * (kD * 2);
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)a);
+        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(a + 8 * (kD * 2)));
+        return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+
+#pragma unroll 1
+    for (int i = i0; i < i1; ++i) {
+        const int st = (i - i0) % ST;
+        // this wave's DMA of tile i landed; after the barrier every wave's has, and nobody reads tile i - 1 any more
+        wait_vmcnt<(ST - 2) * 2 * kBlk>();
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        issue(i + ST - 1, (st + ST - 1) % ST);
+        const int8_t *stage = smem + st * kStage;
+        // ---- S^T = K Q^T: rows = keys of the tile, column = this lane's row ----
+        f32x16 sc = {};
+        auto kfrag = [&](int s) {
+            return __builtin_bit_cast(bf16x8, *(const u32x4 *)(stage + l32 * (kD * 2) + (((2 * s + hi) ^ l32) << 4)));
+        };
+        bf16x8 ka = kfrag(0), kb = kfrag(1);
+#pragma unroll
+        for (int s = 0; s < kD / 16; ++s) {
+            const bf16x8 a = (s & 1) ? kb : ka;
+            if (s + 2 < kD / 16) {
+                if (s & 1) kb = kfrag(s + 2);
+                else ka = kfrag(s + 2);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            sc = mfma_bf16(a, qf[s], sc);
+        }
+        // ---- keys that a row does not see: score -inf, weight 0 (score r of a lane is key 8 (r / 4) + 4 hi + r % 4) ----
+        bool masked = false, own = false;
+        if constexpr (TREE) {
+            own = i >= tl.n0;
+            masked = own || (i + 1) * kBK > keys;
+            if (own) {
+                const uint32_t w = words[row % NB * p.tw + (i - tl.n0)] >> (4 * hi);
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    sc[r] = (w >> (8 * (r >> 2) + (r & 3))) & 1u ? sc[r] : -__builtin_inff();
+            } else if (masked) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    sc[r] = i * kBK + 8 * (r >> 2) + 4 * hi + (r & 3) < keys ? sc[r] : -__builtin_inff();
+            }
+        } else {
+            const int k0 = tl.tile(i) * kBK, first = keys - p.Sq + q0;
+            masked = k0 + kBK - 1 > first || (k0 <= first + NB - 1 - p.window && k0 + kBK > p.sinks);
+            if (masked) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int key = k0 + 8 * (r >> 2) + 4 * hi + (r & 3);
+                    const bool sees = key <= pos && (key > pos - p.window || key < p.sinks);
+                    sc[r] = sees ? sc[r] : -__builtin_inff();
+                }
+            }
+        }
+        // ---- online softmax in log2 units; the reference moves only when the maximum exceeds it by more than 8 ----
+        float mx = -__builtin_inff();
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = __builtin_fmaxf(mx, sc[r]);
+        mx = half_swap_max(mx) * p.scale_log2;
+        const bool grow = mx > m + 8.0f;
+        const float alpha = grow ? __builtin_amdgcn_exp2f(m - mx) : 1.0f;
+        if (grow) m = mx;
+        if (__builtin_amdgcn_ballot_w64(grow)) {
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) O[dt] *= alpha;
+            lsum *= alpha;
+        }
+        const float ref = m == -__builtin_inff() ? 0.0f : m; // a row that has seen nothing yet: exp2(-inf - 0) = 0
+        bf16x8 pb[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            u32x4 w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * s + 2 * e], p.scale_log2, -ref));
+                const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * s + 2 * e + 1], p.scale_log2, -ref));
+                lsum += p0 + p1;
+                w[e] = pack_bf16x2(p0, p1); // the matrix cores' operand type; the sum keeps the unrounded weights
+            }
+            pb[s] = __builtin_bit_cast(bf16x8, w);
+        }
+        // A value that is not finite must not reach the rows that do not see its key (0 x inf = NaN): looked for in
+        // the tiles where rows see different keys.  (Rows past the last key are zeros, and where all rows see all
+        // keys there is no such row.)
+        if (masked) {
+            uint32_t odd = 0;
+#pragma unroll 2
+            for (int x = 0; x < kTile / 1024; ++x) {
+                const u32x4 w = *(const u32x4 *)(stage + kTile + x * 1024 + lane * 16);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) odd |= (w[e] & 0x7f807f80u) + 0x00800080u;
+            }
+            if (__builtin_amdgcn_ballot_w64((odd & 0x80008000u) != 0)) { // the same for every wave: all scan the tile
+                // into the rows that give their keys a weight, then zeros in their place
+                bf16x8 ind[2];
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    u32x4 w = __builtin_bit_cast(u32x4, pb[s]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = ((w[e] & 0xffffu) ? 0x7f00u : 0u) | ((w[e] >> 16) ? 0x7f000000u : 0u);
+                    ind[s] = __builtin_bit_cast(bf16x8, w);
+                }
+#pragma unroll
+                for (int x = 0; x < 4 * NDT; ++x) {
+                    const int s = x & 1, dt = x >> 2;
+                    const uint32_t sign = x & 2 ? 0x8000u : 0u;
+                    u32x4 w = __builtin_bit_cast(u32x4, vfrag(stage, s, dt));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        w[e] = odd_value(w[e] & 0xffffu, sign) | (odd_value(w[e] >> 16, sign) << 16);
+                    O[dt] = mfma_bf16(__builtin_bit_cast(bf16x8, w), ind[s], O[dt]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                __syncthreads();
+#pragma unroll 1
+                for (int x = tid; x < kTile / 4; x += kThreads) {
+                    uint32_t *w = (uint32_t *)(smem + st * kStage + kTile) + x;
+                    *w &= (odd_value(*w & 0xffffu, 0) ? 0u : 0xffffu) | (odd_value(*w >> 16, 0) ? 0u : 0xffff0000u);
+                }
+                __syncthreads();
+            }
+        }
+        // ---- O^T += V^T P^T, the fragments read two steps ahead ----
+        bf16x8 va = vfrag(stage, 0, 0), vb = vfrag(stage, 1 / NDT, 1 % NDT);
+#pragma unroll
+        for (int x = 0; x < 2 * NDT; ++x) {
+            const bf16x8 a = (x & 1) ? vb : va;
+            if (x + 2 < 2 * NDT) {
+                if (x & 1) vb = vfrag(stage, (x + 2) / NDT, (x + 2) % NDT);
+                else va = vfrag(stage, (x + 2) / NDT, (x + 2) % NDT);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            O[x % NDT] = mfma_bf16(a, pb[x / NDT], O[x % NDT]);
+        }
+    }
+    wait_vmcnt<0>();  // the ring's last (empty) loads have written before the stages are used again or given up
+    float ltot = half_swap_sum(lsum);
+    if (absent) { // (its cached keys were computed like the others': nothing of them leaves)
+        m = -__builtin_inff(), ltot = 0.0f;
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) O[dt] = f32x16{};
+    }
+    if (p.nchunk > 1) {
+        const long long blk = (long long)unit * p.nqb + qb;
+        float *po = p.part_o + ((blk * kWaves + wave) * (NDT * 4) * 64 + lane) * 4;
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4)
+                *(float4 *)(po + (dt * 4 + r4) * 256) =
+                    float4{O[dt][4 * r4], O[dt][4 * r4 + 1], O[dt][4 * r4 + 2], O[dt][4 * r4 + 3]};
+        if (dt0 == 0 && hi == 0) p.part_ml[blk * (32 * R) + row] = float2{m, ltot};
+        return;
+    }
+    // ---- normalise, stage in LDS (32 R rows x 512 B), write 16-byte row pieces ----
+    const float inv = ltot == 0.0f ? 0.0f : 1.0f / ltot;
+    __syncthreads();
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+            const int d = (dt0 + dt) * 32 + 8 * r4 + 4 * hi;
+            u32x2 w;
+            w[0] = pack_bf16x2(O[dt][4 * r4] * inv, O[dt][4 * r4 + 1] * inv);
+            w[1] = pack_bf16x2(O[dt][4 * r4 + 2] * inv, O[dt][4 * r4 + 3] * inv);
+            *(u32x2 *)(smem + row * (kD * 2) + (((d >> 3) ^ l32) << 4) + (d & 4) * 2) = w;
+        }
+    __syncthreads();
+#pragma unroll 2
+    for (int x = tid; x < 32 * R * 32; x += kThreads) {
+        const int rr = x >> 5, ch = x & 31, tt = q0 + rr % NB;
+        if (tt < p.Sq)
+            *(u32x4 *)(p.o + b * p.sbo + (long long)(hk * kGroup + rr / NB) * p.sho + (long long)tt * p.ldo + ch * 8) =
+                *(const u32x4 *)(smem + rr * (kD * 2) + ((ch ^ (rr & 31)) << 4));
+    }
+}
+
+// The partial states of a block's chunks joined: with M = max_c m_c, w_c = 2^(m_c - M), o = (sum w_c O_c) / (sum w_c l_c).
+// One wave takes 64 lanes x 16 bytes of the forward kernel's accumulators (4 dims of 32 rows x 2) of every chunk.
+template <int R, int D, bool TREE>
+__global__ __launch_bounds__(256) void ca_merge_kernel(CaParams p) {
+    constexpr int NB = 8 * R, NDT = kD / 32 / D, kFrags = R * D * NDT * 4; // = 32 R
+    const int lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5;
+    const int f = (blockIdx.x % (kFrags / 4)) * 4 + (threadIdx.x >> 6), blk = blockIdx.x / (kFrags / 4);
+    const int qb = blk % p.nqb, hk = blk / p.nqb % p.HK, b = blk / p.nqb / p.HK;
+    const int q0 = qb * NB, row = f / (NDT * 4 * D) * 32 + l32;
+    const Tiles<TREE> tl(p, key_count(p, b), q0, min(NB, p.Sq - q0));
+    const int n = (tl.n + p.chunk - 1) / p.chunk;
+    const long long u0 = (long long)b * p.nchunk * p.HK + hk; // chunk c is unit u0 + c HK
+    float mx = -__builtin_inff();
+    for (int c = 0; c < n; ++c) mx = __builtin_fmaxf(mx, p.part_ml[((u0 + (long long)c * p.HK) * p.nqb + qb) * (32 * R) + row].x);
+    float l = 0.0f;
+    float4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int c = 0; c < n; ++c) {
+        const long long u = (u0 + (long long)c * p.HK) * p.nqb + qb;
+        const float2 ml = p.part_ml[u * (32 * R) + row];
+        const float4 o = *(const float4 *)(p.part_o + ((u * kFrags + f) * 64 + lane) * 4);
+        // a row that no chunk has keys for: weights 1 on zeros (a sum that is NaN stays one)
+        const float w = mx == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(ml.x - mx);
+        l += w * ml.y;
+        acc.x += w * o.x;
+        acc.y += w * o.y;
+        acc.z += w * o.z;
+        acc.w += w * o.w;
+    }
+    const int t = q0 + row % NB;
+    if (t >= p.Sq) return;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const int fr = f % (NDT * 4), dt = f / (NDT * 4) % D * NDT + fr / 4, d = dt * 32 + 8 * (fr % 4) + 4 * hi;
+    u32x2 w;
+    w[0] = pack_bf16x2(acc.x * inv, acc.y * inv);
+    w[1] = pack_bf16x2(acc.z * inv, acc.w * inv);
+    *(u32x2 *)(p.o + b * p.sbo + (long long)(hk * kGroup + row / NB) * p.sho + (long long)t * p.ldo + d) = w;
+}
+
+// ---- host side ----
+
+// How a call is divided: row blocks (R) and dim parts (D) of a workgroup, LDS stages, tiles a workgroup, chunks.
+struct Plan {
+    int R, D, ST, nqb, gq, chunk, nchunk;
+    long long wgs, states; // workgroups; partial rows (0: one chunk)
+};
+
+Plan plan(int B, int Sq, int HK, int max_tiles) {
+    Plan pl{};
+    pl.R = Sq <= 8 ? 1 : Sq <= 16 ? 2 : Sq <= 32 ? 4 : 4;
+    pl.D = 4 / pl.R;
+    pl.ST = pl.R < 4 ? 4 : 2;
+    pl.nqb = (Sq + 8 * pl.R - 1) / (8 * pl.R);
+    pl.gq = pl.nqb < 8 ? pl.nqb : 8;
+    const long long base = (long long)B * HK * pl.nqb, want = base ? (kSlots * (pl.ST == 2 ? 2 : 1) + base - 1) / base : 1;
+    long long chunk = (max_tiles + want - 1) / want;
+    if (chunk < 4) chunk = 4;
+    pl.chunk = (int)chunk;
+    pl.nchunk = max_tiles > chunk ? (int)((max_tiles + chunk - 1) / chunk) : 1;
+    const long long units = (long long)B * pl.nchunk * HK, groups = units * ((pl.nqb + pl.gq - 1) / pl.gq);
+    pl.wgs = (groups + 7) / 8 * 8 * pl.gq;
+    pl.states = pl.nchunk > 1 ? units * pl.nqb * 32 * pl.R : 0;
+    return pl;
+}
+
+int tree_tiles(int N, int cap) { return (cap + kBK - 1) / kBK + (N + kBK - 1) / kBK; }
+// most tiles of a block of Sq <= 32 or 32 queries: the sinks', the window's and the block's own, never more than the keys'
+int window_tiles(int Sq, int Sk, int window, int sinks) {
+    const long long all = ((long long)Sk + kBK - 1) / kBK;
+    const long long span = ((long long)window + (Sq < 32 ? Sq : 32) + 2 * kBK - 3) / kBK + 1;
+    const long long n = (sinks + kBK - 1ll) / kBK + span;
+    return (int)(n < all ? n : all);
+}
+long long state_bytes(const Plan &pl) { return pl.states * (kD * 4 + 8); }
+
+template <bool TREE>
+int launch(CaParams &p, const Plan &pl, void *workspace, hipStream_t st) {
+    p.nqb = pl.nqb, p.gq = pl.gq, p.chunk = pl.chunk, p.nchunk = pl.nchunk;
+    p.part_o = (float *)workspace;
+    p.part_ml = (float2 *)((char *)workspace + pl.states * kD * 4);
+    if (pl.wgs >= (1LL << 31)) return MICA_MISS_RANGE;
+    const dim3 grid((unsigned)pl.wgs), threads(64 * pl.R * pl.D);
+    if (pl.R == 1) hipLaunchKernelGGL((ca_fwd_kernel<1, 4, 4, TREE>), grid, threads, 0, st, p);
+    else if (pl.R == 2) hipLaunchKernelGGL((ca_fwd_kernel<2, 2, 4, TREE>), grid, threads, 0, st, p);
+    else hipLaunchKernelGGL((ca_fwd_kernel<4, 1, 2, TREE>), grid, threads, 0, st, p);
+    if (const int rc = mica_err(hipGetLastError())) return rc;
+    if (pl.nchunk == 1) return 0;
+    const dim3 mgrid((unsigned)((long long)p.B * p.HK * pl.nqb * 8 * pl.R));
+    if (pl.R == 1) hipLaunchKernelGGL((ca_merge_kernel<1, 4, TREE>), mgrid, dim3(256), 0, st, p);
+    else if (pl.R == 2) hipLaunchKernelGGL((ca_merge_kernel<2, 2, TREE>), mgrid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((ca_merge_kernel<4, 1, TREE>), mgrid, dim3(256), 0, st, p);
+    return mica_err(hipGetLastError());
+}
+
+// a row stride of `rows` rows that are read by DMA: 32 rows within a buffer's 31-bit range, none overlapping
+int row_stride(long long &ld, long long rows) {
+    if (rows <= 1) ld = kD; // (never used; the range check of a tile counts on it)
+    if (ld < kD || ld % 8) return MICA_MISS_STRIDE;
+    return ld * 2 * kBK >= (1LL << 31) ? MICA_MISS_RANGE : 0;
+}
+bool strides_ok(std::initializer_list<long long> v) {
+    for (long long x : v)
+        if (x < 0 || x % 8) return false;
+    return true;
+}
+// common checks of sizes; 0 when the call goes on
+int check_sizes(int B, int Sq, int HQ, int HK, int head_dim, float scale) {
+    if (head_dim != kD || HK <= 0 || HK > (1 << 20) || HQ != HK * kGroup || B < 0 || Sq < 0) return MICA_MISS_SHAPE;
+    if (!(scale > 0.0f) || !(scale < __builtin_inff())) return MICA_MISS_ARG;
+    if ((long long)B * HK * ((Sq + 7) / 8) >= (1LL << 24)) return MICA_MISS_RANGE;
+    return 0;
+}
+
+}  // namespace
+
+extern "C" long long mica_attention_tree_workspace_bytes(int B, int N, int HK, int cache_cap) {
+    if (B < 0 || N < 0 || N > kMaxNodes || HK <= 0 || cache_cap < 0) return -1;
+    return state_bytes(plan(B, N, HK, tree_tiles(N, cache_cap)));
+}
+
+extern "C" int mica_attention_tree(const void *q, long long sbq, long long shq, long long ldq, const void *k, long long sbk,
+                                   long long shk, long long ldk, const void *v, long long sbv, long long shv,
+                                   long long ldv, const void *k_cache, long long sbkc, long long shkc, long long ldkc,
+                                   const void *v_cache, long long sbvc, long long shvc, long long ldvc, int cache_cap,
+                                   const int *cache_len, const unsigned long long *tree, long long sbt, void *o,
+                                   long long sbo, long long sho, long long ldo, int B, int N, int HQ, int HK, int head_dim,
+                                   float scale, void *workspace, long long workspace_bytes, mica_stream_t stream) {
+    if (const int rc = check_sizes(B, N, HQ, HK, head_dim, scale)) return rc;
+    if (N > kMaxNodes || cache_cap < 0) return MICA_MISS_SHAPE;
+    if (B == 0 || N == 0) return 0;
+    if (!q || !k || !v || !o || !tree || (cache_cap > 0 && (!k_cache || !v_cache))) return MICA_MISS_ARG;
+    if (!strides_ok({sbq, shq, ldq, sbk, shk, sbv, shv, sbo, sho, ldo}) || sbt < 0) return MICA_MISS_STRIDE;
+    if (cache_cap > 0 && !strides_ok({sbkc, shkc, sbvc, shvc})) return MICA_MISS_STRIDE;
+    if (cache_cap == 0) ldkc = ldvc = kD;
+    const struct { long long *ld; long long rows; } ch[4] = {{&ldk, N}, {&ldv, N}, {&ldkc, cache_cap}, {&ldvc, cache_cap}};
+    for (const auto &x : ch)
+        if (const int rc = row_stride(*x.ld, x.rows)) return rc;
+    if (!mica_aligned16(q) || !mica_aligned16(k) || !mica_aligned16(v) || !mica_aligned16(o) || ((uintptr_t)tree & 7) ||
+        (cache_cap > 0 && (!mica_aligned16(k_cache) || !mica_aligned16(v_cache))))
+        return MICA_MISS_ALIGN;
+    const Plan pl = plan(B, N, HK, tree_tiles(N, cache_cap));
+    if (pl.states && (!workspace || !mica_aligned16(workspace) || workspace_bytes < state_bytes(pl))) return MICA_MISS_ARG;
+    CaParams p{};
+    p.q = (const uint16_t *)q; p.sbq = sbq; p.shq = shq; p.ldq = ldq;
+    p.k = (const uint16_t *)k; p.sbk = sbk; p.shk = shk; p.ldk = ldk;
+    p.v = (const uint16_t *)v; p.sbv = sbv; p.shv = shv; p.ldv = ldv;
+    p.kc = (const uint16_t *)k_cache; p.sbkc = sbkc; p.shkc = shkc; p.ldkc = ldkc;
+    p.vc = (const uint16_t *)v_cache; p.sbvc = sbvc; p.shvc = shvc; p.ldvc = ldvc;
+    p.o = (uint16_t *)o; p.sbo = sbo; p.sho = sho; p.ldo = ldo;
+    p.len = cache_len; p.cap = cache_cap;
+    p.tree = (const uint32_t *)tree; p.sbt = 2 * sbt; p.tw = 2 * ((N + 63) / 64);
+    p.B = B; p.Sq = N; p.HK = HK;
+    p.scale_log2 = scale * 1.44269504088896341f;
+    return launch<true>(p, pl, workspace, (hipStream_t)stream);
+}
+
+extern "C" long long mica_attention_window_workspace_bytes(int B, int Sq, int Sk, int HK, int window, int sinks) {
+    if (B < 0 || Sq < 0 || Sk < 0 || HK <= 0 || window < 1 || sinks < 0) return -1;
+    return state_bytes(plan(B, Sq, HK, window_tiles(Sq, Sk, window, sinks)));
+}
+
+extern "C" int mica_attention_window(const void *q, long long sbq, long long shq, long long ldq, const void *k,
+                                     long long sbk, long long shk, long long ldk, const void *v, long long sbv,
+                                     long long shv, long long ldv, void *o, long long sbo, long long sho, long long ldo,
+                                     int B, int Sq, int Sk, int HQ, int HK, int head_dim, float scale, int window, int sinks,
+                                     const int *kv_len, void *workspace, long long workspace_bytes, mica_stream_t stream) {
+    if (const int rc = check_sizes(B, Sq, HQ, HK, head_dim, scale)) return rc;
+    if (Sk < 0 || window < 1 || sinks < 0) return MICA_MISS_SHAPE;
+    if (B == 0 || Sq == 0) return 0;
+    if (!q || !o || (Sk > 0 && (!k || !v))) return MICA_MISS_ARG;
+    if (!strides_ok({sbq, shq, ldq, sbk, shk, sbv, shv, sbo, sho, ldo})) return MICA_MISS_STRIDE;
+    if (const int rc = row_stride(ldk, Sk)) return rc;
+    if (const int rc = row_stride(ldv, Sk)) return rc;
+    if (!mica_aligned16(q) || !mica_aligned16(o) || (Sk > 0 && (!mica_aligned16(k) || !mica_aligned16(v)))) return MICA_MISS_ALIGN;
+    const Plan pl = plan(B, Sq, HK, window_tiles(Sq, Sk, window, sinks));
+    if (pl.states && (!workspace || !mica_aligned16(workspace) || workspace_bytes < state_bytes(pl))) return MICA_MISS_ARG;
+    CaParams p{};
+    p.q = (const uint16_t *)q; p.sbq = sbq; p.shq = shq; p.ldq = ldq;
+    p.k = (const uint16_t *)k; p.sbk = sbk; p.shk = shk; p.ldk = ldk;
+    p.v = (const uint16_t *)v; p.sbv = sbv; p.shv = shv; p.ldv = ldv;
+    p.o = (uint16_t *)o; p.sbo = sbo; p.sho = sho; p.ldo = ldo;
+    p.len = kv_len; p.cap = Sk;
+    p.B = B; p.Sq = Sq; p.HK = HK; p.window = window; p.sinks = sinks;
+    p.scale_log2 = scale * 1.44269504088896341f;
+    return launch<false>(p, pl, workspace, (hipStream_t)stream);
+}

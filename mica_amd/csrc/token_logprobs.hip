@@ -1,0 +1,432 @@
+// Log probabilities of given tokens, the entropy and the top alternatives of rows of logits, in one pass over them.
+//
+//   M = max_v x_v,  S = sum_v e^(x_v - M),  lp(v) = (x_v - M) - ln S,  H = ln S - (sum_v e^(x_v - M) (x_v - M)) / S
+//   top: the `top` largest by (value, then lowest index); NaN counts as the largest value, -0 equals 0
+//
+// A workgroup walks a row's (or a part's) logits in blocks of 256 threads x 32 elements, the next block's loads in flight
+// while it works on one.  Every thread keeps a running (m, s, t) of its own elements in fp32, so the statistics need no
+// barrier.  For the alternatives the workgroup keeps a list of candidates in LDS and a threshold, of which it knows that
+// `top` elements reach it: at first the top-th largest of 64 group maxima of the first block (found bit by bit with
+// ballots), later the top-th largest candidate.  Only elements that reach it are looked at one by one.  A block of which
+// too many do (long runs of ties) is selected exactly, bit by bit over values and then indices.
+//
+// Few rows are divided over several workgroups each; lp_merge_kernel then joins their (m, s, t) and candidates.
+#include "common.h"
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxTop = 32;
+constexpr int kElems = 32;             // elements a thread holds of a block
+constexpr int kBlock = kThreads * kElems;
+constexpr int kCap = 1024;             // candidates in LDS
+constexpr int kMaxParts = 64;
+constexpr float kLog2e = 1.44269504088896341f;
+constexpr float kFar = -1.0e4f;        // e^-10000 is 0 in fp32: differences are cut here, so that 0 x inf never is
+
+struct LpParams {
+    const void *x; long long ldx;      // logits [T][V], rows ldx elements apart
+    const void *tok; int tok64;        // given tokens, int32 or int64 [T][C]
+    int T, V, C, top;
+    int parts, bpp;                    // workgroups a row, blocks each
+    float *lp;                         // [T][C]
+    float *ent;                        // [T]
+    long long *ids;                    // [T][top]
+    float *tlp;                        // [T][top]
+    float4 *pm;                        // partial (m, s, t) [T][parts]
+    unsigned long long *pk;            // partial candidates [T][parts][top], the best first
+};
+
+// values in order as whole numbers: NaN above all, -0 as 0
+MICA_DEVICE uint32_t order_of(float v) {
+    const uint32_t b = __float_as_uint(v + 0.0f);
+    return v != v ? 0xffffffffu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+MICA_DEVICE float value_of(uint32_t o) {
+    return o == 0xffffffffu ? __builtin_nanf("") : __uint_as_float((o & 0x80000000u) ? o & 0x7fffffffu : ~o);
+}
+// larger: the larger value, then the lower index; every element of a row has a key of its own, and none is 0
+MICA_DEVICE unsigned long long key_of(float v, int idx) {
+    return ((unsigned long long)order_of(v) << 32) | (uint32_t)~idx;
+}
+
+template <int DT> struct Elem; // the logits' type: elements in 16 bytes, bits that order_of() leaves free
+template <> struct Elem<MICA_BF16> {
+    static constexpr int N = 8, kBits = 16;
+    static MICA_DEVICE float get(const u32x4 &w, int e) { return (e & 1) ? bf16_hi(w[e >> 1]) : bf16_lo(w[e >> 1]); }
+    static MICA_DEVICE float load(const void *p, long long i) { return bf16_to_f32(((const uint16_t *)p)[i]); }
+    static constexpr uint32_t kLow = 0xff80ff80u; // -inf
+};
+template <> struct Elem<MICA_FP16> {
+    static constexpr int N = 8, kBits = 19;
+    static MICA_DEVICE float get(const u32x4 &w, int e) { return f16_to_f32((uint16_t)(w[e >> 1] >> (16 * (e & 1)))); }
+    static MICA_DEVICE float load(const void *p, long long i) { return f16_to_f32(((const uint16_t *)p)[i]); }
+    static constexpr uint32_t kLow = 0xfc00fc00u;
+};
+template <> struct Elem<MICA_FP32> {
+    static constexpr int N = 4, kBits = 32;
+    static MICA_DEVICE float get(const u32x4 &w, int e) { return __uint_as_float(w[e]); }
+    static MICA_DEVICE float load(const void *p, long long i) { return ((const float *)p)[i]; }
+    static constexpr uint32_t kLow = 0xff800000u;
+};
+
+// (m, s, t): s = sum e^(x - m), t = sum e^(x - m) (x - m); no element yet: (-inf, 0, 0)
+struct Stat { float m, s, t; };
+MICA_DEVICE void rebase(Stat &a, float m) { // m >= a.m
+    const float d = __builtin_fmaxf(a.m - m, kFar); // (also for a.m = m = -inf, whose difference is NaN)
+    const float f = __builtin_amdgcn_exp2f(d * kLog2e);
+    a.t = f * __builtin_fmaf(a.s, d, a.t);
+    a.s *= f;
+    a.m = m;
+}
+
+// the order number of the n-th largest of 64 lanes' values, bit by bit from the top; lower bits than BITS are 0
+template <int BITS>
+MICA_DEVICE uint32_t nth_of_wave(uint32_t o, int n) {
+    uint32_t at = 0;
+#pragma unroll
+    for (int b = 31; b > 31 - BITS; --b) {
+        const uint32_t c = at | (1u << b);
+        if (__builtin_popcountll(__builtin_amdgcn_ballot_w64(o >= c)) >= n) at = c;
+    }
+    return at;
+}
+
+// The best `top` of the list's n keys, in order, at its start (n <= kCap; every thread calls).  Returns how many.
+MICA_DEVICE int keep_best(unsigned long long *list, int n, int top) {
+    unsigned long long mine[kCap / kThreads];
+    int rank[kCap / kThreads];
+    int cnt = 0;
+    for (int i = threadIdx.x, j = 0; i < n; i += kThreads, ++j) cnt = j + 1;
+#pragma unroll
+    for (int j = 0; j < kCap / kThreads; ++j)
+        if (j < cnt) {
+            const unsigned long long k = list[threadIdx.x + j * kThreads];
+            int r = 0;
+            for (int i = 0; i < n; ++i) r += list[i] > k;
+            mine[j] = k, rank[j] = r;
+        }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kCap / kThreads; ++j)
+        if (j < cnt && rank[j] < top) list[rank[j]] = mine[j];
+    __syncthreads();
+    return n < top ? n : top;
+}
+
+// the results of a row from its whole statistics; every thread of a workgroup calls
+template <int DT>
+MICA_DEVICE void finish(const LpParams &p, int row, const Stat &a, const unsigned long long *best) {
+    const void *x = (const char *)p.x + (long long)row * p.ldx * (DT == MICA_FP32 ? 4 : 2);
+    const float ls = logf(a.s);
+    for (int c = threadIdx.x; c < p.C; c += kThreads) {
+        const long long at = (long long)row * p.C + c;
+        const long long id = p.tok64 ? ((const long long *)p.tok)[at] : ((const int *)p.tok)[at];
+        // an id that is no token: NaN, and no access
+        p.lp[at] = id >= 0 && id < p.V ? (Elem<DT>::load(x, id) - a.m) - ls : __builtin_nanf("");
+    }
+    if (threadIdx.x == 0) p.ent[row] = ls - a.t / a.s;
+    if ((int)threadIdx.x < p.top) {
+        const unsigned long long k = best[threadIdx.x];
+        const long long at = (long long)row * p.top + threadIdx.x;
+        p.ids[at] = (long long)(uint32_t)~(uint32_t)k;
+        p.tlp[at] = (value_of((uint32_t)(k >> 32)) - a.m) - ls;
+    }
+}
+
+// one (m, s, t) of the workgroup's 256; every thread gets it
+MICA_DEVICE Stat block_stat(Stat a, float (*red)[4]) {
+    rebase(a, wave_max(a.m));
+    a.s = wave_sum(a.s), a.t = wave_sum(a.t);
+    const int wave = threadIdx.x >> 6;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[wave][0] = a.m, red[wave][1] = a.s, red[wave][2] = a.t;
+    __syncthreads();
+    float m = red[0][0];
+#pragma unroll
+    for (int w = 1; w < kThreads / 64; ++w) m = __builtin_fmaxf(m, red[w][0]);
+    Stat r = {m, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < kThreads / 64; ++w) {
+        Stat b = {red[w][0], red[w][1], red[w][2]};
+        rebase(b, m);
+        r.s += b.s, r.t += b.t;
+    }
+    return r;
+}
+
+template <int DT, bool TOP>
+__global__ __launch_bounds__(kThreads, 4) void lp_rows_kernel(LpParams p) {
+    using E = Elem<DT>;
+    constexpr int U = kElems / E::N, kSize = 16 / E::N;
+    __shared__ float red[kThreads / 64][4];
+    __shared__ float gmax[64];
+    __shared__ unsigned long long list[TOP ? kCap : 1];
+    __shared__ int count, wcount[kThreads / 64];
+    const int row = blockIdx.x / p.parts, part = blockIdx.x % p.parts, tid = threadIdx.x;
+    const char *x = (const char *)p.x + (long long)row * p.ldx * kSize;
+    // the row as up to N - 1 single elements, 16-byte vectors from the first aligned address, up to N - 1 single ones
+    const int head = min((int)((0 - (uintptr_t)x) & 15) / kSize, p.V), nv = (p.V - head) / E::N;
+    const int tail = p.V - head - nv * E::N;
+    const char *body = x + head * kSize;
+    const int v0 = part * p.bpp * (kThreads * U), v1 = min(v0 + p.bpp * (kThreads * U), nv);
+    const bool first_part = part == 0, last_part = part == p.parts - 1;
+    if (TOP && tid == 0) count = 0;
+
+    auto load = [&](int v, u32x4 (&w)[U]) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int at = v + u * kThreads + tid;
+            w[u] = u32x4{E::kLow, E::kLow, E::kLow, E::kLow};
+            if (at < v1) w[u] = __builtin_nontemporal_load((const u32x4 *)(body + (long long)at * 16));
+        }
+    };
+    u32x4 cur[U], nxt[U];
+    load(v0, cur);
+    // a single element a thread: the head's in the first part, the tail's in the last
+    float one = -__builtin_inff();
+    int one_at = -1;
+    if (first_part && tid < head) one_at = tid;
+    if (last_part && tid >= 8 && tid < 8 + tail) one_at = p.V - tail + tid - 8;
+    if (one_at >= 0) one = E::load(x, one_at);
+
+    Stat a = {-__builtin_inff(), 0.0f, 0.0f};
+    float thr = -__builtin_inff(); // elements not below it are candidates;
+    bool above = false;            // or only those above it
+    int kept = 0;                  // candidates of earlier blocks
+    for (int v = v0; v == v0 || v < v1; v += kThreads * U) {
+        const bool first = v == v0;
+        if (v + kThreads * U < v1) load(v + kThreads * U, nxt);
+        float mx = first ? one : -__builtin_inff();
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int e = 0; e < E::N; ++e) mx = __builtin_fmaxf(mx, E::get(cur[u], e));
+        if (__builtin_amdgcn_ballot_w64(mx > a.m)) rebase(a, __builtin_fmaxf(a.m, mx));
+        const float ref = a.m == -__builtin_inff() ? 0.0f : a.m;
+        auto add = [&](float xv) {
+            const float y = xv - ref, ex = __builtin_amdgcn_exp2f(y * kLog2e);
+            a.s += ex;
+            a.t = __builtin_fmaf(ex, __builtin_fmaxf(y, kFar), a.t);
+        };
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int e = 0; e < E::N; ++e) add(E::get(cur[u], e));
+            __asm__ volatile("" : "+v"(a.s), "+v"(a.t)); // the sums here: left alone they follow all 32 exponentials
+        }
+        if (first) add(one);
+        // keeps what the compiler makes of the elements (their unpacked values, their order numbers) from staying in
+        // registers from one use to the next
+        auto forget = [&] {
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) __asm__ volatile("" : "+v"(cur[u][i]));
+        };
+        if constexpr (TOP) {
+            forget();
+            if (first) {
+                float g = mx;
+                g = __builtin_fmaxf(g, __shfl_xor(g, 1, 64));
+                g = __builtin_fmaxf(g, __shfl_xor(g, 2, 64));
+                if ((tid & 3) == 0) gmax[tid >> 2] = g;
+                __syncthreads();
+                thr = value_of(nth_of_wave<E::kBits>(order_of(gmax[tid & 63]), p.top));
+                if (thr != thr) thr = -__builtin_inff(); // (the number below -inf's is a NaN's)
+            }
+            auto reaches = [&](float xv) { return above ? !(xv <= thr) : !(xv < thr); }; // (as a NaN does)
+            // The elements of the block that a thread picks (bit N u + e: element e of its vector u) go to the list.
+            // Their values are read again, by index: taken from registers, each of the 32 would have code of its own.
+            auto push = [&](float xv, int idx) {
+                const int at = atomicAdd(&count, 1);
+                if (at < kCap) list[at] = key_of(xv, idx);
+            };
+            auto push_all = [&](uint32_t bits) {
+                while (bits) {
+                    const int i = __builtin_ctz(bits);
+                    bits &= bits - 1;
+                    const int idx = head + (v + i / E::N * kThreads + tid) * E::N + i % E::N;
+                    push(E::load(x, idx), idx);
+                }
+            };
+            auto pick = [&](auto test) { // test(value, index)
+                uint32_t bits = 0;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int at = v + u * kThreads + tid;
+                    uint32_t mine = 0;
+#pragma unroll
+                    for (int e = 0; e < E::N; ++e) mine |= test(E::get(cur[u], e), head + at * E::N + e) ? 1u << e : 0u;
+                    bits |= at < v1 ? mine << (u * E::N) : 0u;
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                return bits;
+            };
+            // (the maximum passes over NaNs: a thread that has seen one looks at all its elements from then on)
+            if (reaches(mx) || a.s != a.s) {
+                push_all(pick([&](float xv, int) { return reaches(xv); }));
+                if (first && one_at >= 0 && reaches(one)) push(one, one_at);
+            }
+            __syncthreads();
+            int n = count;
+            __syncthreads(); // nobody adds the next block's before everybody has read it
+            const bool exact = n > kCap;
+            if (exact) { // too many reach the threshold: this block's best, exactly
+                // the value of the top-th best element, then the index up to which elements of that value belong
+                auto belongs = [](float xv, int idx, uint32_t o, uint32_t last) { // above order o, or at it by `last`
+                    const uint32_t q = order_of(xv);
+                    return q > o || (q == o && (uint32_t)idx <= last);
+                };
+                auto tally = [&](uint32_t o, uint32_t last) {
+                    forget();
+                    int c = __popc(pick([&](float xv, int idx) { return belongs(xv, idx, o, last); }));
+                    if (first && one_at >= 0) c += belongs(one, one_at, o, last);
+                    const float w = wave_sum((float)c); // (whole numbers below 2^24)
+                    __syncthreads();
+                    if ((tid & 63) == 0) wcount[tid >> 6] = (int)w;
+                    __syncthreads();
+                    return wcount[0] + wcount[1] + wcount[2] + wcount[3];
+                };
+                uint32_t o = 0;
+#pragma unroll 1
+                for (int b = 31; b >= 0; --b) {
+                    const uint32_t c = o | (1u << b);
+                    if (tally(c, 0xffffffffu) >= p.top) o = c;
+                }
+                uint32_t last = 0x7fffffffu; // the least index that still gives `top` elements
+#pragma unroll 1
+                for (int b = 30; b >= 0; --b) {
+                    const uint32_t c = last & ~(1u << b);
+                    if (tally(o, c) >= p.top) last = c;
+                }
+                if (tid == 0) count = kept;
+                __syncthreads();
+                forget();
+                push_all(pick([&](float xv, int idx) { return belongs(xv, idx, o, last); }));
+                if (first && one_at >= 0 && belongs(one, one_at, o, last)) push(one, one_at);
+                __syncthreads();
+                n = count;
+                __syncthreads();
+            }
+            kept = n;
+            if (exact || n > p.top + 16) { // keep the best and raise the threshold
+                kept = keep_best(list, n, p.top);
+                const unsigned long long least = list[p.top - 1];
+                thr = value_of((uint32_t)(least >> 32));
+                if (thr != thr) thr = __builtin_inff();
+                // indices grow from block to block, but for the single elements of the row's end
+                above = (int)~(uint32_t)least < p.V - tail;
+                if (tid == 0) count = kept;
+                __syncthreads();
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) cur[u] = nxt[u];
+    }
+    const Stat all = block_stat(a, red);
+    if constexpr (TOP) kept = keep_best(list, kept, p.top);
+    if (p.parts == 1) {
+        finish<DT>(p, row, all, list);
+        return;
+    }
+    if (tid == 0) p.pm[blockIdx.x] = float4{all.m, all.s, all.t, 0.0f};
+    if (TOP && tid < p.top) p.pk[(long long)blockIdx.x * p.top + tid] = tid < kept ? list[tid] : 0ull;
+}
+
+template <int DT>
+__global__ __launch_bounds__(kThreads) void lp_merge_kernel(LpParams p) {
+    __shared__ unsigned long long list[kCap], all[kMaxParts * kMaxTop];
+    __shared__ int count;
+    const int row = blockIdx.x, tid = threadIdx.x;
+    const float4 *pm = p.pm + (long long)row * p.parts;
+    const float4 mine = (tid & 63) < p.parts ? pm[tid & 63] : float4{-__builtin_inff(), 0.0f, 0.0f, 0.0f};
+    Stat a = {mine.x, mine.y, mine.z};
+    rebase(a, wave_max(a.m));
+    a.s = wave_sum(a.s), a.t = wave_sum(a.t);
+    if (p.top > 0) {
+        const int n = p.parts * p.top;
+        const unsigned long long *pk = p.pk + (long long)row * n;
+        for (int i = tid; i < n; i += kThreads) all[i] = pk[i];
+        if (tid == 0) count = 0;
+        __syncthreads();
+        // every part's r-th best, r = top / parts rounded up: together top keys at least reach the least of them
+        const int r = (p.top + p.parts - 1) / p.parts;
+        unsigned long long least = ~0ull;
+        for (int c = 0; c < p.parts; ++c) least = min(least, all[c * p.top + r - 1]);
+        for (int i = tid; i < n; i += kThreads)
+            if (all[i] >= least && all[i] != 0) {
+                const int at = atomicAdd(&count, 1);
+                if (at < kCap) list[at] = all[i];
+            }
+        __syncthreads();
+        const int c = count;
+        if (c <= kCap) {
+            keep_best(list, c, p.top);
+        } else { // (parts of ascending values)  rank among all keys
+            for (int i = tid; i < n; i += kThreads) {
+                int k = 0;
+                for (int j = 0; j < n; ++j) k += all[j] > all[i];
+                if (k < p.top && all[i] != 0) list[k] = all[i];
+            }
+            __syncthreads();
+        }
+    }
+    finish<DT>(p, row, a, list);
+}
+
+// Workgroups a row, and blocks each: enough for the chip (256 CUs), whole blocks each.
+void divide(int T, int V, int elems, int &parts, int &bpp) {
+    const int blocks = max(1, (V / elems + kThreads * (kElems / elems) - 1) / (kThreads * (kElems / elems)));
+    const int want = T >= 1024 ? 1 : min((1024 + T - 1) / T, kMaxParts);
+    bpp = (blocks + want - 1) / want;
+    parts = (blocks + bpp - 1) / bpp;
+}
+long long part_bytes(int T, int parts, int top) { return parts > 1 ? (long long)T * parts * (16 + 8 * top) : 0; }
+
+template <int DT>
+void launch(const LpParams &p, hipStream_t st) {
+    const dim3 grid((unsigned)((long long)p.T * p.parts));
+    if (p.top > 0) hipLaunchKernelGGL((lp_rows_kernel<DT, true>), grid, dim3(kThreads), 0, st, p);
+    else hipLaunchKernelGGL((lp_rows_kernel<DT, false>), grid, dim3(kThreads), 0, st, p);
+    if (p.parts > 1) hipLaunchKernelGGL((lp_merge_kernel<DT>), dim3(p.T), dim3(kThreads), 0, st, p);
+}
+
+}  // namespace
+
+extern "C" long long mica_token_logprobs_workspace_bytes(int T, int V, int dtype, int top) {
+    if (T < 0 || V < 1 || top < 0 || top > kMaxTop || top > V) return -1;
+    if (dtype != MICA_BF16 && dtype != MICA_FP16 && dtype != MICA_FP32) return -1;
+    if (T == 0) return 0;
+    int parts, bpp;
+    divide(T, V, dtype == MICA_FP32 ? 4 : 8, parts, bpp);
+    return part_bytes(T, parts, top);
+}
+
+extern "C" int mica_token_logprobs(const void *logits, int dtype, long long ldx, int T, int V, const void *tokens,
+                                   int tokens_64, int C, int top, float *logprobs, float *entropy, long long *top_ids,
+                                   float *top_logprobs, void *workspace, long long workspace_bytes,
+                                   mica_stream_t stream) {
+    if (dtype != MICA_BF16 && dtype != MICA_FP16 && dtype != MICA_FP32) return MICA_MISS_DTYPE;
+    if (T < 0 || V < 1 || C < 0 || top < 0 || top > kMaxTop || top > V) return MICA_MISS_SHAPE;
+    if (T == 0) return 0;
+    if (!logits || !entropy || (C > 0 && (!tokens || !logprobs)) || (top > 0 && (!top_ids || !top_logprobs))) return MICA_MISS_ARG;
+    if (ldx < V && T > 1) return MICA_MISS_STRIDE;
+    const int size = dtype == MICA_FP32 ? 4 : 2;
+    if ((uintptr_t)logits % size || (uintptr_t)tokens % (tokens_64 ? 8 : 4) || (uintptr_t)top_ids % 8 ||
+        (uintptr_t)logprobs % 4 || (uintptr_t)entropy % 4 || (uintptr_t)top_logprobs % 4)
+        return MICA_MISS_ALIGN;
+    LpParams p{};
+    p.x = logits; p.ldx = ldx; p.tok = tokens; p.tok64 = tokens_64 != 0; p.T = T; p.V = V; p.C = C; p.top = top;
+    p.lp = logprobs; p.ent = entropy; p.ids = top_ids; p.tlp = top_logprobs;
+    divide(T, V, 16 / size, p.parts, p.bpp);
+    const long long need = part_bytes(T, p.parts, top);
+    if (need && (!workspace || !mica_aligned16(workspace) || workspace_bytes < need)) return MICA_MISS_ARG;
+    if (V > (1 << 30) || (long long)T * p.parts >= (1LL << 31)) return MICA_MISS_RANGE;
+    p.pm = (float4 *)workspace;
+    p.pk = (unsigned long long *)((char *)workspace + (long long)T * p.parts * 16);
+    if (dtype == MICA_BF16) launch<MICA_BF16>(p, (hipStream_t)stream);
+    else if (dtype == MICA_FP16) launch<MICA_FP16>(p, (hipStream_t)stream);
+    else launch<MICA_FP32>(p, (hipStream_t)stream);
+    return mica_err(hipGetLastError());
+}

@@ -7,6 +7,8 @@ v0.5/serving/lib/release_runtime.py:298-306) applied to ``body.norm`` of the las
 """
 from __future__ import annotations
 
+from typing import NamedTuple
+
 import torch
 
 from . import _lib
@@ -98,3 +100,56 @@ def gather_logits(h, last_idx, norm_w, eps, label_W, n_opts, offset=1.0):
     _, probs = ro(h, last_idx, norm_w, eps, offset, lo=lo, cnt=torch.tensor(cnt, dtype=torch.int32),
                   probs_width=max(cnt) if cnt else 0)
     return probs
+
+
+MAX_TOP = 32     # alternatives of token_logprobs
+
+
+class TokenLogprobs(NamedTuple):
+    """token_logprobs' results: fp32 of the tokens' shape, fp32 [T], int64 [T, top], fp32 [T, top]."""
+
+    logprobs: torch.Tensor
+    entropy: torch.Tensor
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
+
+
+def token_logprobs(logits, tokens, top: int = 0) -> TokenLogprobs:
+    """Log probabilities of given tokens under rows of logits, each row's entropy (nats) and its `top` most probable
+    tokens, in one pass over the logits (mica_token_logprobs).
+
+    logits: [T, V] bf16 / fp16 / fp32 with unit column stride (a view of wider rows will do), e.g. a full-vocabulary
+    head's output.  tokens: int32 or int64, one token for each row [T] or several [T, C]; an id outside 0 .. V - 1 gives
+    NaN.  top: 0 .. 32 alternatives, equal logits by the lower id.  A logit of -inf has probability 0; a row with a NaN or
+    +inf logit, or with -inf only, gives NaN."""
+    if not logits.is_cuda:
+        raise ValueError("mica_amd readout runs on the GPU only (got a CPU tensor)")
+    if logits.dim() != 2 or logits.dtype not in DT or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise ValueError("logits must be a 2-D bf16, fp16 or fp32 tensor with unit column stride")
+    dev = logits.device
+    T, V = logits.shape
+    if (tokens.device != dev or tokens.dtype not in (torch.int32, torch.int64) or tokens.dim() not in (1, 2)
+            or tokens.shape[0] != T):
+        raise ValueError("tokens must be an int32 or int64 [T] or [T, C] tensor on the logits' device")
+    top = int(top)
+    if V < 1 or not 0 <= top <= min(MAX_TOP, V):
+        raise ValueError(f"top must be 0 .. {MAX_TOP} and at most the vocabulary")
+    if not _gpu_ok(dev):
+        raise RuntimeError(f"mica_amd kernels need a gfx950 GPU (device {dev})")
+    tokens = tokens.contiguous()
+    C = 1 if tokens.dim() == 1 else tokens.shape[1]
+    out = TokenLogprobs(torch.empty(tokens.shape, dtype=torch.float32, device=dev),
+                        torch.empty(T, dtype=torch.float32, device=dev),
+                        torch.empty((T, top), dtype=torch.int64, device=dev),
+                        torch.empty((T, top), dtype=torch.float32, device=dev))
+    lib = _lib.load()
+    nbytes = int(lib.mica_token_logprobs_workspace_bytes(T, V, DT[logits.dtype], top))
+    ws = torch.empty((max(nbytes, 16),), dtype=torch.uint8, device=dev)
+    rc = _lib.check(_on(dev, lambda: lib.mica_token_logprobs(
+        logits.data_ptr(), DT[logits.dtype], logits.stride(0) if T > 1 else V, T, V, tokens.data_ptr(),
+        int(tokens.dtype == torch.int64), C, top, *(t.data_ptr() for t in out), ws.data_ptr(), nbytes, _stream(dev))),
+        "mica_token_logprobs")
+    if rc > 0:
+        raise ValueError(f"token_logprobs does not support this input ({_lib.status_name(rc)})")
+    _launched()
+    return out
