@@ -91,7 +91,9 @@ SIGNATURES = {
 NATIVE_FNS = ("mica_act_quant", "mica_mm_i8", "mica_rmsnorm_quant", "mica_rmsnorm_quant_multi",
               "mica_attention_prefix_workspace_bytes", "mica_attention_fwd", "mica_attention_fwd_prefix",
               "mica_causal_conv1d", "mica_gdn_chunk", "mica_gdn_chunk_gate", "mica_gdn_workspace_bytes",
-              "mica_gdn_gate", "mica_gated_rmsnorm_quant")
+              "mica_gdn_gate", "mica_gated_rmsnorm_quant", "mica_token_logprobs", "mica_token_logprobs_workspace_bytes",
+              "mica_attention_tree", "mica_attention_tree_workspace_bytes", "mica_attention_window",
+              "mica_attention_window_workspace_bytes")
 
 
 class _NotLoaded:

@@ -263,6 +263,13 @@ def tree_attention(q, k, v, tree, cache=None, cache_len=None, scale: float | Non
     [B, C, HK, 256] or one for all sequences, [1, C, HK, 256] or [C, HK, 256] (a PrefixState's layer), of any strides;
     cache_len: int32 [B] on the device, how many of them sequence b has (None: C; clamped to 0 .. C).  Rows past it are
     never read.  Returns o [B, N, HQ, 256] bf16."""
+    scale = _scale(scale)
+    kc = vc = None
+    if cache is not None:
+        kc, vc = cache = tuple(t.unsqueeze(0) if t.dim() == 3 else t for t in cache)
+    r = _lib.FAST.tree_attention(q, k, v, tree, kc, vc, cache_len, scale)
+    if r is not None:
+        return _native(r, "mica_attention_tree")
     sq, sk, sv = _heads(q, "q"), _heads(k, "k", q.device), _heads(v, "v", q.device)
     dev = q.device
     B, N, HQ, _ = q.shape
@@ -277,14 +284,12 @@ def tree_attention(q, k, v, tree, cache=None, cache_len=None, scale: float | Non
         raise ValueError("tree must be a contiguous int64 [N, ceil(N / 64)] or [B, N, ceil(N / 64)] tensor on q's device")
     C, skc, svc, pk, pv = 0, (0, 0, 0), (0, 0, 0), None, None
     if cache is not None:
-        kc, vc = (t.unsqueeze(0) if t.dim() == 3 else t for t in cache)
         skc, svc = _heads(kc, "cached keys", dev), _heads(vc, "cached values", dev)
         C = kc.shape[1]
         if kc.shape != vc.shape or kc.shape[2] != HK or kc.shape[0] not in (1, B):
             raise ValueError("cached keys and values must both be [B, C, HK, 256] or [1, C, HK, 256]")
         pk, pv = kc.data_ptr(), vc.data_ptr()
     n_len = _counts(cache_len, B, dev, "cache_len")
-    scale = _scale(scale)
     if not _gpu_ok(dev):
         raise RuntimeError(f"mica_amd kernels need a gfx950 GPU (device {dev})")
     L = _lib.load()
@@ -302,6 +307,10 @@ def window_attention(q, k, v, window: int, sinks: int = 0, scale: float | None =
     device, clamped to 0 .. Sk; None: Sk) and its queries are the last Sq of those positions; a query before the first
     key sees nothing, and its output is zeros.  window >= 1, sinks >= 0.  Keys past kv_len or outside every query's
     reach are not read.  Returns o [B, Sq, HQ, 256] bf16."""
+    scale = _scale(scale)
+    r = _lib.FAST.window_attention(q, k, v, window, sinks, kv_len, scale)
+    if r is not None:
+        return _native(r, "mica_attention_window")
     sq, sk, sv = _heads(q, "q"), _heads(k, "k", q.device), _heads(v, "v", q.device)
     dev = q.device
     B, Sq, HQ, _ = q.shape
@@ -313,7 +322,6 @@ def window_attention(q, k, v, window: int, sinks: int = 0, scale: float | None =
         raise ValueError("window must be at least 1 and sinks at least 0")
     window, sinks = min(window, max(Sk, 1)), min(sinks, Sk)
     n_len = _counts(kv_len, B, dev, "kv_len")
-    scale = _scale(scale)
     if not _gpu_ok(dev):
         raise RuntimeError(f"mica_amd kernels need a gfx950 GPU (device {dev})")
     L = _lib.load()

@@ -49,6 +49,12 @@ struct Abi {
     MICA_FN(gdn_workspace_bytes)
     MICA_FN(gdn_gate)
     MICA_FN(gated_rmsnorm_quant)
+    MICA_FN(token_logprobs)
+    MICA_FN(token_logprobs_workspace_bytes)
+    MICA_FN(attention_tree)
+    MICA_FN(attention_tree_workspace_bytes)
+    MICA_FN(attention_window)
+    MICA_FN(attention_window_workspace_bytes)
 #undef MICA_FN
 } abi;
 bool g_bound = false;
@@ -511,6 +517,140 @@ PyObject *py_gated_norm(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+// token_logprobs(logits [T, V], tokens [T] or [T, C], top) -> (logprobs, entropy, top ids, top logprobs)
+PyObject *py_token_logprobs(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    MICA_ARGS(3)
+    const Tensor *x, *tok;
+    Call c;
+    if (!plain(a[0], &x) || !plain(a[1], &tok) || !PyLong_CheckExact(a[2]) || !enter(*x, c)) return none();
+    const long top = PyLong_AsLong(a[2]);
+    if (PyErr_Occurred()) return nullptr;
+    const int dt = code(x->scalar_type());
+    const at::ScalarType tt = tok->scalar_type();
+    if (x->dim() != 2 || dt < 0 || x->stride(1) != 1 || (tt != at::kLong && tt != at::kInt) || !on(c, *tok) ||
+        tok->dim() < 1 || tok->dim() > 2 || tok->size(0) != x->size(0) || !tok->is_contiguous())
+        return none();
+    const int64_t T = x->size(0), V = x->size(1), C = tok->dim() == 1 ? 1 : tok->size(1);
+    if (V < 1 || V >= kI32 || T >= kI32 || C >= kI32 || top < 0 || top > V) return none();
+    const long long nbytes = abi.token_logprobs_workspace_bytes((int)T, (int)V, dt, (int)std::min(top, 1l << 20));
+    if (nbytes < 0) return none();
+    const Tensor lp = make(c, tok->sizes(), at::kFloat), ent = make(c, {T}, at::kFloat), ids = make(c, {T, top}, at::kLong),
+                 best = make(c, {T, top}, at::kFloat);
+    Tensor ws;
+    if (nbytes) ws = make(c, {nbytes}, at::kByte);
+    const int rc = launch([&] {
+        return abi.token_logprobs(x->data_ptr(), dt, T > 1 ? x->stride(0) : V, (int)T, (int)V, tok->data_ptr(),
+                                  tt == at::kLong, (int)C, (int)top, (float *)lp.data_ptr(), (float *)ent.data_ptr(),
+                                  (long long *)ids.data_ptr(), (float *)best.data_ptr(), nbytes ? ws.data_ptr() : nullptr,
+                                  nbytes, c.stream);
+    });
+    if (rc) return bad(rc);
+    return pack({wrap(lp), wrap(ent), wrap(ids), wrap(best)});
+    END_HANDLE_TH_ERRORS
+}
+
+// bf16 [B, S, heads, 256] heads with unit feature stride, 16-byte aligned; their strides, those of one-element axes as 0
+struct Heads {
+    const void *p = nullptr;
+    long long sb = 0, sh = 0, ld = 0;
+    bool of(const Call &c, const Tensor &t) {
+        if (t.dim() != 4 || t.scalar_type() != at::kBFloat16 || t.size(3) != 256 || t.stride(3) != 1 || !on(c, t) || !aligned(t))
+            return false;
+        p = t.data_ptr();
+        sb = t.size(0) > 1 ? t.stride(0) : 0, sh = t.size(2) > 1 ? t.stride(2) : 0, ld = t.size(1) > 1 ? t.stride(1) : 0;
+        return true;
+    }
+};
+// an optional contiguous int32 [B]
+bool counts(const Call &c, const Tensor *t, int64_t B) {
+    return !t || (t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == B && t->is_contiguous() && on(c, *t));
+}
+// q [B, Sq, HQ, 256], k / v [B, Sk, HK, 256], HQ = 4 HK; sizes that an int holds
+bool qkv(const Call &c, const Tensor &q, const Tensor &k, const Tensor &v, Heads &hq, Heads &hk, Heads &hv) {
+    return hq.of(c, q) && hk.of(c, k) && hv.of(c, v) && k.sizes() == v.sizes() && k.size(0) == q.size(0) &&
+           q.size(2) == 4 * k.size(2) && k.size(2) > 0 && q.numel() / 256 < kI32 && k.numel() / 256 < kI32;
+}
+
+// tree_attention(q, k, v, masks, cached keys, cached values, cached counts, scale) -> o
+PyObject *py_tree_attention(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    MICA_ARGS(8)
+    const Tensor *q, *k, *v, *tree, *kc, *vc, *len;
+    Call c;
+    if (!plain(a[0], &q) || !plain(a[1], &k) || !plain(a[2], &v) || !plain(a[3], &tree) || !plain_opt(a[4], &kc) ||
+        !plain_opt(a[5], &vc) || !plain_opt(a[6], &len) || !enter(*q, c))
+        return none();
+    const double scale = PyFloat_AsDouble(a[7]);
+    if (PyErr_Occurred()) return nullptr;
+    Heads hq, hk, hv, hkc, hvc;
+    if (!qkv(c, *q, *k, *v, hq, hk, hv) || (kc == nullptr) != (vc == nullptr)) return none();
+    const int64_t B = q->size(0), N = q->size(1), HK = k->size(2), W = (N + 63) / 64;
+    int64_t C = 0;
+    if (k->size(1) != N || tree->scalar_type() != at::kLong || !tree->is_contiguous() || !on(c, *tree) || !counts(c, len, B))
+        return none();
+    const bool each = tree->dim() == 3;
+    if (each ? tree->size(0) != B || tree->size(1) != N || tree->size(2) != W
+             : tree->dim() != 2 || tree->size(0) != N || tree->size(1) != W)
+        return none();
+    if (kc) {
+        if (!hkc.of(c, *kc) || !hvc.of(c, *vc) || kc->sizes() != vc->sizes() || kc->size(2) != HK ||
+            (kc->size(0) != 1 && kc->size(0) != B))
+            return none();
+        C = kc->size(1);
+        if (C >= kI32) return none();
+    }
+    const long long nbytes = abi.attention_tree_workspace_bytes((int)B, (int)N, (int)HK, (int)C);
+    if (nbytes < 0) return none();
+    const Tensor o = make(c, q->sizes(), at::kBFloat16);
+    Tensor ws;
+    if (nbytes) ws = make(c, {nbytes}, at::kByte);
+    const int rc = launch([&] {
+        return abi.attention_tree(hq.p, hq.sb, hq.sh, hq.ld, hk.p, hk.sb, hk.sh, hk.ld, hv.p, hv.sb, hv.sh, hv.ld, hkc.p,
+                                  hkc.sb, hkc.sh, hkc.ld, hvc.p, hvc.sb, hvc.sh, hvc.ld, (int)C, (const int *)ptr(len),
+                                  (const unsigned long long *)tree->data_ptr(), each ? N * W : 0, o.data_ptr(), o.stride(0),
+                                  o.stride(2), o.stride(1), (int)B, (int)N, (int)(4 * HK), (int)HK, 256, (float)scale,
+                                  nbytes ? ws.data_ptr() : nullptr, nbytes, c.stream);
+    });
+    if (rc) return bad(rc);
+    return wrap(o);
+    END_HANDLE_TH_ERRORS
+}
+
+// window_attention(q, k, v, window, sinks, key counts, scale) -> o
+PyObject *py_window_attention(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    MICA_ARGS(7)
+    const Tensor *q, *k, *v, *len;
+    Call c;
+    if (!plain(a[0], &q) || !plain(a[1], &k) || !plain(a[2], &v) || !PyLong_CheckExact(a[3]) || !PyLong_CheckExact(a[4]) ||
+        !plain_opt(a[5], &len) || !enter(*q, c))
+        return none();
+    const double scale = PyFloat_AsDouble(a[6]);
+    int over = 0;
+    long long window = PyLong_AsLongLongAndOverflow(a[3], &over), sinks = over ? 0 : PyLong_AsLongLongAndOverflow(a[4], &over);
+    if (PyErr_Occurred()) return nullptr;
+    Heads hq, hk, hv;
+    if (over || window < 1 || sinks < 0 || !qkv(c, *q, *k, *v, hq, hk, hv)) return none();
+    const int64_t B = q->size(0), Sq = q->size(1), Sk = k->size(1), HK = k->size(2);
+    if (!counts(c, len, B)) return none();
+    window = std::min<long long>(window, std::max<int64_t>(Sk, 1)), sinks = std::min<long long>(sinks, Sk);
+    const long long nbytes = abi.attention_window_workspace_bytes((int)B, (int)Sq, (int)Sk, (int)HK, (int)window, (int)sinks);
+    if (nbytes < 0) return none();
+    const Tensor o = make(c, q->sizes(), at::kBFloat16);
+    Tensor ws;
+    if (nbytes) ws = make(c, {nbytes}, at::kByte);
+    const int rc = launch([&] {
+        return abi.attention_window(hq.p, hq.sb, hq.sh, hq.ld, hk.p, hk.sb, hk.sh, hk.ld, hv.p, hv.sb, hv.sh, hv.ld,
+                                    o.data_ptr(), o.stride(0), o.stride(2), o.stride(1), (int)B, (int)Sq, (int)Sk,
+                                    (int)(4 * HK), (int)HK, 256, (float)scale, (int)window, (int)sinks, (const int *)ptr(len),
+                                    nbytes ? ws.data_ptr() : nullptr, nbytes, c.stream);
+    });
+    if (rc) return bad(rc);
+    return wrap(o);
+    END_HANDLE_TH_ERRORS
+}
+
 // bind({name: address}): the loaded library's functions
 PyObject *py_bind(PyObject *, PyObject *d) {
     bool all = PyDict_Check(d);
@@ -533,6 +673,12 @@ PyObject *py_bind(PyObject *, PyObject *d) {
     MICA_FN(gdn_workspace_bytes)
     MICA_FN(gdn_gate)
     MICA_FN(gated_rmsnorm_quant)
+    MICA_FN(token_logprobs)
+    MICA_FN(token_logprobs_workspace_bytes)
+    MICA_FN(attention_tree)
+    MICA_FN(attention_tree_workspace_bytes)
+    MICA_FN(attention_window)
+    MICA_FN(attention_window_workspace_bytes)
 #undef MICA_FN
     if (PyErr_Occurred()) return nullptr;
     if (!all) {
@@ -578,6 +724,9 @@ PyMethodDef kMethods[] = {
     MICA_DEF("gdn_chunk_gate", py_gdn_chunk_gate),
     MICA_DEF("gdn_gate", py_gdn_gate),
     MICA_DEF("gated_norm", py_gated_norm),
+    MICA_DEF("token_logprobs", py_token_logprobs),
+    MICA_DEF("tree_attention", py_tree_attention),
+    MICA_DEF("window_attention", py_window_attention),
     {"bind", py_bind, METH_O, nullptr},
     {"device_ok", py_device_ok, METH_O, nullptr},
     MICA_DEF("workspace", py_workspace),

@@ -12,7 +12,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .int8_kernels import DT, _gpu_ok, _launched, _on, _stream
+from .int8_kernels import DT, _gpu_ok, _launched, _native, _on, _stream
 
 
 class LabelReadout:
@@ -122,6 +122,9 @@ def token_logprobs(logits, tokens, top: int = 0) -> TokenLogprobs:
     head's output.  tokens: int32 or int64, one token for each row [T] or several [T, C]; an id outside 0 .. V - 1 gives
     NaN.  top: 0 .. 32 alternatives, equal logits by the lower id.  A logit of -inf has probability 0; a row with a NaN or
     +inf logit, or with -inf only, gives NaN."""
+    r = _lib.FAST.token_logprobs(logits, tokens, top)
+    if r is not None:
+        return TokenLogprobs._make(_native(r, "mica_token_logprobs"))
     if not logits.is_cuda:
         raise ValueError("mica_amd readout runs on the GPU only (got a CPU tensor)")
     if logits.dim() != 2 or logits.dtype not in DT or (logits.shape[1] > 1 and logits.stride(1) != 1):
