@@ -91,6 +91,7 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
     constexpr int NB = 8 * R;                 // query positions of the workgroup
     constexpr int NDT = kD / 32 / D;          // 32-dim tiles of O a wave holds
     constexpr int kBlk = 16 / kWaves;         // 1 KB DMA blocks of K, and of V, a wave issues for a tile
+    constexpr int kPf = D > 1 ? 8 : 2;        // operand fragments read ahead (D = 1: all registers are taken)
     constexpr int kWords = TREE ? NB * (kMaxNodes / 32) : 1;
     static_assert(R * 32 * kD * 2 <= ST * kStage, "the output is staged where the tiles were");
     __shared__ __attribute__((aligned(1024))) int8_t smem[ST * kStage];
@@ -98,6 +99,7 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l32 = lane & 31, hi = lane >> 5;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void *)smem;
     const int rb = wave / D, dt0 = (wave % D) * NDT;
     // Workgroup -> (sequence, chunk, key/value head, query block).  Consecutive workgroups go to the 8 XCDs in turn; the
     // gq query blocks of a group, which read the same keys, stay on one XCD, one after the other.
@@ -150,19 +152,23 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
             (void *)kb, 0, rows > 0 ? (int)((rows - 1) * ldk * 2) + kD * 2 : 0, kBufferFlags);
         const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
             (void *)vb, 0, rows > 0 ? (int)((rows - 1) * ldv * 2) + kD * 2 : 0, kBufferFlags);
-        int8_t *s = smem + st * kStage;
+        // 1 KB block x = key rows 2 x + hi; chunk c of row r lies at c ^ (r % 16) (K), c ^ 2 (r % 8) (V).  The offsets
+        // come from an opaque copy of the lane id at every tile: hoisted out of the loop they take 16 registers, and
+        // what these push into scratch is then loaded back behind the DMA, which every such load waits for.
+        int ln = lane;
+        __asm__ volatile("" : "+v"(ln));
+        const int r0 = 2 * kBlk * wave + (ln >> 5), k2 = (int)(ldk * 2), v2 = (int)(ldv * 2);
+        const int rk0 = r0 * k2, rv0 = r0 * v2;
+        int8_t *s = smem + st * kStage + kBlk * wave * 1024;
 #pragma unroll
-        for (int x = 0; x < kBlk; ++x) {
-            const int blk = wave * kBlk + x, r = 2 * blk + hi; // 1 KB = key rows 2 blk and 2 blk + 1
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void *)(s + blk * 1024), 16,
-                                                     r * (int)(ldk * 2) + ((l32 ^ r) << 4), 0, 0, 0);
-        }
+        for (int x = 0; x < kBlk; ++x)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void *)(s + x * 1024), 16,
+                                                     rk0 + 2 * x * k2 + (((ln & 31) ^ ((r0 + 2 * x) & 15)) << 4), 0, 0, 0);
 #pragma unroll
-        for (int x = 0; x < kBlk; ++x) {
-            const int blk = wave * kBlk + x, r = 2 * blk + hi;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void *)(s + kTile + blk * 1024), 16,
-                                                     r * (int)(ldv * 2) + ((l32 ^ ((r & 7) << 1)) << 4), 0, 0, 0);
-        }
+        for (int x = 0; x < kBlk; ++x)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void *)(s + kTile + x * 1024), 16,
+                                                     rv0 + 2 * x * v2 + (((ln & 31) ^ (((r0 + 2 * x) & 7) << 1)) << 4), 0,
+                                                     0, 0);
     };
 #pragma unroll
     for (int s = 0; s < ST - 1; ++s) issue(i0 + s, s);
@@ -189,17 +195,21 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
     // 16 ((l / 16) % 2) + 4 (l % 4); chunk c of row r lies at c ^ 2 (r % 8), which spreads the 8 rows x 64 bytes of a
     // read over all banks twice, the least 512 bytes can take.
     const int vrow = 4 * hi + ((l32 & 15) >> 2);
-    const int vc0 = (2 * (l32 >> 4) + ((l32 & 3) >> 1)) ^ (vrow << 1);
-    int vaddr[NDT < 4 ? NDT : 4];
-#pragma unroll
-    for (int j = 0; j < (NDT < 4 ? NDT : 4); ++j)
-        vaddr[j] = kTile + vrow * (kD * 2) + (((4 * (dt0 + j)) ^ vc0) << 4) + (l32 & 1) * 8;
+    const uint32_t vbase = lds0 + kTile + vrow * (kD * 2) + (((2 * (l32 >> 4) + ((l32 & 3) >> 1)) ^ (vrow << 1) ^ (4 * dt0)) << 4) +
+                           (l32 & 1) * 8;
+    // K fragment s: chunk 2 s + hi of key row l % 32, at chunk ^ (l % 16).  The chunk's five bits are address bits of
+    // their own in both tiles, so a fragment's address is one exclusive or away from its stage's.
+    const uint32_t kbase = lds0 + l32 * (kD * 2) + ((hi ^ (l32 & 15)) << 4);
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-    auto vfrag = [&](const int8_t *stage, int s, int dt) {
-        const int8_t *a = stage + vaddr[dt & 3] + (dt >> 2) * 256 + s * 16 * (kD * 2);
-        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)a);
-        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(a + 8 * (kD * 2)));
+    typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+    auto kfrag = [](uint32_t stage, int s) { // stage: kbase + the stage's offset
+        return __builtin_bit_cast(bf16x8, *(lds_u32x4 *)(uintptr_t)((stage ^ (s << 5))));
+    };
+    auto vfrag = [](uint32_t stage, int s, int dt) { // stage: vbase + the stage's offset
+        const uint32_t a = (stage ^ (dt << 6)) + s * 16 * (kD * 2);
+        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(uintptr_t)a);
+        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(uintptr_t)(a + 8 * (kD * 2)));
         return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
     };
 
@@ -212,19 +222,16 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
         __builtin_amdgcn_sched_barrier(0);
         issue(i + ST - 1, (st + ST - 1) % ST);
         const int8_t *stage = smem + st * kStage;
-        // ---- S^T = K Q^T: rows = keys of the tile, column = this lane's row ----
+        const uint32_t ks = kbase + st * kStage, vs = vbase + st * kStage;
+        // ---- S^T = K Q^T: rows = keys of the tile, column = this lane's row; fragments read kPf steps ahead ----
         f32x16 sc = {};
-        auto kfrag = [&](int s) {
-            return __builtin_bit_cast(bf16x8, *(const u32x4 *)(stage + l32 * (kD * 2) + (((2 * s + hi) ^ l32) << 4)));
-        };
-        bf16x8 ka = kfrag(0), kb = kfrag(1);
+        bf16x8 kf[kPf];
+#pragma unroll
+        for (int s = 0; s < kPf; ++s) kf[s] = kfrag(ks, s);
 #pragma unroll
         for (int s = 0; s < kD / 16; ++s) {
-            const bf16x8 a = (s & 1) ? kb : ka;
-            if (s + 2 < kD / 16) {
-                if (s & 1) kb = kfrag(s + 2);
-                else ka = kfrag(s + 2);
-            }
+            const bf16x8 a = kf[s % kPf];
+            if (s + kPf < kD / 16) kf[s % kPf] = kfrag(ks, s + kPf);
             __builtin_amdgcn_sched_barrier(0);
             sc = mfma_bf16(a, qf[s], sc);
         }
@@ -307,7 +314,7 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
                 for (int x = 0; x < 4 * NDT; ++x) {
                     const int s = x & 1, dt = x >> 2;
                     const uint32_t sign = x & 2 ? 0x8000u : 0u;
-                    u32x4 w = __builtin_bit_cast(u32x4, vfrag(stage, s, dt));
+                    u32x4 w = __builtin_bit_cast(u32x4, vfrag(vs, s, dt));
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         w[e] = odd_value(w[e] & 0xffffu, sign) | (odd_value(w[e] >> 16, sign) << 16);
@@ -323,15 +330,15 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
                 __syncthreads();
             }
         }
-        // ---- O^T += V^T P^T, the fragments read two steps ahead ----
-        bf16x8 va = vfrag(stage, 0, 0), vb = vfrag(stage, 1 / NDT, 1 % NDT);
+        // ---- O^T += V^T P^T ----
+        constexpr int kPv = kPf < 2 * NDT ? kPf : 2 * NDT;
+        bf16x8 vf[kPv];
+#pragma unroll
+        for (int x = 0; x < kPv; ++x) vf[x] = vfrag(vs, x / NDT, x % NDT);
 #pragma unroll
         for (int x = 0; x < 2 * NDT; ++x) {
-            const bf16x8 a = (x & 1) ? vb : va;
-            if (x + 2 < 2 * NDT) {
-                if (x & 1) vb = vfrag(stage, (x + 2) / NDT, (x + 2) % NDT);
-                else va = vfrag(stage, (x + 2) / NDT, (x + 2) % NDT);
-            }
+            const bf16x8 a = vf[x % kPv];
+            if (x + kPv < 2 * NDT) vf[x % kPv] = vfrag(vs, (x + kPv) / NDT, (x + kPv) % NDT);
             __builtin_amdgcn_sched_barrier(0);
             O[x % NDT] = mfma_bf16(a, pb[x / NDT], O[x % NDT]);
         }
@@ -434,7 +441,7 @@ Plan plan(int B, int Sq, int HK, int max_tiles) {
     pl.gq = pl.nqb < 8 ? pl.nqb : 8;
     const long long base = (long long)B * HK * pl.nqb, want = base ? (kSlots * (pl.ST == 2 ? 2 : 1) + base - 1) / base : 1;
     long long chunk = (max_tiles + want - 1) / want;
-    if (chunk < 4) chunk = 4;
+    if (chunk < 4 * pl.R) chunk = 4 * pl.R;
     pl.chunk = (int)chunk;
     pl.nchunk = max_tiles > chunk ? (int)((max_tiles + chunk - 1) / chunk) : 1;
     const long long units = (long long)B * pl.nchunk * HK, groups = units * ((pl.nqb + pl.gq - 1) / pl.gq);
