@@ -18,8 +18,11 @@
 // memory and its V^T fragments are transposing reads (ds_read_b64_tr_b16: 16 lanes fetch 4 keys x 16 dims and each gets
 // the 4 keys of one dim), so no pass over V comes before.
 //
-// When there are few workgroups, the key tiles are divided into chunks and ca_merge_kernel joins the partial softmax
-// states (fp32).
+// Up to 64 query positions, one row block takes them all, and the key tiles of all sequences, one after the other, are
+// divided evenly over the chip's workgroups (STREAM): a workgroup may end one sequence and begin the next, so
+// key counts that differ, or sequences that do not divide the chip, leave no CU idle.  More positions take a workgroup
+// for each block, their tiles divided into chunks where that leaves too few.  ca_merge_kernel joins the partial softmax
+// states (fp32) of what was divided.
 #include "attn_common.h"
 
 namespace {
@@ -30,7 +33,7 @@ constexpr int kBK = 32;                    // keys per tile
 constexpr int kTile = kBK * kD * 2;        // 16 KB of K or V
 constexpr int kStage = 2 * kTile;
 constexpr int kMaxNodes = 512;             // nodes of a tree
-constexpr int kSlots = 256;                // CUs of the chip
+constexpr int kCus = 256;                  // CUs of the chip
 
 struct CaParams {
     const uint16_t *q; long long sbq, shq, ldq;     // head h of row t of sequence b: q + b sbq + h shq + t ldq
@@ -46,6 +49,7 @@ struct CaParams {
     int window, sinks;
     float scale_log2;                               // softmax scale x log2(e)
     int nqb, gq, chunk, nchunk;                     // query blocks, in groups of gq; tiles a workgroup, chunks a sequence
+    int runs, least;                                // STREAM: runs of tiles, the fewest tiles of one
     float *part_o;                                  // partial O, a wave's accumulators 64 lanes x 16 bytes at a time
     float2 *part_ml;                                // partial (m, l) of each row
 };
@@ -65,8 +69,8 @@ struct Tiles {
             skip = 0;
         } else {
             const int first = keys - p.Sq + q0, last = first + rows - 1; // positions of the block's queries
-            if (last < 0) {
-                n = n0 = skip = 0;
+            if (last < 0) { // no key: one tile that nothing is read for, so that the zeros are written
+                n = 1, n0 = skip = 0;
                 return;
             }
             const int w0 = max(max(first, 0) - (p.window - 1), 0) / kBK;
@@ -78,6 +82,72 @@ struct Tiles {
     MICA_DEVICE int tile(int i) const { return i < n0 ? i : i + skip; } // window: the key tile's index
 };
 
+// How STREAM divides the tiles: those of all sequences, one after the other, into runs, and a workgroup for each run and
+// head.  Workgroups next to each other take the heads of one run: their rows lie side by side in memory (with the heads
+// one after the other instead, 64 single tokens with a window of 4096 took 208 us and not CHECK).  All lanes of a wave call and get
+// the same; a lane reads every 64th sequence's count.
+template <bool TREE>
+struct Stream {
+    int total, per; // tiles of a head, tiles of a run
+    int x, sum;     // this lane's sequence of the first 64: its tiles, those up to and with it
+    MICA_DEVICE static int of(const CaParams &p, int b) { return Tiles<TREE>(p, key_count(p, b), 0, p.Sq).n; }
+    // a wave's running sums
+    MICA_DEVICE static int scan(int x) {
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int y = __shfl_up(x, d, 64);
+            x += (int)(threadIdx.x & 63) >= d ? y : 0;
+        }
+        return x;
+    }
+    MICA_DEVICE void take(const CaParams &p, int base) {
+        const int b = base + (int)(threadIdx.x & 63);
+        x = b < p.B ? of(p, b) : 0;
+        sum = scan(x);
+    }
+    MICA_DEVICE Stream(const CaParams &p) {
+        if (p.len == nullptr) {
+            x = of(p, 0);
+            total = p.B * x;
+        } else {
+            total = 0;
+            for (int base = (p.B - 1) & ~63; base >= 0; base -= 64) { // (the first 64 last: they are kept)
+                take(p, base);
+                total += __builtin_amdgcn_readlane(sum, 63);
+            }
+        }
+        per = max(p.least, (total + p.runs - 1) / p.runs);
+    }
+    // the sequence and its tile at `at` (below total)
+    MICA_DEVICE void find(const CaParams &p, int at, int &b, int &tile) {
+        if (p.len == nullptr) {
+            b = at / x, tile = at % x;
+            return;
+        }
+        for (int base = 0, before = 0;; base += 64) {
+            if (base) take(p, base);
+            const unsigned long long past = __builtin_amdgcn_ballot_w64(before + sum > at);
+            if (past) {
+                const int l = __builtin_ctzll(past);
+                b = base + l, tile = at - before - __builtin_amdgcn_readlane(sum - x, l);
+                return;
+            }
+            before += __builtin_amdgcn_readlane(sum, 63);
+        }
+    }
+    // the first of sequence b's tiles
+    MICA_DEVICE int first(const CaParams &p, int b) {
+        if (p.len == nullptr) return b * x;
+        int before = 0;
+        for (int base = 0; base < b / 64 * 64; base += 64) {
+            if (base) take(p, base);
+            before += __builtin_amdgcn_readlane(sum, 63);
+        }
+        if (b >= 64) take(p, b / 64 * 64);
+        return before + __builtin_amdgcn_readlane(sum - x, b % 64);
+    }
+};
+
 // A V value (bf16 code) that is not finite as the largest finite value of its sign, NaN with the given sign (0 or 0x8000);
 // 0 for a finite one.  Times 2^127 and summed by the matrix cores these give +-inf, and, with both signs, NaN.
 MICA_DEVICE uint32_t odd_value(uint32_t h, uint32_t nan_sign) {
@@ -85,50 +155,76 @@ MICA_DEVICE uint32_t odd_value(uint32_t h, uint32_t nan_sign) {
     return 0x7f7fu | ((h & 0x7fu) ? nan_sign : (h & 0x8000u));
 }
 
-template <int R, int D, int ST, bool TREE>
+template <int R, int D, int ST, bool TREE, bool STREAM>
 __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca_fwd_kernel(CaParams p) {
     constexpr int kWaves = R * D, kThreads = 64 * kWaves;
     constexpr int NB = 8 * R;                 // query positions of the workgroup
     constexpr int NDT = kD / 32 / D;          // 32-dim tiles of O a wave holds
     constexpr int kBlk = 16 / kWaves;         // 1 KB DMA blocks of K, and of V, a wave issues for a tile
     constexpr int kPf = D > 1 ? 8 : 2;        // operand fragments read ahead (D = 1: all registers are taken)
-    constexpr int kWords = TREE ? NB * (kMaxNodes / 32) : 1;
+    constexpr int kWords = TREE ? NB * (STREAM ? 2 : kMaxNodes / 32) : 1; // (STREAM: up to 64 nodes)
     static_assert(R * 32 * kD * 2 <= ST * kStage, "the output is staged where the tiles were");
     __shared__ __attribute__((aligned(1024))) int8_t smem[ST * kStage];
     __shared__ uint32_t words[kWords];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int l32 = lane & 31, hi = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void *)smem;
     const int rb = wave / D, dt0 = (wave % D) * NDT;
-    // Workgroup -> (sequence, chunk, key/value head, query block).  Consecutive workgroups go to the 8 XCDs in turn; the
-    // gq query blocks of a group, which read the same keys, stay on one XCD, one after the other.
-    const int id = blockIdx.x, ngq = (p.nqb + p.gq - 1) / p.gq;
-    const int grp = id / (8 * p.gq) * 8 + id % 8, unit = grp / ngq, qb = grp % ngq * p.gq + id / 8 % p.gq;
-    if (unit >= p.B * p.nchunk * p.HK || qb >= p.nqb) return;
-    const int hk = unit % p.HK, c = unit / p.HK % p.nchunk, b = unit / p.HK / p.nchunk;
+    int b, hk, qb = 0, i0, left = 0; // the sequence, head and query block, its first tile here, tiles left (STREAM)
+    int blk;                         // where its partial state goes
+    if constexpr (STREAM) {
+        Stream<TREE> all(p);
+        hk = blockIdx.x % p.HK;
+        const int at = blockIdx.x / p.HK * all.per;
+        if (at >= all.total) return;
+        all.find(p, at, b, i0);
+        b = __builtin_amdgcn_readfirstlane(b), i0 = __builtin_amdgcn_readfirstlane(i0);
+        left = __builtin_amdgcn_readfirstlane(min(all.per, all.total - at));
+        blk = 2 * blockIdx.x;
+    } else {
+        // Consecutive workgroups go to the 8 XCDs in turn; the gq query blocks of a group, which read the same keys, stay
+        // on one XCD, one after the other.
+        const int id = blockIdx.x, ngq = (p.nqb + p.gq - 1) / p.gq;
+        const int grp = id / (8 * p.gq) * 8 + id % 8, unit = grp / ngq;
+        qb = grp % ngq * p.gq + id / 8 % p.gq;
+        if (unit >= p.B * p.nchunk * p.HK || qb >= p.nqb) return;
+        hk = unit % p.HK, b = unit / p.HK / p.nchunk, i0 = unit / p.HK % p.nchunk * p.chunk;
+        blk = unit * p.nqb + qb;
+    }
+    for (;;) {
+    // what depends on the lane alone is made here, from an opaque copy of its id: the compiler would make it before the
+    // loop and hold it in registers that the tiles need (45 of them spilled)
+    int tid = threadIdx.x;
+    __asm__ volatile("" : "+v"(tid));
+    const int lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
     const int q0 = qb * NB, keys = key_count(p, b);
     const Tiles<TREE> tl(p, keys, q0, min(NB, p.Sq - q0));
-    const int i0 = c * p.chunk, i1 = min(i0 + p.chunk, tl.n);
-    if (i0 >= tl.n && p.nchunk > 1) return; // (a block without tiles writes its zeros when it is alone)
+    const int i1 = min(STREAM ? i0 + left : i0 + p.chunk, tl.n);
+    if (!STREAM && i0 >= tl.n) return;
+    const bool whole = STREAM ? i0 == 0 && i1 == tl.n : p.nchunk == 1;
 
     // this lane's row: a position and a query head
     const int row = rb * 32 + l32, head = hk * kGroup + row / NB, t = q0 + row % NB;
-    bool absent = false; // a tree node without a bit
+    // the block's words and this lane's Q fragments (B operand of S^T: dims 16 s + 8 hi .. + 7 of the row) are on their
+    // way before the first tiles
+    constexpr int kMine = (kWords + kThreads - 1) / kThreads;
+    uint32_t mine[kMine];
     if constexpr (TREE) {
-#pragma unroll 1
-        for (int i = tid; i < NB * p.tw; i += kThreads) {
-            const int node = q0 + i / p.tw, w = i % p.tw;
-            uint32_t x = node < p.Sq ? p.tree[b * p.sbt + (long long)node * p.tw + w] : 0u;
-            const int left = p.Sq - 32 * w; // bits past the last node do not count
-            x = left >= 32 ? x : left <= 0 ? 0u : x & ((1u << left) - 1u);
-            words[i] = x;
+#pragma unroll
+        for (int x = 0; x < kMine; ++x) {
+            const int i = tid + x * kThreads, node = q0 + i / p.tw;
+            mine[x] = i < NB * p.tw && node < p.Sq ? p.tree[b * p.sbt + (long long)node * p.tw + i % p.tw] : 0u;
         }
-        __syncthreads();
-        uint32_t any = 0;
-#pragma unroll 1
-        for (int w = 0; w < p.tw; ++w) any |= words[row % NB * p.tw + w];
-        absent = any == 0;
+    }
+    bf16x8 qf[kD / 16];
+    {
+        const uint16_t *qr = p.q + b * p.sbq + head * p.shq + (long long)t * p.ldq + hi * 8;
+#pragma unroll
+        for (int s = 0; s < kD / 16; ++s) {
+            u32x4 x = {0u, 0u, 0u, 0u};
+            if (t < p.Sq) x = *(const u32x4 *)(qr + s * 16);
+            qf[s] = __builtin_bit_cast(bf16x8, x);
+        }
     }
 
     // DMA of tile i into stage st; past i1 from a zero-sized buffer, so that every step issues as many instructions
@@ -173,16 +269,18 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
 #pragma unroll
     for (int s = 0; s < ST - 1; ++s) issue(i0 + s, s);
 
-    // Q fragments (B operand of S^T): dims 16 s + 8 hi .. + 7 of this lane's row
-    bf16x8 qf[kD / 16];
-    {
-        const uint16_t *qr = p.q + b * p.sbq + head * p.shq + (long long)t * p.ldq + hi * 8;
+    bool absent = false; // a tree node without a bit
+    if constexpr (TREE) {
 #pragma unroll
-        for (int s = 0; s < kD / 16; ++s) {
-            u32x4 x = {0u, 0u, 0u, 0u};
-            if (t < p.Sq) x = *(const u32x4 *)(qr + s * 16);
-            qf[s] = __builtin_bit_cast(bf16x8, x);
+        for (int x = 0; x < kMine; ++x) {
+            const int i = tid + x * kThreads, left = p.Sq - 32 * (i % p.tw); // bits past the last node do not count
+            if (i < NB * p.tw) words[i] = left >= 32 ? mine[x] : left <= 0 ? 0u : mine[x] & ((1u << left) - 1u);
         }
+        __syncthreads();
+        uint32_t any = 0;
+#pragma unroll 1
+        for (int w = 0; w < p.tw; ++w) any |= words[row % NB * p.tw + w];
+        absent = any == 0;
     }
     f32x16 O[NDT];
 #pragma unroll
@@ -350,69 +448,115 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) O[dt] = f32x16{};
     }
-    if (p.nchunk > 1) {
-        const long long blk = (long long)unit * p.nqb + qb;
-        float *po = p.part_o + ((blk * kWaves + wave) * (NDT * 4) * 64 + lane) * 4;
+    if (!whole) {
+        float *po = p.part_o + (((long long)blk * kWaves + wave) * (NDT * 4) * 64 + lane) * 4;
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
             for (int r4 = 0; r4 < 4; ++r4)
                 *(float4 *)(po + (dt * 4 + r4) * 256) =
                     float4{O[dt][4 * r4], O[dt][4 * r4 + 1], O[dt][4 * r4 + 2], O[dt][4 * r4 + 3]};
-        if (dt0 == 0 && hi == 0) p.part_ml[blk * (32 * R) + row] = float2{m, ltot};
-        return;
-    }
-    // ---- normalise, stage in LDS (32 R rows x 512 B), write 16-byte row pieces ----
-    const float inv = ltot == 0.0f ? 0.0f : 1.0f / ltot;
-    __syncthreads();
+        if (dt0 == 0 && hi == 0) p.part_ml[(long long)blk * (32 * R) + row] = float2{m, ltot};
+    } else {
+        // ---- normalise, stage in LDS (32 R rows x 512 B), write 16-byte row pieces ----
+        const float inv = ltot == 0.0f ? 0.0f : 1.0f / ltot;
+        __syncthreads();
 #pragma unroll
-    for (int dt = 0; dt < NDT; ++dt)
+        for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-            const int d = (dt0 + dt) * 32 + 8 * r4 + 4 * hi;
-            u32x2 w;
-            w[0] = pack_bf16x2(O[dt][4 * r4] * inv, O[dt][4 * r4 + 1] * inv);
-            w[1] = pack_bf16x2(O[dt][4 * r4 + 2] * inv, O[dt][4 * r4 + 3] * inv);
-            *(u32x2 *)(smem + row * (kD * 2) + (((d >> 3) ^ l32) << 4) + (d & 4) * 2) = w;
-        }
-    __syncthreads();
+            for (int r4 = 0; r4 < 4; ++r4) {
+                const int d = (dt0 + dt) * 32 + 8 * r4 + 4 * hi;
+                u32x2 w;
+                w[0] = pack_bf16x2(O[dt][4 * r4] * inv, O[dt][4 * r4 + 1] * inv);
+                w[1] = pack_bf16x2(O[dt][4 * r4 + 2] * inv, O[dt][4 * r4 + 3] * inv);
+                *(u32x2 *)(smem + row * (kD * 2) + (((d >> 3) ^ l32) << 4) + (d & 4) * 2) = w;
+            }
+        __syncthreads();
 #pragma unroll 2
-    for (int x = tid; x < 32 * R * 32; x += kThreads) {
-        const int rr = x >> 5, ch = x & 31, tt = q0 + rr % NB;
-        if (tt < p.Sq)
-            *(u32x4 *)(p.o + b * p.sbo + (long long)(hk * kGroup + rr / NB) * p.sho + (long long)tt * p.ldo + ch * 8) =
-                *(const u32x4 *)(smem + rr * (kD * 2) + ((ch ^ (rr & 31)) << 4));
+        for (int x = tid; x < 32 * R * 32; x += kThreads) {
+            const int rr = x >> 5, ch = x & 31, tt = q0 + rr % NB;
+            if (tt < p.Sq)
+                *(u32x4 *)(p.o + b * p.sbo + (long long)(hk * kGroup + rr / NB) * p.sho + (long long)tt * p.ldo + ch * 8) =
+                    *(const u32x4 *)(smem + rr * (kD * 2) + ((ch ^ (rr & 31)) << 4));
+        }
+    }
+    if (!STREAM) return;
+    left -= i1 - i0;
+    if (left == 0) return;
+    i0 = 0, blk = 2 * blockIdx.x + 1; // (what lies between a workgroup's first and last is whole)
+    ++b;
+    __syncthreads(); // everybody is done with the stages and the words
     }
 }
 
-// The partial states of a block's chunks joined: with M = max_c m_c, w_c = 2^(m_c - M), o = (sum w_c O_c) / (sum w_c l_c).
-// One wave takes 64 lanes x 16 bytes of the forward kernel's accumulators (4 dims of 32 rows x 2) of every chunk.
-template <int R, int D, bool TREE>
+// The partial states of a block's parts joined: with M = max_c m_c, w_c = 2^(m_c - M), o = (sum w_c O_c) / (sum w_c l_c).
+// A part's accumulators are taken 64 lanes x 16 bytes at a time (4 dims of 32 rows x 2), by W waves that share the parts.
+template <int R, int D, bool TREE, bool STREAM, int W>
 __global__ __launch_bounds__(256) void ca_merge_kernel(CaParams p) {
-    constexpr int NB = 8 * R, NDT = kD / 32 / D, kFrags = R * D * NDT * 4; // = 32 R
+    constexpr int NB = 8 * R, NDT = kD / 32 / D, kFrags = 32 * R, kPer = 4 / W;
+    __shared__ float4 accs[W > 1 ? 4 : 1][64];
+    __shared__ float2 mls[W > 1 ? 4 : 1][64];
     const int lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5;
-    const int f = (blockIdx.x % (kFrags / 4)) * 4 + (threadIdx.x >> 6), blk = blockIdx.x / (kFrags / 4);
-    const int qb = blk % p.nqb, hk = blk / p.nqb % p.HK, b = blk / p.nqb / p.HK;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int f = (blockIdx.x % (kFrags / kPer)) * kPer + wave / W, u = blockIdx.x / (kFrags / kPer);
+    const int qb = u % p.nqb, hk = u / p.nqb % p.HK, b = u / p.nqb / p.HK;
     const int q0 = qb * NB, row = f / (NDT * 4 * D) * 32 + l32;
-    const Tiles<TREE> tl(p, key_count(p, b), q0, min(NB, p.Sq - q0));
-    const int n = (tl.n + p.chunk - 1) / p.chunk;
-    const long long u0 = (long long)b * p.nchunk * p.HK + hk; // chunk c is unit u0 + c HK
-    float mx = -__builtin_inff();
-    for (int c = 0; c < n; ++c) mx = __builtin_fmaxf(mx, p.part_ml[((u0 + (long long)c * p.HK) * p.nqb + qb) * (32 * R) + row].x);
-    float l = 0.0f;
+    const int tiles = Tiles<TREE>(p, key_count(p, b), q0, min(NB, p.Sq - q0)).n;
+    int n, g0 = 0, per = 0, s = 0; // parts; STREAM: the run of the first, the runs' tiles, the sequence's first tile
+    if constexpr (STREAM) {
+        Stream<TREE> all(p);
+        per = all.per, s = all.first(p, b);
+        g0 = s / per;
+        n = (s + tiles - 1) / per - g0 + 1;
+        if (n == 1) return; // its workgroup wrote it
+    } else {
+        n = (tiles + p.chunk - 1) / p.chunk;
+    }
+    auto part = [&](int c) -> long long {
+        if constexpr (STREAM) return 2 * ((long long)(g0 + c) * p.HK + hk) + ((g0 + c) * per < s);
+        return ((long long)(b * p.nchunk + c) * p.HK + hk) * p.nqb + qb;
+    };
+    float mx = -__builtin_inff(), l = 0.0f;
     float4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int c = 0; c < n; ++c) {
-        const long long u = (u0 + (long long)c * p.HK) * p.nqb + qb;
-        const float2 ml = p.part_ml[u * (32 * R) + row];
-        const float4 o = *(const float4 *)(p.part_o + ((u * kFrags + f) * 64 + lane) * 4);
-        // a row that no chunk has keys for: weights 1 on zeros (a sum that is NaN stays one)
-        const float w = mx == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(ml.x - mx);
+    // a row that no part has keys for: weights 1 on zeros (a sum that is NaN stays one)
+    auto weight = [](float m, float top) { return top == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - top); };
+    auto add = [&](float w, float2 ml, float4 o) {
         l += w * ml.y;
         acc.x += w * o.x;
         acc.y += w * o.y;
         acc.z += w * o.z;
         acc.w += w * o.w;
+    };
+    constexpr int kBatch = W > 1 ? 8 : 4; // parts whose loads are in flight together
+    for (int c0 = wave % W; c0 < n; c0 += W * kBatch) {
+        float2 ml[kBatch];
+        float4 o[kBatch];
+#pragma unroll
+        for (int x = 0; x < kBatch; ++x) {
+            const int c = c0 + x * W;
+            const long long at = part(c < n ? c : c0);
+            ml[x] = p.part_ml[at * (32 * R) + row];
+            o[x] = *(const float4 *)(p.part_o + ((at * kFrags + f) * 64 + lane) * 4);
+            if (c >= n) ml[x] = float2{-__builtin_inff(), 0.0f}, o[x] = float4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        float top = mx;
+#pragma unroll
+        for (int x = 0; x < kBatch; ++x) top = __builtin_fmaxf(top, ml[x].x);
+        const float w = weight(mx, top);
+        l *= w, acc.x *= w, acc.y *= w, acc.z *= w, acc.w *= w;
+        mx = top;
+#pragma unroll
+        for (int x = 0; x < kBatch; ++x) add(weight(ml[x].x, mx), ml[x], o[x]);
+    }
+    if constexpr (W > 1) {
+        accs[wave][lane] = acc, mls[wave][lane] = float2{mx, l};
+        __syncthreads();
+        if (wave > 0) return;
+#pragma unroll
+        for (int w = 1; w < W; ++w) mx = __builtin_fmaxf(mx, mls[w][lane].x);
+        l = 0.0f, acc = float4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < W; ++w) add(weight(mls[w][lane].x, mx), mls[w][lane], accs[w][lane]);
     }
     const int t = q0 + row % NB;
     if (t >= p.Sq) return;
@@ -426,57 +570,84 @@ __global__ __launch_bounds__(256) void ca_merge_kernel(CaParams p) {
 
 // ---- host side ----
 
-// How a call is divided: row blocks (R) and dim parts (D) of a workgroup, LDS stages, tiles a workgroup, chunks.
+// How a call is divided: row blocks (R) and dim parts (D) of a workgroup, LDS stages, and the work.
 struct Plan {
-    int R, D, ST, nqb, gq, chunk, nchunk;
-    long long wgs, states; // workgroups; partial rows (0: one chunk)
+    int R, D, ST, nqb, gq, chunk, nchunk, runs, least;
+    bool stream, wide;
+    long long tiles, wgs, states; // STREAM: a head's tiles; workgroups; partial rows
 };
 
 Plan plan(int B, int Sq, int HK, int max_tiles) {
     Plan pl{};
-    pl.R = Sq <= 8 ? 1 : Sq <= 16 ? 2 : Sq <= 32 ? 4 : 4;
-    pl.D = 4 / pl.R;
-    pl.ST = pl.R < 4 ? 4 : 2;
+    pl.stream = Sq <= 64;
+    pl.R = Sq <= 8 ? 1 : Sq <= 16 ? 2 : Sq <= 32 || !pl.stream ? 4 : 8;
+    pl.D = pl.R < 4 ? 4 / pl.R : 1;
+    pl.ST = pl.R < 8 ? 2 : 4;
     pl.nqb = (Sq + 8 * pl.R - 1) / (8 * pl.R);
     pl.gq = pl.nqb < 8 ? pl.nqb : 8;
-    const long long base = (long long)B * HK * pl.nqb, want = base ? (kSlots * (pl.ST == 2 ? 2 : 1) + base - 1) / base : 1;
-    long long chunk = (max_tiles + want - 1) / want;
-    if (chunk < 4 * pl.R) chunk = 4 * pl.R;
-    pl.chunk = (int)chunk;
-    pl.nchunk = max_tiles > chunk ? (int)((max_tiles + chunk - 1) / chunk) : 1;
-    const long long units = (long long)B * pl.nchunk * HK, groups = units * ((pl.nqb + pl.gq - 1) / pl.gq);
+    pl.chunk = max_tiles, pl.nchunk = 1;
+    const int slots = kCus * (pl.R < 8 ? 2 : 1);
+    const long long units = (long long)B * HK;
+    if (pl.stream) {
+        pl.least = 2 * pl.R;
+        pl.tiles = (long long)B * max_tiles;
+        const long long most = (pl.tiles + pl.least - 1) / pl.least;
+        pl.runs = HK < slots ? slots / HK : 1;
+        if (most < pl.runs) pl.runs = (int)most;
+        pl.wgs = (long long)pl.runs * HK;
+        pl.states = pl.wgs * 2 * 32 * pl.R;
+        pl.wide = 6 * B <= pl.runs;
+        return pl;
+    }
+    // the chunks that take the least time: rounds of workgroups, each as long as its tiles, and with several chunks a
+    // partial state written (128 KB, a tile is 32) and read again
+    const long long base = units * pl.nqb;
+    long long best = -1;
+    for (int n = 1; n <= 16 && base > 0; ++n) {
+        const long long tiles = (max_tiles + n - 1) / n, cost = ((base * n + slots - 1) / slots) * (tiles + (n > 1 ? 10 : 2));
+        if (best < 0 || cost < best) best = cost, pl.chunk = (int)tiles;
+    }
+    pl.nchunk = pl.chunk > 0 ? (max_tiles + pl.chunk - 1) / pl.chunk : 1;
+    const long long groups = units * pl.nchunk * ((pl.nqb + pl.gq - 1) / pl.gq);
     pl.wgs = (groups + 7) / 8 * 8 * pl.gq;
-    pl.states = pl.nchunk > 1 ? units * pl.nqb * 32 * pl.R : 0;
+    pl.states = pl.nchunk > 1 ? base * pl.nchunk * 32 * pl.R : 0;
     return pl;
 }
 
 int tree_tiles(int N, int cap) { return (cap + kBK - 1) / kBK + (N + kBK - 1) / kBK; }
-// most tiles of a block of Sq <= 32 or 32 queries: the sinks', the window's and the block's own, never more than the keys'
+// most tiles of a block of Sq <= 64 or 32 queries: the sinks', the window's and the block's own, never more than the keys'
 int window_tiles(int Sq, int Sk, int window, int sinks) {
-    const long long all = ((long long)Sk + kBK - 1) / kBK;
-    const long long span = ((long long)window + (Sq < 32 ? Sq : 32) + 2 * kBK - 3) / kBK + 1;
+    const long long all = Sk > 0 ? ((long long)Sk + kBK - 1) / kBK : 1;
+    const long long span = ((long long)window + (Sq <= 64 ? Sq : 32) + 2 * kBK - 3) / kBK + 1;
     const long long n = (sinks + kBK - 1ll) / kBK + span;
     return (int)(n < all ? n : all);
 }
 long long state_bytes(const Plan &pl) { return pl.states * (kD * 4 + 8); }
 
+template <int R, int D, int ST, bool TREE, bool STREAM>
+int launch_as(const CaParams &p, const Plan &pl, hipStream_t st) {
+    hipLaunchKernelGGL((ca_fwd_kernel<R, D, ST, TREE, STREAM>), dim3((unsigned)pl.wgs), dim3(64 * R * D), 0, st, p);
+    if (const int rc = mica_err(hipGetLastError())) return rc;
+    if (pl.states == 0) return 0;
+    const long long blocks = (long long)p.B * p.HK * pl.nqb;
+    if (STREAM && pl.wide)
+        hipLaunchKernelGGL((ca_merge_kernel<R, D, TREE, STREAM, STREAM ? 4 : 1>), dim3((unsigned)(blocks * 32 * R)), dim3(256), 0, st, p);
+    else
+        hipLaunchKernelGGL((ca_merge_kernel<R, D, TREE, STREAM, 1>), dim3((unsigned)(blocks * 8 * R)), dim3(256), 0, st, p);
+    return mica_err(hipGetLastError());
+}
+
 template <bool TREE>
 int launch(CaParams &p, const Plan &pl, void *workspace, hipStream_t st) {
-    p.nqb = pl.nqb, p.gq = pl.gq, p.chunk = pl.chunk, p.nchunk = pl.nchunk;
+    p.nqb = pl.nqb, p.gq = pl.gq, p.chunk = pl.chunk, p.nchunk = pl.nchunk, p.runs = pl.runs, p.least = pl.least;
     p.part_o = (float *)workspace;
     p.part_ml = (float2 *)((char *)workspace + pl.states * kD * 4);
-    if (pl.wgs >= (1LL << 31)) return MICA_MISS_RANGE;
-    const dim3 grid((unsigned)pl.wgs), threads(64 * pl.R * pl.D);
-    if (pl.R == 1) hipLaunchKernelGGL((ca_fwd_kernel<1, 4, 4, TREE>), grid, threads, 0, st, p);
-    else if (pl.R == 2) hipLaunchKernelGGL((ca_fwd_kernel<2, 2, 4, TREE>), grid, threads, 0, st, p);
-    else hipLaunchKernelGGL((ca_fwd_kernel<4, 1, 2, TREE>), grid, threads, 0, st, p);
-    if (const int rc = mica_err(hipGetLastError())) return rc;
-    if (pl.nchunk == 1) return 0;
-    const dim3 mgrid((unsigned)((long long)p.B * p.HK * pl.nqb * 8 * pl.R));
-    if (pl.R == 1) hipLaunchKernelGGL((ca_merge_kernel<1, 4, TREE>), mgrid, dim3(256), 0, st, p);
-    else if (pl.R == 2) hipLaunchKernelGGL((ca_merge_kernel<2, 2, TREE>), mgrid, dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((ca_merge_kernel<4, 1, TREE>), mgrid, dim3(256), 0, st, p);
-    return mica_err(hipGetLastError());
+    if (pl.wgs >= (1LL << 31) || pl.tiles >= (1LL << 30)) return MICA_MISS_RANGE;
+    if (!pl.stream) return launch_as<4, 1, 2, TREE, false>(p, pl, st);
+    if (pl.R == 1) return launch_as<1, 4, 2, TREE, true>(p, pl, st);
+    if (pl.R == 2) return launch_as<2, 2, 2, TREE, true>(p, pl, st);
+    if (pl.R == 4) return launch_as<4, 1, 2, TREE, true>(p, pl, st);
+    return launch_as<8, 1, 4, TREE, true>(p, pl, st);
 }
 
 // a row stride of `rows` rows that are read by DMA: 32 rows within a buffer's 31-bit range, none overlapping
