@@ -3,7 +3,7 @@
 //   M = max_v x_v,  S = sum_v e^(x_v - M),  lp(v) = (x_v - M) - ln S,  H = ln S - (sum_v e^(x_v - M) (x_v - M)) / S
 //   top: the `top` largest by (value, then lowest index); NaN counts as the largest value, -0 equals 0
 //
-// A workgroup walks a row's (or a part's) logits in blocks of 256 threads x 32 elements, the next block's loads in flight
+// (in log2 units, see Stat).  A workgroup walks a row's (or a part's) logits in blocks of 256 threads x 64 bytes, the next block's loads in flight
 // while it works on one.  Every thread keeps a running (m, s, t) of its own elements in fp32, so the statistics need no
 // barrier.  For the alternatives the workgroup keeps a list of candidates in LDS and a threshold, of which it knows that
 // `top` elements reach it: at first the top-th largest of 64 group maxima of the first block (found bit by bit with
@@ -17,13 +17,15 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxTop = 32;
-constexpr int kElems = 32;             // elements a thread holds of a block
-constexpr int kBlock = kThreads * kElems;
+constexpr int U = 4;                   // 16-byte vectors a thread holds of a block
 constexpr int kCap = 1024;             // candidates in LDS
 constexpr int kMaxParts = 64;
-constexpr float kLog2e = 1.44269504088896341f;
-constexpr float kFar = -1.0e4f;        // e^-10000 is 0 in fp32: differences are cut here, so that 0 x inf never is
+constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
+constexpr float kFar = -1.0e4f;        // 2^-10000 is 0 in fp32: differences are cut here, so that 0 x inf never is
+constexpr float kNear = 131072.0f;     // references up to here take one fma an element (Stat)
+constexpr float kRaise = 16.0f;        // e^16 times the elements of a row is far from fp32's range
 
+struct Stat;
 struct LpParams {
     const void *x; long long ldx;      // logits [T][V], rows ldx elements apart
     const void *tok; int tok64;        // given tokens, int32 or int64 [T][C]
@@ -33,7 +35,7 @@ struct LpParams {
     float *ent;                        // [T]
     long long *ids;                    // [T][top]
     float *tlp;                        // [T][top]
-    float4 *pm;                        // partial (m, s, t) [T][parts]
+    Stat *pm;                          // partial sums [T][parts]
     unsigned long long *pk;            // partial candidates [T][parts][top], the best first
 };
 
@@ -50,7 +52,7 @@ MICA_DEVICE unsigned long long key_of(float v, int idx) {
     return ((unsigned long long)order_of(v) << 32) | (uint32_t)~idx;
 }
 
-template <int DT> struct Elem; // the logits' type: elements in 16 bytes, bits that order_of() leaves free
+template <int DT> struct Elem; // the logits' type: elements in 16 bytes, the bits of order_of() that a threshold is found to
 template <> struct Elem<MICA_BF16> {
     static constexpr int N = 8, kBits = 16;
     static MICA_DEVICE float get(const u32x4 &w, int e) { return (e & 1) ? bf16_hi(w[e >> 1]) : bf16_lo(w[e >> 1]); }
@@ -64,21 +66,45 @@ template <> struct Elem<MICA_FP16> {
     static constexpr uint32_t kLow = 0xfc00fc00u;
 };
 template <> struct Elem<MICA_FP32> {
-    static constexpr int N = 4, kBits = 32;
+    static constexpr int N = 4, kBits = 19;
     static MICA_DEVICE float get(const u32x4 &w, int e) { return __uint_as_float(w[e]); }
     static MICA_DEVICE float load(const void *p, long long i) { return ((const float *)p)[i]; }
     static constexpr uint32_t kLow = 0xff800000u;
 };
 
-// (m, s, t): s = sum e^(x - m), t = sum e^(x - m) (x - m); no element yet: (-inf, 0, 0)
-struct Stat { float m, s, t; };
-MICA_DEVICE void rebase(Stat &a, float m) { // m >= a.m
-    const float d = __builtin_fmaxf(a.m - m, kFar); // (also for a.m = m = -inf, whose difference is NaN)
-    const float f = __builtin_amdgcn_exp2f(d * kLog2e);
-    a.t = f * __builtin_fmaf(a.s, d, a.t);
-    a.s *= f;
-    a.m = m;
-}
+// s = sum 2^y, t = sum 2^y y over elements y = (x - m) log2(e) + r.  m is the reference, at the end the largest element, and
+// -inf before the first; with c = m log2(e) rounded and r = m log2(e) - c (exact), y is one fma of x, fma(x, log2(e), -c).  Where |m| is so large
+// that r would count (kNear), r is 0 and y takes the difference first.
+struct Stat {
+    float m, r, s, t;
+    MICA_DEVICE static float rest(float m) { return __builtin_fabsf(m) <= kNear ? __builtin_fmaf(m, kLog2e, -(m * kLog2e)) : 0.0f; }
+    MICA_DEVICE void rebase(float to) { // to >= m
+        const float r2 = rest(to);
+        // (also for m = to = -inf, whose difference is NaN)
+        const float d = __builtin_fmaxf(__builtin_fmaf(m - to, kLog2e, r2 - r), kFar);
+        const float f = __builtin_amdgcn_exp2f(d);
+        t = f * __builtin_fmaf(s, d, t);
+        s *= f;
+        m = to, r = r2;
+    }
+    MICA_DEVICE void add(float y) {
+        const float e = __builtin_amdgcn_exp2f(y);
+        s += e;
+        t = __builtin_fmaf(e, __builtin_fmaxf(y, kFar), t);
+    }
+    MICA_DEVICE float y_of(float x) const { return __builtin_fmaf(x - (m == -__builtin_inff() ? 0.0f : m), kLog2e, r); }
+    // ln S, S = sum e^(x - m): not below 0, and 0 where one element alone has a weight (its own 2^r divided by 2^r)
+    MICA_DEVICE float ln_sum() const {
+        const float q = s / __builtin_amdgcn_exp2f(r);
+        return q < 1.0f ? 0.0f : logf(q);
+    }
+    MICA_DEVICE float logprob(float x) const { return (x - m) - ln_sum(); }
+    MICA_DEVICE float entropy() const { // (t and r s round alike where one element alone has a weight)
+        const float h = ln_sum() - (t - r * s) / s * kLn2;
+        return h < 0.0f ? 0.0f : h;
+    }
+};
+constexpr Stat kNone = {-__builtin_inff(), 0.0f, 0.0f, 0.0f};
 
 // the order number of the n-th largest of 64 lanes' values, bit by bit from the top; lower bits than BITS are 0
 template <int BITS>
@@ -96,73 +122,81 @@ MICA_DEVICE uint32_t nth_of_wave(uint32_t o, int n) {
 MICA_DEVICE int keep_best(unsigned long long *list, int n, int top) {
     unsigned long long mine[kCap / kThreads];
     int rank[kCap / kThreads];
-    int cnt = 0;
-    for (int i = threadIdx.x, j = 0; i < n; i += kThreads, ++j) cnt = j + 1;
 #pragma unroll
-    for (int j = 0; j < kCap / kThreads; ++j)
-        if (j < cnt) {
-            const unsigned long long k = list[threadIdx.x + j * kThreads];
+    for (int j = 0; j < kCap / kThreads; ++j) {
+        const int at = threadIdx.x + j * kThreads;
+        rank[j] = kCap;
+        if (j * kThreads < n && at < n) {
+            const unsigned long long k = list[at];
             int r = 0;
-            for (int i = 0; i < n; ++i) r += list[i] > k;
+            for (int i = 0; i < n; i += 8) // 8 reads at a time; those past n do not count
+#pragma unroll
+                for (int x = 0; x < 8; ++x) r += list[i + x] > k && i + x < n;
             mine[j] = k, rank[j] = r;
         }
+    }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < kCap / kThreads; ++j)
-        if (j < cnt && rank[j] < top) list[rank[j]] = mine[j];
+        if (rank[j] < top) list[rank[j]] = mine[j];
     __syncthreads();
     return n < top ? n : top;
 }
 
-// the results of a row from its whole statistics; every thread of a workgroup calls
+// the logit of a row's given token c; NaN for an id that is no token (no access)
 template <int DT>
-MICA_DEVICE void finish(const LpParams &p, int row, const Stat &a, const unsigned long long *best) {
+MICA_DEVICE float given(const LpParams &p, int row, int c) {
+    const long long at = (long long)row * p.C + c;
+    const long long id = p.tok64 ? ((const long long *)p.tok)[at] : ((const int *)p.tok)[at];
     const void *x = (const char *)p.x + (long long)row * p.ldx * (DT == MICA_FP32 ? 4 : 2);
-    const float ls = logf(a.s);
+    return id >= 0 && id < p.V ? Elem<DT>::load(x, id) : __builtin_nanf("");
+}
+
+// the results of a row from its whole statistics; every thread of a workgroup calls, with its given() logit c = threadIdx.x
+template <int DT>
+MICA_DEVICE void finish(const LpParams &p, int row, const Stat &a, const unsigned long long *best, float tok) {
     for (int c = threadIdx.x; c < p.C; c += kThreads) {
-        const long long at = (long long)row * p.C + c;
-        const long long id = p.tok64 ? ((const long long *)p.tok)[at] : ((const int *)p.tok)[at];
-        // an id that is no token: NaN, and no access
-        p.lp[at] = id >= 0 && id < p.V ? (Elem<DT>::load(x, id) - a.m) - ls : __builtin_nanf("");
+        if (c >= kThreads) tok = given<DT>(p, row, c);
+        p.lp[(long long)row * p.C + c] = a.logprob(tok);
     }
-    if (threadIdx.x == 0) p.ent[row] = ls - a.t / a.s;
+    if (threadIdx.x == 0) p.ent[row] = a.entropy();
     if ((int)threadIdx.x < p.top) {
         const unsigned long long k = best[threadIdx.x];
         const long long at = (long long)row * p.top + threadIdx.x;
         p.ids[at] = (long long)(uint32_t)~(uint32_t)k;
-        p.tlp[at] = (value_of((uint32_t)(k >> 32)) - a.m) - ls;
+        p.tlp[at] = a.logprob(value_of((uint32_t)(k >> 32)));
     }
 }
 
 // one (m, s, t) of the workgroup's 256; every thread gets it
-MICA_DEVICE Stat block_stat(Stat a, float (*red)[4]) {
-    rebase(a, wave_max(a.m));
+MICA_DEVICE Stat block_stat(Stat a, Stat *red) {
+    a.rebase(wave_max(a.m));
     a.s = wave_sum(a.s), a.t = wave_sum(a.t);
     const int wave = threadIdx.x >> 6;
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[wave][0] = a.m, red[wave][1] = a.s, red[wave][2] = a.t;
+    if ((threadIdx.x & 63) == 0) red[wave] = a;
     __syncthreads();
-    float m = red[0][0];
+    float m = red[0].m;
 #pragma unroll
-    for (int w = 1; w < kThreads / 64; ++w) m = __builtin_fmaxf(m, red[w][0]);
-    Stat r = {m, 0.0f, 0.0f};
+    for (int w = 1; w < kThreads / 64; ++w) m = __builtin_fmaxf(m, red[w].m);
+    Stat r = {m, Stat::rest(m), 0.0f, 0.0f};
 #pragma unroll
     for (int w = 0; w < kThreads / 64; ++w) {
-        Stat b = {red[w][0], red[w][1], red[w][2]};
-        rebase(b, m);
+        Stat b = red[w];
+        b.rebase(m);
         r.s += b.s, r.t += b.t;
     }
     return r;
 }
 
 template <int DT, bool TOP>
-__global__ __launch_bounds__(kThreads, 4) void lp_rows_kernel(LpParams p) {
+__global__ __launch_bounds__(kThreads, 6) void lp_rows_kernel(LpParams p) {
     using E = Elem<DT>;
-    constexpr int U = kElems / E::N, kSize = 16 / E::N;
-    __shared__ float red[kThreads / 64][4];
+    constexpr int kSize = 16 / E::N;
+    __shared__ Stat red[kThreads / 64];
     __shared__ float gmax[64];
-    __shared__ unsigned long long list[TOP ? kCap : 1];
-    __shared__ int count, wcount[kThreads / 64];
+    __shared__ unsigned long long list[TOP ? kCap : 8];
+    __shared__ int counts[3], wcount[kThreads / 64];
     const int row = blockIdx.x / p.parts, part = blockIdx.x % p.parts, tid = threadIdx.x;
     const char *x = (const char *)p.x + (long long)row * p.ldx * kSize;
     // the row as up to N - 1 single elements, 16-byte vectors from the first aligned address, up to N - 1 single ones
@@ -171,14 +205,19 @@ __global__ __launch_bounds__(kThreads, 4) void lp_rows_kernel(LpParams p) {
     const char *body = x + head * kSize;
     const int v0 = part * p.bpp * (kThreads * U), v1 = min(v0 + p.bpp * (kThreads * U), nv);
     const bool first_part = part == 0, last_part = part == p.parts - 1;
-    if (TOP && tid == 0) count = 0;
+    if (TOP && tid == 0) counts[0] = 0;
 
     auto load = [&](int v, u32x4 (&w)[U]) {
+        if (v + kThreads * U <= v1) { // a full block
+#pragma unroll
+            for (int u = 0; u < U; ++u) w[u] = __builtin_nontemporal_load((const u32x4 *)(body + (v + u * kThreads + tid) * 16ll));
+            return;
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int at = v + u * kThreads + tid;
             w[u] = u32x4{E::kLow, E::kLow, E::kLow, E::kLow};
-            if (at < v1) w[u] = __builtin_nontemporal_load((const u32x4 *)(body + (long long)at * 16));
+            if (at < v1) w[u] = __builtin_nontemporal_load((const u32x4 *)(body + at * 16ll));
         }
     };
     u32x4 cur[U], nxt[U];
@@ -189,33 +228,48 @@ __global__ __launch_bounds__(kThreads, 4) void lp_rows_kernel(LpParams p) {
     if (first_part && tid < head) one_at = tid;
     if (last_part && tid >= 8 && tid < 8 + tail) one_at = p.V - tail + tid - 8;
     if (one_at >= 0) one = E::load(x, one_at);
+    const float tok = p.parts == 1 && tid < p.C ? given<DT>(p, row, tid) : 0.0f;
 
-    Stat a = {-__builtin_inff(), 0.0f, 0.0f};
+    Stat a = kNone;
+    float largest = -__builtin_inff();
+    bool near = false; // every lane's reference is within kNear
     float thr = -__builtin_inff(); // elements not below it are candidates;
     bool above = false;            // or only those above it
-    int kept = 0;                  // candidates of earlier blocks
+    int kept = 0, turn = 0;        // candidates of earlier blocks; the block's counter
     for (int v = v0; v == v0 || v < v1; v += kThreads * U) {
         const bool first = v == v0;
         if (v + kThreads * U < v1) load(v + kThreads * U, nxt);
-        float mx = first ? one : -__builtin_inff();
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int e = 0; e < E::N; ++e) mx = __builtin_fmaxf(mx, E::get(cur[u], e));
-        if (__builtin_amdgcn_ballot_w64(mx > a.m)) rebase(a, __builtin_fmaxf(a.m, mx));
-        const float ref = a.m == -__builtin_inff() ? 0.0f : a.m;
-        auto add = [&](float xv) {
-            const float y = xv - ref, ex = __builtin_amdgcn_exp2f(y * kLog2e);
-            a.s += ex;
-            a.t = __builtin_fmaf(ex, __builtin_fmaxf(y, kFar), a.t);
+        float vmax[U], mx = first ? one : -__builtin_inff(); // the largest of each vector, of the thread's elements
+        // the reference of the sums follows the maximum when a lane's exceeds it by kRaise (with the maximum itself a wave
+        // would rebase at most of its vectors, half a row's elements later still)
+        auto raise = [&](float m) {
+            if (__builtin_amdgcn_ballot_w64(m > a.m + kRaise)) {
+                a.rebase(__builtin_fmaxf(a.m, m));
+                near = __builtin_amdgcn_ballot_w64(__builtin_fabsf(a.m) > kNear) == 0;
+            }
         };
+        if (first) {
+            raise(one);
+            a.add(a.y_of(one));
+        }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
+            vmax[u] = E::get(cur[u], 0);
 #pragma unroll
-            for (int e = 0; e < E::N; ++e) add(E::get(cur[u], e));
-            __asm__ volatile("" : "+v"(a.s), "+v"(a.t)); // the sums here: left alone they follow all 32 exponentials
+            for (int e = 1; e < E::N; ++e) vmax[u] = __builtin_fmaxf(vmax[u], E::get(cur[u], e));
+            mx = __builtin_fmaxf(mx, vmax[u]);
+            raise(vmax[u]);
+            if (near) {
+                const float c = -(a.m * kLog2e);
+#pragma unroll
+                for (int e = 0; e < E::N; ++e) a.add(__builtin_fmaf(E::get(cur[u], e), kLog2e, c));
+            } else { // (or a thread is without any element of its own yet)
+#pragma unroll 1
+                for (int e = 0; e < E::N; ++e) a.add(a.y_of(E::get(cur[u], e)));
+            }
+            __asm__ volatile("" : "+v"(a.s), "+v"(a.t)); // the sums here: left alone they follow all the exponentials
         }
-        if (first) add(one);
+        largest = __builtin_fmaxf(largest, mx);
         // keeps what the compiler makes of the elements (their unpacked values, their order numbers) from staying in
         // registers from one use to the next
         auto forget = [&] {
@@ -236,101 +290,102 @@ __global__ __launch_bounds__(kThreads, 4) void lp_rows_kernel(LpParams p) {
                 if (thr != thr) thr = -__builtin_inff(); // (the number below -inf's is a NaN's)
             }
             auto reaches = [&](float xv) { return above ? !(xv <= thr) : !(xv < thr); }; // (as a NaN does)
-            // The elements of the block that a thread picks (bit N u + e: element e of its vector u) go to the list.
-            // Their values are read again, by index: taken from registers, each of the 32 would have code of its own.
+            // more candidates than the list holds are only counted
             auto push = [&](float xv, int idx) {
-                const int at = atomicAdd(&count, 1);
+                const int at = kept + atomicAdd(&counts[turn], 1);
                 if (at < kCap) list[at] = key_of(xv, idx);
             };
-            auto push_all = [&](uint32_t bits) {
-                while (bits) {
-                    const int i = __builtin_ctz(bits);
-                    bits &= bits - 1;
-                    const int idx = head + (v + i / E::N * kThreads + tid) * E::N + i % E::N;
-                    push(E::load(x, idx), idx);
-                }
-            };
-            auto pick = [&](auto test) { // test(value, index)
-                uint32_t bits = 0;
+            // Three counters in turn, so that one barrier a block is enough: the next block's is cleared here, before the
+            // barrier, two blocks after its last reads.
+            const int next = turn == 2 ? 0 : turn + 1;
+            if (tid == 0) counts[next] = 0;
+            // (the maxima pass over NaNs: a thread that has seen one looks at all its elements from then on)
+            const bool odd = a.s != a.s;
+            if (__builtin_amdgcn_ballot_w64(reaches(mx) || odd)) {
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     const int at = v + u * kThreads + tid;
-                    uint32_t mine = 0;
+                    if ((reaches(vmax[u]) || odd) && at < v1)
 #pragma unroll
-                    for (int e = 0; e < E::N; ++e) mine |= test(E::get(cur[u], e), head + at * E::N + e) ? 1u << e : 0u;
-                    bits |= at < v1 ? mine << (u * E::N) : 0u;
-                    __builtin_amdgcn_sched_barrier(0);
+                        for (int e = 0; e < E::N; ++e) {
+                            const float xv = E::get(cur[u], e);
+                            if (reaches(xv)) push(xv, head + at * E::N + e);
+                        }
                 }
-                return bits;
-            };
-            // (the maximum passes over NaNs: a thread that has seen one looks at all its elements from then on)
-            if (reaches(mx) || a.s != a.s) {
-                push_all(pick([&](float xv, int) { return reaches(xv); }));
                 if (first && one_at >= 0 && reaches(one)) push(one, one_at);
             }
             __syncthreads();
-            int n = count;
-            __syncthreads(); // nobody adds the next block's before everybody has read it
+            int n = kept + counts[turn];
             const bool exact = n > kCap;
             if (exact) { // too many reach the threshold: this block's best, exactly
-                // the value of the top-th best element, then the index up to which elements of that value belong
-                auto belongs = [](float xv, int idx, uint32_t o, uint32_t last) { // above order o, or at it by `last`
+                // the value of the top-th best element, then the index up to which elements of that value belong; the
+                // block is read again for every bit (a loop of few registers beside the ordinary path's)
+                auto each = [&](auto f) {
+#pragma unroll 1
+                    for (int u = 0; u < U; ++u) {
+                        const int at = v + u * kThreads + tid;
+                        if (at >= v1) break;
+                        const u32x4 w = *(const u32x4 *)(body + (long long)at * 16);
+#pragma unroll
+                        for (int e = 0; e < E::N; ++e) f(E::get(w, e), head + at * E::N + e);
+                    }
+                    if (first && one_at >= 0) f(one, one_at);
+                };
+                uint32_t o = 0, last = 0xffffffffu;
+                auto belongs = [&](float xv, int idx) { // above order o, or at it with an index up to `last`
                     const uint32_t q = order_of(xv);
                     return q > o || (q == o && (uint32_t)idx <= last);
                 };
-                auto tally = [&](uint32_t o, uint32_t last) {
-                    forget();
-                    int c = __popc(pick([&](float xv, int idx) { return belongs(xv, idx, o, last); }));
-                    if (first && one_at >= 0) c += belongs(one, one_at, o, last);
+                auto tally = [&] {
+                    int c = 0;
+                    each([&](float xv, int idx) { c += belongs(xv, idx); });
                     const float w = wave_sum((float)c); // (whole numbers below 2^24)
                     __syncthreads();
                     if ((tid & 63) == 0) wcount[tid >> 6] = (int)w;
                     __syncthreads();
                     return wcount[0] + wcount[1] + wcount[2] + wcount[3];
                 };
-                uint32_t o = 0;
 #pragma unroll 1
                 for (int b = 31; b >= 0; --b) {
-                    const uint32_t c = o | (1u << b);
-                    if (tally(c, 0xffffffffu) >= p.top) o = c;
+                    o |= 1u << b;
+                    if (tally() < p.top) o &= ~(1u << b);
                 }
-                uint32_t last = 0x7fffffffu; // the least index that still gives `top` elements
+                last = 0xffffffffu >> __builtin_clz(p.V); // the least index that still gives `top` elements
 #pragma unroll 1
-                for (int b = 30; b >= 0; --b) {
-                    const uint32_t c = last & ~(1u << b);
-                    if (tally(o, c) >= p.top) last = c;
+                for (int b = 31 - __builtin_clz(p.V); b >= 0; --b) {
+                    last &= ~(1u << b);
+                    if (tally() < p.top) last |= 1u << b;
                 }
-                if (tid == 0) count = kept;
+                if (tid == 0) counts[turn] = 0; // (its reads lie before the tallies' barriers)
                 __syncthreads();
-                forget();
-                push_all(pick([&](float xv, int idx) { return belongs(xv, idx, o, last); }));
-                if (first && one_at >= 0 && belongs(one, one_at, o, last)) push(one, one_at);
-                __syncthreads();
-                n = count;
+                each([&](float xv, int idx) {
+                    if (belongs(xv, idx)) list[kept + atomicAdd(&counts[turn], 1)] = key_of(xv, idx);
+                });
+                n = kept + p.top;
                 __syncthreads();
             }
-            kept = n;
-            if (exact || n > p.top + 16) { // keep the best and raise the threshold
+            turn = next;
+            kept = n; // (at most kCap: a block adds what the list holds, and is followed by a shorter list or is the last)
+            if ((exact || n > p.top + 16) && v + kThreads * U < v1) { // keep the best and raise the threshold
                 kept = keep_best(list, n, p.top);
                 const unsigned long long least = list[p.top - 1];
                 thr = value_of((uint32_t)(least >> 32));
                 if (thr != thr) thr = __builtin_inff();
                 // indices grow from block to block, but for the single elements of the row's end
                 above = (int)~(uint32_t)least < p.V - tail;
-                if (tid == 0) count = kept;
-                __syncthreads();
             }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) cur[u] = nxt[u];
     }
+    a.rebase(largest);
     const Stat all = block_stat(a, red);
     if constexpr (TOP) kept = keep_best(list, kept, p.top);
     if (p.parts == 1) {
-        finish<DT>(p, row, all, list);
+        finish<DT>(p, row, all, list, tok);
         return;
     }
-    if (tid == 0) p.pm[blockIdx.x] = float4{all.m, all.s, all.t, 0.0f};
+    if (tid == 0) p.pm[blockIdx.x] = all;
     if (TOP && tid < p.top) p.pk[(long long)blockIdx.x * p.top + tid] = tid < kept ? list[tid] : 0ull;
 }
 
@@ -339,10 +394,10 @@ __global__ __launch_bounds__(kThreads) void lp_merge_kernel(LpParams p) {
     __shared__ unsigned long long list[kCap], all[kMaxParts * kMaxTop];
     __shared__ int count;
     const int row = blockIdx.x, tid = threadIdx.x;
-    const float4 *pm = p.pm + (long long)row * p.parts;
-    const float4 mine = (tid & 63) < p.parts ? pm[tid & 63] : float4{-__builtin_inff(), 0.0f, 0.0f, 0.0f};
-    Stat a = {mine.x, mine.y, mine.z};
-    rebase(a, wave_max(a.m));
+    Stat a = kNone;
+    if ((tid & 63) < p.parts) a = p.pm[(long long)row * p.parts + (tid & 63)];
+    const float tok = tid < p.C ? given<DT>(p, row, tid) : 0.0f;
+    a.rebase(wave_max(a.m));
     a.s = wave_sum(a.s), a.t = wave_sum(a.t);
     if (p.top > 0) {
         const int n = p.parts * p.top;
@@ -350,10 +405,19 @@ __global__ __launch_bounds__(kThreads) void lp_merge_kernel(LpParams p) {
         for (int i = tid; i < n; i += kThreads) all[i] = pk[i];
         if (tid == 0) count = 0;
         __syncthreads();
-        // every part's r-th best, r = top / parts rounded up: together top keys at least reach the least of them
-        const int r = (p.top + p.parts - 1) / p.parts;
-        unsigned long long least = ~0ull;
-        for (int c = 0; c < p.parts; ++c) least = min(least, all[c * p.top + r - 1]);
+        // with r = top / parts rounded up, the (top / r rounded up)-th largest of the parts' r-th best: at least top keys
+        // reach it
+        const int r = (p.top + p.parts - 1) / p.parts, want = (p.top + r - 1) / r;
+        const unsigned long long own = (tid & 63) < p.parts ? all[(tid & 63) * p.top + r - 1] : 0;
+        int rank = 0;
+        for (int c = 0; c < p.parts; ++c) rank += all[c * p.top + r - 1] > own;
+        const unsigned long long at = __builtin_amdgcn_ballot_w64(rank == want - 1);
+        unsigned long long least = 0; // (parts without that many keys)
+        if (at) {
+            const int l = __builtin_ctzll(at);
+            least = (unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(own >> 32), l) << 32 |
+                    (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)own, l);
+        }
         for (int i = tid; i < n; i += kThreads)
             if (all[i] >= least && all[i] != 0) {
                 const int at = atomicAdd(&count, 1);
@@ -372,13 +436,13 @@ __global__ __launch_bounds__(kThreads) void lp_merge_kernel(LpParams p) {
             __syncthreads();
         }
     }
-    finish<DT>(p, row, a, list);
+    finish<DT>(p, row, a, list, tok);
 }
 
-// Workgroups a row, and blocks each: enough for the chip (256 CUs), whole blocks each.
+// Workgroups a row, and blocks each: enough for the chip (256 CUs of six workgroups), whole blocks each.
 void divide(int T, int V, int elems, int &parts, int &bpp) {
-    const int blocks = max(1, (V / elems + kThreads * (kElems / elems) - 1) / (kThreads * (kElems / elems)));
-    const int want = T >= 1024 ? 1 : min((1024 + T - 1) / T, kMaxParts);
+    const int blocks = max(1, (V / elems + kThreads * U - 1) / (kThreads * U));
+    const int want = T >= 1024 ? 1 : min((2048 + T - 1) / T, kMaxParts);
     bpp = (blocks + want - 1) / want;
     parts = (blocks + bpp - 1) / bpp;
 }
@@ -423,7 +487,7 @@ extern "C" int mica_token_logprobs(const void *logits, int dtype, long long ldx,
     const long long need = part_bytes(T, p.parts, top);
     if (need && (!workspace || !mica_aligned16(workspace) || workspace_bytes < need)) return MICA_MISS_ARG;
     if (V > (1 << 30) || (long long)T * p.parts >= (1LL << 31)) return MICA_MISS_RANGE;
-    p.pm = (float4 *)workspace;
+    p.pm = (Stat *)workspace;
     p.pk = (unsigned long long *)((char *)workspace + (long long)T * p.parts * 16);
     if (dtype == MICA_BF16) launch<MICA_BF16>(p, (hipStream_t)stream);
     else if (dtype == MICA_FP16) launch<MICA_FP16>(p, (hipStream_t)stream);
