@@ -49,7 +49,7 @@ struct CaParams {
     int window, sinks;
     float scale_log2;                               // softmax scale x log2(e)
     int nqb, gq, chunk, nchunk;                     // query blocks, in groups of gq; tiles a workgroup, chunks a sequence
-    int runs, least;                                // STREAM: runs of tiles, the fewest tiles of one
+    int runs, dense, least;                         // STREAM: see Plan
     float *part_o;                                  // partial O, a wave's accumulators 64 lanes x 16 bytes at a time
     float2 *part_ml;                                // partial (m, l) of each row
 };
@@ -89,8 +89,9 @@ struct Tiles {
 template <bool TREE>
 struct Stream {
     int total, per; // tiles of a head, tiles of a run
-    int x, sum;     // this lane's sequence of the first 64: its tiles, those up to and with it
-    MICA_DEVICE static int of(const CaParams &p, int b) { return Tiles<TREE>(p, key_count(p, b), 0, p.Sq).n; }
+    int x, sum;     // this lane's sequence of 64 (the first 64 at the end): its tiles, those up to and with it
+    int count;      // and its keys
+    MICA_DEVICE static int of(const CaParams &p, int keys) { return Tiles<TREE>(p, keys, 0, p.Sq).n; }
     // a wave's running sums
     MICA_DEVICE static int scan(int x) {
 #pragma unroll
@@ -102,12 +103,14 @@ struct Stream {
     }
     MICA_DEVICE void take(const CaParams &p, int base) {
         const int b = base + (int)(threadIdx.x & 63);
-        x = b < p.B ? of(p, b) : 0;
+        count = b < p.B ? key_count(p, b) : 0;
+        x = b < p.B ? of(p, count) : 0;
         sum = scan(x);
     }
     MICA_DEVICE Stream(const CaParams &p) {
         if (p.len == nullptr) {
-            x = of(p, 0);
+            count = p.cap;
+            x = of(p, count);
             total = p.B * x;
         } else {
             total = 0;
@@ -116,12 +119,15 @@ struct Stream {
                 total += __builtin_amdgcn_readlane(sum, 63);
             }
         }
-        per = max(p.least, (total + p.runs - 1) / p.runs);
+        per = (total + p.runs - 1) / p.runs;
+        const int half = max(p.runs / 2, 1);
+        if (per < p.dense) per = (total + half - 1) / half;
+        per = max(per, (long long)total * p.HK <= kCus ? p.least : 4);
     }
-    // the sequence and its tile at `at` (below total)
-    MICA_DEVICE void find(const CaParams &p, int at, int &b, int &tile) {
+    // the sequence, its keys and its tile at `at` (below total)
+    MICA_DEVICE void find(const CaParams &p, int at, int &b, int &keys, int &tile) {
         if (p.len == nullptr) {
-            b = at / x, tile = at % x;
+            b = at / x, tile = at % x, keys = count;
             return;
         }
         for (int base = 0, before = 0;; base += 64) {
@@ -129,7 +135,8 @@ struct Stream {
             const unsigned long long past = __builtin_amdgcn_ballot_w64(before + sum > at);
             if (past) {
                 const int l = __builtin_ctzll(past);
-                b = base + l, tile = at - before - __builtin_amdgcn_readlane(sum - x, l);
+                b = base + l, keys = __builtin_amdgcn_readlane(count, l);
+                tile = at - before - __builtin_amdgcn_readlane(sum - x, l);
                 return;
             }
             before += __builtin_amdgcn_readlane(sum, 63);
@@ -161,7 +168,7 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
     constexpr int NB = 8 * R;                 // query positions of the workgroup
     constexpr int NDT = kD / 32 / D;          // 32-dim tiles of O a wave holds
     constexpr int kBlk = 16 / kWaves;         // 1 KB DMA blocks of K, and of V, a wave issues for a tile
-    constexpr int kPf = D > 1 ? 8 : 2;        // operand fragments read ahead (D = 1: all registers are taken)
+    constexpr int kPf = D > 1 ? 8 : 4;        // operand fragments read ahead (D = 1: more would spill)
     constexpr int kWords = TREE ? NB * (STREAM ? 2 : kMaxNodes / 32) : 1; // (STREAM: up to 64 nodes)
     static_assert(R * 32 * kD * 2 <= ST * kStage, "the output is staged where the tiles were");
     __shared__ __attribute__((aligned(1024))) int8_t smem[ST * kStage];
@@ -170,15 +177,16 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void *)smem;
     const int rb = wave / D, dt0 = (wave % D) * NDT;
-    int b, hk, qb = 0, i0, left = 0; // the sequence, head and query block, its first tile here, tiles left (STREAM)
+    int b, hk, qb = 0, i0, keys, left = 0; // the sequence, head, query block, first tile here, keys; tiles left (STREAM)
     int blk;                         // where its partial state goes
     if constexpr (STREAM) {
         Stream<TREE> all(p);
         hk = blockIdx.x % p.HK;
         const int at = blockIdx.x / p.HK * all.per;
         if (at >= all.total) return;
-        all.find(p, at, b, i0);
+        all.find(p, at, b, keys, i0);
         b = __builtin_amdgcn_readfirstlane(b), i0 = __builtin_amdgcn_readfirstlane(i0);
+        keys = __builtin_amdgcn_readfirstlane(keys);
         left = __builtin_amdgcn_readfirstlane(min(all.per, all.total - at));
         blk = 2 * blockIdx.x;
     } else {
@@ -190,6 +198,7 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
         if (unit >= p.B * p.nchunk * p.HK || qb >= p.nqb) return;
         hk = unit % p.HK, b = unit / p.HK / p.nchunk, i0 = unit / p.HK % p.nchunk * p.chunk;
         blk = unit * p.nqb + qb;
+        keys = key_count(p, b);
     }
     for (;;) {
     // what depends on the lane alone is made here, from an opaque copy of its id: the compiler would make it before the
@@ -197,7 +206,7 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
     int tid = threadIdx.x;
     __asm__ volatile("" : "+v"(tid));
     const int lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
-    const int q0 = qb * NB, keys = key_count(p, b);
+    const int q0 = qb * NB;
     const Tiles<TREE> tl(p, keys, q0, min(NB, p.Sq - q0));
     const int i1 = min(STREAM ? i0 + left : i0 + p.chunk, tl.n);
     if (!STREAM && i0 >= tl.n) return;
@@ -205,28 +214,6 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
 
     // this lane's row: a position and a query head
     const int row = rb * 32 + l32, head = hk * kGroup + row / NB, t = q0 + row % NB;
-    // the block's words and this lane's Q fragments (B operand of S^T: dims 16 s + 8 hi .. + 7 of the row) are on their
-    // way before the first tiles
-    constexpr int kMine = (kWords + kThreads - 1) / kThreads;
-    uint32_t mine[kMine];
-    if constexpr (TREE) {
-#pragma unroll
-        for (int x = 0; x < kMine; ++x) {
-            const int i = tid + x * kThreads, node = q0 + i / p.tw;
-            mine[x] = i < NB * p.tw && node < p.Sq ? p.tree[b * p.sbt + (long long)node * p.tw + i % p.tw] : 0u;
-        }
-    }
-    bf16x8 qf[kD / 16];
-    {
-        const uint16_t *qr = p.q + b * p.sbq + head * p.shq + (long long)t * p.ldq + hi * 8;
-#pragma unroll
-        for (int s = 0; s < kD / 16; ++s) {
-            u32x4 x = {0u, 0u, 0u, 0u};
-            if (t < p.Sq) x = *(const u32x4 *)(qr + s * 16);
-            qf[s] = __builtin_bit_cast(bf16x8, x);
-        }
-    }
-
     // DMA of tile i into stage st; past i1 from a zero-sized buffer, so that every step issues as many instructions
     auto issue = [&](int i, int st) {
         const uint16_t *kb, *vb;
@@ -268,6 +255,25 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
     };
 #pragma unroll
     for (int s = 0; s < ST - 1; ++s) issue(i0 + s, s);
+
+    // this lane's Q fragments (B operand of S^T: dims 16 s + 8 hi .. + 7 of the row) and the block's words, all in flight
+    // with the first tiles
+    constexpr int kMine = (kWords + kThreads - 1) / kThreads;
+    uint32_t mine[kMine];
+    if constexpr (TREE) {
+#pragma unroll
+        for (int x = 0; x < kMine; ++x) {
+            const int i = tid + x * kThreads, node = q0 + i / p.tw;
+            mine[x] = i < NB * p.tw && node < p.Sq ? p.tree[b * p.sbt + (long long)node * p.tw + i % p.tw] : 0u;
+        }
+    }
+    bf16x8 qf[kD / 16];
+    {
+        // (rows past the last position repeat it: they are not stored)
+        const uint16_t *qr = p.q + b * p.sbq + head * p.shq + (long long)min(t, p.Sq - 1) * p.ldq + hi * 8;
+#pragma unroll
+        for (int s = 0; s < kD / 16; ++s) qf[s] = __builtin_bit_cast(bf16x8, *(const u32x4 *)(qr + s * 16));
+    }
 
     bool absent = false; // a tree node without a bit
     if constexpr (TREE) {
@@ -323,6 +329,7 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
         const uint32_t ks = kbase + st * kStage, vs = vbase + st * kStage;
         // ---- S^T = K Q^T: rows = keys of the tile, column = this lane's row; fragments read kPf steps ahead ----
         f32x16 sc = {};
+        __builtin_amdgcn_s_setprio(1);
         bf16x8 kf[kPf];
 #pragma unroll
         for (int s = 0; s < kPf; ++s) kf[s] = kfrag(ks, s);
@@ -333,6 +340,7 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
             __builtin_amdgcn_sched_barrier(0);
             sc = mfma_bf16(a, qf[s], sc);
         }
+        __builtin_amdgcn_s_setprio(0);
         // ---- keys that a row does not see: score -inf, weight 0 (score r of a lane is key 8 (r / 4) + 4 hi + r % 4) ----
         bool masked = false, own = false;
         if constexpr (TREE) {
@@ -430,6 +438,7 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
         }
         // ---- O^T += V^T P^T ----
         constexpr int kPv = kPf < 2 * NDT ? kPf : 2 * NDT;
+        __builtin_amdgcn_s_setprio(1);
         bf16x8 vf[kPv];
 #pragma unroll
         for (int x = 0; x < kPv; ++x) vf[x] = vfrag(vs, x / NDT, x % NDT);
@@ -440,6 +449,7 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
             __builtin_amdgcn_sched_barrier(0);
             O[x % NDT] = mfma_bf16(a, pb[x / NDT], O[x % NDT]);
         }
+        __builtin_amdgcn_s_setprio(0);
     }
     wait_vmcnt<0>();  // the ring's last (empty) loads have written before the stages are used again or given up
     float ltot = half_swap_sum(lsum);
@@ -485,6 +495,7 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
     if (left == 0) return;
     i0 = 0, blk = 2 * blockIdx.x + 1; // (what lies between a workgroup's first and last is whole)
     ++b;
+    keys = key_count(p, b);
     __syncthreads(); // everybody is done with the stages and the words
     }
 }
@@ -572,7 +583,8 @@ __global__ __launch_bounds__(256) void ca_merge_kernel(CaParams p) {
 
 // How a call is divided: row blocks (R) and dim parts (D) of a workgroup, LDS stages, and the work.
 struct Plan {
-    int R, D, ST, nqb, gq, chunk, nchunk, runs, least;
+    int R, D, ST, nqb, gq, chunk, nchunk;
+    int runs, dense, least; // STREAM: most runs of tiles; the tiles of a run below which half as many are made; its fewest
     bool stream, wide;
     long long tiles, wgs, states; // STREAM: a head's tiles; workgroups; partial rows
 };
@@ -589,14 +601,20 @@ Plan plan(int B, int Sq, int HK, int max_tiles) {
     const int slots = kCus * (pl.R < 8 ? 2 : 1);
     const long long units = (long long)B * HK;
     if (pl.stream) {
-        pl.least = 2 * pl.R;
+        // Two workgroups a CU, while each gets enough tiles to repay the partial state that it writes (32 R KB) and the merge
+        // reads; else one, of 4 tiles at least, and of fewer only where even so the chip would be nearly empty.  Measured,
+        // us, two / one a CU (nodes, sequences x keys): 8, 16 x 4000 57 / 67, 1 x 32768 41 / 47, 16 x 1000 29 / 28;
+        // 32, 16 x 4000 76 / 81, 8 x 3000 49 / 45, 16 x 1000 42 / 39; tiles a workgroup 2 / 4 / 8: 8, 1 x 500 14 / 16 / 19,
+        // 2 x 2500 23 / 21 / 25; 64, 1 x 500 26 / 23 / 27.
+        pl.dense = pl.R == 8 ? 0 : pl.R == 4 ? 8 : 4;
+        pl.least = pl.R == 8 ? 4 : 2;
         pl.tiles = (long long)B * max_tiles;
         const long long most = (pl.tiles + pl.least - 1) / pl.least;
         pl.runs = HK < slots ? slots / HK : 1;
-        if (most < pl.runs) pl.runs = (int)most;
-        pl.wgs = (long long)pl.runs * HK;
+        pl.wgs = (most < pl.runs ? most : pl.runs) * HK;
         pl.states = pl.wgs * 2 * 32 * pl.R;
-        pl.wide = 6 * B <= pl.runs;
+        // (few waves, then, of many parts each; 8 nodes, 2 x 10000 keys 37 -> 30 us, 16 x 4000 57, but 63 if waves share there)
+        pl.wide = units * pl.R <= 16;
         return pl;
     }
     // the chunks that take the least time: rounds of workgroups, each as long as its tiles, and with several chunks a
@@ -639,7 +657,7 @@ int launch_as(const CaParams &p, const Plan &pl, hipStream_t st) {
 
 template <bool TREE>
 int launch(CaParams &p, const Plan &pl, void *workspace, hipStream_t st) {
-    p.nqb = pl.nqb, p.gq = pl.gq, p.chunk = pl.chunk, p.nchunk = pl.nchunk, p.runs = pl.runs, p.least = pl.least;
+    p.nqb = pl.nqb, p.gq = pl.gq, p.chunk = pl.chunk, p.nchunk = pl.nchunk, p.runs = pl.runs, p.dense = pl.dense, p.least = pl.least;
     p.part_o = (float *)workspace;
     p.part_ml = (float2 *)((char *)workspace + pl.states * kD * 4);
     if (pl.wgs >= (1LL << 31) || pl.tiles >= (1LL << 30)) return MICA_MISS_RANGE;

@@ -92,7 +92,7 @@ def random_parents(N, seed, absent=False):
 @pytest.mark.parametrize("B,N,HK,C,lens", [
     (1, 1, 4, 0, None), (1, 1, 4, 1, None), (1, 8, 4, 500, None), (2, 9, 4, 33, [33, 0]), (3, 16, 4, 64, [64, 1, 31]),
     (1, 17, 4, 1000, None), (2, 32, 4, 96, [95, 32]), (2, 33, 1, 130, [130, 7]), (1, 64, 4, 2050, None),
-    (2, 65, 2, 40, [0, 40]), (1, 255, 4, 300, None), (1, 512, 1, 70, None), (5, 3, 4, 4000, [4000, 17, 0, 1999, 3968])])
+    (2, 65, 2, 40, [0, 40]), (1, 2, 600, 70, None), (70, 2, 1, 90, [90 - i for i in range(70)]), (1, 255, 4, 300, None), (1, 512, 1, 70, None), (5, 3, 4, 4000, [4000, 17, 0, 1999, 3968])])
 def test_tree_against_float64(gpu, B, N, HK, C, lens):
     q, k, v, kc, vc = heads(gpu, N, B, N, HK, C)
     par = [random_parents(N, 7 * b + N, absent=b % 2 == 1) for b in range(B)]
