@@ -192,10 +192,11 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
     } else {
         // Consecutive workgroups go to the 8 XCDs in turn; the gq query blocks of a group, which read the same keys, stay
         // on one XCD, one after the other.
-        const int id = blockIdx.x, ngq = (p.nqb + p.gq - 1) / p.gq;
-        const int grp = id / (8 * p.gq) * 8 + id % 8, unit = grp / ngq;
-        qb = grp % ngq * p.gq + id / 8 % p.gq;
-        if (unit >= p.B * p.nchunk * p.HK || qb >= p.nqb) return;
+        // The last positions, whose windows are the fullest, come first.
+        const int id = blockIdx.x, units = p.B * p.nchunk * p.HK;
+        const int grp = id / (8 * p.gq) * 8 + id % 8, unit = grp % units;
+        qb = p.nqb - 1 - (grp / units * p.gq + id / 8 % p.gq);
+        if (qb < 0) return;
         hk = unit % p.HK, b = unit / p.HK / p.nchunk, i0 = unit / p.HK % p.nchunk * p.chunk;
         blk = unit * p.nqb + qb;
         keys = key_count(p, b);
