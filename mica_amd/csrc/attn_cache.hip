@@ -168,7 +168,11 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
     constexpr int NB = 8 * R;                 // query positions of the workgroup
     constexpr int NDT = kD / 32 / D;          // 32-dim tiles of O a wave holds
     constexpr int kBlk = 16 / kWaves;         // 1 KB DMA blocks of K, and of V, a wave issues for a tile
-    constexpr int kPf = D > 1 ? 8 : 4;        // operand fragments read ahead (D = 1: more would spill)
+    constexpr int kPf = D > 1 ? 8 : 3;        // operand fragments read ahead (D = 1: more would spill)
+    // The next tile's DMA is issued behind the chain of S^T, whose result is waited for anyway (cached keys: 32 x 16 nodes
+    // 106.6 -> 102.1 us, 64 nodes after 32768 75.4 -> 72.0), but before it where the keys are mostly in L2 and the matrix
+    // cores bound (16384 tokens with a window of 2048: 498.7 against 518.1).
+    constexpr bool kLate = STREAM || TREE;
     constexpr int kWords = TREE ? NB * (STREAM ? 2 : kMaxNodes / 32) : 1; // (STREAM: up to 64 nodes)
     static_assert(R * 32 * kD * 2 <= ST * kStage, "the output is staged where the tiles were");
     __shared__ __attribute__((aligned(1024))) int8_t smem[ST * kStage];
@@ -254,11 +258,8 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
                                                      rv0 + 2 * x * v2 + (((ln & 31) ^ (((r0 + 2 * x) & 7) << 1)) << 4), 0,
                                                      0, 0);
     };
-#pragma unroll
-    for (int s = 0; s < ST - 1; ++s) issue(i0 + s, s);
-
-    // this lane's Q fragments (B operand of S^T: dims 16 s + 8 hi .. + 7 of the row) and the block's words, all in flight
-    // with the first tiles
+    // The block's words and this lane's Q fragments (B operand of S^T: dims 16 s + 8 hi .. + 7 of the row) come before the
+    // tiles: loads end in order, and behind the DMA the first step waited for all the stages' tiles.
     constexpr int kMine = (kWords + kThreads - 1) / kThreads;
     uint32_t mine[kMine];
     if constexpr (TREE) {
@@ -275,19 +276,16 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
 #pragma unroll
         for (int s = 0; s < kD / 16; ++s) qf[s] = __builtin_bit_cast(bf16x8, *(const u32x4 *)(qr + s * 16));
     }
-
-    bool absent = false; // a tree node without a bit
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int s = 0; s < ST - 1; ++s) issue(i0 + s, s);
     if constexpr (TREE) {
 #pragma unroll
         for (int x = 0; x < kMine; ++x) {
             const int i = tid + x * kThreads, left = p.Sq - 32 * (i % p.tw); // bits past the last node do not count
             if (i < NB * p.tw) words[i] = left >= 32 ? mine[x] : left <= 0 ? 0u : mine[x] & ((1u << left) - 1u);
         }
-        __syncthreads();
-        uint32_t any = 0;
-#pragma unroll 1
-        for (int w = 0; w < p.tw; ++w) any |= words[row % NB * p.tw + w];
-        absent = any == 0;
+        wait_lgkmcnt0(); // seen by every wave after the first tile's barrier
     }
     f32x16 O[NDT];
 #pragma unroll
@@ -325,7 +323,7 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
         wait_vmcnt<(ST - 2) * 2 * kBlk>();
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
-        issue(i + ST - 1, (st + ST - 1) % ST);
+        if (!kLate) issue(i + ST - 1, (st + ST - 1) % ST);
         const int8_t *stage = smem + st * kStage;
         const uint32_t ks = kbase + st * kStage, vs = vbase + st * kStage;
         // ---- S^T = K Q^T: rows = keys of the tile, column = this lane's row; fragments read kPf steps ahead ----
@@ -342,6 +340,7 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
             sc = mfma_bf16(a, qf[s], sc);
         }
         __builtin_amdgcn_s_setprio(0);
+        if (kLate) issue(i + ST - 1, (st + ST - 1) % ST);
         // ---- keys that a row does not see: score -inf, weight 0 (score r of a lane is key 8 (r / 4) + 4 hi + r % 4) ----
         bool masked = false, own = false;
         if constexpr (TREE) {
@@ -454,7 +453,13 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
     }
     wait_vmcnt<0>();  // the ring's last (empty) loads have written before the stages are used again or given up
     float ltot = half_swap_sum(lsum);
-    if (absent) { // (its cached keys were computed like the others': nothing of them leaves)
+    uint32_t any = 1;
+    if constexpr (TREE) {
+        any = 0;
+#pragma unroll 1
+        for (int w = 0; w < p.tw; ++w) any |= words[row % NB * p.tw + w];
+    }
+    if (any == 0) { // a tree node without a bit (its cached keys were computed like the others': nothing of them leaves)
         m = -__builtin_inff(), ltot = 0.0f;
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) O[dt] = f32x16{};

@@ -18,6 +18,9 @@ MICA_DEVICE void wait_vmcnt() {
     __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
 }
 
+// This wave's LDS accesses have ended.
+MICA_DEVICE void wait_lgkmcnt0() { __builtin_amdgcn_s_waitcnt(0xf | (3 << 14) | (7 << 4)); }
+
 // Combine a value with the one held by lane l ^ 32 (v_permlane32_swap: no LDS round trip).  With the
 // same register as both operands, the swap leaves (own, other) in lanes 0-31 and (other, own) in lanes
 // 32-63, so max and sum come out bit-identical in every lane.
