@@ -20,7 +20,8 @@
 //
 // Up to 64 query positions, one row block takes them all, and the key tiles of all sequences, one after the other, are
 // divided evenly over the chip's workgroups (STREAM): a workgroup may end one sequence and begin the next, so
-// key counts that differ, or sequences that do not divide the chip, leave no CU idle.  More positions take a workgroup
+// key counts that differ, or sequences that do not divide the chip, leave no CU idle.  In that row each sequence has a few
+// empty tiles before its own, for the time its beginning takes.  More positions take a workgroup
 // for each block, their tiles divided into chunks where that leaves too few.  ca_merge_kernel joins the partial softmax
 // states (fp32) of what was divided.
 #include "attn_common.h"
@@ -49,7 +50,7 @@ struct CaParams {
     int window, sinks;
     float scale_log2;                               // softmax scale x log2(e)
     int nqb, gq, chunk, nchunk;                     // query blocks, in groups of gq; tiles a workgroup, chunks a sequence
-    int runs, dense, least;                         // STREAM: see Plan
+    int runs, dense, least, begin;                  // STREAM: see Plan
     float *part_o;                                  // partial O, a wave's accumulators 64 lanes x 16 bytes at a time
     float2 *part_ml;                                // partial (m, l) of each row
 };
@@ -84,14 +85,14 @@ struct Tiles {
 
 // How STREAM divides the tiles: those of all sequences, one after the other, into runs, and a workgroup for each run and
 // head.  Workgroups next to each other take the heads of one run: their rows lie side by side in memory (with the heads
-// one after the other instead, 64 single tokens with a window of 4096 took 208 us and not CHECK).  All lanes of a wave call and get
-// the same; a lane reads every 64th sequence's count.
+// one after the other instead, 64 single tokens with a window of 4096 took 208 us and not 193).  All lanes of a wave call
+// and get the same; a lane reads every 64th sequence's count.
 template <bool TREE>
 struct Stream {
-    int total, per; // tiles of a head, tiles of a run
+    int total, per; // tiles of a head, tiles of a run, p.begin for each sequence's beginning among them
     int x, sum;     // this lane's sequence of 64 (the first 64 at the end): its tiles, those up to and with it
     int count;      // and its keys
-    MICA_DEVICE static int of(const CaParams &p, int keys) { return Tiles<TREE>(p, keys, 0, p.Sq).n; }
+    MICA_DEVICE static int of(const CaParams &p, int keys) { return Tiles<TREE>(p, keys, 0, p.Sq).n + p.begin; }
     // a wave's running sums
     MICA_DEVICE static int scan(int x) {
 #pragma unroll
@@ -192,6 +193,9 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
         b = __builtin_amdgcn_readfirstlane(b), i0 = __builtin_amdgcn_readfirstlane(i0);
         keys = __builtin_amdgcn_readfirstlane(keys);
         left = __builtin_amdgcn_readfirstlane(min(all.per, all.total - at));
+        const int unused = max(p.begin - i0, 0); // of the sequence's beginning
+        left -= unused, i0 += unused - p.begin;
+        if (left <= 0) return;
         blk = 2 * blockIdx.x;
     } else {
         // Consecutive workgroups go to the 8 XCDs in turn; the gq query blocks of a group, which read the same keys, stay
@@ -497,8 +501,8 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
         }
     }
     if (!STREAM) return;
-    left -= i1 - i0;
-    if (left == 0) return;
+    left -= i1 - i0 + p.begin;
+    if (left <= 0) return;
     i0 = 0, blk = 2 * blockIdx.x + 1; // (what lies between a workgroup's first and last is whole)
     ++b;
     keys = key_count(p, b);
@@ -523,8 +527,8 @@ __global__ __launch_bounds__(256) void ca_merge_kernel(CaParams p) {
     if constexpr (STREAM) {
         Stream<TREE> all(p);
         per = all.per, s = all.first(p, b);
-        g0 = s / per;
-        n = (s + tiles - 1) / per - g0 + 1;
+        g0 = (s + p.begin) / per;
+        n = (s + p.begin + tiles - 1) / per - g0 + 1;
         if (n == 1) return; // its workgroup wrote it
     } else {
         n = (tiles + p.chunk - 1) / p.chunk;
@@ -591,6 +595,7 @@ __global__ __launch_bounds__(256) void ca_merge_kernel(CaParams p) {
 struct Plan {
     int R, D, ST, nqb, gq, chunk, nchunk;
     int runs, dense, least; // STREAM: most runs of tiles; the tiles of a run below which half as many are made; its fewest
+    int begin;              // the tiles that a sequence's beginning counts for
     bool stream, wide;
     long long tiles, wgs, states; // STREAM: a head's tiles; workgroups; partial rows
 };
@@ -614,7 +619,11 @@ Plan plan(int B, int Sq, int HK, int max_tiles) {
         // 2 x 2500 23 / 21 / 25; 64, 1 x 500 26 / 23 / 27.
         pl.dense = pl.R == 8 ? 0 : pl.R == 4 ? 8 : 4;
         pl.least = pl.R == 8 ? 4 : 2;
-        pl.tiles = (long long)B * max_tiles;
+        // A sequence's beginning (its words, queries and first tile are waited for) takes a workgroup as long as a few tiles:
+        // counted for none / 4 tiles, 32 x 16 nodes 103.7 / 100.4 us, 2 x 32 nodes after 10000 43.8 / 38.1; 64 nodes, none /
+        // 4 / 6: 2 x 10000 62.7 / 51.9 / 52.5, 16 x 4000 105.1 / 102.1 / 96.1.
+        pl.begin = B == 1 ? 0 : pl.R == 8 ? 6 : 4;
+        pl.tiles = (long long)B * (max_tiles + pl.begin);
         const long long most = (pl.tiles + pl.least - 1) / pl.least;
         pl.runs = HK < slots ? slots / HK : 1;
         pl.wgs = (most < pl.runs ? most : pl.runs) * HK;
@@ -663,7 +672,7 @@ int launch_as(const CaParams &p, const Plan &pl, hipStream_t st) {
 
 template <bool TREE>
 int launch(CaParams &p, const Plan &pl, void *workspace, hipStream_t st) {
-    p.nqb = pl.nqb, p.gq = pl.gq, p.chunk = pl.chunk, p.nchunk = pl.nchunk, p.runs = pl.runs, p.dense = pl.dense, p.least = pl.least;
+    p.nqb = pl.nqb, p.gq = pl.gq, p.chunk = pl.chunk, p.nchunk = pl.nchunk, p.runs = pl.runs, p.dense = pl.dense, p.least = pl.least, p.begin = pl.begin;
     p.part_o = (float *)workspace;
     p.part_ml = (float2 *)((char *)workspace + pl.states * kD * 4);
     if (pl.wgs >= (1LL << 31) || pl.tiles >= (1LL << 30)) return MICA_MISS_RANGE;
