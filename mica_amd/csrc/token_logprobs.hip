@@ -3,12 +3,15 @@
 //   M = max_v x_v,  S = sum_v e^(x_v - M),  lp(v) = (x_v - M) - ln S,  H = ln S - (sum_v e^(x_v - M) (x_v - M)) / S
 //   top: the `top` largest by (value, then lowest index); NaN counts as the largest value, -0 equals 0
 //
-// (in log2 units, see Stat).  A workgroup walks a row's (or a part's) logits in blocks of 256 threads x 64 bytes, the next block's loads in flight
-// while it works on one.  Every thread keeps a running (m, s, t) of its own elements in fp32, so the statistics need no
-// barrier.  For the alternatives the workgroup keeps a list of candidates in LDS and a threshold, of which it knows that
-// `top` elements reach it: at first the top-th largest of 64 group maxima of the first block (found bit by bit with
-// ballots), later the top-th largest candidate.  Only elements that reach it are looked at one by one.  A block of which
-// too many do (long runs of ties) is selected exactly, bit by bit over values and then indices.
+// (in log2 units, see Stat).  A workgroup walks a row's (or a part's) logits in blocks of 256 threads x 64 bytes, the next
+// block's loads in flight while it works on one.  Every thread keeps a running (m, s, t) of its own elements in fp32, so
+// the statistics need no barrier.  For the alternatives the workgroup keeps a list of candidates in LDS and a threshold, of
+// which it knows that `top` elements reach it: at first the top-th largest of 64 group maxima of the first block (found bit
+// by bit with ballots), later the top-th largest candidate.  The 16-byte vectors whose maximum reaches it go into a queue
+// whole; when 32 of them wait, their elements are looked at, four threads a vector, and the best of the list found anew
+// (with the elements looked at where they were found, a wave took 400 cycles for each, and 2048 x 151936 bf16 with 20
+// alternatives 157 us instead of 135).  A block of which too many vectors reach the threshold (long runs of ties) is
+// selected exactly, bit by bit over values and then indices.
 //
 // Few rows are divided over several workgroups each; lp_merge_kernel then joins their (m, s, t) and candidates.
 #include "common.h"
@@ -19,6 +22,8 @@ constexpr int kThreads = 256;
 constexpr int kMaxTop = 32;
 constexpr int U = 4;                   // 16-byte vectors a thread holds of a block
 constexpr int kCap = 1024;             // candidates in LDS
+constexpr int kQueue = 256;            // vectors in LDS that hold an element that reaches the threshold
+constexpr int kFlush = 32;             // as many wait for the next look at their elements
 constexpr int kMaxParts = 64;
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 constexpr float kFar = -1.0e4f;        // 2^-10000 is 0 in fp32: differences are cut here, so that 0 x inf never is
@@ -189,14 +194,17 @@ MICA_DEVICE Stat block_stat(Stat a, Stat *red) {
     return r;
 }
 
+// (six workgroups a CU; five leave fp32 the registers that it would spill: 1024 x 151936 with 20 alternatives 117.5 -> 107.9 us)
 template <int DT, bool TOP>
-__global__ __launch_bounds__(kThreads, 6) void lp_rows_kernel(LpParams p) {
+__global__ __launch_bounds__(kThreads, DT == MICA_FP32 ? 5 : 6) void lp_rows_kernel(LpParams p) {
     using E = Elem<DT>;
     constexpr int kSize = 16 / E::N;
     __shared__ Stat red[kThreads / 64];
     __shared__ float gmax[64];
     __shared__ unsigned long long list[TOP ? kCap : 8];
-    __shared__ int counts[3], wcount[kThreads / 64];
+    __shared__ u32x4 queue[TOP ? kQueue : 1];
+    __shared__ int queue_at[TOP ? kQueue : 1];
+    __shared__ int counts[3], listed, wcount[kThreads / 64];
     const int row = blockIdx.x / p.parts, part = blockIdx.x % p.parts, tid = threadIdx.x;
     const char *x = (const char *)p.x + (long long)row * p.ldx * kSize;
     // the row as up to N - 1 single elements, 16-byte vectors from the first aligned address, up to N - 1 single ones
@@ -205,7 +213,7 @@ __global__ __launch_bounds__(kThreads, 6) void lp_rows_kernel(LpParams p) {
     const char *body = x + head * kSize;
     const int v0 = part * p.bpp * (kThreads * U), v1 = min(v0 + p.bpp * (kThreads * U), nv);
     const bool first_part = part == 0, last_part = part == p.parts - 1;
-    if (TOP && tid == 0) counts[0] = 0;
+    if (TOP && tid == 0) counts[0] = listed = 0;
 
     auto load = [&](int v, u32x4 (&w)[U]) {
         if (v + kThreads * U <= v1) { // a full block
@@ -235,7 +243,8 @@ __global__ __launch_bounds__(kThreads, 6) void lp_rows_kernel(LpParams p) {
     bool near = false; // every lane's reference is within kNear
     float thr = -__builtin_inff(); // elements not below it are candidates;
     bool above = false;            // or only those above it
-    int kept = 0, turn = 0;        // candidates of earlier blocks; the block's counter
+    int kept = 0, queued = 0;      // candidates; vectors of earlier blocks in the queue
+    int turn = 0;                  // the block's counter
     for (int v = v0; v == v0 || v < v1; v += kThreads * U) {
         const bool first = v == v0;
         if (v + kThreads * U < v1) load(v + kThreads * U, nxt);
@@ -290,10 +299,40 @@ __global__ __launch_bounds__(kThreads, 6) void lp_rows_kernel(LpParams p) {
                 if (thr != thr) thr = -__builtin_inff(); // (the number below -inf's is a NaN's)
             }
             auto reaches = [&](float xv) { return above ? !(xv <= thr) : !(xv < thr); }; // (as a NaN does)
-            // more candidates than the list holds are only counted
-            auto push = [&](float xv, int idx) {
-                const int at = kept + atomicAdd(&counts[turn], 1);
-                if (at < kCap) list[at] = key_of(xv, idx);
+            const bool more = v + kThreads * U < v1;
+            auto push = [&](float xv, int idx) { list[atomicAdd(&listed, 1)] = key_of(xv, idx); };
+            auto best = [&] { // the best of the list, and their threshold
+                const bool full = kept >= p.top;
+                kept = keep_best(list, kept, p.top);
+                if (full) {
+                    const unsigned long long least = list[p.top - 1];
+                    thr = value_of((uint32_t)(least >> 32));
+                    if (thr != thr) thr = __builtin_inff();
+                    // indices grow from block to block, but for the single elements of the row's end
+                    above = (int)~(uint32_t)least < p.V - tail;
+                }
+                if (tid == 0) listed = kept;
+                __syncthreads();
+            };
+            // the elements of the queue's first n vectors, four threads a vector, 64 vectors at a time
+            auto expand = [&](int n) {
+                kept = listed; // (with n = 0 the single elements)
+                for (int q = 0; q < n; q += kThreads / 4) {
+                    const int i = q + (tid >> 2);
+                    if (i < n) {
+                        const u32x4 w = queue[i];
+                        const uint32_t word = (tid & 2) ? ((tid & 1) ? w[3] : w[2]) : ((tid & 1) ? w[1] : w[0]);
+#pragma unroll
+                        for (int e = 0; e < E::N / 4; ++e) {
+                            const float xv = E::get(u32x4{word, 0, 0, 0}, e);
+                            // (not below, also where `above`: that is for the blocks to come)
+                            if (!(xv < thr)) push(xv, head + queue_at[i] * E::N + (tid & 3) * (E::N / 4) + e);
+                        }
+                    }
+                    __syncthreads();
+                    kept = listed;
+                    if (q + kThreads / 4 < n || (more && kept > p.top + 16)) best();
+                }
             };
             // Three counters in turn, so that one barrier a block is enough: the next block's is cleared here, before the
             // barrier, two blocks after its last reads.
@@ -305,19 +344,23 @@ __global__ __launch_bounds__(kThreads, 6) void lp_rows_kernel(LpParams p) {
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
                     const int at = v + u * kThreads + tid;
-                    if ((reaches(vmax[u]) || odd) && at < v1)
-#pragma unroll
-                        for (int e = 0; e < E::N; ++e) {
-                            const float xv = E::get(cur[u], e);
-                            if (reaches(xv)) push(xv, head + at * E::N + e);
-                        }
+                    if ((reaches(vmax[u]) || odd) && at < v1) { // (a queue that is full is only counted)
+                        const int to = queued + atomicAdd(&counts[turn], 1);
+                        if (to < kQueue) queue[to] = cur[u], queue_at[to] = at;
+                    }
                 }
                 if (first && one_at >= 0 && reaches(one)) push(one, one_at);
             }
             __syncthreads();
-            int n = kept + counts[turn];
-            const bool exact = n > kCap;
-            if (exact) { // too many reach the threshold: this block's best, exactly
+            const int n = queued + counts[turn];
+            const bool exact = n > kQueue;
+            if (exact || n > kFlush || !more) {
+                expand(exact ? queued : n);
+                queued = 0;
+            } else {
+                queued = n;
+            }
+            if (exact) { // too many reach the threshold: the best of this block's vectors, exactly
                 // the value of the top-th best element, then the index up to which elements of that value belong; the
                 // block is read again for every bit (a loop of few registers beside the ordinary path's)
                 auto each = [&](auto f) {
@@ -329,7 +372,6 @@ __global__ __launch_bounds__(kThreads, 6) void lp_rows_kernel(LpParams p) {
 #pragma unroll
                         for (int e = 0; e < E::N; ++e) f(E::get(w, e), head + at * E::N + e);
                     }
-                    if (first && one_at >= 0) f(one, one_at);
                 };
                 uint32_t o = 0, last = 0xffffffffu;
                 auto belongs = [&](float xv, int idx) { // above order o, or at it with an index up to `last`
@@ -356,24 +398,14 @@ __global__ __launch_bounds__(kThreads, 6) void lp_rows_kernel(LpParams p) {
                     last &= ~(1u << b);
                     if (tally() < p.top) last |= 1u << b;
                 }
-                if (tid == 0) counts[turn] = 0; // (its reads lie before the tallies' barriers)
-                __syncthreads();
                 each([&](float xv, int idx) {
-                    if (belongs(xv, idx)) list[kept + atomicAdd(&counts[turn], 1)] = key_of(xv, idx);
+                    if (belongs(xv, idx)) push(xv, idx);
                 });
-                n = kept + p.top;
                 __syncthreads();
+                kept = listed;
+                if (more) best();
             }
             turn = next;
-            kept = n; // (at most kCap: a block adds what the list holds, and is followed by a shorter list or is the last)
-            if ((exact || n > p.top + 16) && v + kThreads * U < v1) { // keep the best and raise the threshold
-                kept = keep_best(list, n, p.top);
-                const unsigned long long least = list[p.top - 1];
-                thr = value_of((uint32_t)(least >> 32));
-                if (thr != thr) thr = __builtin_inff();
-                // indices grow from block to block, but for the single elements of the row's end
-                above = (int)~(uint32_t)least < p.V - tail;
-            }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) cur[u] = nxt[u];
