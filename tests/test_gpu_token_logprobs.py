@@ -91,6 +91,35 @@ def test_ties_go_to_the_lowest_index(gpu, dtype, T):
     check(token_logprobs(x, tokens, 20), x, tokens, 20)
 
 
+@pytest.mark.parametrize("top", [1, 20, 32])
+@pytest.mark.parametrize("T", [4, 1026])
+def test_orders_that_bring_many_candidates(gpu, T, top):
+    """Rising rows (every element is the largest so far), and rows whose blocks bring from a few to thousands of them."""
+    V = 50021
+    x = rows(gpu, T, V, torch.float32, 9)
+    up = torch.arange(V, device=gpu, dtype=torch.float32)
+    x[0] = up / 4096
+    x[1] = up // 8 / 4096 - up % 8                 # eight rising runs
+    x[2] += up / 2000                               # a slope under the noise: some of each block
+    x[3] = torch.where(up % 37 == 0, up / 4096, x[3] - 9)
+    tokens = torch.randint(0, V, (T,), device=gpu)
+    check(token_logprobs(x, tokens, top), x, tokens, top)
+
+
+@pytest.mark.parametrize("T", [3, 1026])
+def test_a_nan_in_every_thread(gpu, T):
+    V = 30000
+    x = rows(gpu, T, V, torch.bfloat16, 4)
+    x[0, ::7] = math.nan
+    x[1, ::301] = math.nan                          # from then on a thread looks at all its elements
+    x[2, 5::8192] = math.nan
+    out = token_logprobs(x, torch.zeros(T, dtype=torch.int64, device=gpu), 32)
+    for row, step in ((0, 7), (1, 301)):
+        assert out.top_ids[row].tolist() == [i * step for i in range(32)] and torch.isnan(out.entropy[row])
+    best = torch.sort(torch.nan_to_num(x[2].float(), nan=-math.inf), descending=True, stable=True).indices
+    assert out.top_ids[2].tolist() == [5, 8197, 16389, 24581] + best[:28].tolist()
+
+
 @pytest.mark.parametrize("T", [6, 1030])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_infinite_and_nan_logits(gpu, dtype, T):
