@@ -163,6 +163,17 @@ MICA_DEVICE uint32_t odd_value(uint32_t h, uint32_t nan_sign) {
     return 0x7f7fu | ((h & 0x7fu) ? nan_sign : (h & 0x8000u));
 }
 
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+// A transposing read.  The compiler knows nothing of what the DMA in flight writes, and would let every one of these reads
+// wait for all of it, the next tile's too.  `w`, which nothing is accessed through, says that the read meets no unknown
+// store; the waits are the loop's own.  (16 x 64 nodes after 4000 keys 97.9 -> 94.5 us, 2 x 32 nodes after 10000 38.3 -> 36.)
+MICA_DEVICE s16x4 tr_read(lds_s16x4 *p, lds_void *__restrict w) {
+    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(p);
+    __builtin_assume(w != nullptr);
+    return x;
+}
+
 template <int R, int D, int ST, bool TREE, bool STREAM>
 __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca_fwd_kernel(CaParams p) {
     constexpr int kWaves = R * D, kThreads = 64 * kWaves;
@@ -174,10 +185,10 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
     // 106.6 -> 102.1 us, 64 nodes after 32768 75.4 -> 72.0), but before it where the keys are mostly in L2 and the matrix
     // cores bound (16384 tokens with a window of 2048: 498.7 against 518.1).
     constexpr bool kLate = STREAM || TREE;
-    constexpr int kWords = TREE ? NB * (STREAM ? 2 : kMaxNodes / 32) : 1; // (STREAM: up to 64 nodes)
+    constexpr int kWords = TREE ? NB * (STREAM ? 2 : kMaxNodes / 32) : 0; // (STREAM: up to 64 nodes)
     static_assert(R * 32 * kD * 2 <= ST * kStage, "the output is staged where the tiles were");
-    __shared__ __attribute__((aligned(1024))) int8_t smem[ST * kStage];
-    __shared__ uint32_t words[kWords];
+    __shared__ __attribute__((aligned(1024))) int8_t smem[ST * kStage + kWords * 4];
+    uint32_t *const words = (uint32_t *)(smem + ST * kStage);
 
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void *)smem;
@@ -244,7 +255,7 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
             (void *)kb, 0, rows > 0 ? (int)((rows - 1) * ldk * 2) + kD * 2 : 0, kBufferFlags);
         const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
             (void *)vb, 0, rows > 0 ? (int)((rows - 1) * ldv * 2) + kD * 2 : 0, kBufferFlags);
-        // 1 KB block x = key rows 2 x + hi; chunk c of row r lies at c ^ (r % 16) (K), c ^ 2 (r % 8) (V).  The offsets
+        // 1 KB block x = key rows 2 x + hi; chunk c of row r lies at c ^ (r % 16) (K), c ^ 4 (r % 4) (V).  The offsets
         // come from an opaque copy of the lane id at every tile: hoisted out of the loop they take 16 registers, and
         // what these push into scratch is then loaded back behind the DMA, which every such load waits for.
         int ln = lane;
@@ -259,13 +270,13 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
 #pragma unroll
         for (int x = 0; x < kBlk; ++x)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void *)(s + kTile + x * 1024), 16,
-                                                     rv0 + 2 * x * v2 + (((ln & 31) ^ (((r0 + 2 * x) & 7) << 1)) << 4), 0,
+                                                     rv0 + 2 * x * v2 + (((ln & 31) ^ (((r0 + 2 * x) & 3) << 2)) << 4), 0,
                                                      0, 0);
     };
     // The block's words and this lane's Q fragments (B operand of S^T: dims 16 s + 8 hi .. + 7 of the row) come before the
     // tiles: loads end in order, and behind the DMA the first step waited for all the stages' tiles.
     constexpr int kMine = (kWords + kThreads - 1) / kThreads;
-    uint32_t mine[kMine];
+    uint32_t mine[TREE ? kMine : 1];
     if constexpr (TREE) {
 #pragma unroll
         for (int x = 0; x < kMine; ++x) {
@@ -299,24 +310,23 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
 
     // V^T fragment of 32-dim tile dt, step s: keys 16 s + 4 hi .. + 3 and 16 s + 8 + 4 hi .. + 3 (the keys of P^T's
     // accumulator rows 8 s .. 8 s + 7) of dim 32 dt + l % 32.  The lane's address: key row 4 hi + (l % 16) / 4, dims
-    // 16 ((l / 16) % 2) + 4 (l % 4); chunk c of row r lies at c ^ 2 (r % 8), which spreads the 8 rows x 64 bytes of a
-    // read over all banks twice, the least 512 bytes can take.
+    // 16 ((l / 16) % 2) + 4 (l % 4); chunk c of row r lies at c ^ 4 (r % 4), which spreads the 4 rows x 64 bytes of
+    // each half of a read over all banks (c ^ 2 (r % 8) spreads all 8 rows, but a half over half of the banks: it cost 1.3
+    // conflict cycles an LDS instruction, 1% of the time).
     const int vrow = 4 * hi + ((l32 & 15) >> 2);
-    const uint32_t vbase = lds0 + kTile + vrow * (kD * 2) + (((2 * (l32 >> 4) + ((l32 & 3) >> 1)) ^ (vrow << 1) ^ (4 * dt0)) << 4) +
+    const uint32_t vbase = lds0 + kTile + vrow * (kD * 2) + (((2 * (l32 >> 4) + ((l32 & 3) >> 1)) ^ ((vrow & 3) << 2) ^ (4 * dt0)) << 4) +
                            (l32 & 1) * 8;
     // K fragment s: chunk 2 s + hi of key row l % 32, at chunk ^ (l % 16).  The chunk's five bits are address bits of
     // their own in both tiles, so a fragment's address is one exclusive or away from its stage's.
     const uint32_t kbase = lds0 + l32 * (kD * 2) + ((hi ^ (l32 & 15)) << 4);
-    typedef short s16x4 __attribute__((ext_vector_type(4)));
-    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
     typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
     auto kfrag = [](uint32_t stage, int s) { // stage: kbase + the stage's offset
         return __builtin_bit_cast(bf16x8, *(lds_u32x4 *)(uintptr_t)((stage ^ (s << 5))));
     };
     auto vfrag = [](uint32_t stage, int s, int dt) { // stage: vbase + the stage's offset
         const uint32_t a = (stage ^ (dt << 6)) + s * 16 * (kD * 2);
-        const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(uintptr_t)a);
-        const s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(uintptr_t)(a + 8 * (kD * 2)));
+        const s16x4 x = tr_read((lds_s16x4 *)(uintptr_t)a, (lds_void *)smem);
+        const s16x4 y = tr_read((lds_s16x4 *)(uintptr_t)(a + 8 * (kD * 2)), (lds_void *)smem);
         return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
     };
 
