@@ -85,7 +85,7 @@ struct Tiles {
 
 // How STREAM divides the tiles: those of all sequences, one after the other, into runs, and a workgroup for each run and
 // head.  Workgroups next to each other take the heads of one run: their rows lie side by side in memory (with the heads
-// one after the other instead, 64 single tokens with a window of 4096 took 208 us and not 193).  All lanes of a wave call
+// one after the other instead, 64 single tokens with a window of 4096 took 201 us and not 194).  All lanes of a wave call
 // and get the same; a lane reads every 64th sequence's count.
 template <bool TREE>
 struct Stream {
@@ -181,10 +181,6 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
     constexpr int NDT = kD / 32 / D;          // 32-dim tiles of O a wave holds
     constexpr int kBlk = 16 / kWaves;         // 1 KB DMA blocks of K, and of V, a wave issues for a tile
     constexpr int kPf = D > 1 ? 8 : 3;        // operand fragments read ahead (D = 1: more would spill)
-    // The next tile's DMA is issued behind the chain of S^T, whose result is waited for anyway (cached keys: 32 x 16 nodes
-    // 106.6 -> 102.1 us, 64 nodes after 32768 75.4 -> 72.0), but before it where the keys are mostly in L2 and the matrix
-    // cores bound (16384 tokens with a window of 2048: 498.7 against 518.1).
-    constexpr bool kLate = STREAM || TREE;
     constexpr int kWords = TREE ? NB * (STREAM ? 2 : kMaxNodes / 32) : 0; // (STREAM: up to 64 nodes)
     static_assert(R * 32 * kD * 2 <= ST * kStage, "the output is staged where the tiles were");
     __shared__ __attribute__((aligned(1024))) int8_t smem[ST * kStage + kWords * 4];
@@ -337,7 +333,7 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
         wait_vmcnt<(ST - 2) * 2 * kBlk>();
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
-        if (!kLate) issue(i + ST - 1, (st + ST - 1) % ST);
+        issue(i + ST - 1, (st + ST - 1) % ST);
         const int8_t *stage = smem + st * kStage;
         const uint32_t ks = kbase + st * kStage, vs = vbase + st * kStage;
         // ---- S^T = K Q^T: rows = keys of the tile, column = this lane's row; fragments read kPf steps ahead ----
@@ -354,7 +350,6 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
             sc = mfma_bf16(a, qf[s], sc);
         }
         __builtin_amdgcn_s_setprio(0);
-        if (kLate) issue(i + ST - 1, (st + ST - 1) % ST);
         // ---- keys that a row does not see: score -inf, weight 0 (score r of a lane is key 8 (r / 4) + 4 hi + r % 4) ----
         bool masked = false, own = false;
         if constexpr (TREE) {
@@ -623,22 +618,22 @@ Plan plan(int B, int Sq, int HK, int max_tiles) {
     const long long units = (long long)B * HK;
     if (pl.stream) {
         // Two workgroups a CU, while each gets enough tiles to repay the partial state that it writes (32 R KB) and the merge
-        // reads; else one, of 4 tiles at least, and of fewer only where even so the chip would be nearly empty.  Measured,
-        // us, two / one a CU (nodes, sequences x keys): 8, 16 x 4000 57 / 67, 1 x 32768 41 / 47, 16 x 1000 29 / 28;
-        // 32, 16 x 4000 76 / 81, 8 x 3000 49 / 45, 16 x 1000 42 / 39; tiles a workgroup 2 / 4 / 8: 8, 1 x 500 14 / 16 / 19,
-        // 2 x 2500 23 / 21 / 25; 64, 1 x 500 26 / 23 / 27.
-        pl.dense = pl.R == 8 ? 0 : pl.R == 4 ? 8 : 4;
+        // reads (R = 1: 8, else 12); else one, of 4 tiles at least, and of fewer only where even so the chip would be nearly
+        // empty.  Measured, us, two / one a CU (nodes, sequences x keys): 4, 8 x 5000 44.3 / 46.5, 2 x 10000 27.1 / 24.1;
+        // 16, 32 x 4096 102 / 110, 1 x 32768 45.6 / 41.3; 32, 16 x 2000 56.8 / 50.1, 16 x 4000 84 / 85.  Tiles a workgroup
+        // 2 / 4 in a nearly empty chip: 8, 1 x 500 14.1 / 15.9; 64, 1 x 500 23.5 / 22.8.
+        pl.dense = pl.R == 8 ? 0 : pl.R == 1 ? 8 : 12;
         pl.least = pl.R == 8 ? 4 : 2;
         // A sequence's beginning (its words, queries and first tile are waited for) takes a workgroup as long as a few tiles:
-        // counted for none / 4 tiles, 32 x 16 nodes 103.7 / 100.4 us, 2 x 32 nodes after 10000 43.8 / 38.1; 64 nodes, none /
-        // 4 / 6: 2 x 10000 62.7 / 51.9 / 52.5, 16 x 4000 105.1 / 102.1 / 96.1.
+        // counted for none / 4 tiles, 16 x 32 nodes after 4000 keys 89.4 / 83.9 us, 2 x 10000 42.8 / 36.4; 64 nodes, none / 4 /
+        // 6: 2 x 10000 62.7 / 51.9 / 52.5, 16 x 4000 105 / 102 / 96.
         pl.begin = B == 1 ? 0 : pl.R == 8 ? 6 : 4;
         pl.tiles = (long long)B * (max_tiles + pl.begin);
         const long long most = (pl.tiles + pl.least - 1) / pl.least;
         pl.runs = HK < slots ? slots / HK : 1;
         pl.wgs = (most < pl.runs ? most : pl.runs) * HK;
         pl.states = pl.wgs * 2 * 32 * pl.R;
-        // (few waves, then, of many parts each; 8 nodes, 2 x 10000 keys 37 -> 30 us, 16 x 4000 57, but 63 if waves share there)
+        // (few waves, then, of many parts each; 8 nodes, 1 x 32768 keys 54.6 -> 40.2 us, but 16 x 4000 64.2 -> 68.9 if waves share there)
         pl.wide = units * pl.R <= 16;
         return pl;
     }
