@@ -101,6 +101,19 @@ def test_tree_against_float64(gpu, B, N, HK, C, lens):
     check(o, q, torch.cat((kc, k), 1), torch.cat((vc, v), 1), tree_sees(par, lens or [C] * B, C, gpu))
 
 
+@pytest.mark.parametrize("N", [3, 12, 30, 60])
+@pytest.mark.parametrize("B,C", [(130, 40), (70, 400), (9, 2900)])
+def test_tree_sequences_of_every_length_side_by_side(gpu, B, C, N):
+    """Workgroups begin and end anywhere in the row of all sequences' keys: at a sequence's first tile, in its last, within
+    the new keys."""
+    q, k, v, kc, vc = heads(gpu, B + N, B, N, 1, C)
+    g = torch.Generator().manual_seed(B * N)
+    lens = torch.randint(-C // 4, C + 1, (B,), generator=g).clamp(0).tolist()
+    par = [random_parents(N, b, absent=b % 3 == 0) for b in range(B)]
+    o = tree_attention(q, k, v, tree_masks(par, gpu), (kc, vc), torch.tensor(lens, dtype=torch.int32, device=gpu))
+    check(o, q, torch.cat((kc, k), 1), torch.cat((vc, v), 1), tree_sees(par, lens, C, gpu))
+
+
 def test_tree_shared_cache_one_tree_and_scale(gpu):
     q, k, v, kc, vc = heads(gpu, 3, 4, 20, 4, 777)
     par = random_parents(20, 5)
@@ -178,6 +191,15 @@ def test_window_against_float64(gpu, B, n, S, window, sinks, lens):
     t = None if lens is None else torch.tensor(lens, dtype=torch.int32, device=gpu)
     o = window_attention(q, k, v, window, sinks, kv_len=t)
     check(o, q, k, v, window_sees(B, n, S, window, sinks, lens or [S] * B, gpu))
+
+
+@pytest.mark.parametrize("n,window", [(1, 500), (3, 40), (14, 300), (30, 64), (60, 129)])
+def test_window_sequences_of_every_length_side_by_side(gpu, n, window):
+    B, S = 67, 700
+    q, _, _, k, v = heads(gpu, n, B, n, 1, S)
+    lens = torch.randint(-S // 4, S + 1, (B,), generator=torch.Generator().manual_seed(n)).clamp(0).tolist()
+    o = window_attention(q, k, v, window, 4, kv_len=torch.tensor(lens, dtype=torch.int32, device=gpu))
+    check(o, q, k, v, window_sees(B, n, S, window, 4, lens, gpu))
 
 
 def test_window_wider_than_the_keys_is_causal_attention(gpu):
