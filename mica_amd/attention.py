@@ -6,6 +6,9 @@ and the torch SDPA path taken without it.  ``causal_gqa_attention(q, k, v)`` tak
 views -- typically of the fused QKV projection output, no copies -- with 4 query heads per key/value
 head, and returns o [B, S, HQ, 256] bf16 (the O projection's [B * S, HQ * 256] rows).
 GPU only; no fallback.
+
+``tree_attention`` and ``window_attention`` take the same heads: a tree of drafted tokens over a cache, and causal attention
+within a sliding window.
 """
 from __future__ import annotations
 

@@ -174,6 +174,13 @@ MICA_DEVICE s16x4 tr_read(lds_s16x4 *p, lds_void *__restrict w) {
     return x;
 }
 
+// What bounds it, and the whole call's time (at the rates of a large copy, 4.87 TB/s, and a large matrix product, 1401 TFLOP/s):
+// few rows, the cache's bytes: 64 single tokens with a window of 4096 take 190 us, 5.7 TB/s; 32 x 16 nodes over up to 4096
+// keys 97 us of 86.  Many rows, the matrix cores beside the softmax, with two waves a SIMD: 16384 tokens with a window of 2048
+// 476 us of 368; 64 nodes after 32768 keys 65 us of 28, of them 8 for the first tiles and 20 for writing and joining 64 MB of
+// partial states; 4 x 255 nodes after 2048 shared keys 63 us of 24.5.  A short call is two launches: 8 nodes after 500 keys
+// 13 us.  (Four stages with fewer than eight waves, fragments read further ahead, 64 rows a wave, two chains for S^T: no
+// faster, or slower for the registers that they spill.)
 template <int R, int D, int ST, bool TREE, bool STREAM>
 __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca_fwd_kernel(CaParams p) {
     constexpr int kWaves = R * D, kThreads = 64 * kWaves;
@@ -517,6 +524,8 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
 
 // The partial states of a block's parts joined: with M = max_c m_c, w_c = 2^(m_c - M), o = (sum w_c O_c) / (sum w_c l_c).
 // A part's accumulators are taken 64 lanes x 16 bytes at a time (4 dims of 32 rows x 2), by W waves that share the parts.
+// Bound by reading the states that were just written: 64 MB take 15 us, 4.3 TB/s (more waves, more loads in flight or
+// nontemporal ones: no faster); 1 MB takes 4 us.
 template <int R, int D, bool TREE, bool STREAM, int W>
 __global__ __launch_bounds__(256) void ca_merge_kernel(CaParams p) {
     constexpr int NB = 8 * R, NDT = kD / 32 / D, kFrags = 32 * R, kPer = 4 / W;

@@ -4,6 +4,9 @@ embedding are ever multiplied, and only at each request's last token.
 Reference: the readout closure built in HFJudge.__init__ (akivet/Mica
 v0.5/serving/lib/release_runtime.py:298-306) applied to ``body.norm`` of the last hidden row
 (prefill_engine.py:280-304), then the slice + softmax of judge_many (release_runtime.py:509-517).
+
+``token_logprobs`` reads whole rows of logits instead: the log probabilities of given tokens, the entropy and the best
+alternatives.
 """
 from __future__ import annotations
 
