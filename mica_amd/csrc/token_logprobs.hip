@@ -124,7 +124,24 @@ MICA_DEVICE uint32_t nth_of_wave(uint32_t o, int n) {
 }
 
 // The best `top` of the list's n keys, in order, at its start (n <= kCap; every thread calls).  Returns how many.
+// QUADS: up to 64 keys take four threads each (64 x 151936 fp32 21.9 -> 20.3 us; the 16-bit rows' kernel would spill for it,
+// 8192 x 16000 with 5 alternatives 66.4 -> 71.1).
+template <bool QUADS>
 MICA_DEVICE int keep_best(unsigned long long *list, int n, int top) {
+    if (QUADS && n <= kThreads / 4) { // four threads a key
+        const int at = threadIdx.x >> 2;
+        const unsigned long long k = at < n ? list[at] : 0;
+        int r = 0;
+        for (int i = threadIdx.x & 3; i < n; i += 16)
+#pragma unroll
+            for (int x = 0; x < 16; x += 4) r += list[i + x] > k && i + x < n;
+        r += __shfl_xor(r, 1, 64);
+        r += __shfl_xor(r, 2, 64);
+        __syncthreads();
+        if (at < n && (threadIdx.x & 3) == 0 && r < top) list[r] = k;
+        __syncthreads();
+        return n < top ? n : top;
+    }
     unsigned long long mine[kCap / kThreads];
     int rank[kCap / kThreads];
 #pragma unroll
@@ -196,7 +213,7 @@ MICA_DEVICE Stat block_stat(Stat a, Stat *red) {
 
 // One pass over the row, bound by HBM without alternatives: 4096 x 151936 bf16 take 198 us, 6.3 TB/s; with 20 of them nearly
 // as much by VALU issue, 2048 rows 131 us, 4.8 TB/s.  Rows of a block or two are bound by their latency (load, threshold,
-// candidates, join): 64 x 151936 fp32 with 20 alternatives 20.7 us, without 12; one row 11.
+// candidates, join): 64 x 151936 fp32 with 20 alternatives 20.3 us, without 12; one row 11.
 // (six workgroups a CU; five leave fp32 the registers that it would spill: 1024 x 151936 with 20 alternatives 117.5 -> 107.9 us)
 template <int DT, bool TOP>
 __global__ __launch_bounds__(kThreads, DT == MICA_FP32 ? 5 : 6) void lp_rows_kernel(LpParams p) {
@@ -306,7 +323,7 @@ __global__ __launch_bounds__(kThreads, DT == MICA_FP32 ? 5 : 6) void lp_rows_ker
             auto push = [&](float xv, int idx) { list[atomicAdd(&listed, 1)] = key_of(xv, idx); };
             auto best = [&] { // the best of the list, and their threshold
                 const bool full = kept >= p.top;
-                kept = keep_best(list, kept, p.top);
+                kept = keep_best<DT == MICA_FP32>(list, kept, p.top);
                 if (full) {
                     const unsigned long long least = list[p.top - 1];
                     thr = value_of((uint32_t)(least >> 32));
@@ -415,7 +432,7 @@ __global__ __launch_bounds__(kThreads, DT == MICA_FP32 ? 5 : 6) void lp_rows_ker
     }
     a.rebase(largest);
     const Stat all = block_stat(a, red);
-    if constexpr (TOP) kept = keep_best(list, kept, p.top);
+    if constexpr (TOP) kept = keep_best<DT == MICA_FP32>(list, kept, p.top);
     if (p.parts == 1) {
         finish<DT>(p, row, all, list, tok);
         return;
@@ -447,7 +464,9 @@ __global__ __launch_bounds__(kThreads) void lp_merge_kernel(LpParams p) {
         const int r = (p.top + p.parts - 1) / p.parts, want = (p.top + r - 1) / r;
         const unsigned long long own = (tid & 63) < p.parts ? all[(tid & 63) * p.top + r - 1] : 0;
         int rank = 0;
-        for (int c = 0; c < p.parts; ++c) rank += all[c * p.top + r - 1] > own;
+        for (int c = 0; c < p.parts; c += 8) // 8 reads at a time (past the last part within `all`); those do not count
+#pragma unroll
+            for (int x = 0; x < 8; ++x) rank += all[(c + x) * p.top + r - 1] > own && c + x < p.parts;
         const unsigned long long at = __builtin_amdgcn_ballot_w64(rank == want - 1);
         unsigned long long least = 0; // (parts without that many keys)
         if (at) {
@@ -463,7 +482,7 @@ __global__ __launch_bounds__(kThreads) void lp_merge_kernel(LpParams p) {
         __syncthreads();
         const int c = count;
         if (c <= kCap) {
-            keep_best(list, c, p.top);
+            keep_best<true>(list, c, p.top);
         } else { // (parts of ascending values)  rank among all keys
             for (int i = tid; i < n; i += kThreads) {
                 int k = 0;
