@@ -13,7 +13,7 @@
 // the others) and 256 / D dims of O^T += V^T P^T.  With few rows, D > 1 waves share a row block: they repeat its scores
 // (cheap beside the tile's memory time) and divide the dims of O.
 //
-// Data movement: K and V tiles of 32 rows come by LDS DMA into a ring of ST stages, 16-byte chunks XOR-swizzled by row,
+// Data movement: K and V tiles of 32 rows come by LDS DMA into two stages in turn, 16-byte chunks XOR-swizzled by row,
 // rows past the last key as zeros (the buffer's range check).  K fragments are 16-byte reads; V is kept as it lies in
 // memory and its V^T fragments are transposing reads (ds_read_b64_tr_b16: 16 lanes fetch 4 keys x 16 dims and each gets
 // the 4 keys of one dim), so no pass over V comes before.
@@ -179,19 +179,19 @@ MICA_DEVICE s16x4 tr_read(lds_s16x4 *p, lds_void *__restrict w) {
 // keys 97 us of 86.  Many rows, the matrix cores beside the softmax, with two waves a SIMD: 16384 tokens with a window of 2048
 // 476 us of 368; 64 nodes after 32768 keys 65 us of 28, of them 8 for the first tiles and 20 for writing and joining 64 MB of
 // partial states; 4 x 255 nodes after 2048 shared keys 63 us of 24.5.  A short call is two launches: 8 nodes after 500 keys
-// 13 us.  (Four stages with fewer than eight waves, fragments read further ahead, 64 rows a wave, two chains for S^T: no
-// faster, or slower for the registers that they spill.)
-template <int R, int D, int ST, bool TREE, bool STREAM>
-__global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca_fwd_kernel(CaParams p) {
+// 13 us.  (Four stages with one workgroup a CU 1 to 5 us slower, with eight waves 1 us; fragments read further ahead, 64 rows
+// a wave, two chains for S^T: no faster, or slower for the registers that they spill.)
+template <int R, int D, bool TREE, bool STREAM>
+__global__ __launch_bounds__(64 * R * D, 2) void ca_fwd_kernel(CaParams p) {
     constexpr int kWaves = R * D, kThreads = 64 * kWaves;
     constexpr int NB = 8 * R;                 // query positions of the workgroup
     constexpr int NDT = kD / 32 / D;          // 32-dim tiles of O a wave holds
     constexpr int kBlk = 16 / kWaves;         // 1 KB DMA blocks of K, and of V, a wave issues for a tile
     constexpr int kPf = D > 1 ? 8 : 3;        // operand fragments read ahead (D = 1: more would spill)
     constexpr int kWords = TREE ? NB * (STREAM ? 2 : kMaxNodes / 32) : 0; // (STREAM: up to 64 nodes)
-    static_assert(R * 32 * kD * 2 <= ST * kStage, "the output is staged where the tiles were");
-    __shared__ __attribute__((aligned(1024))) int8_t smem[ST * kStage + kWords * 4];
-    uint32_t *const words = (uint32_t *)(smem + ST * kStage);
+    constexpr int kSmem = R * 32 * kD * 2 > 2 * kStage ? R * 32 * kD * 2 : 2 * kStage; // the tiles; the output, in the end
+    __shared__ __attribute__((aligned(1024))) int8_t smem[kSmem + kWords * 4];
+    uint32_t *const words = (uint32_t *)(smem + kSmem);
 
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void *)smem;
@@ -277,7 +277,7 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
                                                      0, 0);
     };
     // The block's words and this lane's Q fragments (B operand of S^T: dims 16 s + 8 hi .. + 7 of the row) come before the
-    // tiles: loads end in order, and behind the DMA the first step waited for all the stages' tiles.
+    // first tile: loads end in order.
     constexpr int kMine = (kWords + kThreads - 1) / kThreads;
     uint32_t mine[TREE ? kMine : 1];
     if constexpr (TREE) {
@@ -295,8 +295,7 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
         for (int s = 0; s < kD / 16; ++s) qf[s] = __builtin_bit_cast(bf16x8, *(const u32x4 *)(qr + s * 16));
     }
     __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int s = 0; s < ST - 1; ++s) issue(i0 + s, s);
+    issue(i0, 0);
     if constexpr (TREE) {
 #pragma unroll
         for (int x = 0; x < kMine; ++x) {
@@ -335,12 +334,12 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
 
 #pragma unroll 1
     for (int i = i0; i < i1; ++i) {
-        const int st = (i - i0) % ST;
+        const int st = (i - i0) & 1;
         // this wave's DMA of tile i landed; after the barrier every wave's has, and nobody reads tile i - 1 any more
-        wait_vmcnt<(ST - 2) * 2 * kBlk>();
+        wait_vmcnt<0>();
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
-        issue(i + ST - 1, (st + ST - 1) % ST);
+        issue(i + 1, 1 - st);
         const int8_t *stage = smem + st * kStage;
         const uint32_t ks = kbase + st * kStage, vs = vbase + st * kStage;
         // ---- S^T = K Q^T: rows = keys of the tile, column = this lane's row; fragments read kPf steps ahead ----
@@ -467,7 +466,7 @@ __global__ __launch_bounds__(64 * R * D, (R * D > 4 || ST == 2) ? 2 : 1) void ca
         }
         __builtin_amdgcn_s_setprio(0);
     }
-    wait_vmcnt<0>();  // the ring's last (empty) loads have written before the stages are used again or given up
+    wait_vmcnt<0>();  // the last (empty) loads have written before the stages are used again or given up
     float ltot = half_swap_sum(lsum);
     uint32_t any = 1;
     if constexpr (TREE) {
@@ -605,9 +604,9 @@ __global__ __launch_bounds__(256) void ca_merge_kernel(CaParams p) {
 
 // ---- host side ----
 
-// How a call is divided: row blocks (R) and dim parts (D) of a workgroup, LDS stages, and the work.
+// How a call is divided: row blocks (R) and dim parts (D) of a workgroup, and the work.
 struct Plan {
-    int R, D, ST, nqb, gq, chunk, nchunk;
+    int R, D, nqb, gq, chunk, nchunk;
     int runs, dense, least; // STREAM: most runs of tiles; the tiles of a run below which half as many are made; its fewest
     int begin;              // the tiles that a sequence's beginning counts for
     bool stream, wide;
@@ -619,7 +618,6 @@ Plan plan(int B, int Sq, int HK, int max_tiles) {
     pl.stream = Sq <= 64;
     pl.R = Sq <= 8 ? 1 : Sq <= 16 ? 2 : Sq <= 32 || !pl.stream ? 4 : 8;
     pl.D = pl.R < 4 ? 4 / pl.R : 1;
-    pl.ST = pl.R < 8 ? 2 : 4;
     pl.nqb = (Sq + 8 * pl.R - 1) / (8 * pl.R);
     pl.gq = pl.nqb < 8 ? pl.nqb : 8;
     pl.chunk = max_tiles, pl.nchunk = 1;
@@ -674,9 +672,9 @@ int window_tiles(int Sq, int Sk, int window, int sinks) {
 }
 long long state_bytes(const Plan &pl) { return pl.states * (kD * 4 + 8); }
 
-template <int R, int D, int ST, bool TREE, bool STREAM>
+template <int R, int D, bool TREE, bool STREAM>
 int launch_as(const CaParams &p, const Plan &pl, hipStream_t st) {
-    hipLaunchKernelGGL((ca_fwd_kernel<R, D, ST, TREE, STREAM>), dim3((unsigned)pl.wgs), dim3(64 * R * D), 0, st, p);
+    hipLaunchKernelGGL((ca_fwd_kernel<R, D, TREE, STREAM>), dim3((unsigned)pl.wgs), dim3(64 * R * D), 0, st, p);
     if (const int rc = mica_err(hipGetLastError())) return rc;
     if (pl.states == 0) return 0;
     const long long blocks = (long long)p.B * p.HK * pl.nqb;
@@ -693,11 +691,11 @@ int launch(CaParams &p, const Plan &pl, void *workspace, hipStream_t st) {
     p.part_o = (float *)workspace;
     p.part_ml = (float2 *)((char *)workspace + pl.states * kD * 4);
     if (pl.wgs >= (1LL << 31) || pl.tiles >= (1LL << 30)) return MICA_MISS_RANGE;
-    if (!pl.stream) return launch_as<4, 1, 2, TREE, false>(p, pl, st);
-    if (pl.R == 1) return launch_as<1, 4, 2, TREE, true>(p, pl, st);
-    if (pl.R == 2) return launch_as<2, 2, 2, TREE, true>(p, pl, st);
-    if (pl.R == 4) return launch_as<4, 1, 2, TREE, true>(p, pl, st);
-    return launch_as<8, 1, 4, TREE, true>(p, pl, st);
+    if (!pl.stream) return launch_as<4, 1, TREE, false>(p, pl, st);
+    if (pl.R == 1) return launch_as<1, 4, TREE, true>(p, pl, st);
+    if (pl.R == 2) return launch_as<2, 2, TREE, true>(p, pl, st);
+    if (pl.R == 4) return launch_as<4, 1, TREE, true>(p, pl, st);
+    return launch_as<8, 1, TREE, true>(p, pl, st);
 }
 
 // a row stride of `rows` rows that are read by DMA: 32 rows within a buffer's 31-bit range, none overlapping
