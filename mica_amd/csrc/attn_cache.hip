@@ -163,6 +163,13 @@ MICA_DEVICE uint32_t odd_value(uint32_t h, uint32_t nan_sign) {
     return 0x7f7fu | ((h & 0x7fu) ? nan_sign : (h & 0x8000u));
 }
 
+// A workgroup barrier that waits for nothing else; no access to memory moves across it.
+MICA_DEVICE void meet() {
+    __asm__ volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    __asm__ volatile("" ::: "memory");
+}
+
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 // A transposing read.  The compiler knows nothing of what the DMA in flight writes, and would let every one of these reads
@@ -190,8 +197,9 @@ __global__ __launch_bounds__(64 * R * D, 2) void ca_fwd_kernel(CaParams p) {
     constexpr int kPf = D > 1 ? 8 : 3;        // operand fragments read ahead (D = 1: more would spill)
     constexpr int kWords = TREE ? NB * (STREAM ? 2 : kMaxNodes / 32) : 0; // (STREAM: up to 64 nodes)
     constexpr int kSmem = R * 32 * kD * 2 > 2 * kStage ? R * 32 * kD * 2 : 2 * kStage; // the tiles; the output, in the end
-    __shared__ __attribute__((aligned(1024))) int8_t smem[kSmem + kWords * 4];
-    uint32_t *const words = (uint32_t *)(smem + kSmem);
+    __shared__ __attribute__((aligned(1024))) int8_t smem[kSmem + 16 + kWords * 4];
+    int *const odd_tile = (int *)(smem + kSmem); // the last tile that held a value that is not finite
+    uint32_t *const words = (uint32_t *)(smem + kSmem + 16);
 
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void *)smem;
@@ -302,8 +310,9 @@ __global__ __launch_bounds__(64 * R * D, 2) void ca_fwd_kernel(CaParams p) {
             const int i = tid + x * kThreads, left = p.Sq - 32 * (i % p.tw); // bits past the last node do not count
             if (i < NB * p.tw) words[i] = left >= 32 ? mine[x] : left <= 0 ? 0u : mine[x] & ((1u << left) - 1u);
         }
-        wait_lgkmcnt0(); // seen by every wave after the first tile's barrier
     }
+    if (tid == 0) *odd_tile = -1;
+    wait_lgkmcnt0(); // seen by every wave after the first tile's barrier
     f32x16 O[NDT];
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) O[dt] = f32x16{};
@@ -337,9 +346,13 @@ __global__ __launch_bounds__(64 * R * D, 2) void ca_fwd_kernel(CaParams p) {
         const int st = (i - i0) & 1;
         // this wave's DMA of tile i landed; after the barrier every wave's has, and nobody reads tile i - 1 any more
         wait_vmcnt<0>();
-        __builtin_amdgcn_s_barrier();
+        meet();
         __builtin_amdgcn_sched_barrier(0);
         issue(i + 1, 1 - st);
+        if constexpr (TREE && !STREAM) { // new keys that none of the block's nodes sees, as those after them (2 x 500 nodes
+                                         // after 500 keys 58.4 -> 45.8 us; up to 64 nodes there are hardly any)
+            if (i >= tl.n0 && !__builtin_amdgcn_ballot_w64(words[lane % NB * p.tw + (i - tl.n0)])) continue;
+        }
         const int8_t *stage = smem + st * kStage;
         const uint32_t ks = kbase + st * kStage, vs = vbase + st * kStage;
         // ---- S^T = K Q^T: rows = keys of the tile, column = this lane's row; fragments read kPf steps ahead ----
@@ -411,17 +424,21 @@ __global__ __launch_bounds__(64 * R * D, 2) void ca_fwd_kernel(CaParams p) {
             pb[s] = __builtin_bit_cast(bf16x8, w);
         }
         // A value that is not finite must not reach the rows that do not see its key (0 x inf = NaN): looked for in
-        // the tiles where rows see different keys.  (Rows past the last key are zeros, and where all rows see all
-        // keys there is no such row.)
+        // the tiles where rows see different keys, by every wave in its part of the tile (by each in all of it, 3 x 1111
+        // tokens with a window of 200 took 32.1 us and not 30.5, and 2000 with one of 100 21.4 and not 19.4).  (Rows past
+        // the last key are zeros, and where all rows see all keys there is no such row.)
         if (masked) {
             uint32_t odd = 0;
-#pragma unroll 2
-            for (int x = 0; x < kTile / 1024; ++x) {
-                const u32x4 w = *(const u32x4 *)(stage + kTile + x * 1024 + lane * 16);
+#pragma unroll
+            for (int x = 0; x < kBlk; ++x) {
+                const u32x4 w = *(const u32x4 *)(stage + kTile + (kBlk * wave + x) * 1024 + lane * 16);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) odd |= (w[e] & 0x7f807f80u) + 0x00800080u;
             }
-            if (__builtin_amdgcn_ballot_w64((odd & 0x80008000u) != 0)) { // the same for every wave: all scan the tile
+            if (__builtin_amdgcn_ballot_w64((odd & 0x80008000u) != 0) && lane == 0) *odd_tile = i;
+            wait_lgkmcnt0();
+            meet(); // (not __syncthreads, which waits for the DMA too)
+            if (*odd_tile == i) { // the same for every wave
                 // into the rows that give their keys a weight, then zeros in their place
                 bf16x8 ind[2];
 #pragma unroll
