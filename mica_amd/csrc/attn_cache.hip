@@ -550,18 +550,31 @@ __global__ __launch_bounds__(256) void ca_merge_kernel(CaParams p) {
     const int lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int f = (blockIdx.x % (kFrags / kPer)) * kPer + wave / W, u = blockIdx.x / (kFrags / kPer);
-    const int qb = u % p.nqb, hk = u / p.nqb % p.HK, b = u / p.nqb / p.HK;
+    const int qb = u % p.nqb, hk = u / p.nqb % p.HK;
+    int b = u / p.nqb / p.HK;
     const int q0 = qb * NB, row = f / (NDT * 4 * D) * 32 + l32;
-    const int tiles = Tiles<TREE>(p, key_count(p, b), q0, min(NB, p.Sq - q0)).n;
     int n, g0 = 0, per = 0, s = 0; // parts; STREAM: the run of the first, the runs' tiles, the sequence's first tile
     if constexpr (STREAM) {
         Stream<TREE> all(p);
-        per = all.per, s = all.first(p, b);
+        per = all.per;
+        int keys;
+        if (p.B > p.runs) { // the sequence in which run b + 1 begins, if no run before begins in it
+            const int at = (b + 1) * per;
+            if (at >= all.total) return;
+            int tile;
+            all.find(p, at, b, keys, tile);
+            s = at - tile;
+            if (tile <= p.begin || (s + p.begin) / per < at / per - 1) return;
+        } else {
+            keys = key_count(p, b);
+            s = all.first(p, b);
+        }
+        const int tiles = Tiles<TREE>(p, keys, q0, min(NB, p.Sq - q0)).n;
         g0 = (s + p.begin) / per;
         n = (s + p.begin + tiles - 1) / per - g0 + 1;
         if (n == 1) return; // its workgroup wrote it
     } else {
-        n = (tiles + p.chunk - 1) / p.chunk;
+        n = (Tiles<TREE>(p, key_count(p, b), q0, min(NB, p.Sq - q0)).n + p.chunk - 1) / p.chunk;
     }
     auto part = [&](int c) -> long long {
         if constexpr (STREAM) return 2 * ((long long)(g0 + c) * p.HK + hk) + ((g0 + c) * per < s);
@@ -694,7 +707,10 @@ int launch_as(const CaParams &p, const Plan &pl, hipStream_t st) {
     hipLaunchKernelGGL((ca_fwd_kernel<R, D, TREE, STREAM>), dim3((unsigned)pl.wgs), dim3(64 * R * D), 0, st, p);
     if (const int rc = mica_err(hipGetLastError())) return rc;
     if (pl.states == 0) return 0;
-    const long long blocks = (long long)p.B * p.HK * pl.nqb;
+    // STREAM: a sequence is divided where a run begins in it, so that there are no more of these than runs (every workgroup
+    // walks all the key counts: with workgroups for all sequences, 3000 tokens of up to 200 keys each took 2052 us and not 498)
+    const long long blocks = (long long)(STREAM && p.B > pl.runs ? pl.runs - 1 : p.B) * p.HK * pl.nqb;
+    if (blocks == 0) return 0;
     if (STREAM && pl.wide)
         hipLaunchKernelGGL((ca_merge_kernel<R, D, TREE, STREAM, STREAM ? 4 : 1>), dim3((unsigned)(blocks * 32 * R)), dim3(256), 0, st, p);
     else

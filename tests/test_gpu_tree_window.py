@@ -102,7 +102,7 @@ def test_tree_against_float64(gpu, B, N, HK, C, lens):
 
 
 @pytest.mark.parametrize("N", [3, 12, 30, 60])
-@pytest.mark.parametrize("B,C", [(130, 40), (70, 400), (9, 2900)])
+@pytest.mark.parametrize("B,C", [(130, 40), (70, 400), (9, 2900), (600, 50)])
 def test_tree_sequences_of_every_length_side_by_side(gpu, B, C, N):
     """Workgroups begin and end anywhere in the row of all sequences' keys: at a sequence's first tile, in its last, within
     the new keys."""
