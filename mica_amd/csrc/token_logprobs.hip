@@ -220,7 +220,7 @@ __global__ __launch_bounds__(kThreads, DT == MICA_FP32 ? 5 : 6) void lp_rows_ker
     using E = Elem<DT>;
     constexpr int kSize = 16 / E::N;
     __shared__ Stat red[kThreads / 64];
-    __shared__ float gmax[64];
+    __shared__ float gmax[kThreads / 2];
     __shared__ unsigned long long list[TOP ? kCap : 8];
     __shared__ u32x4 queue[TOP ? kQueue : 1];
     __shared__ int queue_at[TOP ? kQueue : 1];
@@ -310,12 +310,12 @@ __global__ __launch_bounds__(kThreads, DT == MICA_FP32 ? 5 : 6) void lp_rows_ker
         if constexpr (TOP) {
             forget();
             if (first) {
-                float g = mx;
-                g = __builtin_fmaxf(g, __shfl_xor(g, 1, 64));
-                g = __builtin_fmaxf(g, __shfl_xor(g, 2, 64));
-                if ((tid & 3) == 0) gmax[tid >> 2] = g;
+                // groups of lanes l and l + 32 of two waves: a short row fills as many as it has vectors (of four lanes side by
+                // side, 300 elements filled 10, and everything was a candidate: 8192 rows with 20 alternatives 155 us, not 54)
+                const float g = __builtin_fmaxf(mx, __shfl_xor(mx, 32, 64));
+                if ((tid & 32) == 0) gmax[(tid >> 6) * 32 + (tid & 31)] = g;
                 __syncthreads();
-                thr = value_of(nth_of_wave<E::kBits>(order_of(gmax[tid & 63]), p.top));
+                thr = value_of(nth_of_wave<E::kBits>(order_of(__builtin_fmaxf(gmax[tid & 63], gmax[64 + (tid & 63)])), p.top));
                 if (thr != thr) thr = -__builtin_inff(); // (the number below -inf's is a NaN's)
             }
             auto reaches = [&](float xv) { return above ? !(xv <= thr) : !(xv < thr); }; // (as a NaN does)
@@ -495,10 +495,12 @@ __global__ __launch_bounds__(kThreads) void lp_merge_kernel(LpParams p) {
     finish<DT>(p, row, a, list, tok);
 }
 
-// Workgroups a row, and blocks each: enough for the chip (256 CUs of six workgroups), whole blocks each.
-void divide(int T, int V, int elems, int &parts, int &bpp) {
+// Workgroups a row, and blocks each: enough for the chip (256 CUs of six workgroups), whole blocks each.  A row that is short,
+// or one of many, takes one workgroup and no join: up to 2 blocks with alternatives (which each block's candidates delay:
+// 500 x 9000 bf16 with 20 16.6 -> 10.9 us, but 260 x 24000 14.4 -> 15.4), up to 4 without (260 x 24000 12.3 -> 8.8).
+void divide(int T, int V, int elems, int top, int &parts, int &bpp) {
     const int blocks = max(1, (V / elems + kThreads * U - 1) / (kThreads * U));
-    const int want = T >= 1024 ? 1 : min((2048 + T - 1) / T, kMaxParts);
+    const int want = T >= 1024 || blocks <= (top ? 2 : 4) ? 1 : min((2048 + T - 1) / T, kMaxParts);
     bpp = (blocks + want - 1) / want;
     parts = (blocks + bpp - 1) / bpp;
 }
@@ -519,7 +521,7 @@ extern "C" long long mica_token_logprobs_workspace_bytes(int T, int V, int dtype
     if (dtype != MICA_BF16 && dtype != MICA_FP16 && dtype != MICA_FP32) return -1;
     if (T == 0) return 0;
     int parts, bpp;
-    divide(T, V, dtype == MICA_FP32 ? 4 : 8, parts, bpp);
+    divide(T, V, dtype == MICA_FP32 ? 4 : 8, top, parts, bpp);
     return part_bytes(T, parts, top);
 }
 
@@ -539,7 +541,7 @@ extern "C" int mica_token_logprobs(const void *logits, int dtype, long long ldx,
     LpParams p{};
     p.x = logits; p.ldx = ldx; p.tok = tokens; p.tok64 = tokens_64 != 0; p.T = T; p.V = V; p.C = C; p.top = top;
     p.lp = logprobs; p.ent = entropy; p.ids = top_ids; p.tlp = top_logprobs;
-    divide(T, V, 16 / size, p.parts, p.bpp);
+    divide(T, V, 16 / size, top, p.parts, p.bpp);
     const long long need = part_bytes(T, p.parts, top);
     if (need && (!workspace || !mica_aligned16(workspace) || workspace_bytes < need)) return MICA_MISS_ARG;
     if (V > (1 << 30) || (long long)T * p.parts >= (1LL << 31)) return MICA_MISS_RANGE;
