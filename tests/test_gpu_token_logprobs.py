@@ -106,6 +106,38 @@ def test_orders_that_bring_many_candidates(gpu, T, top):
     check(token_logprobs(x, tokens, top), x, tokens, top)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [40, 250, 1015, 1016, 1017, 1500, 2031, 2032, 2033, 2050])
+def test_short_rows(gpu, dtype, V):
+    """Rows of up to a few vectors a lane: ordinary ones, ties, -inf, rising and falling ones, at every alignment."""
+    T = 2060
+    x = rows(gpu, T, V + 1, dtype, V)[:, 1:]            # (rows V + 1 apart: each begins elsewhere)
+    up = torch.arange(V, device=gpu)
+    x[0], x[1], x[2], x[3] = 0.0, -math.inf, up // 9, -up // 9
+    x[4, 3:] = -math.inf
+    x[5], x[6] = torch.finfo(dtype).min, up % 2
+    x[7, ::5] = -math.inf
+    for top in (0, 1, 20, 32):
+        tokens = torch.randint(0, V, (T, 3), device=gpu)
+        out = token_logprobs(x, tokens, top)
+        assert torch.isnan(out.logprobs[1]).all() and out.top_ids[1].tolist() == list(range(top))
+        keep = [i for i in range(T) if i != 1]
+        check(type(out)(*(o[keep] for o in out)), x[keep], tokens[keep], top)
+
+
+@pytest.mark.parametrize("dtype,V", [(torch.bfloat16, 2100), (torch.bfloat16, 4064), (torch.float16, 4065), (torch.float32, 2032)])
+def test_many_short_rows(gpu, dtype, V):
+    T = 4099
+    x = rows(gpu, T, V, dtype, V)
+    up = torch.arange(V, device=gpu)
+    x[0], x[1], x[2], x[3] = 0.0, up % 2, up // 17, -up // 17
+    x[4, : V // 2] = -math.inf
+    x[5, V // 2:] = -math.inf
+    tokens = torch.randint(0, V, (T,), device=gpu)
+    for top in (0, 32):
+        check(token_logprobs(x, tokens, top), x, tokens, top)
+
+
 @pytest.mark.parametrize("T", [3, 1026])
 def test_a_nan_in_every_thread(gpu, T):
     V = 30000
