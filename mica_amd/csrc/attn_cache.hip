@@ -677,10 +677,11 @@ Plan plan(int B, int Sq, int HK, int max_tiles) {
     // The chunks that take the least time, in 1/20 us: a tile of a workgroup alone on its CU 30, beside another 44; with
     // several chunks the partial states (128 KB a workgroup) written and joined.  Counted as rounds of tiles, and 10 tiles
     // for the states, instead: 8 x 255 nodes after 300 keys 60.1 us, now 42.6; 2000 tokens with a window of 1000 60.6, now
-    // 50.5; 3 x 130 nodes after 3500 keys 53.9, now 53.1.  Up to 24 chunks (65 nodes after 32768 keys; with 16 94 us, now 78).
+    // 50.5; 3 x 130 nodes after 3500 keys 53.9, now 53.1.  Up to 64 chunks (65 nodes after 32768 keys: with 16 94
+    // us, with 24 88, now 78).
     const long long base = units * pl.nqb;
     long long best = -1;
-    for (int n = 1; n <= 24 && base > 0; ++n) {
+    for (int n = 1; n <= 64 && base > 0; ++n) {
         const long long tiles = (max_tiles + n - 1) / n, wgs = base * n, full = wgs / slots, rest = wgs % slots;
         const long long cost = tiles * (full * 44 + (rest > kCus ? 44 : rest ? 30 : 0)) + (n > 1 ? 180 + wgs * 17 / 20 : 0);
         if (best < 0 || cost < best) best = cost, pl.chunk = (int)tiles;
