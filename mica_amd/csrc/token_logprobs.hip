@@ -214,7 +214,7 @@ MICA_DEVICE Stat block_stat(Stat a, Stat *red) {
 
 // One pass over the row, bound by HBM without alternatives: 4096 x 151936 bf16 take 197 us, 6.3 TB/s; with 20 of them nearly
 // as much by VALU issue, 2048 rows 130 us, 4.8 TB/s.  Rows of a block or two are bound by their latency (load, threshold,
-// candidates, join): 64 x 151936 fp32 with 20 alternatives 19.7 us, without 12; one row 11.
+// candidates, join): 64 x 151936 fp32 with 20 alternatives 19.3 us, without 12; one row 11.
 // (six workgroups a CU; five leave fp32 the registers that it would spill: 1024 x 151936 with 20 alternatives 117.5 -> 107.9 us)
 template <int DT, bool TOP, int NT>
 __global__ __launch_bounds__(NT, DT == MICA_FP32 ? 5 : 6) void lp_rows_kernel(LpParams p) {
