@@ -20,11 +20,14 @@
 //
 // Up to 64 query positions, one row block takes them all, and the key tiles of all sequences, one after the other, are
 // divided evenly over the chip's workgroups (STREAM): a workgroup may end one sequence and begin the next, so
-// key counts that differ, or sequences that do not divide the chip, leave no CU idle.  In that row each sequence has a few
+// key counts that differ, or sequences that do not divide the chip, leave no CU idle.  Many or short sequences have a
+// workgroup each.  In that row each sequence has a few
 // empty tiles before its own, for the time its beginning takes.  More positions take a workgroup
 // for each block, their tiles divided into chunks where that leaves too few.  ca_merge_kernel joins the partial softmax
 // states (fp32) of what was divided.
 #include "attn_common.h"
+
+#include <algorithm>
 
 namespace {
 
@@ -206,7 +209,11 @@ __global__ __launch_bounds__(64 * R * D, 2) void ca_fwd_kernel(CaParams p) {
     const int rb = wave / D, dt0 = (wave % D) * NDT;
     int b, hk, qb = 0, i0, keys, left = 0; // the sequence, head, query block, first tile here, keys; tiles left (STREAM)
     int blk;                         // where its partial state goes
-    if constexpr (STREAM) {
+    if (STREAM && p.runs == 0) { // a whole sequence
+        hk = blockIdx.x % p.HK, b = blockIdx.x / p.HK, i0 = 0, blk = 0;
+        keys = key_count(p, b);
+        left = Tiles<TREE>(p, keys, 0, p.Sq).n;
+    } else if constexpr (STREAM) {
         Stream<TREE> all(p);
         hk = blockIdx.x % p.HK;
         const int at = blockIdx.x / p.HK * all.per;
@@ -637,7 +644,7 @@ __global__ __launch_bounds__(256) void ca_merge_kernel(CaParams p) {
 // How a call is divided: row blocks (R) and dim parts (D) of a workgroup, and the work.
 struct Plan {
     int R, D, nqb, gq, chunk, nchunk;
-    int runs, dense, least; // STREAM: most runs of tiles; the tiles of a run below which half as many are made; its fewest
+    int runs, dense, least; // STREAM: most runs of tiles (0: every sequence whole); the tiles of a run below which half as many are made; its fewest
     int begin;              // the tiles that a sequence's beginning counts for
     bool stream, wide;
     long long tiles, wgs, states; // STREAM: a head's tiles; workgroups; partial rows
@@ -653,6 +660,15 @@ Plan plan(int B, int Sq, int HK, int max_tiles) {
     pl.chunk = max_tiles, pl.nchunk = 1;
     const int slots = kCus * (pl.R < 8 ? 2 : 1);
     const long long units = (long long)B * HK;
+    // A workgroup a sequence and head, undivided, where those are many or short: no state to write and join, no sequence
+    // begun behind another's end.  The longest of a batch is then waited for, so up to as many tiles as the whole batch, at
+    // full length, takes all workgroups twice over at most.  Divided / whole, us (nodes, sequences x keys): 4, 1 x 60 13.2 /
+    // 8.9, 32 x 1000 31.9 / 42.4, 64 x 500 43.7 / 32.0, 200 x 3500 394 / 362; 16, 32 x 1000 40.8 / 45.0, 64 x 500 43.0 / 35.0;
+    // 32, 32 x 1000 51.5 / 47.7, 600 x 800 554 / 423; 64, 8 x 250 30.4 / 26.1, 64 x 2000 179 / 139.
+    if (pl.stream && max_tiles <= std::max(10ll, 10ll * std::max(pl.R, 2) * (units / 128))) {
+        pl.wgs = units;
+        return pl;
+    }
     if (pl.stream) {
         // Two workgroups a CU, while each gets enough tiles to repay the partial state that it writes (32 R KB) and the merge
         // reads (R = 1: 8, else 12); else one, of 4 tiles at least, and of fewer only where even so the chip would be nearly

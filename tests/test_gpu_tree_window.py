@@ -114,6 +114,20 @@ def test_tree_sequences_of_every_length_side_by_side(gpu, B, C, N):
     check(o, q, torch.cat((kc, k), 1), torch.cat((vc, v), 1), tree_sees(par, lens, C, gpu))
 
 
+@pytest.mark.parametrize("N", [3, 12])
+def test_tree_a_few_long_sequences_among_many(gpu, N):
+    """More sequences than runs of key tiles: most lie within a run, the long ones are divided over many."""
+    B, C = 140, 2700
+    q, k, v, kc, vc = heads(gpu, N, B, N, 4, C)
+    g = torch.Generator().manual_seed(N)
+    lens = torch.randint(0, 70, (B,), generator=g).tolist()
+    for b in (0, 63, 64, 100, 101, 139):
+        lens[b] = C - b
+    par = [random_parents(N, b) for b in range(B)]
+    o = tree_attention(q, k, v, tree_masks(par, gpu), (kc, vc), torch.tensor(lens, dtype=torch.int32, device=gpu))
+    check(o, q, torch.cat((kc, k), 1), torch.cat((vc, v), 1), tree_sees(par, lens, C, gpu))
+
+
 def test_tree_shared_cache_one_tree_and_scale(gpu):
     q, k, v, kc, vc = heads(gpu, 3, 4, 20, 4, 777)
     par = random_parents(20, 5)
