@@ -516,18 +516,29 @@ void divide(int T, int V, int elems, int top, int &parts, int &bpp) {
 }
 long long part_bytes(int T, int parts, int top) { return parts > 1 ? (long long)T * parts * (16 + 8 * top) : 0; }
 
+// Rows of one launch: a grid of 2^32 work-items or more wraps round without an error, and the rows behind it were not written.
+constexpr int kGridRows = 1 << 23;
+
 template <int DT>
-void launch(LpParams &p, hipStream_t st) {
-    const dim3 grid((unsigned)((long long)p.T * p.parts));
+void launch(LpParams p, hipStream_t st) {
+    constexpr int kSize = 16 / Elem<DT>::N;
     // A row of one block of 64 threads (two, where rows are so many that they wait for each other) takes a wave: 8192 x 300
     // bf16 with 20 alternatives 53.6 -> 23.9 us, 8192 x 4000 44.5 -> 36.1; but two blocks of 2000 x 4000 15.2 / 17.2.
     const bool wave = p.parts == 1 && p.V <= ((p.T >= 4096 ? 2 : 1) * 64 * U - 2) * Elem<DT>::N;
     if (wave) p.bpp *= kThreads / 64;
-    if (p.top > 0 && wave) hipLaunchKernelGGL((lp_rows_kernel<DT, true, 64>), grid, dim3(64), 0, st, p);
-    else if (p.top > 0) hipLaunchKernelGGL((lp_rows_kernel<DT, true, kThreads>), grid, dim3(kThreads), 0, st, p);
-    else if (wave) hipLaunchKernelGGL((lp_rows_kernel<DT, false, 64>), grid, dim3(64), 0, st, p);
-    else hipLaunchKernelGGL((lp_rows_kernel<DT, false, kThreads>), grid, dim3(kThreads), 0, st, p);
-    if (p.parts > 1) hipLaunchKernelGGL((lp_merge_kernel<DT>), dim3(p.T), dim3(kThreads), 0, st, p);
+    for (int left = p.T; left > 0; left -= kGridRows) { // (rows of several parts are few)
+        p.T = min(left, kGridRows);
+        const dim3 grid((unsigned)(p.T * p.parts));
+        if (p.top > 0 && wave) hipLaunchKernelGGL((lp_rows_kernel<DT, true, 64>), grid, dim3(64), 0, st, p);
+        else if (p.top > 0) hipLaunchKernelGGL((lp_rows_kernel<DT, true, kThreads>), grid, dim3(kThreads), 0, st, p);
+        else if (wave) hipLaunchKernelGGL((lp_rows_kernel<DT, false, 64>), grid, dim3(64), 0, st, p);
+        else hipLaunchKernelGGL((lp_rows_kernel<DT, false, kThreads>), grid, dim3(kThreads), 0, st, p);
+        if (p.parts > 1) hipLaunchKernelGGL((lp_merge_kernel<DT>), dim3(p.T), dim3(kThreads), 0, st, p);
+        const long long n = p.T;
+        p.x = (const char *)p.x + n * p.ldx * kSize;
+        p.tok = (const char *)p.tok + n * p.C * (p.tok64 ? 8 : 4);
+        p.lp += n * p.C, p.ent += n, p.ids += n * p.top, p.tlp += n * p.top;
+    }
 }
 
 }  // namespace

@@ -1,0 +1,23 @@
+"""The scoring operators at the ends of their ranges."""
+import pytest
+import torch
+
+from mica_amd.readout import token_logprobs
+
+pytestmark = pytest.mark.gpu
+
+
+def test_more_rows_than_a_grid_holds(gpu):
+    """2^26 workgroups of 64 threads are 2^32 work-items, one more than a grid may have."""
+    T = 2 ** 26 + 5
+    x = torch.zeros(T, 2, dtype=torch.bfloat16, device=gpu)
+    x[:, 1] = (torch.arange(T, device=gpu) % 97).to(torch.bfloat16) / 16 - 3
+    tokens = (torch.arange(T, device=gpu) % 2).int()
+    out = token_logprobs(x, tokens, 1)
+    lp = torch.log_softmax(x[:97].double(), 1).tile(T // 97 + 1, 1)[:T]
+    want = torch.where(tokens == 0, lp[:, 0], lp[:, 1])
+    # two terms: a few fp32 steps of values below 4
+    assert ((out.logprobs.double() - want).abs() <= 2 ** -20).all()
+    assert torch.equal(out.top_ids[:, 0], (x[:, 1] > 0).long())
+    assert ((out.top_logprobs[:, 0].double() - lp.amax(1)).abs() <= 2 ** -20).all()
+    assert ((out.entropy.double() + (lp.exp() * lp).sum(1)).abs() <= 2 ** -20).all()
