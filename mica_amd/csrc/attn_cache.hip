@@ -694,10 +694,11 @@ Plan plan(int B, int Sq, int HK, int max_tiles) {
     // several chunks the partial states (128 KB a workgroup) written and joined.  Counted as rounds of tiles, and 10 tiles
     // for the states, instead: 8 x 255 nodes after 300 keys 60.1 us, now 42.6; 2000 tokens with a window of 1000 60.6, now
     // 50.5; 3 x 130 nodes after 3500 keys 53.9, now 53.1.  Up to 64 chunks (65 nodes after 32768 keys: with 16 94
-    // us, with 24 88, now 78).
+    // us, with 24 88, now 78).  Never so many workgroups that a grid, here or of the join (8 R workgroups a block), would reach
+    // 2^32 work-items: it would wrap round without an error.
     const long long base = units * pl.nqb;
     long long best = -1;
-    for (int n = 1; n <= 64 && base > 0; ++n) {
+    for (int n = 1; n <= 64 && base > 0 && (n == 1 || base * n < (1 << 20)); ++n) {
         const long long tiles = (max_tiles + n - 1) / n, wgs = base * n, full = wgs / slots, rest = wgs % slots;
         const long long cost = tiles * (full * 44 + (rest > kCus ? 44 : rest ? 30 : 0)) + (n > 1 ? 180 + wgs * 17 / 20 : 0);
         if (best < 0 || cost < best) best = cost, pl.chunk = (int)tiles;
