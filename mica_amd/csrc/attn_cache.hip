@@ -492,14 +492,16 @@ __global__ __launch_bounds__(64 * R * D, 2) void ca_fwd_kernel(CaParams p) {
     }
     wait_vmcnt<0>();  // the last (empty) loads have written before the stages are used again or given up
     float ltot = half_swap_sum(lsum);
-    uint32_t any = 1;
+    // A row that sees no key (a tree node without a bit, a position before the first key) has zeros, and -1 in the place of
+    // its sum.  One that sees keys has a sum of 0 only where all their scores are -inf: no softmax, 0 / 0.
+    uint32_t sees = pos >= 0;
     if constexpr (TREE) {
-        any = 0;
+        sees = 0;
 #pragma unroll 1
-        for (int w = 0; w < p.tw; ++w) any |= words[row % NB * p.tw + w];
+        for (int w = 0; w < p.tw; ++w) sees |= words[row % NB * p.tw + w];
     }
-    if (any == 0) { // a tree node without a bit (its cached keys were computed like the others': nothing of them leaves)
-        m = -__builtin_inff(), ltot = 0.0f;
+    if (sees == 0) { // (a node's cached keys were computed like the others': nothing of them leaves)
+        m = -__builtin_inff(), ltot = -1.0f;
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) O[dt] = f32x16{};
     }
@@ -514,7 +516,7 @@ __global__ __launch_bounds__(64 * R * D, 2) void ca_fwd_kernel(CaParams p) {
         if (dt0 == 0 && hi == 0) p.part_ml[(long long)blk * (32 * R) + row] = float2{m, ltot};
     } else {
         // ---- normalise, stage in LDS (32 R rows x 512 B), write 16-byte row pieces ----
-        const float inv = ltot == 0.0f ? 0.0f : 1.0f / ltot;
+        const float inv = ltot < 0.0f ? 0.0f : 1.0f / ltot;
         __syncthreads();
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt)
@@ -589,7 +591,7 @@ __global__ __launch_bounds__(256) void ca_merge_kernel(CaParams p) {
     };
     float mx = -__builtin_inff(), l = 0.0f;
     float4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    // a row that no part has keys for: weights 1 on zeros (a sum that is NaN stays one)
+    // no part has a key that counts: weights 1 on zeros (a sum that is NaN or -1 stays so)
     auto weight = [](float m, float top) { return top == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - top); };
     auto add = [&](float w, float2 ml, float4 o) {
         l += w * ml.y;
@@ -631,7 +633,7 @@ __global__ __launch_bounds__(256) void ca_merge_kernel(CaParams p) {
     }
     const int t = q0 + row % NB;
     if (t >= p.Sq) return;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    const float inv = l < 0.0f ? 0.0f : 1.0f / l; // (a row that sees no key: the parts' -1)
     const int fr = f % (NDT * 4), dt = f / (NDT * 4) % D * NDT + fr / 4, d = dt * 32 + 8 * (fr % 4) + 4 * hi;
     u32x2 w;
     w[0] = pack_bf16x2(acc.x * inv, acc.y * inv);
