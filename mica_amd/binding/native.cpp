@@ -524,8 +524,9 @@ PyObject *py_token_logprobs(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
     const Tensor *x, *tok;
     Call c;
     if (!plain(a[0], &x) || !plain(a[1], &tok) || !PyLong_CheckExact(a[2]) || !enter(*x, c)) return none();
-    const long top = PyLong_AsLong(a[2]);
-    if (PyErr_Occurred()) return nullptr;
+    int over = 0;
+    const long top = PyLong_AsLongAndOverflow(a[2], &over);
+    if (over) return none();
     const int dt = code(x->scalar_type());
     const at::ScalarType tt = tok->scalar_type();
     if (x->dim() != 2 || dt < 0 || x->stride(1) != 1 || (tt != at::kLong && tt != at::kInt) || !on(c, *tok) ||

@@ -21,3 +21,10 @@ def test_more_rows_than_a_grid_holds(gpu):
     assert torch.equal(out.top_ids[:, 0], (x[:, 1] > 0).long())
     assert ((out.top_logprobs[:, 0].double() - lp.amax(1)).abs() <= 2 ** -20).all()
     assert ((out.entropy.double() + (lp.exp() * lp).sum(1)).abs() <= 2 ** -20).all()
+
+
+def test_a_top_that_no_int_holds(gpu):
+    x, tokens = torch.zeros(2, 50, device=gpu), torch.zeros(2, dtype=torch.long, device=gpu)
+    for top in (2 ** 40, 2 ** 70, -2 ** 70):
+        with pytest.raises(ValueError):
+            token_logprobs(x, tokens, top)
