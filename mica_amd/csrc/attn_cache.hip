@@ -66,13 +66,15 @@ MICA_DEVICE int key_count(const CaParams &p, int b) { return p.len ? min(max(p.l
 template <bool TREE>
 struct Tiles {
     int n, n0, skip; // tiles; of them cached (tree) or before the window (window); tiles skipped after those (window)
+    int end;         // the new keys (tree); the keys up to the block's last position (window)
     MICA_DEVICE Tiles(const CaParams &p, int keys, int q0, int rows) {
         if constexpr (TREE) {
             n0 = (keys + kBK - 1) / kBK;
             n = n0 + (p.Sq + kBK - 1) / kBK;
-            skip = 0;
+            skip = 0, end = p.Sq;
         } else {
             const int first = keys - p.Sq + q0, last = first + rows - 1; // positions of the block's queries
+            end = max(last + 1, 0);
             if (last < 0) { // no key: one tile that nothing is read for, so that the zeros are written
                 n = 1, n0 = skip = 0;
                 return;
@@ -266,7 +268,7 @@ __global__ __launch_bounds__(64 * R * D, 2) void ca_fwd_kernel(CaParams p) {
             const int j = TREE ? i - tl.n0 : tl.tile(i);
             kb = p.k + b * p.sbk + hk * p.shk + (long long)j * kBK * ldk;
             vb = p.v + b * p.sbv + hk * p.shv + (long long)j * kBK * ldv;
-            rows = (TREE ? p.Sq : keys) - j * kBK;
+            rows = tl.end - j * kBK;
         }
         rows = i < i1 ? min(rows, kBK) : 0;
         const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
