@@ -395,12 +395,13 @@ __global__ __launch_bounds__(64 * R * D, 2) void ca_fwd_kernel(CaParams p) {
             }
         } else {
             const int k0 = tl.tile(i) * kBK, first = keys - p.Sq + q0;
-            masked = k0 + kBK - 1 > first || (k0 <= first + NB - 1 - p.window && k0 + kBK > p.sinks);
+            // (differences of positions, which are small: a window up to the largest int would overflow taken from one)
+            masked = k0 + kBK - 1 > first || (first + NB - 1 - k0 >= p.window && k0 + kBK > p.sinks);
             if (masked) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const int key = k0 + 8 * (r >> 2) + 4 * hi + (r & 3);
-                    const bool sees = key <= pos && (key > pos - p.window || key < p.sinks);
+                    const bool sees = key <= pos && (pos - key < p.window || key < p.sinks);
                     sc[r] = sees ? sc[r] : -__builtin_inff();
                 }
             }
@@ -714,7 +715,7 @@ Plan plan(int B, int Sq, int HK, int max_tiles) {
     return pl;
 }
 
-int tree_tiles(int N, int cap) { return (cap + kBK - 1) / kBK + (N + kBK - 1) / kBK; }
+int tree_tiles(int N, int cap) { return (int)((cap + (kBK - 1ll)) / kBK) + (N + kBK - 1) / kBK; }
 // most tiles of a block of Sq <= 64 or 32 queries: the sinks', the window's and the block's own, never more than the keys'
 int window_tiles(int Sq, int Sk, int window, int sinks) {
     const long long all = Sk > 0 ? ((long long)Sk + kBK - 1) / kBK : 1;

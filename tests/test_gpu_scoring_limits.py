@@ -5,6 +5,7 @@ import pytest
 import torch
 from test_gpu_tree_window import check, heads, window_sees
 
+from mica_amd import _lib
 from mica_amd.attention import window_attention
 from mica_amd.readout import token_logprobs
 
@@ -49,3 +50,20 @@ def test_window_blocks_before_the_first_key(gpu, n, lens):
     assert torch.isinf(o[0, -1]).all() and torch.isfinite(o[0, :-1]).all()
     for b, length in enumerate(lens):
         assert not o[b, :n - length].any()
+
+
+@pytest.mark.parametrize("n", [5, 100])
+def test_a_window_of_the_largest_int(gpu, n):
+    """Through the C entry, which does not cut it to the keys: positions before the first key, and window and sinks beyond."""
+    q, _, _, k, v = heads(gpu, 9 + n, 2, n, 4, 300)
+    lens = [300, n // 2]
+    t = torch.tensor(lens, dtype=torch.int32, device=gpu)
+    L, big = _lib.load(), 2 ** 31 - 1
+    for window, sinks in ((big, 0), (big, big), (2, big)):
+        o = torch.empty_like(q, memory_format=torch.contiguous_format)
+        need = L.mica_attention_window_workspace_bytes(2, n, 300, 4, window, sinks)
+        ws = torch.empty(max(need, 16), dtype=torch.uint8, device=gpu)
+        st = lambda x: (x.data_ptr(), x.stride(0), x.stride(2), x.stride(1))  # noqa: E731
+        assert L.mica_attention_window(*st(q), *st(k), *st(v), *st(o), 2, n, 300, 16, 4, 256, 1 / 16, window, sinks, t.data_ptr(),
+                                       ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream) == 0
+        check(o, q, k, v, window_sees(2, n, 300, big, 0, lens, gpu))
