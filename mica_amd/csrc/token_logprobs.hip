@@ -484,23 +484,13 @@ __global__ __launch_bounds__(kThreads) void lp_merge_kernel(LpParams p) {
             least = (unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(own >> 32), l) << 32 |
                     (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)own, l);
         }
+        // At most top^2 keys reach it: with up to top parts there are no more; with more parts r is 1 and want is top, so
+        // want - 1 parts have keys above `least`, and one more has it.
+        static_assert(kMaxTop * kMaxTop <= kCap<kThreads>, "the keys that reach the bound fit the list");
         for (int i = tid; i < n; i += kThreads)
-            if (all[i] >= least && all[i] != 0) {
-                const int at = atomicAdd(&count, 1);
-                if (at < kCap<kThreads>) list[at] = all[i];
-            }
+            if (all[i] >= least && all[i] != 0) list[atomicAdd(&count, 1)] = all[i];
         __syncthreads();
-        const int c = count;
-        if (c <= kCap<kThreads>) {
-            keep_best<true, kThreads>(list, c, p.top);
-        } else { // (parts of ascending values)  rank among all keys
-            for (int i = tid; i < n; i += kThreads) {
-                int k = 0;
-                for (int j = 0; j < n; ++j) k += all[j] > all[i];
-                if (k < p.top && all[i] != 0) list[k] = all[i];
-            }
-            __syncthreads();
-        }
+        keep_best<true, kThreads>(list, count, p.top);
     }
     finish<DT, kThreads>(p, row, a, list, tok);
 }

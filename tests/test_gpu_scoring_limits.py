@@ -67,3 +67,23 @@ def test_a_window_of_the_largest_int(gpu, n):
         assert L.mica_attention_window(*st(q), *st(k), *st(v), *st(o), 2, n, 300, 16, 4, 256, 1 / 16, window, sinks, t.data_ptr(),
                                        ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream) == 0
         check(o, q, k, v, window_sees(2, n, 300, big, 0, lens, gpu))
+
+
+@pytest.mark.parametrize("top", [1, 5, 31, 32])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("parts", [2, 7, 31, 32, 33, 64])
+def test_the_join_of_every_order_of_parts(gpu, parts, dtype, top):
+    """Parts of one block each (16 KB) whose best keys rise, fall, lie in one part or one in each; the last part with all its
+    keys, one, or none of its own but the row's end."""
+    block = 16384 // dtype.itemsize
+    for V in (parts * block, (parts - 1) * block + 8, (parts - 1) * block + 8 + 3):
+        at = torch.arange(V, device=gpu)
+        x = torch.randn(5, V, generator=torch.Generator(device=gpu).manual_seed(parts), device=gpu)
+        x[0] += at // block * 8                                # rising by parts
+        x[1] -= at // block * 8
+        x[2, V // 2:V // 2 + 40] += 20                         # one part has them all (or two)
+        x[3, ::block] += 20                                    # one in each
+        x[4] = torch.where(at // block % 3 == 1, -math.inf, x[4])
+        x = x.to(dtype)
+        out = token_logprobs(x, at[:5], top)
+        assert torch.equal(out.top_ids, torch.sort(x, dim=1, descending=True, stable=True).indices[:, :top])
