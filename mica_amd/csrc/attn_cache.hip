@@ -241,312 +241,312 @@ __global__ __launch_bounds__(64 * R * D, 2) void ca_fwd_kernel(CaParams p) {
         keys = key_count(p, b);
     }
     for (;;) {
-    // what depends on the lane alone is made here, from an opaque copy of its id: the compiler would make it before the
-    // loop and hold it in registers that the tiles need (45 of them spilled)
-    int tid = threadIdx.x;
-    __asm__ volatile("" : "+v"(tid));
-    const int lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
-    const int q0 = qb * NB;
-    const Tiles<TREE> tl(p, keys, q0, min(NB, p.Sq - q0));
-    const int i1 = min(STREAM ? i0 + left : i0 + p.chunk, tl.n);
-    if (!STREAM && i0 >= tl.n) return;
-    const bool whole = STREAM ? i0 == 0 && i1 == tl.n : p.nchunk == 1;
+        // what depends on the lane alone is made here, from an opaque copy of its id: the compiler would make it before the
+        // loop and hold it in registers that the tiles need (45 of them spilled)
+        int tid = threadIdx.x;
+        __asm__ volatile("" : "+v"(tid));
+        const int lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
+        const int q0 = qb * NB;
+        const Tiles<TREE> tl(p, keys, q0, min(NB, p.Sq - q0));
+        const int i1 = min(STREAM ? i0 + left : i0 + p.chunk, tl.n);
+        if (!STREAM && i0 >= tl.n) return;
+        const bool whole = STREAM ? i0 == 0 && i1 == tl.n : p.nchunk == 1;
 
-    // this lane's row: a position and a query head
-    const int row = rb * 32 + l32, head = hk * kGroup + row / NB, t = q0 + row % NB;
-    // DMA of tile i into stage st; past i1 from a zero-sized buffer, so that every step issues as many instructions
-    auto issue = [&](int i, int st) {
-        const uint16_t *kb, *vb;
-        long long ldk = p.ldk, ldv = p.ldv;
-        int rows;
-        if (TREE && i < tl.n0) {
-            ldk = p.ldkc, ldv = p.ldvc;
-            kb = p.kc + b * p.sbkc + hk * p.shkc + (long long)i * kBK * ldk;
-            vb = p.vc + b * p.sbvc + hk * p.shvc + (long long)i * kBK * ldv;
-            rows = keys - i * kBK;
-        } else {
-            const int j = TREE ? i - tl.n0 : tl.tile(i);
-            kb = p.k + b * p.sbk + hk * p.shk + (long long)j * kBK * ldk;
-            vb = p.v + b * p.sbv + hk * p.shv + (long long)j * kBK * ldv;
-            rows = tl.end - j * kBK;
-        }
-        rows = i < i1 ? min(rows, kBK) : 0;
-        const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
-            (void *)kb, 0, rows > 0 ? (int)((rows - 1) * ldk * 2) + kD * 2 : 0, kBufferFlags);
-        const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
-            (void *)vb, 0, rows > 0 ? (int)((rows - 1) * ldv * 2) + kD * 2 : 0, kBufferFlags);
-        // 1 KB block x = key rows 2 x + hi; chunk c of row r lies at c ^ (r % 16) (K), c ^ 4 (r % 4) (V).  The offsets
-        // come from an opaque copy of the lane id at every tile: hoisted out of the loop they take 16 registers, and
-        // what these push into scratch is then loaded back behind the DMA, which every such load waits for.
-        int ln = lane;
-        __asm__ volatile("" : "+v"(ln));
-        const int r0 = 2 * kBlk * wave + (ln >> 5), k2 = (int)(ldk * 2), v2 = (int)(ldv * 2);
-        const int rk0 = r0 * k2, rv0 = r0 * v2;
-        int8_t *s = smem + st * kStage + kBlk * wave * 1024;
+        // this lane's row: a position and a query head
+        const int row = rb * 32 + l32, head = hk * kGroup + row / NB, t = q0 + row % NB;
+        // DMA of tile i into stage st; past i1 from a zero-sized buffer, so that every step issues as many instructions
+        auto issue = [&](int i, int st) {
+            const uint16_t *kb, *vb;
+            long long ldk = p.ldk, ldv = p.ldv;
+            int rows;
+            if (TREE && i < tl.n0) {
+                ldk = p.ldkc, ldv = p.ldvc;
+                kb = p.kc + b * p.sbkc + hk * p.shkc + (long long)i * kBK * ldk;
+                vb = p.vc + b * p.sbvc + hk * p.shvc + (long long)i * kBK * ldv;
+                rows = keys - i * kBK;
+            } else {
+                const int j = TREE ? i - tl.n0 : tl.tile(i);
+                kb = p.k + b * p.sbk + hk * p.shk + (long long)j * kBK * ldk;
+                vb = p.v + b * p.sbv + hk * p.shv + (long long)j * kBK * ldv;
+                rows = tl.end - j * kBK;
+            }
+            rows = i < i1 ? min(rows, kBK) : 0;
+            const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
+                (void *)kb, 0, rows > 0 ? (int)((rows - 1) * ldk * 2) + kD * 2 : 0, kBufferFlags);
+            const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
+                (void *)vb, 0, rows > 0 ? (int)((rows - 1) * ldv * 2) + kD * 2 : 0, kBufferFlags);
+            // 1 KB block x = key rows 2 x + hi; chunk c of row r lies at c ^ (r % 16) (K), c ^ 4 (r % 4) (V).  The offsets
+            // come from an opaque copy of the lane id at every tile: hoisted out of the loop they take 16 registers, and
+            // what these push into scratch is then loaded back behind the DMA, which every such load waits for.
+            int ln = lane;
+            __asm__ volatile("" : "+v"(ln));
+            const int r0 = 2 * kBlk * wave + (ln >> 5), k2 = (int)(ldk * 2), v2 = (int)(ldv * 2);
+            const int rk0 = r0 * k2, rv0 = r0 * v2;
+            int8_t *s = smem + st * kStage + kBlk * wave * 1024;
 #pragma unroll
-        for (int x = 0; x < kBlk; ++x)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void *)(s + x * 1024), 16,
-                                                     rk0 + 2 * x * k2 + (((ln & 31) ^ ((r0 + 2 * x) & 15)) << 4), 0, 0, 0);
+            for (int x = 0; x < kBlk; ++x)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void *)(s + x * 1024), 16,
+                                                         rk0 + 2 * x * k2 + (((ln & 31) ^ ((r0 + 2 * x) & 15)) << 4), 0, 0, 0);
 #pragma unroll
-        for (int x = 0; x < kBlk; ++x)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void *)(s + kTile + x * 1024), 16,
-                                                     rv0 + 2 * x * v2 + (((ln & 31) ^ (((r0 + 2 * x) & 3) << 2)) << 4), 0,
-                                                     0, 0);
-    };
-    // The block's words and this lane's Q fragments (B operand of S^T: dims 16 s + 8 hi .. + 7 of the row) come before the
-    // first tile: loads end in order.
-    constexpr int kMine = (kWords + kThreads - 1) / kThreads;
-    uint32_t mine[TREE ? kMine : 1];
-    if constexpr (TREE) {
-#pragma unroll
-        for (int x = 0; x < kMine; ++x) {
-            const int i = tid + x * kThreads, node = q0 + i / p.tw;
-            mine[x] = i < NB * p.tw && node < p.Sq ? p.tree[b * p.sbt + (long long)node * p.tw + i % p.tw] : 0u;
-        }
-    }
-    bf16x8 qf[kD / 16];
-    {
-        // (rows past the last position repeat it: they are not stored)
-        const uint16_t *qr = p.q + b * p.sbq + head * p.shq + (long long)min(t, p.Sq - 1) * p.ldq + hi * 8;
-#pragma unroll
-        for (int s = 0; s < kD / 16; ++s) qf[s] = __builtin_bit_cast(bf16x8, *(const u32x4 *)(qr + s * 16));
-    }
-    __builtin_amdgcn_sched_barrier(0);
-    issue(i0, 0);
-    if constexpr (TREE) {
-#pragma unroll
-        for (int x = 0; x < kMine; ++x) {
-            const int i = tid + x * kThreads, left = p.Sq - 32 * (i % p.tw); // bits past the last node do not count
-            if (i < NB * p.tw) words[i] = left >= 32 ? mine[x] : left <= 0 ? 0u : mine[x] & ((1u << left) - 1u);
-        }
-    }
-    if (tid == 0) *odd_tile = -1;
-    wait_lgkmcnt0(); // seen by every wave after the first tile's barrier
-    f32x16 O[NDT];
-#pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) O[dt] = f32x16{};
-    float m = -__builtin_inff(), lsum = 0.0f;
-    const int pos = keys - p.Sq + t; // window: this row's position
-
-    // V^T fragment of 32-dim tile dt, step s: keys 16 s + 4 hi .. + 3 and 16 s + 8 + 4 hi .. + 3 (the keys of P^T's
-    // accumulator rows 8 s .. 8 s + 7) of dim 32 dt + l % 32.  The lane's address: key row 4 hi + (l % 16) / 4, dims
-    // 16 ((l / 16) % 2) + 4 (l % 4); chunk c of row r lies at c ^ 4 (r % 4), which spreads the 4 rows x 64 bytes of
-    // each half of a read over all banks (c ^ 2 (r % 8) spreads all 8 rows, but a half over half of the banks: it cost 1.3
-    // conflict cycles an LDS instruction, 1% of the time).
-    const int vrow = 4 * hi + ((l32 & 15) >> 2);
-    const uint32_t vbase = lds0 + kTile + vrow * (kD * 2) + (((2 * (l32 >> 4) + ((l32 & 3) >> 1)) ^ ((vrow & 3) << 2) ^ (4 * dt0)) << 4) +
-                           (l32 & 1) * 8;
-    // K fragment s: chunk 2 s + hi of key row l % 32, at chunk ^ (l % 16).  The chunk's five bits are address bits of
-    // their own in both tiles, so a fragment's address is one exclusive or away from its stage's.
-    const uint32_t kbase = lds0 + l32 * (kD * 2) + ((hi ^ (l32 & 15)) << 4);
-    typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
-    auto kfrag = [](uint32_t stage, int s) { // stage: kbase + the stage's offset
-        return __builtin_bit_cast(bf16x8, *(lds_u32x4 *)(uintptr_t)((stage ^ (s << 5))));
-    };
-    auto vfrag = [](uint32_t stage, int s, int dt) { // stage: vbase + the stage's offset
-        const uint32_t a = (stage ^ (dt << 6)) + s * 16 * (kD * 2);
-        const s16x4 x = tr_read((lds_s16x4 *)(uintptr_t)a, (lds_void *)smem);
-        const s16x4 y = tr_read((lds_s16x4 *)(uintptr_t)(a + 8 * (kD * 2)), (lds_void *)smem);
-        return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-    };
-
-#pragma unroll 1
-    for (int i = i0; i < i1; ++i) {
-        const int st = (i - i0) & 1;
-        // this wave's DMA of tile i landed; after the barrier every wave's has, and nobody reads tile i - 1 any more
-        wait_vmcnt<0>();
-        meet();
-        __builtin_amdgcn_sched_barrier(0);
-        issue(i + 1, 1 - st);
-        if constexpr (TREE && !STREAM) { // new keys that none of the block's nodes sees, as those after them (2 x 500 nodes
-                                         // after 500 keys 58.4 -> 45.8 us; up to 64 nodes there are hardly any)
-            if (i >= tl.n0 && !__builtin_amdgcn_ballot_w64(words[lane % NB * p.tw + (i - tl.n0)])) continue;
-        }
-        const int8_t *stage = smem + st * kStage;
-        const uint32_t ks = kbase + st * kStage, vs = vbase + st * kStage;
-        // ---- S^T = K Q^T: rows = keys of the tile, column = this lane's row; fragments read kPf steps ahead ----
-        f32x16 sc = {};
-        __builtin_amdgcn_s_setprio(1);
-        bf16x8 kf[kPf];
-#pragma unroll
-        for (int s = 0; s < kPf; ++s) kf[s] = kfrag(ks, s);
-#pragma unroll
-        for (int s = 0; s < kD / 16; ++s) {
-            const bf16x8 a = kf[s % kPf];
-            if (s + kPf < kD / 16) kf[s % kPf] = kfrag(ks, s + kPf);
-            __builtin_amdgcn_sched_barrier(0);
-            sc = mfma_bf16(a, qf[s], sc);
-        }
-        __builtin_amdgcn_s_setprio(0);
-        // ---- keys that a row does not see: score -inf, weight 0 (score r of a lane is key 8 (r / 4) + 4 hi + r % 4) ----
-        bool masked = false, own = false;
+            for (int x = 0; x < kBlk; ++x)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void *)(s + kTile + x * 1024), 16,
+                                                         rv0 + 2 * x * v2 + (((ln & 31) ^ (((r0 + 2 * x) & 3) << 2)) << 4), 0,
+                                                         0, 0);
+        };
+        // The block's words and this lane's Q fragments (B operand of S^T: dims 16 s + 8 hi .. + 7 of the row) come before the
+        // first tile: loads end in order.
+        constexpr int kMine = (kWords + kThreads - 1) / kThreads;
+        uint32_t mine[TREE ? kMine : 1];
         if constexpr (TREE) {
-            own = i >= tl.n0;
-            masked = own || (i + 1) * kBK > keys;
-            if (own) {
-                const uint32_t w = words[row % NB * p.tw + (i - tl.n0)] >> (4 * hi);
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    sc[r] = (w >> (8 * (r >> 2) + (r & 3))) & 1u ? sc[r] : -__builtin_inff();
-            } else if (masked) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    sc[r] = i * kBK + 8 * (r >> 2) + 4 * hi + (r & 3) < keys ? sc[r] : -__builtin_inff();
-            }
-        } else {
-            const int k0 = tl.tile(i) * kBK, first = keys - p.Sq + q0;
-            // (differences of positions, which are small: a window up to the largest int would overflow taken from one)
-            masked = k0 + kBK - 1 > first || (first + NB - 1 - k0 >= p.window && k0 + kBK > p.sinks);
-            if (masked) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int key = k0 + 8 * (r >> 2) + 4 * hi + (r & 3);
-                    const bool sees = key <= pos && (pos - key < p.window || key < p.sinks);
-                    sc[r] = sees ? sc[r] : -__builtin_inff();
-                }
+            for (int x = 0; x < kMine; ++x) {
+                const int i = tid + x * kThreads, node = q0 + i / p.tw;
+                mine[x] = i < NB * p.tw && node < p.Sq ? p.tree[b * p.sbt + (long long)node * p.tw + i % p.tw] : 0u;
             }
         }
-        // ---- online softmax in log2 units; the reference moves only when the maximum exceeds it by more than 8 ----
-        float mx = -__builtin_inff();
+        bf16x8 qf[kD / 16];
+        {
+            // (rows past the last position repeat it: they are not stored)
+            const uint16_t *qr = p.q + b * p.sbq + head * p.shq + (long long)min(t, p.Sq - 1) * p.ldq + hi * 8;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) mx = __builtin_fmaxf(mx, sc[r]);
-        mx = half_swap_max(mx) * p.scale_log2;
-        const bool grow = mx > m + 8.0f;
-        const float alpha = grow ? __builtin_amdgcn_exp2f(m - mx) : 1.0f;
-        if (grow) m = mx;
-        if (__builtin_amdgcn_ballot_w64(grow)) {
-#pragma unroll
-            for (int dt = 0; dt < NDT; ++dt) O[dt] *= alpha;
-            lsum *= alpha;
+            for (int s = 0; s < kD / 16; ++s) qf[s] = __builtin_bit_cast(bf16x8, *(const u32x4 *)(qr + s * 16));
         }
-        const float ref = m == -__builtin_inff() ? 0.0f : m; // a row that has seen nothing yet: exp2(-inf - 0) = 0
-        bf16x8 pb[2];
+        __builtin_amdgcn_sched_barrier(0);
+        issue(i0, 0);
+        if constexpr (TREE) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            u32x4 w;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * s + 2 * e], p.scale_log2, -ref));
-                const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * s + 2 * e + 1], p.scale_log2, -ref));
-                lsum += p0 + p1;
-                w[e] = pack_bf16x2(p0, p1); // the matrix cores' operand type; the sum keeps the unrounded weights
-            }
-            pb[s] = __builtin_bit_cast(bf16x8, w);
-        }
-        // A value that is not finite must not reach the rows that do not see its key (0 x inf = NaN): looked for in
-        // the tiles where rows see different keys, by every wave in its part of the tile (by each in all of it, 3 x 1111
-        // tokens with a window of 200 took 32.1 us and not 30.5, and 2000 with one of 100 21.4 and not 19.4).  (Rows past
-        // the last key are zeros, and where all rows see all keys there is no such row.)
-        if (masked) {
-            uint32_t odd = 0;
-#pragma unroll
-            for (int x = 0; x < kBlk; ++x) {
-                const u32x4 w = *(const u32x4 *)(stage + kTile + (kBlk * wave + x) * 1024 + lane * 16);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) odd |= (w[e] & 0x7f807f80u) + 0x00800080u;
-            }
-            if (__builtin_amdgcn_ballot_w64((odd & 0x80008000u) != 0) && lane == 0) *odd_tile = i;
-            wait_lgkmcnt0();
-            meet(); // (not __syncthreads, which waits for the DMA too)
-            if (*odd_tile == i) { // the same for every wave
-                // into the rows that give their keys a weight, then zeros in their place
-                bf16x8 ind[2];
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    u32x4 w = __builtin_bit_cast(u32x4, pb[s]);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) w[e] = ((w[e] & 0xffffu) ? 0x7f00u : 0u) | ((w[e] >> 16) ? 0x7f000000u : 0u);
-                    ind[s] = __builtin_bit_cast(bf16x8, w);
-                }
-#pragma unroll
-                for (int x = 0; x < 4 * NDT; ++x) {
-                    const int s = x & 1, dt = x >> 2;
-                    const uint32_t sign = x & 2 ? 0x8000u : 0u;
-                    u32x4 w = __builtin_bit_cast(u32x4, vfrag(vs, s, dt));
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        w[e] = odd_value(w[e] & 0xffffu, sign) | (odd_value(w[e] >> 16, sign) << 16);
-                    O[dt] = mfma_bf16(__builtin_bit_cast(bf16x8, w), ind[s], O[dt]);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-                __syncthreads();
-#pragma unroll 1
-                for (int x = tid; x < kTile / 4; x += kThreads) {
-                    uint32_t *w = (uint32_t *)(smem + st * kStage + kTile) + x;
-                    *w &= (odd_value(*w & 0xffffu, 0) ? 0u : 0xffffu) | (odd_value(*w >> 16, 0) ? 0u : 0xffff0000u);
-                }
-                __syncthreads();
+            for (int x = 0; x < kMine; ++x) {
+                const int i = tid + x * kThreads, left = p.Sq - 32 * (i % p.tw); // bits past the last node do not count
+                if (i < NB * p.tw) words[i] = left >= 32 ? mine[x] : left <= 0 ? 0u : mine[x] & ((1u << left) - 1u);
             }
         }
-        // ---- O^T += V^T P^T ----
-        constexpr int kPv = kPf < 2 * NDT ? kPf : 2 * NDT;
-        __builtin_amdgcn_s_setprio(1);
-        bf16x8 vf[kPv];
-#pragma unroll
-        for (int x = 0; x < kPv; ++x) vf[x] = vfrag(vs, x / NDT, x % NDT);
-#pragma unroll
-        for (int x = 0; x < 2 * NDT; ++x) {
-            const bf16x8 a = vf[x % kPv];
-            if (x + kPv < 2 * NDT) vf[x % kPv] = vfrag(vs, (x + kPv) / NDT, (x + kPv) % NDT);
-            __builtin_amdgcn_sched_barrier(0);
-            O[x % NDT] = mfma_bf16(a, pb[x / NDT], O[x % NDT]);
-        }
-        __builtin_amdgcn_s_setprio(0);
-    }
-    wait_vmcnt<0>();  // the last (empty) loads have written before the stages are used again or given up
-    float ltot = half_swap_sum(lsum);
-    // A row that sees no key (a tree node without a bit, a position before the first key) has zeros, and -1 in the place of
-    // its sum.  One that sees keys has a sum of 0 only where all their scores are -inf: no softmax, 0 / 0.
-    uint32_t sees = pos >= 0;
-    if constexpr (TREE) {
-        sees = 0;
-#pragma unroll 1
-        for (int w = 0; w < p.tw; ++w) sees |= words[row % NB * p.tw + w];
-    }
-    if (sees == 0) { // (a node's cached keys were computed like the others': nothing of them leaves)
-        m = -__builtin_inff(), ltot = -1.0f;
+        if (tid == 0) *odd_tile = -1;
+        wait_lgkmcnt0(); // seen by every wave after the first tile's barrier
+        f32x16 O[NDT];
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) O[dt] = f32x16{};
-    }
-    if (!whole) {
-        float *po = p.part_o + (((long long)blk * kWaves + wave) * (NDT * 4) * 64 + lane) * 4;
-#pragma unroll
-        for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-            for (int r4 = 0; r4 < 4; ++r4)
-                *(float4 *)(po + (dt * 4 + r4) * 256) =
-                    float4{O[dt][4 * r4], O[dt][4 * r4 + 1], O[dt][4 * r4 + 2], O[dt][4 * r4 + 3]};
-        if (dt0 == 0 && hi == 0) p.part_ml[(long long)blk * (32 * R) + row] = float2{m, ltot};
-    } else {
-        // ---- normalise, stage in LDS (32 R rows x 512 B), write 16-byte row pieces ----
-        const float inv = ltot < 0.0f ? 0.0f : 1.0f / ltot;
-        __syncthreads();
-#pragma unroll
-        for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-            for (int r4 = 0; r4 < 4; ++r4) {
-                const int d = (dt0 + dt) * 32 + 8 * r4 + 4 * hi;
-                u32x2 w;
-                w[0] = pack_bf16x2(O[dt][4 * r4] * inv, O[dt][4 * r4 + 1] * inv);
-                w[1] = pack_bf16x2(O[dt][4 * r4 + 2] * inv, O[dt][4 * r4 + 3] * inv);
-                *(u32x2 *)(smem + row * (kD * 2) + (((d >> 3) ^ l32) << 4) + (d & 4) * 2) = w;
+        float m = -__builtin_inff(), lsum = 0.0f;
+        const int pos = keys - p.Sq + t; // window: this row's position
+
+        // V^T fragment of 32-dim tile dt, step s: keys 16 s + 4 hi .. + 3 and 16 s + 8 + 4 hi .. + 3 (the keys of P^T's
+        // accumulator rows 8 s .. 8 s + 7) of dim 32 dt + l % 32.  The lane's address: key row 4 hi + (l % 16) / 4, dims
+        // 16 ((l / 16) % 2) + 4 (l % 4); chunk c of row r lies at c ^ 4 (r % 4), which spreads the 4 rows x 64 bytes of
+        // each half of a read over all banks (c ^ 2 (r % 8) spreads all 8 rows, but a half over half of the banks: it cost 1.3
+        // conflict cycles an LDS instruction, 1% of the time).
+        const int vrow = 4 * hi + ((l32 & 15) >> 2);
+        const int vchunk = (2 * (l32 >> 4) + ((l32 & 3) >> 1)) ^ ((vrow & 3) << 2) ^ (4 * dt0);
+        const uint32_t vbase = lds0 + kTile + vrow * (kD * 2) + (vchunk << 4) + (l32 & 1) * 8;
+        // K fragment s: chunk 2 s + hi of key row l % 32, at chunk ^ (l % 16).  The chunk's five bits are address bits of
+        // their own in both tiles, so a fragment's address is one exclusive or away from its stage's.
+        const uint32_t kbase = lds0 + l32 * (kD * 2) + ((hi ^ (l32 & 15)) << 4);
+        typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+        auto kfrag = [](uint32_t stage, int s) { // stage: kbase + the stage's offset
+            return __builtin_bit_cast(bf16x8, *(lds_u32x4 *)(uintptr_t)((stage ^ (s << 5))));
+        };
+        auto vfrag = [](uint32_t stage, int s, int dt) { // stage: vbase + the stage's offset
+            const uint32_t a = (stage ^ (dt << 6)) + s * 16 * (kD * 2);
+            const s16x4 x = tr_read((lds_s16x4 *)(uintptr_t)a, (lds_void *)smem);
+            const s16x4 y = tr_read((lds_s16x4 *)(uintptr_t)(a + 8 * (kD * 2)), (lds_void *)smem);
+            return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+        };
+
+#pragma unroll 1
+        for (int i = i0; i < i1; ++i) {
+            const int st = (i - i0) & 1;
+            // this wave's DMA of tile i landed; after the barrier every wave's has, and nobody reads tile i - 1 any more
+            wait_vmcnt<0>();
+            meet();
+            __builtin_amdgcn_sched_barrier(0);
+            issue(i + 1, 1 - st);
+            if constexpr (TREE && !STREAM) { // new keys that none of the block's nodes sees, as those after them (2 x 500 nodes
+                                             // after 500 keys 58.4 -> 45.8 us; up to 64 nodes there are hardly any)
+                if (i >= tl.n0 && !__builtin_amdgcn_ballot_w64(words[lane % NB * p.tw + (i - tl.n0)])) continue;
             }
-        __syncthreads();
-#pragma unroll 2
-        for (int x = tid; x < 32 * R * 32; x += kThreads) {
-            const int rr = x >> 5, ch = x & 31, tt = q0 + rr % NB;
-            if (tt < p.Sq)
-                *(u32x4 *)(p.o + b * p.sbo + (long long)(hk * kGroup + rr / NB) * p.sho + (long long)tt * p.ldo + ch * 8) =
-                    *(const u32x4 *)(smem + rr * (kD * 2) + ((ch ^ (rr & 31)) << 4));
+            const int8_t *stage = smem + st * kStage;
+            const uint32_t ks = kbase + st * kStage, vs = vbase + st * kStage;
+            // ---- S^T = K Q^T: rows = keys of the tile, column = this lane's row; fragments read kPf steps ahead ----
+            f32x16 sc = {};
+            __builtin_amdgcn_s_setprio(1);
+            bf16x8 kf[kPf];
+#pragma unroll
+            for (int s = 0; s < kPf; ++s) kf[s] = kfrag(ks, s);
+#pragma unroll
+            for (int s = 0; s < kD / 16; ++s) {
+                const bf16x8 a = kf[s % kPf];
+                if (s + kPf < kD / 16) kf[s % kPf] = kfrag(ks, s + kPf);
+                __builtin_amdgcn_sched_barrier(0);
+                sc = mfma_bf16(a, qf[s], sc);
+            }
+            __builtin_amdgcn_s_setprio(0);
+            // ---- keys that a row does not see: score -inf, weight 0 (score r of a lane is key 8 (r / 4) + 4 hi + r % 4) ----
+            bool masked = false, own = false;
+            if constexpr (TREE) {
+                own = i >= tl.n0;
+                masked = own || (i + 1) * kBK > keys;
+                if (own) {
+                    const uint32_t w = words[row % NB * p.tw + (i - tl.n0)] >> (4 * hi);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        sc[r] = (w >> (8 * (r >> 2) + (r & 3))) & 1u ? sc[r] : -__builtin_inff();
+                } else if (masked) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        sc[r] = i * kBK + 8 * (r >> 2) + 4 * hi + (r & 3) < keys ? sc[r] : -__builtin_inff();
+                }
+            } else {
+                const int k0 = tl.tile(i) * kBK, first = keys - p.Sq + q0;
+                // (differences of positions, which are small: a window up to the largest int would overflow taken from one)
+                masked = k0 + kBK - 1 > first || (first + NB - 1 - k0 >= p.window && k0 + kBK > p.sinks);
+                if (masked) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int key = k0 + 8 * (r >> 2) + 4 * hi + (r & 3);
+                        const bool sees = key <= pos && (pos - key < p.window || key < p.sinks);
+                        sc[r] = sees ? sc[r] : -__builtin_inff();
+                    }
+                }
+            }
+            // ---- online softmax in log2 units; the reference moves only when the maximum exceeds it by more than 8 ----
+            float mx = -__builtin_inff();
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mx = __builtin_fmaxf(mx, sc[r]);
+            mx = half_swap_max(mx) * p.scale_log2;
+            const bool grow = mx > m + 8.0f;
+            const float alpha = grow ? __builtin_amdgcn_exp2f(m - mx) : 1.0f;
+            if (grow) m = mx;
+            if (__builtin_amdgcn_ballot_w64(grow)) {
+#pragma unroll
+                for (int dt = 0; dt < NDT; ++dt) O[dt] *= alpha;
+                lsum *= alpha;
+            }
+            const float ref = m == -__builtin_inff() ? 0.0f : m; // a row that has seen nothing yet: exp2(-inf - 0) = 0
+            bf16x8 pb[2];
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                u32x4 w;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * s + 2 * e], p.scale_log2, -ref));
+                    const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * s + 2 * e + 1], p.scale_log2, -ref));
+                    lsum += p0 + p1;
+                    w[e] = pack_bf16x2(p0, p1); // the matrix cores' operand type; the sum keeps the unrounded weights
+                }
+                pb[s] = __builtin_bit_cast(bf16x8, w);
+            }
+            // A value that is not finite must not reach the rows that do not see its key (0 x inf = NaN): looked for in
+            // the tiles where rows see different keys, by every wave in its part of the tile (by each in all of it, 3 x 1111
+            // tokens with a window of 200 took 32.1 us and not 30.5, and 2000 with one of 100 21.4 and not 19.4).  (Rows past
+            // the last key are zeros, and where all rows see all keys there is no such row.)
+            if (masked) {
+                uint32_t odd = 0;
+#pragma unroll
+                for (int x = 0; x < kBlk; ++x) {
+                    const u32x4 w = *(const u32x4 *)(stage + kTile + (kBlk * wave + x) * 1024 + lane * 16);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) odd |= (w[e] & 0x7f807f80u) + 0x00800080u;
+                }
+                if (__builtin_amdgcn_ballot_w64((odd & 0x80008000u) != 0) && lane == 0) *odd_tile = i;
+                wait_lgkmcnt0();
+                meet(); // (not __syncthreads, which waits for the DMA too)
+                if (*odd_tile == i) { // the same for every wave
+                    // into the rows that give their keys a weight, then zeros in their place
+                    bf16x8 ind[2];
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        u32x4 w = __builtin_bit_cast(u32x4, pb[s]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) w[e] = ((w[e] & 0xffffu) ? 0x7f00u : 0u) | ((w[e] >> 16) ? 0x7f000000u : 0u);
+                        ind[s] = __builtin_bit_cast(bf16x8, w);
+                    }
+#pragma unroll
+                    for (int x = 0; x < 4 * NDT; ++x) {
+                        const int s = x & 1, dt = x >> 2;
+                        const uint32_t sign = x & 2 ? 0x8000u : 0u;
+                        u32x4 w = __builtin_bit_cast(u32x4, vfrag(vs, s, dt));
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            w[e] = odd_value(w[e] & 0xffffu, sign) | (odd_value(w[e] >> 16, sign) << 16);
+                        O[dt] = mfma_bf16(__builtin_bit_cast(bf16x8, w), ind[s], O[dt]);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    __syncthreads();
+#pragma unroll 1
+                    for (int x = tid; x < kTile / 4; x += kThreads) {
+                        uint32_t *w = (uint32_t *)(smem + st * kStage + kTile) + x;
+                        *w &= (odd_value(*w & 0xffffu, 0) ? 0u : 0xffffu) | (odd_value(*w >> 16, 0) ? 0u : 0xffff0000u);
+                    }
+                    __syncthreads();
+                }
+            }
+            // ---- O^T += V^T P^T ----
+            constexpr int kPv = kPf < 2 * NDT ? kPf : 2 * NDT;
+            __builtin_amdgcn_s_setprio(1);
+            bf16x8 vf[kPv];
+#pragma unroll
+            for (int x = 0; x < kPv; ++x) vf[x] = vfrag(vs, x / NDT, x % NDT);
+#pragma unroll
+            for (int x = 0; x < 2 * NDT; ++x) {
+                const bf16x8 a = vf[x % kPv];
+                if (x + kPv < 2 * NDT) vf[x % kPv] = vfrag(vs, (x + kPv) / NDT, (x + kPv) % NDT);
+                __builtin_amdgcn_sched_barrier(0);
+                O[x % NDT] = mfma_bf16(a, pb[x / NDT], O[x % NDT]);
+            }
+            __builtin_amdgcn_s_setprio(0);
         }
-    }
-    if (!STREAM) return;
-    left -= i1 - i0 + p.begin;
-    if (left <= 0) return;
-    i0 = 0, blk = 2 * blockIdx.x + 1; // (what lies between a workgroup's first and last is whole)
-    ++b;
-    keys = key_count(p, b);
-    __syncthreads(); // everybody is done with the stages and the words
+        wait_vmcnt<0>();  // the last (empty) loads have written before the stages are used again or given up
+        float ltot = half_swap_sum(lsum);
+        // A row that sees no key (a tree node without a bit, a position before the first key) has zeros, and -1 in the place of
+        // its sum.  One that sees keys has a sum of 0 only where all their scores are -inf: no softmax, 0 / 0.
+        uint32_t sees = pos >= 0;
+        if constexpr (TREE) {
+            sees = 0;
+#pragma unroll 1
+            for (int w = 0; w < p.tw; ++w) sees |= words[row % NB * p.tw + w];
+        }
+        if (sees == 0) { // (a node's cached keys were computed like the others': nothing of them leaves)
+            m = -__builtin_inff(), ltot = -1.0f;
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) O[dt] = f32x16{};
+        }
+        if (!whole) {
+            float *po = p.part_o + (((long long)blk * kWaves + wave) * (NDT * 4) * 64 + lane) * 4;
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                for (int r4 = 0; r4 < 4; ++r4)
+                    *(float4 *)(po + (dt * 4 + r4) * 256) =
+                        float4{O[dt][4 * r4], O[dt][4 * r4 + 1], O[dt][4 * r4 + 2], O[dt][4 * r4 + 3]};
+            if (dt0 == 0 && hi == 0) p.part_ml[(long long)blk * (32 * R) + row] = float2{m, ltot};
+        } else {
+            // ---- normalise, stage in LDS (32 R rows x 512 B), write 16-byte row pieces ----
+            const float inv = ltot < 0.0f ? 0.0f : 1.0f / ltot;
+            __syncthreads();
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                for (int r4 = 0; r4 < 4; ++r4) {
+                    const int d = (dt0 + dt) * 32 + 8 * r4 + 4 * hi;
+                    u32x2 w;
+                    w[0] = pack_bf16x2(O[dt][4 * r4] * inv, O[dt][4 * r4 + 1] * inv);
+                    w[1] = pack_bf16x2(O[dt][4 * r4 + 2] * inv, O[dt][4 * r4 + 3] * inv);
+                    *(u32x2 *)(smem + row * (kD * 2) + (((d >> 3) ^ l32) << 4) + (d & 4) * 2) = w;
+                }
+            __syncthreads();
+#pragma unroll 2
+            for (int x = tid; x < 32 * R * 32; x += kThreads) {
+                const int rr = x >> 5, ch = x & 31, tt = q0 + rr % NB;
+                if (tt < p.Sq)
+                    *(u32x4 *)(p.o + b * p.sbo + (long long)(hk * kGroup + rr / NB) * p.sho + (long long)tt * p.ldo + ch * 8) =
+                        *(const u32x4 *)(smem + rr * (kD * 2) + ((ch ^ (rr & 31)) << 4));
+            }
+        }
+        if (!STREAM) return;
+        left -= i1 - i0 + p.begin;
+        if (left <= 0) return;
+        i0 = 0, blk = 2 * blockIdx.x + 1; // (what lies between a workgroup's first and last is whole)
+        ++b;
+        keys = key_count(p, b);
+        __syncthreads(); // everybody is done with the stages and the words
     }
 }
 
@@ -649,8 +649,8 @@ __global__ __launch_bounds__(256) void ca_merge_kernel(CaParams p) {
 // How a call is divided: row blocks (R) and dim parts (D) of a workgroup, and the work.
 struct Plan {
     int R, D, nqb, gq, chunk, nchunk;
-    int runs, dense, least; // STREAM: most runs of tiles (0: every sequence whole); the tiles of a run below which half as many are made; its fewest
-    int begin;              // the tiles that a sequence's beginning counts for
+    int runs, dense;  // STREAM: most runs of tiles (0: every sequence whole); the tiles of a run below which half as many are made
+    int least, begin; // a run's fewest tiles; the tiles that a sequence's beginning counts for
     bool stream, wide;
     long long tiles, wgs, states; // STREAM: a head's tiles; workgroups; partial rows
 };
@@ -691,7 +691,8 @@ Plan plan(int B, int Sq, int HK, int max_tiles) {
         pl.runs = HK < slots ? slots / HK : 1;
         pl.wgs = (most < pl.runs ? most : pl.runs) * HK;
         pl.states = pl.wgs * 2 * 32 * pl.R;
-        // (few waves, then, of many parts each; 8 nodes, 1 x 32768 keys 54.6 -> 40.2 us, but 16 x 4000 64.2 -> 68.9 if waves share there)
+        // (few waves, then, of many parts each; 8 nodes, 1 x 32768 keys 54.6 -> 40.2 us, but 16 x 4000 64.2 -> 68.9 if waves
+        // share there)
         pl.wide = units * pl.R <= 16;
         return pl;
     }
@@ -734,16 +735,16 @@ int launch_as(const CaParams &p, const Plan &pl, hipStream_t st) {
     // walks all the key counts: with workgroups for all sequences, 3000 tokens of up to 200 keys each took 2052 us and not 498)
     const long long blocks = (long long)(STREAM && p.B > pl.runs ? pl.runs - 1 : p.B) * p.HK * pl.nqb;
     if (blocks == 0) return 0;
-    if (STREAM && pl.wide)
-        hipLaunchKernelGGL((ca_merge_kernel<R, D, TREE, STREAM, STREAM ? 4 : 1>), dim3((unsigned)(blocks * 32 * R)), dim3(256), 0, st, p);
-    else
-        hipLaunchKernelGGL((ca_merge_kernel<R, D, TREE, STREAM, 1>), dim3((unsigned)(blocks * 8 * R)), dim3(256), 0, st, p);
+    const dim3 one((unsigned)(blocks * 8 * R)), four((unsigned)(blocks * 32 * R));
+    if (STREAM && pl.wide) hipLaunchKernelGGL((ca_merge_kernel<R, D, TREE, STREAM, STREAM ? 4 : 1>), four, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((ca_merge_kernel<R, D, TREE, STREAM, 1>), one, dim3(256), 0, st, p);
     return mica_err(hipGetLastError());
 }
 
 template <bool TREE>
 int launch(CaParams &p, const Plan &pl, void *workspace, hipStream_t st) {
-    p.nqb = pl.nqb, p.gq = pl.gq, p.chunk = pl.chunk, p.nchunk = pl.nchunk, p.runs = pl.runs, p.dense = pl.dense, p.least = pl.least, p.begin = pl.begin;
+    p.nqb = pl.nqb, p.gq = pl.gq, p.chunk = pl.chunk, p.nchunk = pl.nchunk;
+    p.runs = pl.runs, p.dense = pl.dense, p.least = pl.least, p.begin = pl.begin;
     p.part_o = (float *)workspace;
     p.part_ml = (float2 *)((char *)workspace + pl.states * kD * 4);
     if (pl.wgs >= (1LL << 31) || pl.tiles >= (1LL << 30)) return MICA_MISS_RANGE;
@@ -833,7 +834,8 @@ extern "C" int mica_attention_window(const void *q, long long sbq, long long shq
     if (!strides_ok({sbq, shq, ldq, sbk, shk, sbv, shv, sbo, sho, ldo})) return MICA_MISS_STRIDE;
     if (const int rc = row_stride(ldk, Sk)) return rc;
     if (const int rc = row_stride(ldv, Sk)) return rc;
-    if (!mica_aligned16(q) || !mica_aligned16(o) || (Sk > 0 && (!mica_aligned16(k) || !mica_aligned16(v)))) return MICA_MISS_ALIGN;
+    if (!mica_aligned16(q) || !mica_aligned16(o) || (Sk > 0 && (!mica_aligned16(k) || !mica_aligned16(v))))
+        return MICA_MISS_ALIGN;
     const Plan pl = plan(B, Sq, HK, window_tiles(Sq, Sk, window, sinks));
     if (pl.states && (!workspace || !mica_aligned16(workspace) || workspace_bytes < state_bytes(pl))) return MICA_MISS_ARG;
     CaParams p{};
