@@ -372,9 +372,11 @@ int mica_attention_fwd_rope(const void *q, long long sbq, long long shq, long lo
  *   o[b, i, h] = sum_{u in S} softmax_u(scale q[b, i, h] . key_u[h / 4]) value_u[h / 4],
  *   S = the sequence's cached keys and the nodes j with bit j % 64 of word tree[b sbt + i W + j / 64] set, W = ceil(N / 64).
  * A node whose words hold no bit below N is absent (a padded batch): it sees nothing, the cache neither, and its output is
- * zeros.  No order of the nodes is assumed.  q / k / v / o: bf16; head j of node t of sequence b at ptr + b sb + j sh + t ld
- * (elements, all % 8); k_cache / v_cache: [cache_cap] rows likewise, a batch stride of 0 shares them.  tree: device memory,
- * 8-byte aligned; sbt words between sequences (0: one tree for all).  N <= 512; scale positive.  Keys past cache_len are
+ * zeros; the softmax of scores that are all -inf is NaN.  No order of the nodes is assumed.  q / k / v / o: bf16, 16-byte
+ * aligned; head j of node t of sequence b at ptr + b sb + j sh + t ld (elements, all % 8 and not negative; rows of k and v
+ * at least 256 and less than 2^25 apart); k_cache / v_cache: [cache_cap] rows likewise, a batch stride of 0 shares them.
+ * tree: device memory, 8-byte aligned; sbt words between sequences (0: one tree for all).  N <= 512; scale positive and
+ * finite; B HK ceil(N / 8) < 2^24.  Keys past cache_len are
  * never read; a key or value that is not finite reaches only the nodes that see it.  fp32 softmax and sums, the weights
  * rounded to bf16 for the product with v.  workspace: mica_attention_tree_workspace_bytes(B, N, HK, cache_cap) bytes (0:
  * none), 16-byte aligned, no initialisation needed.  No counterpart in the reference, which runs every candidate as a
@@ -394,8 +396,8 @@ long long mica_attention_tree_workspace_bytes(int B, int N, int HK, int cache_ca
  * kv_len[b] keys (int32 [B], device memory, clamped to 0 .. Sk; NULL: Sk); its Sq queries are its last Sq positions:
  * query i is at position p = kv_len[b] - Sq + i and sees the keys u <= p with u > p - window or u < sinks.
  *   o[b, i, h] = sum_u softmax_u(scale q[b, i, h] . k[b, u, h / 4]) v[b, u, h / 4];  zeros where p < 0.
- * window >= 1, sinks >= 0; Sk may be less than Sq.  Layouts, types and values that are not finite as in
- * mica_attention_tree.  workspace: mica_attention_window_workspace_bytes(B, Sq, Sk, HK, window, sinks) bytes (0: none),
+ * window >= 1, sinks >= 0; Sk may be less than Sq.  Keys past kv_len are never read.  Layouts, types, limits and values that
+ * are not finite as in mica_attention_tree.  workspace: mica_attention_window_workspace_bytes(B, Sq, Sk, HK, window, sinks) bytes (0: none),
  * 16-byte aligned, no initialisation needed.  No counterpart in the reference (its attention sees every key).
  */
 int mica_attention_window(const void *q, long long sbq, long long shq, long long ldq, const void *k, long long sbk,

@@ -263,9 +263,10 @@ def tree_attention(q, k, v, tree, cache=None, cache_len=None, scale: float | Non
     q [B, N, HQ, 256], k / v [B, N, HK, 256]: the new nodes' heads, bf16 views (e.g. of the fused QKV output), with their
     positions already applied, HQ = 4 HK, N <= 512.  tree: int64 masks [N, W] for every sequence or [B, N, W]
     (tree_masks(parents)); a node without a bit is padding: it sees nothing and its output is zeros.  cache: (keys, values),
-    [B, C, HK, 256] or one for all sequences, [1, C, HK, 256] or [C, HK, 256] (a PrefixState's layer), of any strides;
-    cache_len: int32 [B] on the device, how many of them sequence b has (None: C; clamped to 0 .. C).  Rows past it are
-    never read.  Returns o [B, N, HQ, 256] bf16."""
+    [B, C, HK, 256] or one for all sequences, [1, C, HK, 256] or [C, HK, 256] (a PrefixState's layer).  All of them views
+    with unit feature stride, other strides of whole 16 bytes, and no two rows of one sequence in one place.  cache_len:
+    int32 [B] on the device, how many cached keys sequence b has (None: C; clamped to 0 .. C).  Rows past it are never
+    read.  Returns o [B, N, HQ, 256] bf16."""
     scale = _scale(scale)
     kc = vc = None
     if cache is not None:
@@ -308,8 +309,9 @@ def window_attention(q, k, v, window: int, sinks: int = 0, scale: float | None =
 
     q [B, Sq, HQ, 256], k / v [B, Sk, HK, 256] bf16 views, HQ = 4 HK.  Sequence b has kv_len[b] keys (int32 [B] on the
     device, clamped to 0 .. Sk; None: Sk) and its queries are the last Sq of those positions; a query before the first
-    key sees nothing, and its output is zeros.  window >= 1, sinks >= 0.  Keys past kv_len or outside every query's
-    reach are not read.  Returns o [B, Sq, HQ, 256] bf16."""
+    key sees nothing, and its output is zeros.  window >= 1, sinks >= 0.  Keys past kv_len are not read, nor most of those
+    outside every query's reach (32 at a time); what these hold does not matter.  Strides as in tree_attention.  Returns o
+    [B, Sq, HQ, 256] bf16."""
     scale = _scale(scale)
     r = _lib.FAST.window_attention(q, k, v, window, sinks, kv_len, scale)
     if r is not None:

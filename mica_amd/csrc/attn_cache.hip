@@ -2,7 +2,8 @@
 // candidate tokens over a cache (mica_attention_tree) and causal attention within a sliding window and over a few
 // first tokens (mica_attention_window).
 //
-//   o[i, h] = sum_{u in S(i)} softmax_u(scale q[i, h] . k[u, h / 4]) v[u, h / 4];   zeros where S(i) is empty
+//   o[i, h] = sum_{u in S(i)} softmax_u(scale q[i, h] . k[u, h / 4]) v[u, h / 4];   zeros where S(i) is empty, NaN where
+//   all its scores are -inf
 //   tree:    S(i) = the sequence's first cache_len cached keys and the new keys j whose bit is set in node i's words
 //            (a node without any bit is absent and sees nothing)
 //   window:  S(i) = { u : u <= p and (u > p - window or u < sinks) },  p = position of query i
@@ -20,11 +21,10 @@
 //
 // Up to 64 query positions, one row block takes them all, and the key tiles of all sequences, one after the other, are
 // divided evenly over the chip's workgroups (STREAM): a workgroup may end one sequence and begin the next, so
-// key counts that differ, or sequences that do not divide the chip, leave no CU idle.  Many or short sequences have a
-// workgroup each.  In that row each sequence has a few
-// empty tiles before its own, for the time its beginning takes.  More positions take a workgroup
-// for each block, their tiles divided into chunks where that leaves too few.  ca_merge_kernel joins the partial softmax
-// states (fp32) of what was divided.
+// key counts that differ, or sequences that do not divide the chip, leave no CU idle.  In that row of tiles each sequence
+// has a few empty ones before its own, for the time its beginning takes.  Many or short sequences are not divided: a
+// workgroup each.  More positions take a workgroup for each block, their tiles divided into chunks where that leaves too
+// few.  ca_merge_kernel joins the partial softmax states (fp32) of what was divided.
 #include "attn_common.h"
 
 #include <algorithm>
@@ -666,8 +666,10 @@ Plan plan(int B, int Sq, int HK, int max_tiles) {
     const int slots = kCus * (pl.R < 8 ? 2 : 1);
     const long long units = (long long)B * HK;
     // A workgroup a sequence and head, undivided, where those are many or short: no state to write and join, no sequence
-    // begun behind another's end.  The longest of a batch is then waited for, so up to as many tiles as the whole batch, at
-    // full length, takes all workgroups twice over at most.  Divided / whole, us (nodes, sequences x keys): 4, 1 x 60 13.2 /
+    // begun behind another's end.  The longest of a batch is then waited for, alone in the end, so only up to a length that
+    // grows with how full the chip is: 10 tiles, or 10 max(R, 2) for every 128 sequences x heads.  (These workgroups, evenly
+    // divided, would have a quarter of a sequence's tiles each at 128 sequences x heads, or half with R = 8, and states to
+    // write and join.)  Divided / whole, us (nodes, sequences x keys): 4, 1 x 60 13.2 /
     // 8.9, 32 x 1000 31.9 / 42.4, 64 x 500 43.7 / 32.0, 200 x 3500 394 / 362; 16, 32 x 1000 40.8 / 45.0, 64 x 500 43.0 / 35.0;
     // 32, 32 x 1000 51.5 / 47.7, 600 x 800 554 / 423; 64, 8 x 250 30.4 / 26.1, 64 x 2000 179 / 139.
     if (pl.stream && max_tiles <= std::max(10ll, 10ll * std::max(pl.R, 2) * (units / 128))) {

@@ -213,8 +213,12 @@ MICA_DEVICE Stat block_stat(Stat a, Stat *red) {
 }
 
 // One pass over the row, bound by HBM without alternatives: 4096 x 151936 bf16 take 197 us, 6.3 TB/s; with 20 of them nearly
-// as much by VALU issue, 2048 rows 130 us, 4.8 TB/s.  Rows of a block or two are bound by their latency (load, threshold,
-// candidates, join): 64 x 151936 fp32 with 20 alternatives 19.3 us, without 12; one row 11.
+// as much by VALU issue, 2048 rows 130 us, 4.8 TB/s (calls one behind the other: a call by itself takes 155 to 160).  Rows
+// of a block or two are bound by their latency (load, threshold, candidates, join): 64 x 151936 fp32 with 20 alternatives
+// 19.3 us, without 12; one row 11.  Rows of which nearly everything is -inf are slower: lanes that have seen nothing else
+// send their wave through the loop of single elements, and with fewer than `top` groups of the first block that hold a
+// finite element the exact selection runs: 30 finite elements of 151936, 20 alternatives, one row 102 us, 2048 rows 447 (139
+// without alternatives); 3000 finite ones 12.5 and 148.
 // (six workgroups a CU; five leave fp32 the registers that it would spill: 1024 x 151936 with 20 alternatives 117.5 -> 107.9 us)
 template <int DT, bool TOP, int NT>
 __global__ __launch_bounds__(NT, DT == MICA_FP32 ? 5 : 6) void lp_rows_kernel(LpParams p) {
@@ -495,9 +499,13 @@ __global__ __launch_bounds__(kThreads) void lp_merge_kernel(LpParams p) {
     finish<DT, kThreads>(p, row, a, list, tok);
 }
 
-// Workgroups a row, and blocks each: enough for the chip (256 CUs of six workgroups), whole blocks each.  A row that is short,
-// or one of many, takes one workgroup and no join: up to 2 blocks with alternatives (which each block's candidates delay:
-// 500 x 9000 bf16 with 20 16.6 -> 10.9 us, but 260 x 24000 14.4 -> 15.4), up to 4 without (260 x 24000 12.3 -> 8.8).
+// Workgroups a row, and whole blocks each: about 2048 in all, a third more than the chip holds at a time (256 CUs of six,
+// fp32 five).  No more than it holds (1536, fp32 1280), rounded down, us, 2048 / those: 20 alternatives, bf16 100 x 151936
+// 18.2 / 22.3, 300 37 / 33, 1000 75 / 70, fp32 300 x 151936 44 / 40; without, 300 x 151936 21.0 / 21.8, 700 41.8 / 44.5,
+// 1000 56.7 / 53.2; fp16 517 x 32003 with 7 18.6 / 18.2.  Neither is better everywhere.
+// A row that is short, or one of many, takes one workgroup and no join: up to 2 blocks with alternatives (which each block's
+// candidates delay: 500 x 9000 bf16 with 20 16.6 -> 10.9 us, but 260 x 24000 14.4 -> 15.4), up to 4 without (260 x 24000
+// 12.3 -> 8.8).
 void divide(int T, int V, int elems, int top, int &parts, int &bpp) {
     const int blocks = max(1, (V / elems + kThreads * U - 1) / (kThreads * U));
     const int want = T >= 1024 || blocks <= (top ? 2 : 4) ? 1 : min((2048 + T - 1) / T, kMaxParts);
