@@ -188,10 +188,10 @@ MICA_DEVICE s16x4 tr_read(lds_s16x4 *p, lds_void *__restrict w) {
 
 // What bounds it, and the whole call's time (at the rates of a large copy, 4.87 TB/s, and a large matrix product, 1401
 // TFLOP/s): few rows, the cache's bytes: 64 single tokens with a window of 4096 take 190 us, 5.7 TB/s; 32 x 16 nodes over up
-// to 4096 keys 96 us of 86.  Many rows, the matrix cores beside the softmax, with two waves a SIMD: 16384 tokens with a
-// window of 2048 470 us of 368; 64 nodes after 32768 keys 61 to 64 us of 28, of them 8 for the first tile and 20 for writing
-// and joining 64 MB of partial states; 4 x 255 nodes after 2048 shared keys 60 us of 24.5.  A short call is two launches: 8 nodes
-// after 500 keys 12.5 us.  (Four stages with one workgroup a CU 1 to 5 us slower, with eight waves 1 us; fragments read
+// to 4096 keys 97 us of 86.  Many rows, the matrix cores beside the softmax, with two waves a SIMD: 16384 tokens with a
+// window of 2048 469 us of 368 (548 in a long run of nothing else); 64 nodes after 32768 keys 63 us of 28, of them 8 for the
+// first tile and 20 for writing and joining 64 MB of partial states; 4 x 255 nodes after 2048 shared keys 59 us of 24.5.  A
+// short call is two launches: 8 nodes after 500 keys 12.5 us.  (Four stages with one workgroup a CU 1 to 5 us slower, with eight waves 1 us; fragments read
 // further ahead, 64 rows a wave, two chains for S^T: no faster, or slower for the registers that they spill.)
 template <int R, int D, bool TREE, bool STREAM>
 __global__ __launch_bounds__(64 * R * D, 2) void ca_fwd_kernel(CaParams p) {
@@ -429,7 +429,9 @@ __global__ __launch_bounds__(64 * R * D, 2) void ca_fwd_kernel(CaParams p) {
                     const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * s + 2 * e], p.scale_log2, -ref));
                     const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * s + 2 * e + 1], p.scale_log2, -ref));
                     lsum += p0 + p1;
-                    w[e] = pack_bf16x2(p0, p1); // the matrix cores' operand type; the sum keeps the unrounded weights
+                    // the matrix cores' operand type; the sum keeps the unrounded weights.  The result is then 0.0022 of its
+                    // norm off, where its own rounding to bf16 alone makes 0.0017 (as causal_gqa_attention's)
+                    w[e] = pack_bf16x2(p0, p1);
                 }
                 pb[s] = __builtin_bit_cast(bf16x8, w);
             }
