@@ -376,10 +376,10 @@ int mica_attention_fwd_rope(const void *q, long long sbq, long long shq, long lo
  * aligned; head j of node t of sequence b at ptr + b sb + j sh + t ld (elements, all % 8 and not negative; rows of k and v
  * at least 256 and less than 2^25 apart); k_cache / v_cache: [cache_cap] rows likewise, a batch stride of 0 shares them.
  * tree: device memory, 8-byte aligned; sbt words between sequences (0: one tree for all).  N <= 512; scale positive and
- * finite; B HK ceil(N / 8) < 2^24.  Keys past cache_len are
- * never read; a key or value that is not finite reaches only the nodes that see it.  fp32 softmax and sums, the weights
- * rounded to bf16 for the product with v.  workspace: mica_attention_tree_workspace_bytes(B, N, HK, cache_cap) bytes (0:
- * none), 16-byte aligned, no initialisation needed.  No counterpart in the reference, which runs every candidate as a
+ * finite; B HK ceil(N / 8) < 2^24.  Keys past cache_len are never read; a key or value that is not finite reaches only the
+ * nodes that see it.  fp32 softmax and sums, the weights rounded to bf16 for the product with v.
+ * workspace: mica_attention_tree_workspace_bytes(B, N, HK, cache_cap) bytes (0: none), 16-byte aligned, no initialisation
+ * needed.  No counterpart in the reference, which runs every candidate as a
  * request of its own.
  */
 int mica_attention_tree(const void *q, long long sbq, long long shq, long long ldq, const void *k, long long sbk,
@@ -397,8 +397,8 @@ long long mica_attention_tree_workspace_bytes(int B, int N, int HK, int cache_ca
  * query i is at position p = kv_len[b] - Sq + i and sees the keys u <= p with u > p - window or u < sinks.
  *   o[b, i, h] = sum_u softmax_u(scale q[b, i, h] . k[b, u, h / 4]) v[b, u, h / 4];  zeros where p < 0.
  * window >= 1, sinks >= 0; Sk may be less than Sq.  Keys past kv_len are never read.  Layouts, types, limits and values that
- * are not finite as in mica_attention_tree.  workspace: mica_attention_window_workspace_bytes(B, Sq, Sk, HK, window, sinks) bytes (0: none),
- * 16-byte aligned, no initialisation needed.  No counterpart in the reference (its attention sees every key).
+ * are not finite as in mica_attention_tree.  workspace: mica_attention_window_workspace_bytes(B, Sq, Sk, HK, window, sinks)
+ * bytes (0: none), 16-byte aligned, no initialisation needed.  No counterpart in the reference (its attention sees every key).
  */
 int mica_attention_window(const void *q, long long sbq, long long shq, long long ldq, const void *k, long long sbk,
                           long long shk, long long ldk, const void *v, long long sbv, long long shv, long long ldv, void *o,

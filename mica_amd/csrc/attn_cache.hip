@@ -191,8 +191,8 @@ MICA_DEVICE s16x4 tr_read(lds_s16x4 *p, lds_void *__restrict w) {
 // to 4096 keys 97 us of 86.  Many rows, the matrix cores beside the softmax, with two waves a SIMD: 16384 tokens with a
 // window of 2048 469 us of 368 (548 in a long run of nothing else); 64 nodes after 32768 keys 63 us of 28, of them 8 for the
 // first tile and 20 for writing and joining 64 MB of partial states; 4 x 255 nodes after 2048 shared keys 59 us of 24.5.  A
-// short call is two launches: 8 nodes after 500 keys 12.5 us.  (Four stages with one workgroup a CU 1 to 5 us slower, with eight waves 1 us; fragments read
-// further ahead, 64 rows a wave, two chains for S^T: no faster, or slower for the registers that they spill.)
+// short call is two launches: 8 nodes after 500 keys 12.5 us.  (Four stages with one workgroup a CU 1 to 5 us slower, with
+// eight waves 1 us; fragments read further ahead, 64 rows a wave, two chains for S^T: no faster, or slower for the registers that they spill.)
 template <int R, int D, bool TREE, bool STREAM>
 __global__ __launch_bounds__(64 * R * D, 2) void ca_fwd_kernel(CaParams p) {
     constexpr int kWaves = R * D, kThreads = 64 * kWaves;

@@ -213,7 +213,7 @@ MICA_DEVICE Stat block_stat(Stat a, Stat *red) {
 }
 
 // One pass over the row, bound by HBM without alternatives: 4096 x 151936 bf16 take 197 us, 6.3 TB/s; with 20 of them nearly
-// as much by VALU issue, 2048 rows 130 us, 4.8 TB/s (calls one behind the other: a call by itself takes 155 to 160).  Rows
+// as much by VALU issue, 2048 rows 130 us, 4.8 TB/s (calls one behind the other: a call by itself takes 147 to 160).  Rows
 // of a block or two are bound by their latency (load, threshold, candidates, join): 64 x 151936 fp32 with 20 alternatives
 // 19.3 us, without 12; one row 11.  Rows of which nearly everything is -inf are slower: lanes that have seen nothing else
 // send their wave through the loop of single elements, and with fewer than `top` groups of the first block that hold a
@@ -514,7 +514,7 @@ void divide(int T, int V, int elems, int top, int &parts, int &bpp) {
 }
 long long part_bytes(int T, int parts, int top) { return parts > 1 ? (long long)T * parts * (16 + 8 * top) : 0; }
 
-// Rows of one launch: a grid of 2^32 work-items or more wraps round without an error, and the rows behind it were not written.
+// Rows of one launch: a grid of 2^32 work-items or more wraps round without an error and leaves the rows behind it unwritten.
 constexpr int kGridRows = 1 << 23;
 
 template <int DT>
