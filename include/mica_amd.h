@@ -407,6 +407,84 @@ int mica_attention_window(const void *q, long long sbq, long long shq, long long
                           mica_stream_t stream);
 long long mica_attention_window_workspace_bytes(int B, int Sq, int Sk, int HK, int window, int sinks);
 
+/*
+ * Causal attention over prompts of different lengths packed one behind the other, head dim 256, HQ = 4 HK.  starts: int32
+ * [B + 1], device memory, not falling: rows starts[b] .. starts[b + 1] - 1 of T are sequence b's (values are clamped to 0 .. T,
+ * so that no others are touched whatever they are; sequences that overlap have no defined results).  Row t attends to the
+ * rows of its sequence up to itself:
+ *   o[t, h] = sum_{u in seq(t), u <= t} softmax_u(scale q[t, h] . k[u, h / 4]) v[u, h / 4].
+ * Rows of no sequence, before the first or behind the last, become zeros with fill != 0 and are left as they were without.
+ * q / k / v / o: bf16, 16-byte aligned; head j of row t at ptr + j sh + t ld (elements, all % 8 and not negative; rows of k and
+ * v at least 256 and less than 2^25 apart).  scale positive and finite.  fp32 softmax and sums, the weights rounded to bf16 for the
+ * product with v; the softmax of scores that are all -inf is NaN; a key or value that is not finite reaches only the rows
+ * that see it.  longest: the rows of the longest sequence, or 0 for T, where the host knows it: a hint for the division of the
+ * work.  workspace: mica_attention_packed_workspace_bytes(B, T, HK, longest) bytes (0: none), 16-byte aligned, no
+ * initialisation needed.  The reference pads a batch to a common width (prefill_engine.py:171-418).
+ */
+int mica_attention_packed(const void *q, long long shq, long long ldq, const void *k, long long shk, long long ldk,
+                          const void *v, long long shv, long long ldv, void *o, long long sho, long long ldo,
+                          const int *starts, int B, int T, int HQ, int HK, int head_dim, float scale, int fill, int longest,
+                          void *workspace, long long workspace_bytes, mica_stream_t stream);
+long long mica_attention_packed_workspace_bytes(int B, int T, int HK, int longest);
+
+/* ---- paged key/value cache in 8 bits ----------------------------------------------------------- */
+
+/*
+ * A cache of the keys and values of one layer (head dim 256) for many sequences.  A sequence's tokens lie in blocks of 32.  A
+ * finished block is a page: int8 values with one fp32 scale for each head and side (0 keys, 1 values), s = max(max |x|, 1e-8)
+ * / 127 and q = round_half_even(x / s) over the block's bf16 rows x.  The block that a sequence has not filled yet, its rest,
+ * stays in bf16 in the sequence's slot, so that what the cache holds depends on the tokens and not on the calls that brought
+ * them.  A block with a value that is not finite has the scale NaN: all of it is NaN.
+ *   data   int8 [pages][2][HK][8192]: keys [8 groups of 32 dims][32 tokens][32 dims]; values [256 dims][32 tokens, in fours
+ *          in the order 0 4 2 6 1 5 3 7]
+ *   scales fp32 [pages][2][HK]
+ *   recent bf16 [n_slots][2][HK][32][256]
+ *   table  int32 [B][width], rows ldt apart: the page of block j of sequence b; pages may be shared
+ *   lens   int32 [B]: the sequence's tokens (clamped to 0 .. 32 width + 31); slots int32 [B]: its slot, NULL: b
+ * starts / B / T: the call's rows, packed as in mica_attention_packed.  All of these in device memory; data and recent 16-byte
+ * aligned.  A block without a page (an entry outside 0 .. pages - 1, or past the table) is not stored, and reads as NaN; a
+ * sequence whose slot is outside 0 .. n_slots - 1 is not stored, and its rest reads as NaN.  No counterpart in the reference,
+ * which keeps its keys and values in bf16, one tensor a prefix (prefill_engine.py:218-226).
+ */
+
+/*
+ * New rows into the cache: row i of sequence b becomes its token lens[b] + i (lens as before the call; the caller adds the rows
+ * afterwards).  k / v: bf16, head j of row t at ptr + j sh + t ld (elements, % 8), 16-byte aligned, not changed.  Before a key
+ * is stored its head is normed, (x / sqrt(mean(x^2) + norm_eps)) (norm_offset + w), with norm_w (bf16 [256]; NULL: not), then
+ * rotated over its first rot_dim dims (0: not; 16, 32, 64, 128 or 256): (x_i, x_{i + rot_dim / 2}) -> (x_i cos - x_{i +
+ * rot_dim / 2} sin, x_{i + rot_dim / 2} cos + x_i sin) with cos_tab / sin_tab [n_pos][rot_dim / 2] (MICA_BF16 or MICA_FP32,
+ * 16-byte aligned) at the row's position pos[t] (int32 [T]; NULL: lens[b] + i), not at all outside the tables.  Both in fp32,
+ * rounded to bf16 once.  longest as in mica_attention_packed.  Two sequences of one call must not share a slot or a page that
+ * the call writes.
+ */
+int mica_kv_append(const void *k, long long shk, long long ldk, const void *v, long long shv, long long ldv, const int *starts,
+                   int B, int T, void *data, float *scales, void *recent, int pages, int n_slots, int HK, int head_dim,
+                   const int *table, long long ldt, int width, const int *lens, const int *slots, const void *norm_w,
+                   float norm_offset, float norm_eps, int rot_dim, const void *cos_tab, const void *sin_tab, int tab_dtype,
+                   int n_pos, const int *pos, int longest, mica_stream_t stream);
+
+/*
+ * The cache's rows back in bf16, each value rounded once: k / v [T][HK][256], contiguous, 16-byte aligned; the n rows of sequence
+ * b are its last n tokens (zeros for those before its first, and for rows of no sequence).
+ */
+int mica_kv_read(void *k, void *v, const int *starts, int B, int T, const void *data, const float *scales, const void *recent,
+                 int pages, int n_slots, int HK, int head_dim, const int *table, long long ldt, int width, const int *lens,
+                 const int *slots, mica_stream_t stream);
+
+/*
+ * Attention of each sequence's last rows over the cache, HQ = 4 HK: row i of the n of sequence b is at position p = lens[b] - n
+ * + i (its keys and values are in the cache already) and sees the tokens 0 .. p:
+ *   o[t, h] = sum_{u <= p} softmax_u(scale q[t, h] . key_u[h / 4]) value_u[h / 4];   zeros where p < 0.
+ * q / o, fill, scale, longest, workspace and values that are not finite as in mica_attention_packed.  The products are of int8
+ * values, exact in bf16: a block's scales multiply its scores and weights in fp32, before the weights are rounded.
+ */
+int mica_attention_paged(const void *q, long long shq, long long ldq, void *o, long long sho, long long ldo, const int *starts,
+                         int B, int T, int HQ, const void *data, const float *scales, const void *recent, int pages,
+                         int n_slots, int HK, int head_dim, const int *table, long long ldt, int width, const int *lens,
+                         const int *slots, float scale, int fill, int longest, void *workspace, long long workspace_bytes,
+                         mica_stream_t stream);
+long long mica_attention_paged_workspace_bytes(int B, int T, int HK, int width, int longest);
+
 /* ---- gated delta net (GDN) token mixer ------------------------------------------------------- */
 
 /*

@@ -33,6 +33,9 @@ _I = ctypes.c_int
 _F = ctypes.c_float
 _LL = ctypes.c_longlong
 
+# the paged cache: data, scales, recent, pages, slots, heads, head dim, table, its row stride and width, lens, slots
+_PAGED = [_P, _P, _P, _I, _I, _I, _I, _P, _LL, _I, _P, _P]
+
 # name -> (restype, argtypes); the order of arguments is that of include/mica_amd.h
 SIGNATURES = {
     "mica_version": (_I, []),
@@ -77,6 +80,12 @@ SIGNATURES = {
     "mica_attention_tree_workspace_bytes": (_LL, [_I, _I, _I, _I]),
     "mica_attention_window": (_I, [*[_P, _LL, _LL, _LL] * 4, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P, _P, _LL, _P]),
     "mica_attention_window_workspace_bytes": (_LL, [_I, _I, _I, _I, _I, _I]),
+    "mica_attention_packed": (_I, [*[_P, _LL, _LL] * 4, _P, _I, _I, _I, _I, _I, _F, _I, _I, _P, _LL, _P]),
+    "mica_attention_packed_workspace_bytes": (_LL, [_I, _I, _I, _I]),
+    "mica_kv_append": (_I, [*[_P, _LL, _LL] * 2, _P, _I, _I, *_PAGED, _P, _F, _F, _I, _P, _P, _I, _I, _P, _I, _P]),
+    "mica_kv_read": (_I, [_P, _P, _P, _I, _I, *_PAGED, _P]),
+    "mica_attention_paged": (_I, [*[_P, _LL, _LL] * 2, _P, _I, _I, _I, *_PAGED, _F, _I, _I, _P, _LL, _P]),
+    "mica_attention_paged_workspace_bytes": (_LL, [_I, _I, _I, _I, _I]),
     "mica_causal_conv1d": (_I, [_P, _LL, _I, _P, _P, _I, _I, _P, _P, _P, _LL, _I, _I, _I, _I, _I, _I, _F, _P]),
     "mica_gdn_chunk": (_I, [_P, _LL, _I, _P, _LL, _I, _P, _LL, _I, _P, _P, _I, _P, _P, _P, _F, _I, _I, _I, _I, _P,
                             _LL, _P]),

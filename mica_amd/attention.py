@@ -8,7 +8,7 @@ head, and returns o [B, S, HQ, 256] bf16 (the O projection's [B * S, HQ * 256] r
 GPU only; no fallback.
 
 ``tree_attention`` and ``window_attention`` take the same heads: a tree of drafted tokens over a cache, and causal attention
-within a sliding window.
+within a sliding window.  ``packed_attention`` takes prompts of different lengths packed one behind the other.
 """
 from __future__ import annotations
 
@@ -334,3 +334,76 @@ def window_attention(q, k, v, window: int, sinks: int = 0, scale: float | None =
     return _cache_call("mica_attention_window", q, nbytes, lambda o, so, ws, st: L.mica_attention_window(
         q.data_ptr(), *sq, k.data_ptr(), *sk, v.data_ptr(), *sv, o, *so, B, Sq, Sk, HQ, HK, HEAD_DIM, scale, window,
         sinks, n_len, ws, nbytes, st))
+
+
+def _rows(t, what, dev=None):
+    """Checks a bf16 [T, heads, 256] view; its (head, row) strides, those of axes of one element as 0."""
+    if not t.is_cuda:
+        raise ValueError("mica_amd attention runs on the GPU only (got a CPU tensor)")
+    if t.dim() != 3 or t.dtype != torch.bfloat16 or t.shape[2] != HEAD_DIM or t.stride(2) != 1:
+        raise ValueError(f"{what} must be a bf16 [T, heads, 256] tensor with unit feature stride")
+    if dev is not None and t.device != dev:
+        raise ValueError(f"{what} is on another device than the others")
+    return tuple(t.stride(i) if t.shape[i] > 1 else 0 for i in (1, 0))
+
+
+def _starts(starts, dev):
+    """Checks the packed sequences' starts, int32 [B + 1]; B."""
+    if starts.dtype != torch.int32 or starts.device != dev or starts.dim() != 1 or not starts.numel() or not starts.is_contiguous():
+        raise ValueError("starts must be a contiguous int32 [B + 1] tensor on the rows' device")
+    return starts.numel() - 1
+
+
+def _hint(longest):
+    longest = 0 if longest is None else int(longest)
+    if longest < 0:
+        raise ValueError("longest must not be negative")
+    return min(longest, 2 ** 31 - 1)
+
+
+def _out(out, q):
+    """The output [T, HQ, 256] of packed rows (None: a new one), its strides, and whether rows of no sequence become zeros."""
+    if out is None:
+        o = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
+        return o, (o.stride(1), o.stride(0)), 1
+    so = _rows(out, "out", q.device)
+    if out.shape != q.shape:
+        raise ValueError("out must have q's shape")
+    if any(n > 1 and st < HEAD_DIM for n, st in zip(out.shape[1::-1], so)):
+        raise ValueError("out's rows and heads must not overlap")
+    return out, so, 0
+
+
+def packed_attention(q, k, v, starts, longest: int | None = None, scale: float | None = None, out=None):
+    """Causal attention over prompts of different lengths packed one behind the other, without padding
+    (mica_attention_packed).
+
+    q [T, HQ, 256], k / v [T, HK, 256]: bf16 views with unit feature stride (e.g. of the fused QKV rows), positions applied,
+    HQ = 4 HK.  starts: int32 [B + 1] on the device, not falling: rows starts[b] .. starts[b + 1] - 1 are sequence b's, and each
+    attends to those up to itself; a sequence may be empty.  longest: the longest sequence's rows where the host knows it (a
+    hint: it changes the division of the work and so roundings, not what is computed).  Strides of whole 16 bytes, rows of k
+    and v at least 256 elements apart.  Returns o [T, HQ, 256] bf16, zeros in rows of no sequence; with out= (such a view) that,
+    whose rows of no sequence are left as they were."""
+    scale = _scale(scale)
+    sq, sk, sv = _rows(q, "q"), _rows(k, "k", q.device), _rows(v, "v", q.device)
+    dev = q.device
+    T, HQ, _ = q.shape
+    HK = k.shape[1]
+    if k.shape != v.shape or k.shape[0] != T or HQ != GROUP * HK:
+        raise ValueError("q / k / v shapes do not match (4 query heads per key/value head, one key per row)")
+    B, longest = _starts(starts, dev), _hint(longest)
+    if not _gpu_ok(dev):
+        raise RuntimeError(f"mica_amd kernels need a gfx950 GPU (device {dev})")
+    L = _lib.load()
+    o, so, fill = _out(out, q)
+    nbytes = int(L.mica_attention_packed_workspace_bytes(B, T, HK, longest))
+    if nbytes < 0:
+        raise ValueError("attention: invalid sizes")
+    ws = torch.empty((max(nbytes, 16),), dtype=torch.uint8, device=dev)
+    rc = _lib.check(_on(dev, lambda: L.mica_attention_packed(
+        q.data_ptr(), *sq, k.data_ptr(), *sk, v.data_ptr(), *sv, o.data_ptr(), *so, starts.data_ptr(), B, T, HQ, HK, HEAD_DIM,
+        scale, fill, longest, ws.data_ptr(), nbytes, _stream(dev))), "mica_attention_packed")
+    if rc:
+        raise ValueError(f"attention: unsupported input ({_lib.status_name(rc)})")
+    _launched()
+    return o

@@ -161,31 +161,6 @@ struct Stream {
     }
 };
 
-// A V value (bf16 code) that is not finite as the largest finite value of its sign, NaN with the given sign (0 or 0x8000);
-// 0 for a finite one.  Times 2^127 and summed by the matrix cores these give +-inf, and, with both signs, NaN.
-MICA_DEVICE uint32_t odd_value(uint32_t h, uint32_t nan_sign) {
-    if ((h & 0x7f80u) != 0x7f80u) return 0u;
-    return 0x7f7fu | ((h & 0x7fu) ? nan_sign : (h & 0x8000u));
-}
-
-// A workgroup barrier that waits for nothing else; no access to memory moves across it.
-MICA_DEVICE void meet() {
-    __asm__ volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    __asm__ volatile("" ::: "memory");
-}
-
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-// A transposing read.  The compiler knows nothing of what the DMA in flight writes, and would let every one of these reads
-// wait for all of it, the next tile's too.  `w`, which nothing is accessed through, says that the read meets no unknown
-// store; the waits are the loop's own.  (16 x 64 nodes after 4000 keys 97.9 -> 94.5 us, 2 x 32 nodes after 10000 38.3 -> 36.)
-MICA_DEVICE s16x4 tr_read(lds_s16x4 *p, lds_void *__restrict w) {
-    const s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(p);
-    __builtin_assume(w != nullptr);
-    return x;
-}
-
 // What bounds it, and the whole call's time (at the rates of a large copy, 4.87 TB/s, and a large matrix product, 1401
 // TFLOP/s): few rows, the cache's bytes: 64 single tokens with a window of 4096 take 190 us, 5.7 TB/s; 32 x 16 nodes over up
 // to 4096 keys 97 us of 86.  Many rows, the matrix cores beside the softmax, with two waves a SIMD: 16384 tokens with a

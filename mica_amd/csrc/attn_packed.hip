@@ -1,0 +1,294 @@
+// Causal grouped-query attention over prompts of different lengths packed one behind the other (mica_attention_packed), head
+// dim 256, 4 query heads per key/value head.
+//
+//   o[t, h] = sum_{u in seq(t), u <= t} softmax_u(scale q[t, h] . k[u, h / 4]) v[u, h / 4]
+//
+// Work split: a workgroup takes one key/value head and a block of 32 rows of one sequence; wave w takes query head 4 hk + w, so
+// that every tile of 32 keys brought into LDS serves four heads.  It computes S^T = K Q^T (32 keys x 32 rows,
+// v_mfma_f32_32x32x16_bf16), the online softmax of its rows (a lane holds 16 of a row's 32 scores, lane l ^ 32 the others) and
+// O^T += V^T P^T.  Blocks are found on the device from the sequences' starts, so that nothing is padded.
+//
+// Data movement: K and V tiles come by LDS DMA into two stages in turn, 16-byte chunks XOR-swizzled by row, rows past the
+// sequence's end as zeros (the buffer's range check); V is kept as it lies in memory and its V^T fragments are transposing
+// reads (ds_read_b64_tr_b16: 16 lanes fetch 4 keys x 16 dims and each gets the 4 keys of one dim).
+#include "attn_common.h"
+#include "ragged.h"
+
+namespace {
+
+constexpr int kD = 256;             // head dim
+constexpr int kGroup = 4;           // query heads per key/value head, a wave each
+constexpr int kB = 32;              // rows of a block, keys of a tile
+constexpr int kThreads = 64 * kGroup;
+constexpr int kTile = kB * kD * 2;  // 16 KB of K or V
+constexpr int kStage = 2 * kTile;
+
+struct PackedParams {
+    const uint16_t *q; long long shq, ldq; // head h of row t: q + h shq + t ldq
+    const uint16_t *k; long long shk, ldk;
+    const uint16_t *v; long long shv, ldv;
+    uint16_t *o; long long sho, ldo;
+    Ragged rows;
+    int HK, fill;                          // fill: rows of no sequence become zeros
+    float scale_log2;                      // softmax scale x log2(e)
+};
+
+// zeros for rows i0 .. i0 + 31 of those that no sequence has (the rows before the first and behind the last sequence)
+MICA_DEVICE void fill_rows(const PackedParams &p, int hk, int i0) {
+    const int before = p.rows.at(0), behind = p.rows.at(p.rows.B);
+    for (int x = threadIdx.x; x < kB * kGroup * (kD / 8); x += kThreads) {
+        const int i = i0 + x / (kGroup * (kD / 8)), c = x % (kGroup * (kD / 8));
+        const long long t = i < before ? i : (long long)behind + i - before;
+        if (t < p.rows.T) *(u32x4 *)(p.o + (hk * kGroup + c / (kD / 8)) * p.sho + t * p.ldo + c % (kD / 8) * 8) = u32x4{0u, 0u, 0u, 0u};
+    }
+}
+
+__global__ __launch_bounds__(kThreads, 2) void pk_fwd_kernel(PackedParams p) {
+    constexpr int kSmem = kGroup * kB * kD * 2 > 2 * kStage ? kGroup * kB * kD * 2 : 2 * kStage; // the stages; the output, in the end
+    __shared__ __attribute__((aligned(1024))) int8_t smem[kSmem + 16];
+    int *const odd_tile = (int *)(smem + kSmem); // whether the diagonal tile holds a value that is not finite
+
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
+    const int hk = blockIdx.x % p.HK, id = blockIdx.x / p.HK;
+    int b, u;
+    if (!find_unit(p.rows.B, [&](int i) { return (p.rows.rows(i) + kB - 1) / kB; }, id, b, u)) {
+        if (p.fill) fill_rows(p, hk, (id - b) * kB);
+        return;
+    }
+    b = __builtin_amdgcn_readfirstlane(b), u = __builtin_amdgcn_readfirstlane(u);
+    const int first = p.rows.at(b), n = p.rows.rows(b);
+    const int qb = (n + kB - 1) / kB - 1 - u; // a sequence's longest blocks first
+    const int q0 = qb * kB;
+
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void *)smem;
+    const uint16_t *const kb = p.k + hk * p.shk + (long long)first * p.ldk;
+    const uint16_t *const vb = p.v + hk * p.shv + (long long)first * p.ldv;
+    // DMA of tile i into stage st; past the block's last from a zero-sized buffer
+    auto issue = [&](int i, int st) {
+        const int rows = i <= qb ? min(n - i * kB, kB) : 0;
+        const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
+            (void *)(kb + (long long)i * kB * p.ldk), 0, rows > 0 ? (int)((rows - 1) * p.ldk * 2) + kD * 2 : 0, kBufferFlags);
+        const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
+            (void *)(vb + (long long)i * kB * p.ldv), 0, rows > 0 ? (int)((rows - 1) * p.ldv * 2) + kD * 2 : 0, kBufferFlags);
+        // 1 KB block x = key rows 2 x + hi; chunk c of row r lies at c ^ (r % 16) (K), c ^ 4 (r % 4) (V).  The offsets come from
+        // an opaque copy of the lane id at every tile: hoisted out of the loop they take registers that the tiles need.
+        int ln = lane;
+        __asm__ volatile("" : "+v"(ln));
+        const int r0 = 8 * wave + (ln >> 5), k2 = (int)(p.ldk * 2), v2 = (int)(p.ldv * 2);
+        const int rk0 = r0 * k2, rv0 = r0 * v2;
+        int8_t *s = smem + st * kStage + 4 * wave * 1024;
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void *)(s + x * 1024), 16,
+                                                     rk0 + 2 * x * k2 + (((ln & 31) ^ ((r0 + 2 * x) & 15)) << 4), 0, 0, 0);
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void *)(s + kTile + x * 1024), 16,
+                                                     rv0 + 2 * x * v2 + (((ln & 31) ^ (((r0 + 2 * x) & 3) << 2)) << 4), 0, 0, 0);
+    };
+    // Q fragments (B operand of S^T: dims 16 s + 8 hi .. + 7 of row q0 + l % 32); rows past the sequence repeat its last
+    bf16x8 qf[kD / 16];
+    {
+        const uint16_t *qr = p.q + (hk * kGroup + wave) * p.shq + (long long)(first + min(q0 + l32, n - 1)) * p.ldq + hi * 8;
+#pragma unroll
+        for (int s = 0; s < kD / 16; ++s) qf[s] = __builtin_bit_cast(bf16x8, *(const u32x4 *)(qr + s * 16));
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    issue(0, 0);
+    if (tid == 0) *odd_tile = 0;
+    wait_lgkmcnt0(); // seen by every wave after the first tile's barrier
+    f32x16 O[kD / 32];
+#pragma unroll
+    for (int dt = 0; dt < kD / 32; ++dt) O[dt] = f32x16{};
+    float m = -__builtin_inff(), lsum = 0.0f;
+
+    // V^T fragment of 32-dim tile dt, step s: keys 16 s + 4 hi .. + 3 and 16 s + 8 + 4 hi .. + 3 (the keys of P^T's accumulator
+    // rows 8 s .. 8 s + 7) of dim 32 dt + l % 32
+    const int vrow = 4 * hi + ((l32 & 15) >> 2);
+    const int vchunk = (2 * (l32 >> 4) + ((l32 & 3) >> 1)) ^ ((vrow & 3) << 2);
+    const uint32_t vbase = lds0 + kTile + vrow * (kD * 2) + (vchunk << 4) + (l32 & 1) * 8;
+    // K fragment s: chunk 2 s + hi of key row l % 32, at chunk ^ (l % 16)
+    const uint32_t kbase = lds0 + l32 * (kD * 2) + ((hi ^ (l32 & 15)) << 4);
+    typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+    auto kfrag = [](uint32_t stage, int s) { return __builtin_bit_cast(bf16x8, *(lds_u32x4 *)(uintptr_t)((stage ^ (s << 5)))); };
+    auto vfrag = [&](uint32_t stage, int s, int dt) {
+        const uint32_t a = (stage ^ (dt << 6)) + s * 16 * (kD * 2);
+        const s16x4 x = tr_read((lds_s16x4 *)(uintptr_t)a, (lds_void *)smem);
+        const s16x4 y = tr_read((lds_s16x4 *)(uintptr_t)(a + 8 * (kD * 2)), (lds_void *)smem);
+        return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    constexpr int kPf = 3; // operand fragments read ahead
+#pragma unroll 1
+    for (int i = 0; i <= qb; ++i) {
+        const int st = i & 1;
+        // this wave's DMA of tile i landed; after the barrier every wave's has, and nobody reads tile i - 1 any more
+        wait_vmcnt<0>();
+        meet();
+        __builtin_amdgcn_sched_barrier(0);
+        issue(i + 1, 1 - st);
+        const int8_t *stage = smem + st * kStage;
+        const uint32_t ks = kbase + st * kStage, vs = vbase + st * kStage;
+        // ---- S^T = K Q^T: rows = keys of the tile, column = this lane's row ----
+        f32x16 sc = {};
+        __builtin_amdgcn_s_setprio(1);
+        bf16x8 kf[kPf];
+#pragma unroll
+        for (int s = 0; s < kPf; ++s) kf[s] = kfrag(ks, s);
+#pragma unroll
+        for (int s = 0; s < kD / 16; ++s) {
+            const bf16x8 a = kf[s % kPf];
+            if (s + kPf < kD / 16) kf[s % kPf] = kfrag(ks, s + kPf);
+            __builtin_amdgcn_sched_barrier(0);
+            sc = mfma_bf16(a, qf[s], sc);
+        }
+        __builtin_amdgcn_s_setprio(0);
+        // ---- the diagonal tile: score r of a lane is key 8 (r / 4) + 4 hi + r % 4, seen by rows from it on ----
+        if (i == qb) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sc[r] = 8 * (r >> 2) + 4 * hi + (r & 3) <= l32 ? sc[r] : -__builtin_inff();
+        }
+        // ---- online softmax in log2 units; the reference moves only when the maximum exceeds it by more than 8 ----
+        float mx = -__builtin_inff();
+#pragma unroll
+        for (int r = 0; r < 16; ++r) mx = __builtin_fmaxf(mx, sc[r]);
+        mx = half_swap_max(mx) * p.scale_log2;
+        const bool grow = mx > m + 8.0f;
+        const float alpha = grow ? __builtin_amdgcn_exp2f(m - mx) : 1.0f;
+        if (grow) m = mx;
+        if (__builtin_amdgcn_ballot_w64(grow)) {
+#pragma unroll
+            for (int dt = 0; dt < kD / 32; ++dt) O[dt] *= alpha;
+            lsum *= alpha;
+        }
+        const float ref = m == -__builtin_inff() ? 0.0f : m; // nothing but scores of -inf yet: exp2(-inf - 0) = 0
+        bf16x8 pb[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            u32x4 w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * s + 2 * e], p.scale_log2, -ref));
+                const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[8 * s + 2 * e + 1], p.scale_log2, -ref));
+                lsum += p0 + p1;
+                w[e] = pack_bf16x2(p0, p1); // the matrix cores' operand type; the sum keeps the unrounded weights
+            }
+            pb[s] = __builtin_bit_cast(bf16x8, w);
+        }
+        // A value that is not finite must not reach the rows before its own (0 x inf = NaN): looked for in the diagonal tile
+        // by all waves, each in its part.
+        if (i == qb) {
+            uint32_t odd = 0;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const u32x4 w = *(const u32x4 *)(stage + kTile + (4 * wave + x) * 1024 + lane * 16);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) odd |= (w[e] & 0x7f807f80u) + 0x00800080u;
+            }
+            if (__builtin_amdgcn_ballot_w64((odd & 0x80008000u) != 0) && lane == 0) *odd_tile = 1;
+            wait_lgkmcnt0();
+            meet();
+            if (*odd_tile) { // the same for every wave: into the rows that give their keys a weight, then zeros in their place
+                bf16x8 ind[2];
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    u32x4 w = __builtin_bit_cast(u32x4, pb[s]);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = ((w[e] & 0xffffu) ? 0x7f00u : 0u) | ((w[e] >> 16) ? 0x7f000000u : 0u);
+                    ind[s] = __builtin_bit_cast(bf16x8, w);
+                }
+#pragma unroll
+                for (int x = 0; x < 4 * (kD / 32); ++x) {
+                    const int s = x & 1, dt = x >> 2;
+                    const uint32_t sign = x & 2 ? 0x8000u : 0u;
+                    u32x4 w = __builtin_bit_cast(u32x4, vfrag(vs, s, dt));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = odd_value(w[e] & 0xffffu, sign) | (odd_value(w[e] >> 16, sign) << 16);
+                    O[dt] = mfma_bf16(__builtin_bit_cast(bf16x8, w), ind[s], O[dt]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                __syncthreads();
+#pragma unroll 1
+                for (int x = tid; x < kTile / 4; x += kThreads) {
+                    uint32_t *w = (uint32_t *)(smem + st * kStage + kTile) + x;
+                    *w &= (odd_value(*w & 0xffffu, 0) ? 0u : 0xffffu) | (odd_value(*w >> 16, 0) ? 0u : 0xffff0000u);
+                }
+                __syncthreads();
+            }
+        }
+        // ---- O^T += V^T P^T ----
+        __builtin_amdgcn_s_setprio(1);
+        bf16x8 vf[kPf];
+#pragma unroll
+        for (int x = 0; x < kPf; ++x) vf[x] = vfrag(vs, x >> 3, x & 7);
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+            const bf16x8 a = vf[x % kPf];
+            if (x + kPf < 16) vf[x % kPf] = vfrag(vs, (x + kPf) >> 3, (x + kPf) & 7);
+            __builtin_amdgcn_sched_barrier(0);
+            O[x & 7] = mfma_bf16(a, pb[x >> 3], O[x & 7]);
+        }
+        __builtin_amdgcn_s_setprio(0);
+    }
+    wait_vmcnt<0>(); // the last (empty) loads have written before the stages are used again
+    // ---- normalise (a row whose scores are all -inf has no softmax: 0 / 0), stage in LDS, write 16-byte row pieces ----
+    const float inv = 1.0f / half_swap_sum(lsum);
+    __syncthreads();
+#pragma unroll
+    for (int dt = 0; dt < kD / 32; ++dt)
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+            const int d = dt * 32 + 8 * r4 + 4 * hi;
+            u32x2 w;
+            w[0] = pack_bf16x2(O[dt][4 * r4] * inv, O[dt][4 * r4 + 1] * inv);
+            w[1] = pack_bf16x2(O[dt][4 * r4 + 2] * inv, O[dt][4 * r4 + 3] * inv);
+            *(u32x2 *)(smem + (wave * kB + l32) * (kD * 2) + (((d >> 3) ^ l32) << 4) + (d & 4) * 2) = w;
+        }
+    __syncthreads();
+#pragma unroll 2
+    for (int x = tid; x < kGroup * kB * 32; x += kThreads) {
+        const int rr = x >> 5, ch = x & 31, t = q0 + rr % kB;
+        if (t < n)
+            *(u32x4 *)(p.o + (long long)(hk * kGroup + rr / kB) * p.sho + (long long)(first + t) * p.ldo + ch * 8) =
+                *(const u32x4 *)(smem + rr * (kD * 2) + ((ch ^ (rr & 31)) << 4));
+    }
+}
+
+}  // namespace
+
+extern "C" int mica_attention_packed(const void *q, long long shq, long long ldq, const void *k, long long shk, long long ldk,
+                                     const void *v, long long shv, long long ldv, void *o, long long sho, long long ldo,
+                                     const int *starts, int B, int T, int HQ, int HK, int head_dim, float scale, int fill,
+                                     int longest, void *workspace, long long workspace_bytes, mica_stream_t stream) {
+    if (head_dim != kD || HK <= 0 || HK > (1 << 20) || HQ != HK * kGroup || B < 0 || T < 0) return MICA_MISS_SHAPE;
+    if (!(scale > 0.0f) || !(scale < __builtin_inff())) return MICA_MISS_ARG;
+    if (T == 0 || (B == 0 && !fill)) return 0;
+    if (!q || !k || !v || !o || !starts) return MICA_MISS_ARG;
+    if (T == 1) ldk = ldv = kD; // (never used; the range check of a tile counts on it)
+    for (long long x : {shq, ldq, shk, ldk, shv, ldv, sho, ldo})
+        if (x < 0 || x % 8) return MICA_MISS_STRIDE;
+    for (long long x : {ldk, ldv}) {
+        if (x < kD) return MICA_MISS_STRIDE;
+        if (x * 2 * kB >= (1LL << 31)) return MICA_MISS_RANGE; // a tile's rows within a buffer's range
+    }
+    if (!mica_aligned16(q) || !mica_aligned16(k) || !mica_aligned16(v) || !mica_aligned16(o) || ((uintptr_t)starts & 3))
+        return MICA_MISS_ALIGN;
+    // blocks of all sequences and of the rows of none: at most (n + 31) / 32 and n of each
+    const long long most = ((long long)T + 31ll * B + 31) / 32, units = most < T ? most : T;
+    if (units * HK >= (1 << 24)) return MICA_MISS_RANGE; // (a grid of 2^32 work-items wraps round)
+    PackedParams p{};
+    p.q = (const uint16_t *)q; p.shq = shq; p.ldq = ldq;
+    p.k = (const uint16_t *)k; p.shk = shk; p.ldk = ldk;
+    p.v = (const uint16_t *)v; p.shv = shv; p.ldv = ldv;
+    p.o = (uint16_t *)o; p.sho = sho; p.ldo = ldo;
+    p.rows = Ragged{starts, B, T};
+    p.HK = HK; p.fill = fill;
+    p.scale_log2 = scale * 1.44269504088896341f;
+    hipLaunchKernelGGL(pk_fwd_kernel, dim3((unsigned)(units * HK)), dim3(kThreads), 0, (hipStream_t)stream, p);
+    return mica_err(hipGetLastError());
+}
+
+extern "C" long long mica_attention_packed_workspace_bytes(int B, int T, int HK, int longest) {
+    if (B < 0 || T < 0 || HK <= 0) return -1;
+    return 0;
+}
