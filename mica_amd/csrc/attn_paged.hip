@@ -4,16 +4,16 @@
 //   o[t, h] = sum_{u <= p} softmax_u(scale q[t, h] . key_u[h / 4]) value_u[h / 4],   p = len - n + i  for row i of n
 //   key_u = s_K q_u for a block's scale s_K and int8 q_u, bf16 in the rest; values likewise; zeros where p < 0
 //
-// Work split: a workgroup takes one key/value head and a block of 8 R rows of one sequence, 32 R (row, head) pairs.  Each of
-// its R x D waves holds 32 of them: it computes S^T = K Q^T (32 keys x 32 pairs, v_mfma_f32_32x32x16_bf16), the online softmax
-// of its pairs (a lane holds 16 of a pair's 32 scores, lane l ^ 32 the others) and 256 / D dims of O^T += V^T P^T.
-//
 // The products are of whole numbers: int8 values are exact in bf16, so a block's key scale multiplies the scores and its value
 // scale the weights, once each, and nothing is rounded that a bf16 cache would not round.
 //
-// Data movement: a page's 16 KB of a head are 16 pieces of 1 KB, 16 bytes a lane, in the order of the matrix cores' operands.
-// Every wave loads its share of the next page into registers while this one is computed, widens it to bf16 once for all waves
-// and writes it to one of two LDS stages, from which every operand is one contiguous 16-byte read a lane.
+// Division: the tiles (pages, and the rest) of all units (a sequence's blocks of nb rows), one behind the other, are divided
+// evenly over runs, and a worker takes a run for one key/value head: it may end one unit and begin the next, so that
+// lengths that differ, or sequences that do not divide the chip, leave nothing idle.  pg_merge_kernel joins the partial
+// softmax states (fp32) of the units that are divided.  Everything is found on the device from starts and lens.
+//
+// Two kernels: few rows (pg_few_kernel: a worker is a wave, which takes pages from memory into registers by itself) and more
+// (pg_fwd_kernel: a worker is a workgroup, whose waves share each page through LDS).
 #include "attn_common.h"
 #include "paged.h"
 
@@ -32,6 +32,129 @@ struct PagedParams {
     Pages c;
     int fill;                              // rows of no sequence become zeros
     float scale_log2;                      // softmax scale x log2(e)
+    int nb;                                // rows of a unit: a workgroup's (or a wave's) pairs are 4 nb
+    int runs, least, begin;                // most runs; a run's fewest tiles; the tiles that a unit's beginning counts for
+    float4 *part_o;                        // partial O: [part][64 fours of dims][4 nb pairs]
+    float2 *part_ml;                       // partial (m, l): [part][4 nb pairs]
+};
+
+// zeros for rows i0 .. i0 + rows - 1 of those that no sequence has (the rows before the first and behind the last sequence)
+MICA_DEVICE void fill_rows(const PagedParams &p, int hk, int i0, int rows, int tid, int threads) {
+    const int before = p.rows.at(0), behind = p.rows.at(p.rows.B);
+    for (int x = tid; x < rows * kGroup * (kD / 8); x += threads) {
+        const int i = i0 + x / (kGroup * (kD / 8)), c = x % (kGroup * (kD / 8));
+        const long long t = i < before ? i : (long long)behind + i - before;
+        if (t < p.rows.T) *(u32x4 *)(p.o + (hk * kGroup + c / (kD / 8)) * p.sho + t * p.ldo + c % (kD / 8) * 8) = u32x4{0u, 0u, 0u, 0u};
+    }
+}
+
+// The row of all units' tiles and its division.  All lanes of a wave call and get the same; a lane reads every 64th
+// sequence's lengths.
+struct Walk {
+    int total, per;   // places in the row: tiles, and p.begin for each unit's beginning; those of a run
+    int x, sum, base; // this lane's sequence of the 64 from `base` on: its places, those up to and with it
+    MICA_DEVICE static int tiles(const PagedParams &p, int n, int len, int qb) {
+        const int last = len - n + min(n, (qb + 1) * p.nb) - 1;
+        return last < 0 ? 1 : last / kBK + 1; // (rows before the first token: a tile of which they see nothing)
+    }
+    MICA_DEVICE void take(const PagedParams &p, int from) {
+        const int b = from + (int)(threadIdx.x & 63);
+        base = from, x = 0;
+        if (b < p.rows.B) {
+            const int n = p.rows.rows(b), len = p.c.len(b);
+            for (int qb = 0; qb * p.nb < n; ++qb) x += tiles(p, n, len, qb) + p.begin;
+        }
+        sum = wave_scan(x);
+    }
+    MICA_DEVICE Walk(const PagedParams &p) {
+        total = 0;
+        for (int from = (p.rows.B - 1) & ~63; from >= 0; from -= 64) { // (the first 64 last: they are kept)
+            take(p, from);
+            total += __builtin_amdgcn_readlane(sum, 63);
+        }
+        per = max((total + p.runs - 1) / p.runs, p.least + p.begin);
+    }
+    // the unit at place `at` (below total), and the place where it begins; called once
+    MICA_DEVICE void find(const PagedParams &p, int at, int &b, int &qb, int &from) {
+        int before = 0;
+        for (;;) {
+            const unsigned long long past = __builtin_amdgcn_ballot_w64(before + sum > at);
+            if (past != 0 || base + 64 >= p.rows.B) {
+                const int l = past ? __builtin_ctzll(past) : 0;
+                b = __builtin_amdgcn_readfirstlane(base + l);
+                from = before + __builtin_amdgcn_readlane(sum - x, l);
+                break;
+            }
+            before += __builtin_amdgcn_readlane(sum, 63);
+            take(p, base + 64);
+        }
+        const int n = p.rows.rows(b), len = p.c.len(b);
+        qb = 0;
+        for (int t; (qb + 1) * p.nb < n && at >= from + (t = tiles(p, n, len, qb) + p.begin); ++qb) from += t;
+        qb = __builtin_amdgcn_readfirstlane(qb), from = __builtin_amdgcn_readfirstlane(from);
+    }
+};
+
+// A worker's place in its run: a unit, and the tiles of it that are this worker's
+struct Piece {
+    int b, qb;               // the unit
+    int left;                // places of the run that are left
+    int i0, i1, all;         // this worker's tiles; the unit's
+    int part;                // where the partial state goes, for one head
+    int n, len, first;       // the sequence's rows, tokens, first row
+    MICA_DEVICE bool begin(const PagedParams &p, int run) {
+        Walk w(p);
+        const int at = run * w.per;
+        if (at >= w.total) return false;
+        int from;
+        w.find(p, at, b, qb, from);
+        left = __builtin_amdgcn_readfirstlane(min(w.per, w.total - at));
+        i0 = __builtin_amdgcn_readfirstlane(at - from - p.begin);
+        part = 2 * run;
+        return open(p);
+    }
+    MICA_DEVICE bool next(const PagedParams &p) { // the run's next unit
+        left -= i1 - i0;
+        ++qb;
+        if (qb * p.nb >= n) {
+            qb = 0;
+            do {
+                if (++b >= p.rows.B) return false;
+            } while (__builtin_amdgcn_readfirstlane(p.rows.rows(b)) == 0);
+        }
+        i0 = -p.begin;
+        part |= 1; // (what lies between a run's first and last unit is whole)
+        return open(p);
+    }
+    MICA_DEVICE bool whole() const { return i0 == 0 && i1 == all; }
+
+private:
+    MICA_DEVICE bool open(const PagedParams &p) {
+        n = __builtin_amdgcn_readfirstlane(p.rows.rows(b));
+        len = __builtin_amdgcn_readfirstlane(p.c.len(b));
+        first = __builtin_amdgcn_readfirstlane(p.rows.at(b));
+        all = Walk::tiles(p, n, len, qb);
+        if (i0 < 0) left += i0, i0 = 0; // the rest of the unit's beginning
+        i1 = min(i0 + left, all);
+        return left > 0;
+    }
+};
+
+// Pages and scales of 64 tiles of a sequence, a lane each: one round trip to memory for all of them.
+struct Index {
+    int base, page;
+    float sk, sv;
+    MICA_DEVICE void load(const PagedParams &p, int b, int hk, int whole, int from) {
+        const int i = from + (int)(threadIdx.x & 63);
+        base = from;
+        page = i < whole ? p.c.page(b, i) : -1;
+        // (a block without a page: NaN, for the rows that see it)
+        sk = page >= 0 ? p.c.scales[p.c.index(page, 0, hk)] : __builtin_nanf("");
+        sv = page >= 0 ? p.c.scales[p.c.index(page, 1, hk)] : __builtin_nanf("");
+    }
+    MICA_DEVICE int page_of(int i) const { return __builtin_amdgcn_readlane(page, i - base); }
+    MICA_DEVICE float sk_of(int i) const { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sk), i - base)); }
+    MICA_DEVICE float sv_of(int i) const { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sv), i - base)); }
 };
 
 // four int8 as two packed bf16 pairs
@@ -41,166 +164,24 @@ MICA_DEVICE u32x2 widen4(uint32_t w) {
     x[1] = pack_bf16x2((float)(int8_t)(w >> 16), (float)((int32_t)w >> 24));
     return x;
 }
+MICA_DEVICE bf16x8 widen8(uint32_t a, uint32_t b) {
+    const u32x2 x = widen4(a), y = widen4(b);
+    return __builtin_bit_cast(bf16x8, u32x4{x[0], x[1], y[0], y[1]});
+}
 
-template <int R, int D>
-__global__ __launch_bounds__(64 * R * D, 2) void pg_fwd_kernel(PagedParams p) {
-    constexpr int kWaves = R * D, kThreads = 64 * kWaves;
-    constexpr int NB = 8 * R;               // rows of the workgroup
-    constexpr int NDT = kD / 32 / D;        // 32-dim tiles of O a wave holds
-    constexpr int kOwn = 16 / kWaves;       // pieces of a page a wave brings
-    constexpr int kSmem = R * 32 * kD * 2 > 2 * kStage ? R * 32 * kD * 2 : 2 * kStage; // the stages; the output, in the end
-    __shared__ __attribute__((aligned(1024))) int8_t smem[kSmem + 16];
-    int *const odd_rest = (int *)(smem + kSmem); // whether the rest holds a value that is not finite
-
-    const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int rb = wave / D, dt0 = (wave % D) * NDT;
-    const int hk = blockIdx.x % p.c.HK, id = blockIdx.x / p.c.HK;
-    int b, qb;
-    if (!find_unit(p.rows.B, [&](int i) { return (p.rows.rows(i) + NB - 1) / NB; }, id, b, qb)) {
-        if (p.fill) {
-            const int i0 = (id - b) * NB, before = p.rows.at(0), behind = p.rows.at(p.rows.B);
-            for (int x = tid; x < NB * kGroup * (kD / 8); x += kThreads) {
-                const int i = i0 + x / (kGroup * (kD / 8)), c = x % (kGroup * (kD / 8));
-                const long long t = i < before ? i : (long long)behind + i - before;
-                if (t < p.rows.T)
-                    *(u32x4 *)(p.o + (hk * kGroup + c / (kD / 8)) * p.sho + t * p.ldo + c % (kD / 8) * 8) = u32x4{0u, 0u, 0u, 0u};
-            }
-        }
-        return;
-    }
-    b = __builtin_amdgcn_readfirstlane(b), qb = __builtin_amdgcn_readfirstlane(qb);
-    const int first = p.rows.at(b), n = p.rows.rows(b), len = p.c.len(b), slot = p.c.slot(b);
-    const int q0 = qb * NB, from = len - n;                  // the block's first row; the position of the sequence's
-    const int last = from + min(n, q0 + NB) - 1;             // position of the block's last row
-    const int tiles = last < 0 ? 0 : last / kBK + 1, whole = len / kBK;
-
-    // this lane's pair: a row and a query head
-    const int pair = rb * 32 + l32, head = hk * kGroup + pair / NB, t = q0 + pair % NB, pos = from + t;
-    // Q fragments (B operand of S^T): step 2 c + e takes dims 32 c + 16 hi + 8 e .. + 7, as a page's bytes lie; rows past the
-    // last repeat it
-    bf16x8 qf[kD / 16];
-    {
-        const uint16_t *qr = p.q + head * p.shq + (long long)(first + min(t, n - 1)) * p.ldq + hi * 16;
-#pragma unroll
-        for (int s = 0; s < kD / 16; ++s) qf[s] = __builtin_bit_cast(bf16x8, *(const u32x4 *)(qr + (s >> 1) * 32 + (s & 1) * 8));
-    }
-    // Pieces 0 .. 7 of a page are keys (32 dims of each token), 8 .. 15 values (32 dims' rows); this wave brings kOwn of them.
-    u32x4 raw[kOwn];
-    float sk = 0.0f, sv = 0.0f, sk_next = 0.0f, sv_next = 0.0f;  // the tile's scales
-    auto fetch = [&](int i) { // tile i's pieces into registers, and its scales
-        if (i >= tiles) return;
-        if (i >= whole) { // (the rest: see below)
-            const bool bad = slot < 0;
-            sk_next = sv_next = bad ? __builtin_nanf("") : 1.0f;
-            return;
-        }
-        const int page = p.c.page(b, i);
-        // (a block without a page: NaN, for the rows that see it)
-        sk_next = page >= 0 ? p.c.scales[p.c.index(page, 0, hk)] : __builtin_nanf("");
-        sv_next = page >= 0 ? p.c.scales[p.c.index(page, 1, hk)] : __builtin_nanf("");
-#pragma unroll
-        for (int x = 0; x < kOwn; ++x) {
-            const int piece = wave * kOwn + x;
-            raw[x] = page >= 0 ? *(const u32x4 *)(p.c.block(page, piece >> 3, hk) + (piece & 7) * 1024 + l32 * 32 + hi * 16)
-                               : u32x4{0u, 0u, 0u, 0u};
-        }
-    };
-    // Tile i into LDS stage st: piece x becomes two operands of 64 lanes x 16 bytes.  Keys: bytes 8 e .. 8 e + 7 are step
-    // 2 c + e's; values: fours s and s + 2 are step s's (tokens 16 s + 4 hi .. + 3 and 8 more on: P^T's accumulator rows).
-    auto stage_in = [&](int i, int st) {
-        int8_t *s = smem + st * kStage + lane * 16;
-        if (i < whole) {
-#pragma unroll
-            for (int x = 0; x < kOwn; ++x) {
-                const int piece = wave * kOwn + x;
-                const u32x2 w0 = widen4(raw[x][0]), w1 = widen4(raw[x][1]), w2 = widen4(raw[x][2]), w3 = widen4(raw[x][3]);
-                const bool value = piece >= 8;
-                u32x4 a = {w0[0], w0[1], w1[0], w1[1]}, c = {w2[0], w2[1], w3[0], w3[1]};
-                if (value) a = u32x4{w0[0], w0[1], w2[0], w2[1]}, c = u32x4{w1[0], w1[1], w3[0], w3[1]};
-                *(u32x4 *)(s + piece * 2048) = a;
-                *(u32x4 *)(s + piece * 2048 + 1024) = c;
-            }
-            return;
-        }
-        // The rest: bf16 rows, the same operands; zeros past its last token.
-        const int have = slot < 0 ? 0 : len - whole * kBK;
-        const uint16_t *kr = p.c.rest(max(slot, 0), 0, hk), *vr = p.c.rest(max(slot, 0), 1, hk);
-        uint32_t odd = 0;
-#pragma unroll 1
-        for (int x = 0; x < kOwn; ++x) {
-            const int piece = wave * kOwn + x;
-            u32x4 a = {}, c = {};
-            if (piece < 8) {
-                if (l32 < have) {
-                    const u32x4 *src = (const u32x4 *)(kr + l32 * kD + piece * 32 + hi * 16);
-                    a = src[0], c = src[1];
-                }
-            } else {
-                const uint16_t *src = vr + (piece - 8) * 32 + l32;
-                uint32_t w[16];
-#pragma unroll
-                for (int e = 0; e < 16; ++e) { // step e / 8, its token e % 8
-                    const int token = 16 * (e >> 3) + 8 * ((e >> 2) & 1) + 4 * hi + (e & 3);
-                    w[e] = token < have ? src[token * kD] : 0u;
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) a[e] = w[2 * e] | w[2 * e + 1] << 16, c[e] = w[8 + 2 * e] | w[9 + 2 * e] << 16;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) odd |= ((a[e] & 0x7f807f80u) + 0x00800080u) | ((c[e] & 0x7f807f80u) + 0x00800080u);
-            }
-            *(u32x4 *)(s + piece * 2048) = a;
-            *(u32x4 *)(s + piece * 2048 + 1024) = c;
-        }
-        if (__builtin_amdgcn_ballot_w64((odd & 0x80008000u) != 0) && lane == 0) *odd_rest = 1;
-    };
-    typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
-    const uint32_t base = (uint32_t)(uintptr_t)(lds_void *)smem + lane * 16;
-    auto kfrag = [](uint32_t a, int s) { return __builtin_bit_cast(bf16x8, *(lds_u32x4 *)(uintptr_t)(a + s * 1024)); };
-    auto vfrag = [&](uint32_t a, int s, int dt) {
-        return __builtin_bit_cast(bf16x8, *(lds_u32x4 *)(uintptr_t)(a + kTile + (dt0 + dt) * 2048 + s * 1024));
-    };
-
-    f32x16 O[NDT];
-#pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) O[dt] = f32x16{};
-    float m = -__builtin_inff(), lsum = 0.0f;
-    if (tid == 0) *odd_rest = 0;
-    __syncthreads();
-    fetch(0);
-#pragma unroll 1
-    for (int i = 0; i < tiles; ++i) {
-        const int st = i & 1;
-        stage_in(i, st);
-        sk = sk_next, sv = sv_next;
-        fetch(i + 1);
-        // every wave's pieces are there; nobody reads the other stage (tile i - 1) any more when tile i + 1 is written to it
-        wait_lgkmcnt0();
-        meet();
-        const uint32_t at = base + st * kStage;
-        // ---- S^T = K Q^T: rows = keys of the tile, column = this lane's pair ----
-        constexpr int kPf = 3; // operands read ahead
-        f32x16 sc = {};
-        __builtin_amdgcn_s_setprio(1);
-        bf16x8 kf[kPf];
-#pragma unroll
-        for (int s = 0; s < kPf; ++s) kf[s] = kfrag(at, s);
-#pragma unroll
-        for (int s = 0; s < kD / 16; ++s) {
-            const bf16x8 a = kf[s % kPf];
-            if (s + kPf < kD / 16) kf[s % kPf] = kfrag(at, s + kPf);
-            __builtin_amdgcn_sched_barrier(0);
-            sc = mfma_bf16(a, qf[s], sc);
-        }
-        __builtin_amdgcn_s_setprio(0);
-        const float scale = p.scale_log2 * sk;
-        // ---- keys past a row's position: score -inf (score r of a lane is key 8 (r / 4) + 4 hi + r % 4) ----
-        const bool masked = (i + 1) * kBK - 1 > from + q0;
+// The running softmax of a lane's pair, in log2 units relative to m
+struct Softmax {
+    float m, lsum;
+    MICA_DEVICE void clear() { m = -__builtin_inff(), lsum = 0.0f; }
+    // Scores sc of a tile (score r of a lane is key k0 + 8 (r / 4) + 4 hi + r % 4) become weights, unscaled ones in the sum and
+    // sv times them in sc; `masked`: keys past pos get none.  The reference moves only when the maximum exceeds it by more than
+    // 8, and then O with it.
+    template <int NDT>
+    MICA_DEVICE void add(f32x16 &sc, f32x16 (&O)[NDT], float scale, float sv, bool masked, int k0, int pos, int hi) {
         if (masked) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sc[r] = i * kBK + 8 * (r >> 2) + 4 * hi + (r & 3) <= pos ? sc[r] : -__builtin_inff();
+            for (int r = 0; r < 16; ++r) sc[r] = k0 + 8 * (r >> 2) + 4 * hi + (r & 3) <= pos ? sc[r] : -__builtin_inff();
         }
-        // ---- online softmax in log2 units; the reference moves only when the maximum exceeds it by more than 8 ----
         float mx = -__builtin_inff();
 #pragma unroll
         for (int r = 0; r < 16; ++r) mx = __builtin_fmaxf(mx, sc[r]);
@@ -214,94 +195,520 @@ __global__ __launch_bounds__(64 * R * D, 2) void pg_fwd_kernel(PagedParams p) {
             lsum *= alpha;
         }
         const float ref = m == -__builtin_inff() ? 0.0f : m; // a row that has seen nothing yet: exp2(-inf - 0) = 0
-        float pr[16];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            pr[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], scale, -ref));
-            if (masked) pr[r] = i * kBK + 8 * (r >> 2) + 4 * hi + (r & 3) <= pos ? pr[r] : 0.0f; // (a scale may be NaN)
+        for (int r = 0; r < 16; ++r) sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], scale, -ref));
+        if (masked && !(scale < __builtin_inff())) { // (a scale of NaN makes NaN of -inf)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sc[r] = k0 + 8 * (r >> 2) + 4 * hi + (r & 3) <= pos ? sc[r] : 0.0f;
         }
-        bf16x8 pb[2];
-        const bool odd_scale = !(sv < __builtin_inff());
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            u32x4 w;
+        for (int r = 0; r < 16; r += 2) lsum += sc[r] + sc[r + 1];
+        if (sv < __builtin_inff()) {
+            sc *= sv;
+        } else { // (a scale of NaN, and keys of no weight)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float p0 = pr[8 * s + 2 * e], p1 = pr[8 * s + 2 * e + 1];
-                lsum += p0 + p1;
-                float v0 = p0 * sv, v1 = p1 * sv;
-                if (odd_scale) v0 = p0 == 0.0f ? 0.0f : v0, v1 = p1 == 0.0f ? 0.0f : v1;
-                w[e] = pack_bf16x2(v0, v1); // the matrix cores' operand type; the sum keeps the unrounded weights
-            }
-            pb[s] = __builtin_bit_cast(bf16x8, w);
+            for (int r = 0; r < 16; ++r) sc[r] = sc[r] == 0.0f ? 0.0f : sc[r] * sv;
         }
-        // A value of the rest that is not finite must not reach the rows before its own (0 x inf = NaN): into the rows that give
-        // its key a weight, then zeros in its place.
-        if (i >= whole && *odd_rest) {
-            bf16x8 ind[2];
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                u32x4 w = __builtin_bit_cast(u32x4, pb[s]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = ((w[e] & 0xffffu) ? 0x7f00u : 0u) | ((w[e] >> 16) ? 0x7f000000u : 0u);
-                ind[s] = __builtin_bit_cast(bf16x8, w);
-            }
-#pragma unroll
-            for (int x = 0; x < 4 * NDT; ++x) {
-                const int s = x & 1, dt = x >> 2;
-                const uint32_t sign = x & 2 ? 0x8000u : 0u;
-                u32x4 w = __builtin_bit_cast(u32x4, vfrag(at, s, dt));
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w[e] = odd_value(w[e] & 0xffffu, sign) | (odd_value(w[e] >> 16, sign) << 16);
-                O[dt] = mfma_bf16(__builtin_bit_cast(bf16x8, w), ind[s], O[dt]);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            __syncthreads();
-#pragma unroll 1
-            for (int x = tid; x < kTile / 4; x += kThreads) {
-                uint32_t *w = (uint32_t *)(smem + st * kStage + kTile) + x;
-                *w &= (odd_value(*w & 0xffffu, 0) ? 0u : 0xffffu) | (odd_value(*w >> 16, 0) ? 0u : 0xffff0000u);
-            }
-            __syncthreads();
-        }
-        // ---- O^T += V^T P^T ----
-        constexpr int kPv = kPf < 2 * NDT ? kPf : 2 * NDT;
-        __builtin_amdgcn_s_setprio(1);
-        bf16x8 vf[kPv];
-#pragma unroll
-        for (int x = 0; x < kPv; ++x) vf[x] = vfrag(at, x / NDT, x % NDT);
-#pragma unroll
-        for (int x = 0; x < 2 * NDT; ++x) {
-            const bf16x8 a = vf[x % kPv];
-            if (x + kPv < 2 * NDT) vf[x % kPv] = vfrag(at, (x + kPv) / NDT, (x + kPv) % NDT);
-            __builtin_amdgcn_sched_barrier(0);
-            O[x % NDT] = mfma_bf16(a, pb[x / NDT], O[x % NDT]);
-        }
-        __builtin_amdgcn_s_setprio(0);
     }
-    // ---- normalise (a row whose scores are all -inf has no softmax: 0 / 0; one that sees no key: zeros), stage, write ----
-    const float inv = pos < 0 ? 0.0f : 1.0f / half_swap_sum(lsum);
-    __syncthreads();
+};
+
+// P^T operand of step s from the scores' place
+MICA_DEVICE bf16x8 weights(const f32x16 &w, int s) {
+    return __builtin_bit_cast(bf16x8, u32x4{pack_bf16x2(w[8 * s], w[8 * s + 1]), pack_bf16x2(w[8 * s + 2], w[8 * s + 3]),
+                                            pack_bf16x2(w[8 * s + 4], w[8 * s + 5]), pack_bf16x2(w[8 * s + 6], w[8 * s + 7])});
+}
+// 2^127 in the place of every weight that is not zero
+MICA_DEVICE bf16x8 indicators(const bf16x8 &x) {
+    u32x4 w = __builtin_bit_cast(u32x4, x);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = ((w[e] & 0xffffu) ? 0x7f00u : 0u) | ((w[e] >> 16) ? 0x7f000000u : 0u);
+    return __builtin_bit_cast(bf16x8, w);
+}
+// the values that are not finite of a V^T operand, see odd_value
+MICA_DEVICE bf16x8 odd_values(const bf16x8 &x, uint32_t sign) {
+    u32x4 w = __builtin_bit_cast(u32x4, x);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = odd_value(w[e] & 0xffffu, sign) | (odd_value(w[e] >> 16, sign) << 16);
+    return __builtin_bit_cast(bf16x8, w);
+}
+MICA_DEVICE uint32_t without_odd(uint32_t w) {
+    return w & ((odd_value(w & 0xffffu, 0) ? 0u : 0xffffu) | (odd_value(w >> 16, 0) ? 0u : 0xffff0000u));
+}
+// bits 15 and 31 are set where a packed value is not finite
+MICA_DEVICE uint32_t odd_bits(uint32_t w) { return (w & 0x7f807f80u) + 0x00800080u; }
+
+// A worker's state of its unit, left for pg_merge_kernel: (m, l) with l = -1 for a row that sees no key
+template <int NDT>
+MICA_DEVICE void leave(const PagedParams &p, long long part, int pair, int dt0, int hi, bool blind, const f32x16 (&O)[NDT],
+                       float m, float l) {
+    const int np = kGroup * p.nb;
+    if (pair >= np) return;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
-            const int d = (dt0 + dt) * 32 + 8 * r4 + 4 * hi;
             const f32x16 x = O[dt];
-            u32x2 w;
-            w[0] = pack_bf16x2(x[4 * r4] * inv, x[4 * r4 + 1] * inv);
-            w[1] = pack_bf16x2(x[4 * r4 + 2] * inv, x[4 * r4 + 3] * inv);
-            *(u32x2 *)(smem + pair * (kD * 2) + (((d >> 3) ^ l32) << 4) + (d & 4) * 2) = w;
+            p.part_o[(part * 64 + ((dt0 + dt) * 4 + r4) * 2 + hi) * np + pair] =
+                blind ? float4{0.0f, 0.0f, 0.0f, 0.0f} : float4{x[4 * r4], x[4 * r4 + 1], x[4 * r4 + 2], x[4 * r4 + 3]};
         }
-    __syncthreads();
-#pragma unroll 2
-    for (int x = tid; x < 32 * R * 32; x += kThreads) {
-        const int rr = x >> 5, ch = x & 31, tt = q0 + rr % NB;
-        if (tt < n)
-            *(u32x4 *)(p.o + (long long)(hk * kGroup + rr / NB) * p.sho + (long long)(first + tt) * p.ldo + ch * 8) =
-                *(const u32x4 *)(smem + rr * (kD * 2) + ((ch ^ (rr & 31)) << 4));
-    }
+    if (dt0 == 0 && hi == 0) p.part_ml[part * np + pair] = blind ? float2{-__builtin_inff(), -1.0f} : float2{m, l};
 }
+
+// ---- few rows: up to 8 of a sequence ----
+// A wave takes tiles by itself: a page's pieces go from memory straight into the registers of the matrix cores' operands, 16
+// bytes a lane, each loaded for the next tile as soon as this one's has been widened, so that a wave has a page (16 KB) in
+// flight all the time.  Nothing is shared, there is no barrier, and the matrix cores' time (of which a single row uses an
+// eighth) is hidden behind the memory's.  The weights are taken as two bf16 summands: they cost products that are free here.
+__global__ __launch_bounds__(256, 1) void pg_few_kernel(PagedParams p) {
+    __shared__ __attribute__((aligned(1024))) int8_t smem[4 * kTile]; // a wave's values of the rest
+    const int lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int worker = blockIdx.x * 4 + wave, hk = worker % p.c.HK, run = worker / p.c.HK;
+    if (run >= p.runs) return;
+    if (p.fill) {
+        const int none = p.rows.at(0) + p.rows.T - p.rows.at(p.rows.B);
+        for (int i = run * 32; i < none; i += p.runs * 32) fill_rows(p, hk, i, 32, lane, 64);
+    }
+    int8_t *const mine = smem + wave * kTile;
+    Piece w;
+    if (!w.begin(p, run)) return;
+    do {
+        const int q0 = w.qb * p.nb, from = w.len - w.n, whole = w.len / kBK;
+        const int t = q0 + (l32 >> 2), head = hk * kGroup + (l32 & 3), pos = from + t; // this lane's pair l32
+        // Q fragments (B operand of S^T): step 2 c + e takes dims 32 c + 16 hi + 8 e .. + 7, as a page's bytes lie; rows past the
+        // last repeat it
+        bf16x8 qf[kD / 16];
+        {
+            const uint16_t *qr = p.q + head * p.shq + (long long)(w.first + min(t, w.n - 1)) * p.ldq + hi * 16;
+#pragma unroll
+            for (int s = 0; s < kD / 16; ++s) qf[s] = __builtin_bit_cast(bf16x8, *(const u32x4 *)(qr + (s >> 1) * 32 + (s & 1) * 8));
+        }
+        f32x16 O[kD / 32];
+#pragma unroll
+        for (int dt = 0; dt < kD / 32; ++dt) O[dt] = f32x16{};
+        Softmax sm;
+        sm.clear();
+        const int end = min(w.i1, whole); // pages; then the rest
+        if (w.i0 < end) {
+            Index ix;
+            ix.load(p, w.b, hk, whole, w.i0);
+            const int at = l32 * 32 + hi * 16;
+            auto source = [&](int page, int side) { // nothing of a block without a page: zeros
+                return __builtin_amdgcn_make_buffer_rsrc((void *)p.c.block(max(page, 0), side, hk), 0, page >= 0 ? kPageBytes : 0,
+                                                         kBufferFlags);
+            };
+            auto piece = [&](const __amdgpu_buffer_rsrc_t &r, int x) {
+                return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, at + x * 1024, 0, 0));
+            };
+            u32x4 rk[8], rv[8];
+            {
+                const int page = ix.page_of(w.i0);
+                const __amdgpu_buffer_rsrc_t sk = source(page, 0), sv = source(page, 1);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) rk[x] = piece(sk, x);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) rv[x] = piece(sv, x);
+            }
+#pragma unroll 1
+            for (int i = w.i0; i < end; ++i) {
+                const float sk = ix.sk_of(i), sv = ix.sv_of(i);
+                if (i + 1 - ix.base == 64) ix.load(p, w.b, hk, whole, i + 1);
+                const int page = i + 1 < end ? ix.page_of(i + 1) : -1;
+                const __amdgpu_buffer_rsrc_t nk = source(page, 0), nv = source(page, 1);
+                f32x16 sc = {};
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {
+                    const bf16x8 a = widen8(rk[x][0], rk[x][1]), c = widen8(rk[x][2], rk[x][3]);
+                    rk[x] = piece(nk, x);
+                    sc = mfma_bf16(a, qf[2 * x], sc);
+                    sc = mfma_bf16(c, qf[2 * x + 1], sc);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                sm.add(sc, O, p.scale_log2 * sk, sv, (i + 1) * kBK - 1 > from + q0, i * kBK, pos, hi);
+                const bf16x8 h0 = weights(sc, 0), h1 = weights(sc, 1);
+                f32x16 lo;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) lo[r] = sc[r] - round_bf16(sc[r]);
+                const bf16x8 g0 = weights(lo, 0), g1 = weights(lo, 1);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {
+                    const bf16x8 a = widen8(rv[x][0], rv[x][2]), c = widen8(rv[x][1], rv[x][3]);
+                    rv[x] = piece(nv, x);
+                    O[x] = mfma_bf16(a, h0, O[x]);
+                    O[x] = mfma_bf16(c, h1, O[x]);
+                    O[x] = mfma_bf16(a, g0, O[x]);
+                    O[x] = mfma_bf16(c, g1, O[x]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        }
+        if (w.i1 > end) {
+            // The rest: keys from memory as operands, values by DMA into this wave's LDS (chunk c of row r at c ^ 4 (r % 4)),
+            // from where they are read transposed; zeros past the last token.
+            const int slot = __builtin_amdgcn_readfirstlane(p.c.slot(w.b)), have = slot < 0 ? 0 : w.len - whole * kBK;
+            const uint16_t *kr = p.c.rest(max(slot, 0), 0, hk);
+            const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void *)p.c.rest(max(slot, 0), 1, hk), 0,
+                                                                                 have * kD * 2, kBufferFlags);
+#pragma unroll
+            for (int x = 0; x < 16; ++x)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_void *)(mine + x * 1024), 16,
+                                                         (2 * x + hi) * (kD * 2) + ((l32 ^ (((2 * x + hi) & 3) << 2)) << 4), 0, 0, 0);
+            f32x16 sc = {};
+#pragma unroll
+            for (int s = 0; s < kD / 16; ++s) {
+                u32x4 a = {0u, 0u, 0u, 0u};
+                if (l32 < have) a = *(const u32x4 *)(kr + l32 * kD + (s >> 1) * 32 + hi * 16 + (s & 1) * 8);
+                sc = mfma_bf16(__builtin_bit_cast(bf16x8, a), qf[s], sc);
+            }
+            const float one = slot < 0 ? __builtin_nanf("") : 1.0f;
+            sm.add(sc, O, p.scale_log2 * one, one, true, whole * kBK, pos, hi);
+            bf16x8 pb[2] = {weights(sc, 0), weights(sc, 1)};
+            wait_vmcnt<0>();
+            __asm__ volatile("" ::: "memory");
+            uint32_t odd = 0;
+#pragma unroll 4
+            for (int x = 0; x < 16; ++x) {
+                const u32x4 v = *(const u32x4 *)(mine + x * 1024 + lane * 16);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) odd |= odd_bits(v[e]);
+            }
+            const uint32_t lds = (uint32_t)(uintptr_t)(lds_void *)mine;
+            const int vrow = 4 * hi + ((l32 & 15) >> 2);
+            const uint32_t vbase = lds + vrow * (kD * 2) + (((2 * (l32 >> 4) + ((l32 & 3) >> 1)) ^ ((vrow & 3) << 2)) << 4) + (l32 & 1) * 8;
+            auto vfrag = [&](int s, int dt) {
+                const uint32_t a = (vbase ^ (dt << 6)) + s * 16 * (kD * 2);
+                const s16x4 x = tr_read((lds_s16x4 *)(uintptr_t)a, (lds_void *)smem);
+                const s16x4 y = tr_read((lds_s16x4 *)(uintptr_t)(a + 8 * (kD * 2)), (lds_void *)smem);
+                return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+            };
+            // A value that is not finite must not reach the rows before its own (0 x inf = NaN): into the rows that give its key a
+            // weight, then zeros in its place.
+            if (__builtin_amdgcn_ballot_w64((odd & 0x80008000u) != 0)) {
+                const bf16x8 i0 = indicators(pb[0]), i1 = indicators(pb[1]);
+#pragma unroll
+                for (int dt = 0; dt < kD / 32; ++dt)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        O[dt] = mfma_bf16(odd_values(vfrag(x & 1, dt), x & 2 ? 0x8000u : 0u), x & 1 ? i1 : i0, O[dt]);
+                wait_lgkmcnt0();
+                __asm__ volatile("" ::: "memory");
+#pragma unroll 1
+                for (int x = lane; x < kTile / 4; x += 64) ((uint32_t *)mine)[x] = without_odd(((uint32_t *)mine)[x]);
+                wait_lgkmcnt0();
+                __asm__ volatile("" ::: "memory");
+            }
+#pragma unroll
+            for (int x = 0; x < 2 * (kD / 32); ++x) O[x >> 1] = mfma_bf16(vfrag(x & 1, x >> 1), pb[x & 1], O[x >> 1]);
+            wait_lgkmcnt0();
+        }
+        const float l = half_swap_sum(sm.lsum);
+        if (!w.whole()) {
+            leave(p, (long long)w.part * p.c.HK + (long long)hk, l32, 0, hi, pos < 0, O, sm.m, l);
+        } else if (t < w.n && (l32 >> 2) < p.nb) {
+            // (a row whose scores are all -inf has no softmax: 0 / 0; one that sees no key: zeros)
+            const float inv = 1.0f / l;
+            uint16_t *out = p.o + head * p.sho + (long long)(w.first + t) * p.ldo + 4 * hi;
+#pragma unroll
+            for (int dt = 0; dt < kD / 32; ++dt)
+#pragma unroll
+                for (int r4 = 0; r4 < 4; ++r4) {
+                    const f32x16 x = O[dt];
+                    u32x2 v = {pack_bf16x2(x[4 * r4] * inv, x[4 * r4 + 1] * inv), pack_bf16x2(x[4 * r4 + 2] * inv, x[4 * r4 + 3] * inv)};
+                    if (pos < 0) v = u32x2{0u, 0u};
+                    *(u32x2 *)(out + dt * 32 + 8 * r4) = v;
+                }
+        }
+    } while (w.next(p));
+}
+
+// ---- more rows ----
+// A workgroup's R x D waves share each page: every wave loads its share of the next one into registers while this one is
+// computed, widens it to bf16 once for all of them and writes it to one of two LDS stages, from which every operand is one
+// contiguous 16-byte read a lane.  A wave holds 32 (row, head) pairs: it computes S^T = K Q^T (32 keys x 32 pairs,
+// v_mfma_f32_32x32x16_bf16), the online softmax of its pairs (a lane holds 16 of a pair's 32 scores, lane l ^ 32 the others)
+// and 256 / D dims of O^T += V^T P^T.
+template <int R, int D>
+__global__ __launch_bounds__(64 * R * D, 2) void pg_fwd_kernel(PagedParams p) {
+    constexpr int kWaves = R * D, kThreads = 64 * kWaves;
+    constexpr int NDT = kD / 32 / D;        // 32-dim tiles of O a wave holds
+    constexpr int kOwn = 16 / kWaves;       // pieces of a page a wave brings
+    constexpr int kSmem = R * 32 * kD * 2 > 2 * kStage ? R * 32 * kD * 2 : 2 * kStage; // the stages; the output, in the end
+    __shared__ __attribute__((aligned(1024))) int8_t smem[kSmem + 16];
+    int *const odd_rest = (int *)(smem + kSmem); // whether the rest holds a value that is not finite
+
+    const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int rb = wave / D, dt0 = (wave % D) * NDT, pair = rb * 32 + l32;
+    const int hk = blockIdx.x % p.c.HK, run = blockIdx.x / p.c.HK;
+    if (p.fill) {
+        const int none = p.rows.at(0) + p.rows.T - p.rows.at(p.rows.B);
+        for (int i = run * 32; i < none; i += p.runs * 32) fill_rows(p, hk, i, 32, tid, kThreads);
+    }
+    Piece w;
+    if (!w.begin(p, run)) return;
+    do {
+        const int q0 = w.qb * p.nb, from = w.len - w.n, whole = w.len / kBK;
+        const int t = q0 + (pair >> 2), head = hk * kGroup + (pair & 3), pos = from + t; // this lane's pair
+        const int slot = __builtin_amdgcn_readfirstlane(p.c.slot(w.b)), have = slot < 0 ? 0 : w.len - whole * kBK;
+        // Q fragments (B operand of S^T): step 2 c + e takes dims 32 c + 16 hi + 8 e .. + 7, as a page's bytes lie; rows past the
+        // last repeat it
+        bf16x8 qf[kD / 16];
+        {
+            const uint16_t *qr = p.q + head * p.shq + (long long)(w.first + min(t, w.n - 1)) * p.ldq + hi * 16;
+#pragma unroll
+            for (int s = 0; s < kD / 16; ++s) qf[s] = __builtin_bit_cast(bf16x8, *(const u32x4 *)(qr + (s >> 1) * 32 + (s & 1) * 8));
+        }
+        // Pieces 0 .. 7 of a page are keys (32 dims of each token), 8 .. 15 values (32 dims' rows); this wave brings kOwn of them.
+        Index ix;
+        ix.load(p, w.b, hk, whole, w.i0);
+        u32x4 raw[kOwn];
+        auto fetch = [&](int i) { // tile i's pieces into registers
+            const int page = i < min(w.i1, whole) ? ix.page_of(i) : -1;
+            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+                (void *)p.c.block(max(page, 0), wave * kOwn >> 3, hk), 0, page >= 0 ? kPageBytes : 0, kBufferFlags);
+#pragma unroll
+            for (int x = 0; x < kOwn; ++x)
+                raw[x] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                       r, l32 * 32 + hi * 16, ((wave * kOwn + x) & 7) * 1024, 0));
+        };
+        // Tile i into LDS stage st: a piece becomes two operands of 64 lanes x 16 bytes.  Keys: bytes 8 e .. 8 e + 7 are step
+        // 2 c + e's; values: fours s and s + 2 are step s's (tokens 16 s + 4 hi .. + 3 and 8 more on: P^T's accumulator rows).
+        auto stage_in = [&](int i, int st) {
+            int8_t *s = smem + st * kStage + lane * 16;
+            if (i < whole) {
+#pragma unroll
+                for (int x = 0; x < kOwn; ++x) {
+                    const int piece = wave * kOwn + x;
+                    const u32x2 w0 = widen4(raw[x][0]), w1 = widen4(raw[x][1]), w2 = widen4(raw[x][2]), w3 = widen4(raw[x][3]);
+                    u32x4 a = {w0[0], w0[1], w1[0], w1[1]}, c = {w2[0], w2[1], w3[0], w3[1]};
+                    if (wave * kOwn >= 8) a = u32x4{w0[0], w0[1], w2[0], w2[1]}, c = u32x4{w1[0], w1[1], w3[0], w3[1]};
+                    *(u32x4 *)(s + piece * 2048) = a;
+                    *(u32x4 *)(s + piece * 2048 + 1024) = c;
+                }
+                return;
+            }
+            // The rest: bf16 rows, the same operands; zeros past its last token.
+            const uint16_t *kr = p.c.rest(max(slot, 0), 0, hk), *vr = p.c.rest(max(slot, 0), 1, hk);
+            uint32_t odd = 0;
+#pragma unroll 1
+            for (int x = 0; x < kOwn; ++x) {
+                const int piece = wave * kOwn + x;
+                u32x4 a = {}, c = {};
+                if (piece < 8) {
+                    if (l32 < have) {
+                        const u32x4 *src = (const u32x4 *)(kr + l32 * kD + piece * 32 + hi * 16);
+                        a = src[0], c = src[1];
+                    }
+                } else {
+                    const uint16_t *src = vr + (piece - 8) * 32 + l32;
+                    uint32_t v[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) { // step e / 8, its token e % 8
+                        const int token = 16 * (e >> 3) + 8 * ((e >> 2) & 1) + 4 * hi + (e & 3);
+                        v[e] = token < have ? src[token * kD] : 0u;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) a[e] = v[2 * e] | v[2 * e + 1] << 16, c[e] = v[8 + 2 * e] | v[9 + 2 * e] << 16;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) odd |= odd_bits(a[e]) | odd_bits(c[e]);
+                }
+                *(u32x4 *)(s + piece * 2048) = a;
+                *(u32x4 *)(s + piece * 2048 + 1024) = c;
+            }
+            if (__builtin_amdgcn_ballot_w64((odd & 0x80008000u) != 0) && lane == 0) *odd_rest = 1;
+        };
+        typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+        const uint32_t base = (uint32_t)(uintptr_t)(lds_void *)smem + lane * 16;
+        auto kfrag = [](uint32_t a, int s) { return __builtin_bit_cast(bf16x8, *(lds_u32x4 *)(uintptr_t)(a + s * 1024)); };
+        auto vfrag = [&](uint32_t a, int s, int dt) {
+            return __builtin_bit_cast(bf16x8, *(lds_u32x4 *)(uintptr_t)(a + kTile + (dt0 + dt) * 2048 + s * 1024));
+        };
+        f32x16 O[NDT];
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) O[dt] = f32x16{};
+        Softmax sm;
+        sm.clear();
+        if (tid == 0) *odd_rest = 0;
+        fetch(w.i0);
+        __syncthreads();
+#pragma unroll 1
+        for (int i = w.i0; i < w.i1; ++i) {
+            const int st = (i - w.i0) & 1;
+            stage_in(i, st);
+            const float none = slot < 0 ? __builtin_nanf("") : 1.0f;
+            const float sk = i < whole ? ix.sk_of(i) : none, sv = i < whole ? ix.sv_of(i) : none;
+            if (i + 1 - ix.base == 64) ix.load(p, w.b, hk, whole, i + 1);
+            fetch(i + 1);
+            // every wave's pieces are there; nobody reads the other stage (tile i - 1) any more when tile i + 1 is written to it
+            wait_lgkmcnt0();
+            meet();
+            const uint32_t at = base + st * kStage;
+            // ---- S^T = K Q^T: rows = keys of the tile, column = this lane's pair ----
+            constexpr int kPf = 3; // operands read ahead
+            f32x16 sc = {};
+            __builtin_amdgcn_s_setprio(1);
+            bf16x8 kf[kPf];
+#pragma unroll
+            for (int s = 0; s < kPf; ++s) kf[s] = kfrag(at, s);
+#pragma unroll
+            for (int s = 0; s < kD / 16; ++s) {
+                const bf16x8 a = kf[s % kPf];
+                if (s + kPf < kD / 16) kf[s % kPf] = kfrag(at, s + kPf);
+                __builtin_amdgcn_sched_barrier(0);
+                sc = mfma_bf16(a, qf[s], sc);
+            }
+            __builtin_amdgcn_s_setprio(0);
+            sm.add(sc, O, p.scale_log2 * sk, sv, (i + 1) * kBK - 1 > from + q0, i * kBK, pos, hi);
+            // the matrix cores' operand type; the sum keeps the unrounded weights
+            const bf16x8 pb[2] = {weights(sc, 0), weights(sc, 1)};
+            // A value of the rest that is not finite must not reach the rows before its own (0 x inf = NaN): into the rows that
+            // give its key a weight, then zeros in its place.
+            if (i >= whole && *odd_rest) {
+                const bf16x8 i0 = indicators(pb[0]), i1 = indicators(pb[1]);
+#pragma unroll
+                for (int x = 0; x < 4 * NDT; ++x) {
+                    O[x >> 2] = mfma_bf16(odd_values(vfrag(at, x & 1, x >> 2), x & 2 ? 0x8000u : 0u), x & 1 ? i1 : i0, O[x >> 2]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                __syncthreads();
+#pragma unroll 1
+                for (int x = tid; x < kTile / 4; x += kThreads) {
+                    uint32_t *v = (uint32_t *)(smem + st * kStage + kTile) + x;
+                    *v = without_odd(*v);
+                }
+                __syncthreads();
+            }
+            // ---- O^T += V^T P^T ----
+            constexpr int kPv = kPf < 2 * NDT ? kPf : 2 * NDT;
+            __builtin_amdgcn_s_setprio(1);
+            bf16x8 vf[kPv];
+#pragma unroll
+            for (int x = 0; x < kPv; ++x) vf[x] = vfrag(at, x / NDT, x % NDT);
+#pragma unroll
+            for (int x = 0; x < 2 * NDT; ++x) {
+                const bf16x8 a = vf[x % kPv];
+                if (x + kPv < 2 * NDT) vf[x % kPv] = vfrag(at, (x + kPv) / NDT, (x + kPv) % NDT);
+                __builtin_amdgcn_sched_barrier(0);
+                O[x % NDT] = mfma_bf16(a, pb[x / NDT], O[x % NDT]);
+            }
+            __builtin_amdgcn_s_setprio(0);
+        }
+        const float l = half_swap_sum(sm.lsum);
+        if (!w.whole()) {
+            leave(p, (long long)w.part * p.c.HK + (long long)hk, pair, dt0, hi, pos < 0, O, sm.m, l);
+            __syncthreads(); // the stages are free again
+        } else {
+            // ---- normalise (a row whose scores are all -inf has no softmax: 0 / 0; one that sees no key: zeros), stage, write ----
+            const float inv = 1.0f / l;
+            __syncthreads();
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                for (int r4 = 0; r4 < 4; ++r4) {
+                    const int d = (dt0 + dt) * 32 + 8 * r4 + 4 * hi;
+                    const f32x16 x = O[dt];
+                    u32x2 v = {pack_bf16x2(x[4 * r4] * inv, x[4 * r4 + 1] * inv), pack_bf16x2(x[4 * r4 + 2] * inv, x[4 * r4 + 3] * inv)};
+                    if (pos < 0) v = u32x2{0u, 0u};
+                    *(u32x2 *)(smem + pair * (kD * 2) + (((d >> 3) ^ l32) << 4) + (d & 4) * 2) = v;
+                }
+            __syncthreads();
+#pragma unroll 2
+            for (int x = tid; x < 32 * R * 32; x += kThreads) {
+                const int rr = x >> 5, ch = x & 31, tt = q0 + (rr >> 2);
+                if (tt < w.n)
+                    *(u32x4 *)(p.o + (long long)(hk * kGroup + (rr & 3)) * p.sho + (long long)(w.first + tt) * p.ldo + ch * 8) =
+                        *(const u32x4 *)(smem + rr * (kD * 2) + ((ch ^ (rr & 31)) << 4));
+            }
+            __syncthreads();
+        }
+    } while (w.next(p));
+}
+
+// The partial states of a divided unit joined: with M = max_c m_c, w_c = 2^(m_c - M), o = (sum w_c O_c) / (sum w_c l_c).  A
+// workgroup goes by the place where run r begins, and joins the unit there if it is the unit's first division; a thread has
+// four dims of one pair.
+__global__ __launch_bounds__(256) void pg_merge_kernel(PagedParams p) {
+    const int np = kGroup * p.nb, blocks = np / 4; // workgroups that share a unit's 64 x np fours
+    const int x = blockIdx.x % blocks * 256 + threadIdx.x, hk = blockIdx.x / blocks % p.c.HK, r = blockIdx.x / blocks / p.c.HK + 1;
+    Walk all(p);
+    const int at = r * all.per;
+    if (at >= all.total) return;
+    int b, qb, from;
+    all.find(p, at, b, qb, from);
+    const int start = from + p.begin, g0 = start / all.per; // the unit's first tile, and the run that has it
+    if (at <= start || g0 != r - 1) return;
+    const int n = p.rows.rows(b), tiles = Walk::tiles(p, n, p.c.len(b), qb);
+    const int parts = (start + tiles - 1) / all.per - g0 + 1;
+    const int pair = x % np, four = x / np;
+    auto part = [&](int c) { // (a unit that begins within a run has the run's second place)
+        return (2 * (long long)(g0 + c) + ((g0 + c) * all.per < from)) * p.c.HK + hk;
+    };
+    float mx = -__builtin_inff(), l = 0.0f;
+    float4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    // no part has a key that counts: weights 1 on zeros (a sum that is NaN or -1 stays so)
+    auto weight = [](float m, float top) { return top == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - top); };
+    constexpr int kBatch = 4; // parts whose loads are in flight together
+    for (int c0 = 0; c0 < parts; c0 += kBatch) {
+        float2 ml[kBatch];
+        float4 o[kBatch];
+#pragma unroll
+        for (int y = 0; y < kBatch; ++y) {
+            const long long k = part(c0 + y < parts ? c0 + y : c0);
+            ml[y] = p.part_ml[k * np + pair];
+            o[y] = p.part_o[(k * 64 + four) * np + pair];
+            if (c0 + y >= parts) ml[y] = float2{-__builtin_inff(), 0.0f}, o[y] = float4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        float top = mx;
+#pragma unroll
+        for (int y = 0; y < kBatch; ++y) top = __builtin_fmaxf(top, ml[y].x);
+        const float w = weight(mx, top);
+        l *= w, acc.x *= w, acc.y *= w, acc.z *= w, acc.w *= w;
+        mx = top;
+#pragma unroll
+        for (int y = 0; y < kBatch; ++y) {
+            const float v = weight(ml[y].x, mx);
+            l += v * ml[y].y;
+            acc.x += v * o[y].x;
+            acc.y += v * o[y].y;
+            acc.z += v * o[y].z;
+            acc.w += v * o[y].w;
+        }
+    }
+    const int t = qb * p.nb + (pair >> 2);
+    if (t >= n) return;
+    const float inv = l < 0.0f ? 0.0f : 1.0f / l; // (a row that sees no key: the parts' -1)
+    const u32x2 w = {pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv)};
+    *(u32x2 *)(p.o + (hk * kGroup + (pair & 3)) * p.sho + (long long)(p.rows.at(b) + t) * p.ldo + four * 4) = w;
+}
+
+// ---- host side ----
+
+constexpr int kCus = 256;
+
+struct Plan {
+    int R;                       // row blocks of a workgroup; 0: pg_few_kernel
+    int nb, runs, least, begin;  // see PagedParams
+    long long units, tiles, states; // most units; most places of the row; partial states
+};
+
+Plan plan(long long B, long long T, int HK, int width, int longest) {
+    Plan pl{};
+    const long long hint = longest > 0 && longest < T ? longest : T;
+    pl.R = hint <= 8 ? 0 : hint <= 16 ? 2 : hint <= 32 ? 4 : 8;
+    pl.nb = hint <= 1 ? 1 : hint <= 2 ? 2 : hint <= 4 ? 4 : hint <= 8 ? 8 : 8 * pl.R;
+    const long long most = (T + (pl.nb - 1) * B) / pl.nb;
+    pl.units = most < T ? most : T;
+    pl.begin = B == 1 && pl.units == 1 ? 0 : pl.R ? 4 : 2;
+    pl.least = pl.R ? 4 : 1;
+    pl.tiles = pl.units * (width + 1ll + pl.begin);
+    const long long slots = pl.R == 0 ? 4 * kCus : pl.R == 8 ? kCus : 2 * kCus;
+    long long runs = slots / HK > 0 ? slots / HK : 1;
+    const long long useful = pl.tiles / (pl.least + pl.begin) + 1; // (no more than can have tiles)
+    pl.runs = (int)(runs < useful ? runs : useful);
+    pl.states = pl.runs > 1 ? 2ll * pl.runs * HK : 0;
+    return pl;
+}
+long long state_bytes(const Plan &pl) { return pl.states * kGroup * pl.nb * (kD * 4 + 8); }
 
 }  // namespace
 
@@ -322,23 +729,31 @@ extern "C" int mica_attention_paged(const void *q, long long shq, long long ldq,
     for (long long x : {shq, ldq, sho, ldo})
         if (x < 0 || x % 8) return MICA_MISS_STRIDE;
     if (!mica_aligned16(q) || !mica_aligned16(o) || ((uintptr_t)starts & 3)) return MICA_MISS_ALIGN;
+    const Plan pl = plan(B, T, HK, width, longest);
+    if (pl.tiles >= (1ll << 30) || B >= (1 << 30) || T >= (1 << 29)) return MICA_MISS_RANGE; // (places are ints)
+    if (pl.states && (!workspace || !mica_aligned16(workspace) || workspace_bytes < state_bytes(pl))) return MICA_MISS_ARG;
     p.q = (const uint16_t *)q; p.shq = shq; p.ldq = ldq;
     p.o = (uint16_t *)o; p.sho = sho; p.ldo = ldo;
     p.rows = Ragged{starts, B, T};
     p.fill = fill;
     p.scale_log2 = scale * 1.44269504088896341f;
-    const int hint = longest > 0 && longest < T ? longest : T;
-    const int R = hint <= 8 ? 1 : hint <= 16 ? 2 : 4, nb = 8 * R;
-    const long long most = ((long long)T + (nb - 1ll) * B + nb - 1) / nb, units = most < T ? most : T, wgs = units * HK;
-    if (wgs >= (1 << 24)) return MICA_MISS_RANGE; // (a grid of 2^32 work-items wraps round)
+    p.nb = pl.nb, p.runs = pl.runs, p.least = pl.least, p.begin = pl.begin;
+    p.part_o = (float4 *)workspace;
+    p.part_ml = (float2 *)((char *)workspace + pl.states * kGroup * pl.nb * kD * 4);
     hipStream_t st = (hipStream_t)stream;
-    if (R == 1) hipLaunchKernelGGL((pg_fwd_kernel<1, 4>), dim3((unsigned)wgs), dim3(256), 0, st, p);
-    else if (R == 2) hipLaunchKernelGGL((pg_fwd_kernel<2, 2>), dim3((unsigned)wgs), dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((pg_fwd_kernel<4, 1>), dim3((unsigned)wgs), dim3(256), 0, st, p);
+    const long long workers = (long long)pl.runs * HK;
+    if (pl.R == 0) hipLaunchKernelGGL(pg_few_kernel, dim3((unsigned)((workers + 3) / 4)), dim3(256), 0, st, p);
+    else if (pl.R == 2) hipLaunchKernelGGL((pg_fwd_kernel<2, 2>), dim3((unsigned)workers), dim3(256), 0, st, p);
+    else if (pl.R == 4) hipLaunchKernelGGL((pg_fwd_kernel<4, 1>), dim3((unsigned)workers), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((pg_fwd_kernel<8, 1>), dim3((unsigned)workers), dim3(512), 0, st, p);
+    if (const int rc = mica_err(hipGetLastError())) return rc;
+    if (pl.states == 0) return 0;
+    hipLaunchKernelGGL(pg_merge_kernel, dim3((unsigned)((pl.runs - 1) * HK * pl.nb)), dim3(256), 0, st, p);
     return mica_err(hipGetLastError());
 }
 
 extern "C" long long mica_attention_paged_workspace_bytes(int B, int T, int HK, int width, int longest) {
-    if (B < 0 || T < 0 || HK <= 0 || width < 0) return -1;
-    return 0;
+    if (B < 0 || T < 0 || HK <= 0 || HK > (1 << 16) || width < 0 || width > (1 << 24)) return -1;
+    if (B == 0 || T == 0) return 0;
+    return state_bytes(plan(B, T, HK, width, longest));
 }
