@@ -57,3 +57,10 @@ MICA_DEVICE s16x4 tr_read(lds_s16x4 *p, lds_void *__restrict w) {
     __builtin_assume(w != nullptr);
     return x;
 }
+// 16 bytes of LDS at address a, likewise.
+typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
+MICA_DEVICE u32x4 lds_read(uint32_t a, lds_void *__restrict w) {
+    const u32x4 x = *(lds_u32x4 *)(uintptr_t)a;
+    __builtin_assume(w != nullptr);
+    return x;
+}

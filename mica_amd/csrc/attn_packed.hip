@@ -112,10 +112,13 @@ __global__ __launch_bounds__(kThreads, 2) void pk_fwd_kernel(PackedParams p) {
     const uint32_t kbase = lds0 + l32 * (kD * 2) + ((hi ^ (l32 & 15)) << 4);
     typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
     auto kfrag = [](uint32_t stage, int s) { return __builtin_bit_cast(bf16x8, *(lds_u32x4 *)(uintptr_t)((stage ^ (s << 5)))); };
-    auto vfrag = [&](uint32_t stage, int s, int dt) {
+    // (opaque: as a constant it would be put into tr_read itself, which then says nothing)
+    lds_void *none = (lds_void *)smem;
+    __asm__ volatile("" : "+s"(none));
+    auto vfrag = [none](uint32_t stage, int s, int dt) {
         const uint32_t a = (stage ^ (dt << 6)) + s * 16 * (kD * 2);
-        const s16x4 x = tr_read((lds_s16x4 *)(uintptr_t)a, (lds_void *)smem);
-        const s16x4 y = tr_read((lds_s16x4 *)(uintptr_t)(a + 8 * (kD * 2)), (lds_void *)smem);
+        const s16x4 x = tr_read((lds_s16x4 *)(uintptr_t)a, none);
+        const s16x4 y = tr_read((lds_s16x4 *)(uintptr_t)(a + 8 * (kD * 2)), none);
         return __builtin_bit_cast(bf16x8, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
     };
     constexpr int kPf = 3; // operand fragments read ahead

@@ -422,106 +422,126 @@ __global__ __launch_bounds__(256, 1) void pg_few_kernel(PagedParams p) {
 }
 
 // ---- more rows ----
-// A workgroup's R x D waves share each page: every wave loads its share of the next one into registers while this one is
-// computed, widens it to bf16 once for all of them and writes it to one of two LDS stages, from which every operand is one
-// contiguous 16-byte read a lane.  A wave holds 32 (row, head) pairs: it computes S^T = K Q^T (32 keys x 32 pairs,
-// v_mfma_f32_32x32x16_bf16), the online softmax of its pairs (a lane holds 16 of a pair's 32 scores, lane l ^ 32 the others)
-// and 256 / D dims of O^T += V^T P^T.
-template <int R, int D>
-__global__ __launch_bounds__(64 * R * D, 2) void pg_fwd_kernel(PagedParams p) {
-    constexpr int kWaves = R * D, kThreads = 64 * kWaves;
-    constexpr int NDT = kD / 32 / D;        // 32-dim tiles of O a wave holds
-    constexpr int kOwn = 16 / kWaves;       // pieces of a page a wave brings
-    constexpr int kSmem = R * 32 * kD * 2 > 2 * kStage ? R * 32 * kD * 2 : 2 * kStage; // the stages; the output, in the end
-    __shared__ __attribute__((aligned(1024))) int8_t smem[kSmem + 16];
-    int *const odd_rest = (int *)(smem + kSmem); // whether the rest holds a value that is not finite
+// A workgroup of 8 waves shares each page, one workgroup a CU.  A page's 16 pieces come by LDS DMA, two of them by each wave,
+// three tiles ahead into a ring; when its two have landed a wave widens them to bf16, once for all waves, into one of two
+// stages, from which every operand is one contiguous 16-byte read a lane.  A wave holds 32 (row, head) pairs (R row blocks): it
+// computes S^T = K Q^T (32 keys x 32 pairs, v_mfma_f32_32x32x16_bf16), the online softmax of its pairs (a lane holds 16 of a
+// pair's 32 scores, lane l ^ 32 the others) and 256 / D dims of O^T += V^T P^T; with few rows D = 8 / R waves repeat a row
+// block's scores and divide its dims.
+constexpr int kWaves = 8, kThreads = 64 * kWaves;
+constexpr int kOwn = 16 / kWaves;       // pieces of a page a wave brings
+constexpr int kRing = 4;                // pages in the ring: one being widened, three on their way
+constexpr int kRaw = 2 * kPageBytes;
 
-    const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int rb = wave / D, dt0 = (wave % D) * NDT, pair = rb * 32 + l32;
+template <int R>
+__global__ __launch_bounds__(kThreads, 2) void pg_fwd_kernel(PagedParams p) {
+    constexpr int D = kWaves / R;           // waves of a row block
+    constexpr int NDT = kD / 32 / D;        // 32-dim tiles of O a wave holds
+    constexpr int kSmem = 2 * kStage + kRing * kRaw; // the stages and the ring; the output, in the end
+    static_assert(kSmem >= R * 32 * kD * 2, "the output is staged in their place");
+    // (one array: with several the compiler lets every operand read wait for all DMA in flight)
+    __shared__ __attribute__((aligned(1024))) int8_t smem[kSmem + kWaves * 64 * 16 + 16];
+    int *const index = (int *)(smem + kSmem) + (threadIdx.x >> 6) * 256; // this wave's: page and scales of 64 tiles, i at i % 64
+    int *const odd_rest = (int *)(smem + kSmem + kWaves * 64 * 16);      // whether the rest holds a value that is not finite
+
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int rb = wave / D, dt0 = (wave % D) * NDT;
     const int hk = blockIdx.x % p.c.HK, run = blockIdx.x / p.c.HK;
     if (p.fill) {
         const int none = p.rows.at(0) + p.rows.T - p.rows.at(p.rows.B);
-        for (int i = run * 32; i < none; i += p.runs * 32) fill_rows(p, hk, i, 32, tid, kThreads);
+        for (int i = run * 32; i < none; i += p.runs * 32) fill_rows(p, hk, i, 32, threadIdx.x, kThreads);
     }
     Piece w;
     if (!w.begin(p, run)) return;
     do {
+        // what depends on the lane alone is made here, from an opaque copy of its id: the compiler would make it before the loop
+        // and hold it in registers that the tiles need
+        int tid = threadIdx.x;
+        __asm__ volatile("" : "+v"(tid));
+        const int lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
         const int q0 = w.qb * p.nb, from = w.len - w.n, whole = w.len / kBK;
-        const int t = q0 + (pair >> 2), head = hk * kGroup + (pair & 3), pos = from + t; // this lane's pair
         const int slot = __builtin_amdgcn_readfirstlane(p.c.slot(w.b)), have = slot < 0 ? 0 : w.len - whole * kBK;
+        const int end = min(w.i1, whole); // pages; then the rest
+        // Pages and scales of tiles i .. i + 31 into this wave's index: one round trip to memory for all of them
+        auto look_up = [&](int i) {
+            const int j = i + (lane & 31), page = j < whole ? p.c.page(w.b, j) : -1;
+            // (a block without a page: NaN, for the rows that see it)
+            const float x = page >= 0 ? p.c.scales[p.c.index(page, hi, hk)] : __builtin_nanf("");
+            index[(j & 63) * 4] = page;
+            index[(j & 63) * 4 + 1 + hi] = __float_as_int(x);
+        };
+        auto found = [&](int i, int what) { return __builtin_amdgcn_readfirstlane(index[(i & 63) * 4 + what]); };
+        int known = w.i0 + 32; // the first tile that is not in the index
+        look_up(w.i0);
+        // DMA of tile i's pieces (of this wave): 0 .. 7 of a page are keys (32 dims of each token), 8 .. 15 values (32 dims'
+        // rows).  Past the last page, and for a block without one, from a zero-sized buffer: every step issues as many.
+        auto fetch = [&](int i) {
+            const int page = i < end ? found(i, 0) : -1;
+            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+                (void *)p.c.block(max(page, 0), wave * kOwn >> 3, hk), 0, page >= 0 ? kPageBytes : 0, kBufferFlags);
+            int ln = lane;
+            __asm__ volatile("" : "+v"(ln));
+            int8_t *s = smem + 2 * kStage + ((i - w.i0) & (kRing - 1)) * kRaw + wave * kOwn * 1024;
+#pragma unroll
+            for (int x = 0; x < kOwn; ++x)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void *)(s + x * 1024), 16,
+                                                         (ln & 31) * 32 + (ln >> 5) * 16 + (wave * kOwn & 7) * 1024 + x * 1024, 0, 0, 0);
+        };
         // Q fragments (B operand of S^T): step 2 c + e takes dims 32 c + 16 hi + 8 e .. + 7, as a page's bytes lie; rows past the
         // last repeat it
+        const int t = q0 + rb * 8 + (l32 >> 2), pos = from + t; // this lane's pair: row t, head l % 4
         bf16x8 qf[kD / 16];
         {
-            const uint16_t *qr = p.q + head * p.shq + (long long)(w.first + min(t, w.n - 1)) * p.ldq + hi * 16;
+            const uint16_t *qr = p.q + (hk * kGroup + (l32 & 3)) * p.shq + (long long)(w.first + min(t, w.n - 1)) * p.ldq + hi * 16;
 #pragma unroll
             for (int s = 0; s < kD / 16; ++s) qf[s] = __builtin_bit_cast(bf16x8, *(const u32x4 *)(qr + (s >> 1) * 32 + (s & 1) * 8));
         }
-        // Pieces 0 .. 7 of a page are keys (32 dims of each token), 8 .. 15 values (32 dims' rows); this wave brings kOwn of them.
-        Index ix;
-        ix.load(p, w.b, hk, whole, w.i0);
-        u32x4 raw[kOwn];
-        auto fetch = [&](int i) { // tile i's pieces into registers
-            const int page = i < min(w.i1, whole) ? ix.page_of(i) : -1;
-            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
-                (void *)p.c.block(max(page, 0), wave * kOwn >> 3, hk), 0, page >= 0 ? kPageBytes : 0, kBufferFlags);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int x = 0; x < kOwn; ++x)
-                raw[x] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                                                       r, l32 * 32 + hi * 16, ((wave * kOwn + x) & 7) * 1024, 0));
-        };
-        // Tile i into LDS stage st: a piece becomes two operands of 64 lanes x 16 bytes.  Keys: bytes 8 e .. 8 e + 7 are step
-        // 2 c + e's; values: fours s and s + 2 are step s's (tokens 16 s + 4 hi .. + 3 and 8 more on: P^T's accumulator rows).
-        auto stage_in = [&](int i, int st) {
-            int8_t *s = smem + st * kStage + lane * 16;
-            if (i < whole) {
-#pragma unroll
-                for (int x = 0; x < kOwn; ++x) {
-                    const int piece = wave * kOwn + x;
-                    const u32x2 w0 = widen4(raw[x][0]), w1 = widen4(raw[x][1]), w2 = widen4(raw[x][2]), w3 = widen4(raw[x][3]);
-                    u32x4 a = {w0[0], w0[1], w1[0], w1[1]}, c = {w2[0], w2[1], w3[0], w3[1]};
-                    if (wave * kOwn >= 8) a = u32x4{w0[0], w0[1], w2[0], w2[1]}, c = u32x4{w1[0], w1[1], w3[0], w3[1]};
-                    *(u32x4 *)(s + piece * 2048) = a;
-                    *(u32x4 *)(s + piece * 2048 + 1024) = c;
-                }
-                return;
-            }
-            // The rest: bf16 rows, the same operands; zeros past its last token.
-            const uint16_t *kr = p.c.rest(max(slot, 0), 0, hk), *vr = p.c.rest(max(slot, 0), 1, hk);
+        for (int x = 0; x < kRing - 1; ++x) {
+            fetch(w.i0 + x);
+        }
+        // The rest into stage st: bf16 rows, the same operands; zeros past its last token (the buffer's range check).
+        auto stage_rest = [&](int st) {
+            const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void *)p.c.rest(max(slot, 0), wave * kOwn >> 3, hk),
+                                                                               0, have * kD * 2, kBufferFlags);
             uint32_t odd = 0;
+            int ln = lane;
+            __asm__ volatile("" : "+v"(ln));
+            const int row = ln & 31, half = ln >> 5;
 #pragma unroll 1
             for (int x = 0; x < kOwn; ++x) {
-                const int piece = wave * kOwn + x;
-                u32x4 a = {}, c = {};
-                if (piece < 8) {
-                    if (l32 < have) {
-                        const u32x4 *src = (const u32x4 *)(kr + l32 * kD + piece * 32 + hi * 16);
-                        a = src[0], c = src[1];
-                    }
+                const int dims = ((wave * kOwn + x) & 7) * 64; // the piece's dims, in bytes of a row
+                u32x4 a, c;
+                if (wave < 4) {
+                    const int at = row * (kD * 2) + dims + half * 32;
+                    a = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0));
+                    c = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, at + 16, 0, 0));
                 } else {
-                    const uint16_t *src = vr + (piece - 8) * 32 + l32;
+                    const int at = 4 * half * (kD * 2) + dims + row * 2;
                     uint32_t v[16];
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) { // step e / 8, its token e % 8
-                        const int token = 16 * (e >> 3) + 8 * ((e >> 2) & 1) + 4 * hi + (e & 3);
-                        v[e] = token < have ? src[token * kD] : 0u;
-                    }
+                    for (int e = 0; e < 16; ++e) // step e / 8, its token e % 8
+                        v[e] = (uint16_t)__builtin_amdgcn_raw_buffer_load_b16(
+                            r, at + (16 * (e >> 3) + 8 * ((e >> 2) & 1) + (e & 3)) * (kD * 2), 0, 0);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) a[e] = v[2 * e] | v[2 * e + 1] << 16, c[e] = v[8 + 2 * e] | v[9 + 2 * e] << 16;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) odd |= odd_bits(a[e]) | odd_bits(c[e]);
                 }
-                *(u32x4 *)(s + piece * 2048) = a;
-                *(u32x4 *)(s + piece * 2048 + 1024) = c;
+                int8_t *s = smem + st * kStage + (wave * kOwn + x) * 2048 + ln * 16;
+                *(u32x4 *)s = a;
+                *(u32x4 *)(s + 1024) = c;
             }
-            if (__builtin_amdgcn_ballot_w64((odd & 0x80008000u) != 0) && lane == 0) *odd_rest = 1;
+            if (__builtin_amdgcn_ballot_w64((odd & 0x80008000u) != 0) && ln == 0) *odd_rest = 1;
         };
-        typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
         const uint32_t base = (uint32_t)(uintptr_t)(lds_void *)smem + lane * 16;
-        auto kfrag = [](uint32_t a, int s) { return __builtin_bit_cast(bf16x8, *(lds_u32x4 *)(uintptr_t)(a + s * 1024)); };
-        auto vfrag = [&](uint32_t a, int s, int dt) {
-            return __builtin_bit_cast(bf16x8, *(lds_u32x4 *)(uintptr_t)(a + kTile + (dt0 + dt) * 2048 + s * 1024));
+        // (opaque: as a constant it would be put into lds_read itself, which then says nothing)
+        lds_void *none = (lds_void *)smem;
+        __asm__ volatile("" : "+s"(none));
+        auto kfrag = [none](uint32_t a, int s) { return __builtin_bit_cast(bf16x8, lds_read(a + s * 1024, none)); };
+        auto vfrag = [none](uint32_t a, int s, int dt) { // a: of the wave's first dims
+            return __builtin_bit_cast(bf16x8, lds_read(a + dt * 2048 + s * 1024, none));
         };
         f32x16 O[NDT];
 #pragma unroll
@@ -529,20 +549,42 @@ __global__ __launch_bounds__(64 * R * D, 2) void pg_fwd_kernel(PagedParams p) {
         Softmax sm;
         sm.clear();
         if (tid == 0) *odd_rest = 0;
-        fetch(w.i0);
-        __syncthreads();
+        wait_vmcnt<(kRing - 1) * kOwn>(); // the queries are there (said here, or the loop's first use waits for all DMA at every tile)
+        wait_lgkmcnt0();
+        meet();
 #pragma unroll 1
         for (int i = w.i0; i < w.i1; ++i) {
-            const int st = (i - w.i0) & 1;
-            stage_in(i, st);
-            const float none = slot < 0 ? __builtin_nanf("") : 1.0f;
-            const float sk = i < whole ? ix.sk_of(i) : none, sv = i < whole ? ix.sv_of(i) : none;
-            if (i + 1 - ix.base == 64) ix.load(p, w.b, hk, whole, i + 1);
-            fetch(i + 1);
+            const uint32_t at = base + ((i - w.i0) & 1) * kStage;
+            float sk, sv;
+            if (i < whole) {
+                // Tile i's pieces of this wave have landed (those of the next two, 2 kOwn, may still be out): each becomes two
+                // operands.  Keys: bytes 8 e .. 8 e + 7 are step 2 c + e's; values: fours s and s + 2 are step s's (tokens 16 s + 4
+                // hi .. + 3 and 8 more on: P^T's accumulator rows).
+                wait_vmcnt<2 * kOwn>();
+                __builtin_amdgcn_sched_barrier(0);
+                const uint32_t src = base + 2 * kStage + ((i - w.i0) & (kRing - 1)) * kRaw + wave * kOwn * 1024;
+                u32x4 raw[kOwn];
+#pragma unroll
+                for (int x = 0; x < kOwn; ++x) raw[x] = lds_read(src + x * 1024, none);
+#pragma unroll
+                for (int x = 0; x < kOwn; ++x) {
+                    const uint32_t m1 = wave < 4 ? raw[x][1] : raw[x][2], m2 = wave < 4 ? raw[x][2] : raw[x][1];
+                    const bf16x8 a = widen8(raw[x][0], m1), c = widen8(m2, raw[x][3]);
+                    const uint32_t to = at + (wave * kOwn + x) * 2048;
+                    *(lds_u32x4 *)(uintptr_t)to = __builtin_bit_cast(u32x4, a);
+                    *(lds_u32x4 *)(uintptr_t)(to + 1024) = __builtin_bit_cast(u32x4, c);
+                }
+                sk = __int_as_float(found(i, 1)), sv = __int_as_float(found(i, 2));
+            } else {
+                stage_rest((i - w.i0) & 1);
+                sk = sv = slot < 0 ? __builtin_nanf("") : 1.0f;
+            }
+            // the next tile of the ring, whose place this wave has read a step ago
+            if (i + kRing - 1 == known && known < end) look_up(known), known += 32;
+            fetch(i + kRing - 1);
             // every wave's pieces are there; nobody reads the other stage (tile i - 1) any more when tile i + 1 is written to it
             wait_lgkmcnt0();
             meet();
-            const uint32_t at = base + st * kStage;
             // ---- S^T = K Q^T: rows = keys of the tile, column = this lane's pair ----
             constexpr int kPf = 3; // operands read ahead
             f32x16 sc = {};
@@ -560,43 +602,53 @@ __global__ __launch_bounds__(64 * R * D, 2) void pg_fwd_kernel(PagedParams p) {
             __builtin_amdgcn_s_setprio(0);
             sm.add(sc, O, p.scale_log2 * sk, sv, (i + 1) * kBK - 1 > from + q0, i * kBK, pos, hi);
             // the matrix cores' operand type; the sum keeps the unrounded weights
-            const bf16x8 pb[2] = {weights(sc, 0), weights(sc, 1)};
-            // A value of the rest that is not finite must not reach the rows before its own (0 x inf = NaN): into the rows that
-            // give its key a weight, then zeros in its place.
-            if (i >= whole && *odd_rest) {
-                const bf16x8 i0 = indicators(pb[0]), i1 = indicators(pb[1]);
-#pragma unroll
-                for (int x = 0; x < 4 * NDT; ++x) {
-                    O[x >> 2] = mfma_bf16(odd_values(vfrag(at, x & 1, x >> 2), x & 2 ? 0x8000u : 0u), x & 1 ? i1 : i0, O[x >> 2]);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
+            bf16x8 pb[2] = {weights(sc, 0), weights(sc, 1)};
+            // A value of the rest that is not finite must not reach the rows before its own (0 x inf = NaN): zeros in its place, and
+            // it goes into the rows that give its key a weight, by products of their own with what the ring then holds (nothing
+            // else does: the rest is a unit's last tile).
+            const bool odd = i >= whole && *odd_rest;
+            if (odd) {
+                wait_vmcnt<0>(); // (the empty loads)
                 __syncthreads();
 #pragma unroll 1
-                for (int x = tid; x < kTile / 4; x += kThreads) {
-                    uint32_t *v = (uint32_t *)(smem + st * kStage + kTile) + x;
+                for (int x = threadIdx.x; x < kTile / 4; x += kThreads) {
+                    uint32_t *v = (uint32_t *)(smem + ((i - w.i0) & 1) * kStage + kTile) + x, *o = (uint32_t *)(smem + 2 * kStage) + x;
+                    const uint32_t lo = *v & 0xffffu, hh = *v >> 16;
+                    o[0] = odd_value(lo, 0) | odd_value(hh, 0) << 16;
+                    o[kTile / 4] = odd_value(lo, 0x8000u) | odd_value(hh, 0x8000u) << 16;
                     *v = without_odd(*v);
                 }
                 __syncthreads();
             }
             // ---- O^T += V^T P^T ----
-            constexpr int kPv = kPf < 2 * NDT ? kPf : 2 * NDT;
-            __builtin_amdgcn_s_setprio(1);
-            bf16x8 vf[kPv];
+            auto product = [&](uint32_t v) { // values at v
+                constexpr int kPv = kPf < 2 * NDT ? kPf : 2 * NDT;
+                __builtin_amdgcn_s_setprio(1);
+                bf16x8 vf[kPv];
 #pragma unroll
-            for (int x = 0; x < kPv; ++x) vf[x] = vfrag(at, x / NDT, x % NDT);
+                for (int x = 0; x < kPv; ++x) vf[x] = vfrag(v, x / NDT, x % NDT);
 #pragma unroll
-            for (int x = 0; x < 2 * NDT; ++x) {
-                const bf16x8 a = vf[x % kPv];
-                if (x + kPv < 2 * NDT) vf[x % kPv] = vfrag(at, (x + kPv) / NDT, (x + kPv) % NDT);
-                __builtin_amdgcn_sched_barrier(0);
-                O[x % NDT] = mfma_bf16(a, pb[x / NDT], O[x % NDT]);
+                for (int x = 0; x < 2 * NDT; ++x) {
+                    const bf16x8 a = vf[x % kPv];
+                    if (x + kPv < 2 * NDT) vf[x % kPv] = vfrag(v, (x + kPv) / NDT, (x + kPv) % NDT);
+                    __builtin_amdgcn_sched_barrier(0);
+                    O[x % NDT] = mfma_bf16(a, pb[x / NDT], O[x % NDT]);
+                }
+                __builtin_amdgcn_s_setprio(0);
+            };
+            product(at + kTile + dt0 * 2048);
+            if (odd) {
+                pb[0] = indicators(pb[0]), pb[1] = indicators(pb[1]);
+#pragma unroll 1
+                for (int x = 0; x < 2; ++x) product(base + 2 * kStage + x * kTile + dt0 * 2048);
             }
-            __builtin_amdgcn_s_setprio(0);
         }
+        wait_vmcnt<0>(); // the last (empty) loads have written before the ring is used again or given up
         const float l = half_swap_sum(sm.lsum);
+        __asm__ volatile("" : "+v"(tid));
+        const int ln = tid & 63, row = rb * 32 + (ln & 31), half = ln >> 5;
         if (!w.whole()) {
-            leave(p, (long long)w.part * p.c.HK + (long long)hk, pair, dt0, hi, pos < 0, O, sm.m, l);
-            __syncthreads(); // the stages are free again
+            leave(p, (long long)w.part * p.c.HK + hk, row, dt0, half, pos < 0, O, sm.m, l);
         } else {
             // ---- normalise (a row whose scores are all -inf has no softmax: 0 / 0; one that sees no key: zeros), stage, write ----
             const float inv = 1.0f / l;
@@ -605,11 +657,11 @@ __global__ __launch_bounds__(64 * R * D, 2) void pg_fwd_kernel(PagedParams p) {
             for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
                 for (int r4 = 0; r4 < 4; ++r4) {
-                    const int d = (dt0 + dt) * 32 + 8 * r4 + 4 * hi;
+                    const int d = (dt0 + dt) * 32 + 8 * r4 + 4 * half;
                     const f32x16 x = O[dt];
                     u32x2 v = {pack_bf16x2(x[4 * r4] * inv, x[4 * r4 + 1] * inv), pack_bf16x2(x[4 * r4 + 2] * inv, x[4 * r4 + 3] * inv)};
                     if (pos < 0) v = u32x2{0u, 0u};
-                    *(u32x2 *)(smem + pair * (kD * 2) + (((d >> 3) ^ l32) << 4) + (d & 4) * 2) = v;
+                    *(u32x2 *)(smem + row * (kD * 2) + (((d >> 3) ^ (ln & 31)) << 4) + (d & 4) * 2) = v;
                 }
             __syncthreads();
 #pragma unroll 2
@@ -619,8 +671,8 @@ __global__ __launch_bounds__(64 * R * D, 2) void pg_fwd_kernel(PagedParams p) {
                     *(u32x4 *)(p.o + (long long)(hk * kGroup + (rr & 3)) * p.sho + (long long)(w.first + tt) * p.ldo + ch * 8) =
                         *(const u32x4 *)(smem + rr * (kD * 2) + ((ch ^ (rr & 31)) << 4));
             }
-            __syncthreads();
         }
+        __syncthreads(); // everybody is done with the stages and the ring
     } while (w.next(p));
 }
 
@@ -701,7 +753,7 @@ Plan plan(long long B, long long T, int HK, int width, int longest) {
     pl.begin = B == 1 && pl.units == 1 ? 0 : pl.R ? 4 : 2;
     pl.least = pl.R ? 4 : 1;
     pl.tiles = pl.units * (width + 1ll + pl.begin);
-    const long long slots = pl.R == 0 ? 4 * kCus : pl.R == 8 ? kCus : 2 * kCus;
+    const long long slots = pl.R == 0 ? 4 * kCus : kCus; // waves or workgroups that the chip holds at once
     long long runs = slots / HK > 0 ? slots / HK : 1;
     const long long useful = pl.tiles / (pl.least + pl.begin) + 1; // (no more than can have tiles)
     pl.runs = (int)(runs < useful ? runs : useful);
@@ -743,9 +795,9 @@ extern "C" int mica_attention_paged(const void *q, long long shq, long long ldq,
     hipStream_t st = (hipStream_t)stream;
     const long long workers = (long long)pl.runs * HK;
     if (pl.R == 0) hipLaunchKernelGGL(pg_few_kernel, dim3((unsigned)((workers + 3) / 4)), dim3(256), 0, st, p);
-    else if (pl.R == 2) hipLaunchKernelGGL((pg_fwd_kernel<2, 2>), dim3((unsigned)workers), dim3(256), 0, st, p);
-    else if (pl.R == 4) hipLaunchKernelGGL((pg_fwd_kernel<4, 1>), dim3((unsigned)workers), dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((pg_fwd_kernel<8, 1>), dim3((unsigned)workers), dim3(512), 0, st, p);
+    else if (pl.R == 2) hipLaunchKernelGGL(pg_fwd_kernel<2>, dim3((unsigned)workers), dim3(kThreads), 0, st, p);
+    else if (pl.R == 4) hipLaunchKernelGGL(pg_fwd_kernel<4>, dim3((unsigned)workers), dim3(kThreads), 0, st, p);
+    else hipLaunchKernelGGL(pg_fwd_kernel<8>, dim3((unsigned)workers), dim3(kThreads), 0, st, p);
     if (const int rc = mica_err(hipGetLastError())) return rc;
     if (pl.states == 0) return 0;
     hipLaunchKernelGGL(pg_merge_kernel, dim3((unsigned)((pl.runs - 1) * HK * pl.nb)), dim3(256), 0, st, p);
