@@ -465,11 +465,12 @@ int mica_kv_append(const void *k, long long shk, long long ldk, const void *v, l
 
 /*
  * The cache's rows back in bf16, each value rounded once: k / v [T][HK][256], contiguous, 16-byte aligned; the n rows of sequence
- * b are its last n tokens (zeros for those before its first, and for rows of no sequence).
+ * b are its last n tokens (zeros for those before its first, and for rows of no sequence).  longest as in
+ * mica_attention_packed.
  */
 int mica_kv_read(void *k, void *v, const int *starts, int B, int T, const void *data, const float *scales, const void *recent,
                  int pages, int n_slots, int HK, int head_dim, const int *table, long long ldt, int width, const int *lens,
-                 const int *slots, mica_stream_t stream);
+                 const int *slots, int longest, mica_stream_t stream);
 
 /*
  * Attention of each sequence's last rows over the cache, HQ = 4 HK: row i of the n of sequence b is at position p = lens[b] - n

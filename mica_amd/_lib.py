@@ -83,7 +83,7 @@ SIGNATURES = {
     "mica_attention_packed": (_I, [*[_P, _LL, _LL] * 4, _P, _I, _I, _I, _I, _I, _F, _I, _I, _P, _LL, _P]),
     "mica_attention_packed_workspace_bytes": (_LL, [_I, _I, _I, _I]),
     "mica_kv_append": (_I, [*[_P, _LL, _LL] * 2, _P, _I, _I, *_PAGED, _P, _F, _F, _I, _P, _P, _I, _I, _P, _I, _P]),
-    "mica_kv_read": (_I, [_P, _P, _P, _I, _I, *_PAGED, _P]),
+    "mica_kv_read": (_I, [_P, _P, _P, _I, _I, *_PAGED, _I, _P]),
     "mica_attention_paged": (_I, [*[_P, _LL, _LL] * 2, _P, _I, _I, _I, *_PAGED, _F, _I, _I, _P, _LL, _P]),
     "mica_attention_paged_workspace_bytes": (_LL, [_I, _I, _I, _I, _I]),
     "mica_causal_conv1d": (_I, [_P, _LL, _I, _P, _P, _I, _I, _P, _P, _P, _LL, _I, _I, _I, _I, _I, _I, _F, _P]),
@@ -102,7 +102,8 @@ NATIVE_FNS = ("mica_act_quant", "mica_mm_i8", "mica_rmsnorm_quant", "mica_rmsnor
               "mica_causal_conv1d", "mica_gdn_chunk", "mica_gdn_chunk_gate", "mica_gdn_workspace_bytes",
               "mica_gdn_gate", "mica_gated_rmsnorm_quant", "mica_token_logprobs", "mica_token_logprobs_workspace_bytes",
               "mica_attention_tree", "mica_attention_tree_workspace_bytes", "mica_attention_window",
-              "mica_attention_window_workspace_bytes")
+              "mica_attention_window_workspace_bytes", "mica_attention_packed", "mica_attention_packed_workspace_bytes",
+              "mica_kv_append", "mica_kv_read", "mica_attention_paged", "mica_attention_paged_workspace_bytes")
 
 
 class _NotLoaded:

@@ -385,6 +385,9 @@ def packed_attention(q, k, v, starts, longest: int | None = None, scale: float |
     and v at least 256 elements apart.  Returns o [T, HQ, 256] bf16, zeros in rows of no sequence; with out= (such a view) that,
     whose rows of no sequence are left as they were."""
     scale = _scale(scale)
+    r = _lib.FAST.packed_attention(q, k, v, starts, longest, scale, out)
+    if r is not None:
+        return _native(r, "mica_attention_packed")
     sq, sk, sv = _rows(q, "q"), _rows(k, "k", q.device), _rows(v, "v", q.device)
     dev = q.device
     T, HQ, _ = q.shape

@@ -55,6 +55,12 @@ struct Abi {
     MICA_FN(attention_tree_workspace_bytes)
     MICA_FN(attention_window)
     MICA_FN(attention_window_workspace_bytes)
+    MICA_FN(attention_packed)
+    MICA_FN(attention_packed_workspace_bytes)
+    MICA_FN(kv_append)
+    MICA_FN(kv_read)
+    MICA_FN(attention_paged)
+    MICA_FN(attention_paged_workspace_bytes)
 #undef MICA_FN
 } abi;
 bool g_bound = false;
@@ -652,6 +658,217 @@ PyObject *py_window_attention(PyObject *, PyObject *const *a, Py_ssize_t nargs) 
     END_HANDLE_TH_ERRORS
 }
 
+// bf16 [T, heads, 256] rows with unit feature stride, 16-byte aligned; their strides, those of one-element axes as 0
+struct Rows {
+    const void *p = nullptr;
+    long long sh = 0, ld = 0;
+    bool of(const Call &c, const Tensor &t) {
+        if (t.dim() != 3 || t.scalar_type() != at::kBFloat16 || t.size(2) != 256 || t.stride(2) != 1 || !on(c, t) ||
+            t.numel() / 256 >= kI32 || !aligned(t))
+            return false;
+        p = t.data_ptr();
+        sh = t.size(1) > 1 ? t.stride(1) : 0, ld = t.size(0) > 1 ? t.stride(0) : 0;
+        return true;
+    }
+};
+// int32 [B + 1], at least one
+bool starts_of(const Call &c, const Tensor &t) {
+    return t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) > 0 && t.is_contiguous() && on(c, t);
+}
+// None or a whole number that is not negative, at most an int
+bool hint_of(PyObject *o, int *v) {
+    *v = 0;
+    if (o == Py_None) return true;
+    if (!PyLong_CheckExact(o)) return false;
+    int over = 0;
+    const long long x = PyLong_AsLongLongAndOverflow(o, &over);
+    if (over < 0 || (!over && x < 0)) return false;
+    *v = over || x >= kI32 ? (int)(kI32 - 1) : (int)x;
+    return true;
+}
+// the output of packed rows: a new tensor of q's shape, or a view whose rows and heads do not overlap
+struct Out {
+    Tensor made;
+    void *p = nullptr;
+    long long sh = 0, ld = 0;
+    int fill = 0;
+    bool of(const Call &c, const Tensor &q, const Tensor *out) {
+        if (out) {
+            Rows r;
+            if (!r.of(c, *out) || out->sizes() != q.sizes() || (out->size(0) > 1 && r.ld < 256) || (out->size(1) > 1 && r.sh < 256))
+                return false;
+            p = out->data_ptr(), sh = r.sh, ld = r.ld;
+            return true;
+        }
+        made = make(c, q.sizes(), at::kBFloat16);
+        p = made.data_ptr(), sh = made.stride(1), ld = made.stride(0), fill = 1;
+        return true;
+    }
+    PyObject *result(PyObject *given) const {
+        if (fill) return wrap(made);
+        Py_INCREF(given);
+        return given;
+    }
+};
+// a cache and its index tensors for B sequences
+struct Cache {
+    const Tensor *data, *scales, *recent, *lens, *table, *slots;
+    int64_t P = 0, HK = 0, S = 0, width = 0, ldt = 0;
+    bool take(PyObject *d, PyObject *sc, PyObject *r) { return plain(d, &data) && plain(sc, &scales) && plain(r, &recent); }
+    bool index(PyObject *l, PyObject *t, PyObject *s) { return plain(l, &lens) && plain(t, &table) && plain_opt(s, &slots); }
+    bool of(const Call &c, int64_t B) {
+        if (data->dim() != 6 || data->scalar_type() != at::kChar || !data->is_contiguous() || !on(c, *data) || !aligned(*data))
+            return false;
+        P = data->size(0), HK = data->size(2), S = recent->dim() == 5 ? recent->size(0) : 0;
+        const int64_t d[6] = {P, 2, HK, 8, 32, 32}, sc[3] = {P, 2, HK}, r[5] = {S, 2, HK, 32, 256};
+        if (HK < 1 || P >= kI32 || S >= kI32 || data->sizes() != at::IntArrayRef(d, 6) || scales->scalar_type() != at::kFloat ||
+            scales->sizes() != at::IntArrayRef(sc, 3) || !scales->is_contiguous() || !on(c, *scales) ||
+            recent->scalar_type() != at::kBFloat16 || recent->sizes() != at::IntArrayRef(r, 5) || !recent->is_contiguous() ||
+            !on(c, *recent) || !aligned(*recent))
+            return false;
+        if (!counts(c, lens, B) || !counts(c, slots, B) || table->scalar_type() != at::kInt || table->dim() != 2 ||
+            table->size(0) != B || !on(c, *table))
+            return false;
+        width = table->size(1);
+        if (width >= kI32 || (width > 1 && table->stride(1) != 1) || (B > 1 && width && table->stride(0) < width)) return false;
+        ldt = B > 1 && width ? table->stride(0) : width;
+        return true;
+    }
+};
+#define MICA_CACHE(k) (k).data->data_ptr(), (float *)(k).scales->data_ptr(), (k).recent->data_ptr(), (int)(k).P, (int)(k).S, \
+                      (int)(k).HK, 256, (const int *)(k).table->data_ptr(), (long long)(k).ldt, (int)(k).width,               \
+                      (const int *)(k).lens->data_ptr(), (const int *)ptr((k).slots)
+
+// packed_attention(q, k, v, starts, longest, scale, out) -> o
+PyObject *py_packed_attention(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    MICA_ARGS(7)
+    const Tensor *q, *k, *v, *st, *out;
+    int longest;
+    Call c;
+    if (!plain(a[0], &q) || !plain(a[1], &k) || !plain(a[2], &v) || !plain(a[3], &st) || !hint_of(a[4], &longest) ||
+        !plain_opt(a[6], &out) || !enter(*q, c))
+        return none();
+    const double scale = PyFloat_AsDouble(a[5]);
+    if (PyErr_Occurred()) return nullptr;
+    Rows rq, rk, rv;
+    Out o;
+    if (!rq.of(c, *q) || !rk.of(c, *k) || !rv.of(c, *v) || k->sizes() != v->sizes() || k->size(0) != q->size(0) ||
+        k->size(1) < 1 || q->size(1) != 4 * k->size(1) || !starts_of(c, *st))
+        return none();
+    const int64_t T = q->size(0), HK = k->size(1), B = st->size(0) - 1;
+    if (B >= kI32) return none();
+    const long long nbytes = abi.attention_packed_workspace_bytes((int)B, (int)T, (int)HK, longest);
+    if (nbytes < 0 || !o.of(c, *q, out)) return none();
+    Tensor ws;
+    if (nbytes) ws = make(c, {nbytes}, at::kByte);
+    const int rc = launch([&] {
+        return abi.attention_packed(rq.p, rq.sh, rq.ld, rk.p, rk.sh, rk.ld, rv.p, rv.sh, rv.ld, o.p, o.sh, o.ld,
+                                    (const int *)st->data_ptr(), (int)B, (int)T, (int)(4 * HK), (int)HK, 256, (float)scale,
+                                    o.fill, longest, nbytes ? ws.data_ptr() : nullptr, nbytes, c.stream);
+    });
+    if (rc) return bad(rc);
+    return o.result(a[6]);
+    END_HANDLE_TH_ERRORS
+}
+
+// append_kv(data, scales, recent, k, v, starts, lens, table, slots, longest, cos, sin, pos, weight, offset, eps) -> True
+PyObject *py_append_kv(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    MICA_ARGS(16)
+    Cache kv;
+    const Tensor *k, *v, *st, *cs, *sn, *pos, *w;
+    int longest;
+    Call c;
+    if (!kv.take(a[0], a[1], a[2]) || !plain(a[3], &k) || !plain(a[4], &v) || !plain(a[5], &st) || !kv.index(a[6], a[7], a[8]) ||
+        !hint_of(a[9], &longest) || !plain_opt(a[10], &cs) || !plain_opt(a[11], &sn) || !plain_opt(a[12], &pos) ||
+        !plain_opt(a[13], &w) || !enter(*k, c))
+        return none();
+    const double offset = PyFloat_AsDouble(a[14]), eps = PyFloat_AsDouble(a[15]);
+    if (PyErr_Occurred()) return nullptr;
+    Rows rk, rv;
+    if (!rk.of(c, *k) || !rv.of(c, *v) || k->sizes() != v->sizes() || !starts_of(c, *st)) return none();
+    const int64_t T = k->size(0), B = st->size(0) - 1;
+    if (B >= kI32 || !kv.of(c, B) || k->size(1) != kv.HK) return none();
+    if (w && (w->scalar_type() != at::kBFloat16 || w->numel() != 256 || !w->is_contiguous() || !on(c, *w))) return none();
+    int64_t rot = 0, n_pos = 0;
+    int dt = MICA_BF16;
+    if ((cs == nullptr) != (sn == nullptr)) return none();
+    if (cs) {
+        dt = code(cs->scalar_type());
+        if ((dt != MICA_BF16 && dt != MICA_FP32) || sn->scalar_type() != cs->scalar_type() || cs->dim() != 2 ||
+            cs->sizes() != sn->sizes() || !cs->is_contiguous() || !sn->is_contiguous() || !on(c, *cs) || !on(c, *sn))
+            return none();
+        rot = 2 * cs->size(1), n_pos = cs->size(0);
+        if (rot < 16 || rot > 256 || (rot & (rot - 1)) || n_pos >= kI32) return none();
+    }
+    if (pos && (!cs || pos->scalar_type() != at::kInt || pos->numel() != T || !pos->is_contiguous() || !on(c, *pos))) return none();
+    const int rc = launch([&] {
+        return abi.kv_append(rk.p, rk.sh, rk.ld, rv.p, rv.sh, rv.ld, (const int *)st->data_ptr(), (int)B, (int)T, MICA_CACHE(kv),
+                             ptr(w), (float)offset, (float)eps, (int)rot, ptr(cs), ptr(sn), dt, (int)n_pos,
+                             (const int *)ptr(pos), longest, c.stream);
+    });
+    if (rc) return bad(rc);
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
+// read_kv(data, scales, recent, rows, starts, lens, table, slots, longest) -> (k, v)
+PyObject *py_read_kv(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    MICA_ARGS(9)
+    Cache kv;
+    const Tensor *st;
+    int longest;
+    Call c;
+    if (!kv.take(a[0], a[1], a[2]) || !PyLong_CheckExact(a[3]) || !plain(a[4], &st) || !kv.index(a[5], a[6], a[7]) ||
+        !hint_of(a[8], &longest) || !enter(*kv.data, c))
+        return none();
+    int over = 0;
+    const long long T = PyLong_AsLongLongAndOverflow(a[3], &over);
+    if (over || T < 0 || T >= kI32 || !starts_of(c, *st) || st->size(0) > kI32 || !kv.of(c, st->size(0) - 1)) return none();
+    const Tensor k = make(c, {T, kv.HK, 256}, at::kBFloat16), v = make(c, {T, kv.HK, 256}, at::kBFloat16);
+    const int rc = launch([&] {
+        return abi.kv_read(k.data_ptr(), v.data_ptr(), (const int *)st->data_ptr(), (int)(st->size(0) - 1), (int)T, MICA_CACHE(kv),
+                           longest, c.stream);
+    });
+    if (rc) return bad(rc);
+    return pack({wrap(k), wrap(v)});
+    END_HANDLE_TH_ERRORS
+}
+
+// paged_attention(q, data, scales, recent, starts, lens, table, slots, longest, scale, out) -> o
+PyObject *py_paged_attention(PyObject *, PyObject *const *a, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    MICA_ARGS(11)
+    Cache kv;
+    const Tensor *q, *st, *out;
+    int longest;
+    Call c;
+    if (!plain(a[0], &q) || !kv.take(a[1], a[2], a[3]) || !plain(a[4], &st) || !kv.index(a[5], a[6], a[7]) ||
+        !hint_of(a[8], &longest) || !plain_opt(a[10], &out) || !enter(*q, c))
+        return none();
+    const double scale = PyFloat_AsDouble(a[9]);
+    if (PyErr_Occurred()) return nullptr;
+    Rows rq;
+    Out o;
+    if (!rq.of(c, *q) || !starts_of(c, *st)) return none();
+    const int64_t T = q->size(0), B = st->size(0) - 1;
+    if (B >= kI32 || !kv.of(c, B) || q->size(1) != 4 * kv.HK) return none();
+    const long long nbytes = abi.attention_paged_workspace_bytes((int)B, (int)T, (int)kv.HK, (int)kv.width, longest);
+    if (nbytes < 0 || !o.of(c, *q, out)) return none();
+    Tensor ws;
+    if (nbytes) ws = make(c, {nbytes}, at::kByte);
+    const int rc = launch([&] {
+        return abi.attention_paged(rq.p, rq.sh, rq.ld, o.p, o.sh, o.ld, (const int *)st->data_ptr(), (int)B, (int)T,
+                                   (int)(4 * kv.HK), MICA_CACHE(kv), (float)scale, o.fill, longest,
+                                   nbytes ? ws.data_ptr() : nullptr, nbytes, c.stream);
+    });
+    if (rc) return bad(rc);
+    return o.result(a[10]);
+    END_HANDLE_TH_ERRORS
+}
+
 // bind({name: address}): the loaded library's functions
 PyObject *py_bind(PyObject *, PyObject *d) {
     bool all = PyDict_Check(d);
@@ -680,6 +897,12 @@ PyObject *py_bind(PyObject *, PyObject *d) {
     MICA_FN(attention_tree_workspace_bytes)
     MICA_FN(attention_window)
     MICA_FN(attention_window_workspace_bytes)
+    MICA_FN(attention_packed)
+    MICA_FN(attention_packed_workspace_bytes)
+    MICA_FN(kv_append)
+    MICA_FN(kv_read)
+    MICA_FN(attention_paged)
+    MICA_FN(attention_paged_workspace_bytes)
 #undef MICA_FN
     if (PyErr_Occurred()) return nullptr;
     if (!all) {
@@ -728,6 +951,10 @@ PyMethodDef kMethods[] = {
     MICA_DEF("token_logprobs", py_token_logprobs),
     MICA_DEF("tree_attention", py_tree_attention),
     MICA_DEF("window_attention", py_window_attention),
+    MICA_DEF("packed_attention", py_packed_attention),
+    MICA_DEF("append_kv", py_append_kv),
+    MICA_DEF("read_kv", py_read_kv),
+    MICA_DEF("paged_attention", py_paged_attention),
     {"bind", py_bind, METH_O, nullptr},
     {"device_ok", py_device_ok, METH_O, nullptr},
     MICA_DEF("workspace", py_workspace),

@@ -254,18 +254,20 @@ MICA_DEVICE void leave(const PagedParams &p, long long part, int pair, int dt0, 
     if (dt0 == 0 && hi == 0) p.part_ml[part * np + pair] = blind ? float2{-__builtin_inff(), -1.0f} : float2{m, l};
 }
 
-// ---- few rows: up to 8 of a sequence ----
+// ---- few rows: up to 8 G of a sequence ----
 // A wave takes tiles by itself: a page's pieces go from memory straight into the registers of the matrix cores' operands, 16
 // bytes a lane, each loaded for the next tile as soon as this one's has been widened, so that a wave has a page (16 KB) in
 // flight all the time.  Nothing is shared, there is no barrier, and the matrix cores' time (of which a single row uses an
 // eighth) is hidden behind the memory's.  The weights are taken as two bf16 summands: they cost products that are free here.
+template <int G>
 __global__ __launch_bounds__(256, 1) void pg_few_kernel(PagedParams p) {
     __shared__ __attribute__((aligned(1024))) int8_t smem[4 * kTile]; // a wave's values of the rest
     const int lane = threadIdx.x & 63, l32 = lane & 31, hi = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int worker = blockIdx.x * 4 + wave, hk = worker % p.c.HK, run = worker / p.c.HK;
+    const int worker = blockIdx.x * (4 / G) + wave / G, rb = wave % G, hk = worker % p.c.HK, run = worker / p.c.HK;
+    const int pair = rb * 32 + l32;
     if (run >= p.runs) return;
-    if (p.fill) {
+    if (p.fill && rb == 0) {
         const int none = p.rows.at(0) + p.rows.T - p.rows.at(p.rows.B);
         for (int i = run * 32; i < none; i += p.runs * 32) fill_rows(p, hk, i, 32, lane, 64);
     }
@@ -274,7 +276,7 @@ __global__ __launch_bounds__(256, 1) void pg_few_kernel(PagedParams p) {
     if (!w.begin(p, run)) return;
     do {
         const int q0 = w.qb * p.nb, from = w.len - w.n, whole = w.len / kBK;
-        const int t = q0 + (l32 >> 2), head = hk * kGroup + (l32 & 3), pos = from + t; // this lane's pair l32
+        const int t = q0 + (pair >> 2), head = hk * kGroup + (pair & 3), pos = from + t; // this lane's pair
         // Q fragments (B operand of S^T): step 2 c + e takes dims 32 c + 16 hi + 8 e .. + 7, as a page's bytes lie; rows past the
         // last repeat it
         bf16x8 qf[kD / 16];
@@ -336,8 +338,10 @@ __global__ __launch_bounds__(256, 1) void pg_few_kernel(PagedParams p) {
                     rv[x] = piece(nv, x);
                     O[x] = mfma_bf16(a, h0, O[x]);
                     O[x] = mfma_bf16(c, h1, O[x]);
-                    O[x] = mfma_bf16(a, g0, O[x]);
-                    O[x] = mfma_bf16(c, g1, O[x]);
+                    if constexpr (G == 1) {
+                        O[x] = mfma_bf16(a, g0, O[x]);
+                        O[x] = mfma_bf16(c, g1, O[x]);
+                    }
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
@@ -403,8 +407,8 @@ __global__ __launch_bounds__(256, 1) void pg_few_kernel(PagedParams p) {
         }
         const float l = half_swap_sum(sm.lsum);
         if (!w.whole()) {
-            leave(p, (long long)w.part * p.c.HK + (long long)hk, l32, 0, hi, pos < 0, O, sm.m, l);
-        } else if (t < w.n && (l32 >> 2) < p.nb) {
+            leave(p, (long long)w.part * p.c.HK + hk, pair, 0, hi, pos < 0, O, sm.m, l);
+        } else if (t < w.n && (pair >> 2) < p.nb) {
             // (a row whose scores are all -inf has no softmax: 0 / 0; one that sees no key: zeros)
             const float inv = 1.0f / l;
             uint16_t *out = p.o + head * p.sho + (long long)(w.first + t) * p.ldo + 4 * hi;
@@ -678,10 +682,15 @@ __global__ __launch_bounds__(kThreads, 2) void pg_fwd_kernel(PagedParams p) {
 
 // The partial states of a divided unit joined: with M = max_c m_c, w_c = 2^(m_c - M), o = (sum w_c O_c) / (sum w_c l_c).  A
 // workgroup goes by the place where run r begins, and joins the unit there if it is the unit's first division; a thread has
-// four dims of one pair.
+// four dims of one pair, or W waves share the parts of theirs.
+template <int W>
 __global__ __launch_bounds__(256) void pg_merge_kernel(PagedParams p) {
-    const int np = kGroup * p.nb, blocks = np / 4; // workgroups that share a unit's 64 x np fours
-    const int x = blockIdx.x % blocks * 256 + threadIdx.x, hk = blockIdx.x / blocks % p.c.HK, r = blockIdx.x / blocks / p.c.HK + 1;
+    __shared__ float4 accs[W > 1 ? 4 : 1][64];
+    __shared__ float2 mls[W > 1 ? 4 : 1][64];
+    const int np = kGroup * p.nb, blocks = np * W / 4; // workgroups that share a unit's 64 x np fours
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int x = (blockIdx.x % blocks * 4 + wave) / W * 64 + lane;
+    const int hk = blockIdx.x / blocks % p.c.HK, r = blockIdx.x / blocks / p.c.HK + 1;
     Walk all(p);
     const int at = r * all.per;
     if (at >= all.total) return;
@@ -699,16 +708,24 @@ __global__ __launch_bounds__(256) void pg_merge_kernel(PagedParams p) {
     float4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
     // no part has a key that counts: weights 1 on zeros (a sum that is NaN or -1 stays so)
     auto weight = [](float m, float top) { return top == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - top); };
-    constexpr int kBatch = 4; // parts whose loads are in flight together
-    for (int c0 = 0; c0 < parts; c0 += kBatch) {
+    auto add = [&](float w, float2 ml, float4 o) {
+        l += w * ml.y;
+        acc.x += w * o.x;
+        acc.y += w * o.y;
+        acc.z += w * o.z;
+        acc.w += w * o.w;
+    };
+    constexpr int kBatch = 8; // parts whose loads are in flight together
+    for (int c0 = wave % W; c0 < parts; c0 += W * kBatch) {
         float2 ml[kBatch];
         float4 o[kBatch];
 #pragma unroll
         for (int y = 0; y < kBatch; ++y) {
-            const long long k = part(c0 + y < parts ? c0 + y : c0);
+            const int c = c0 + y * W;
+            const long long k = part(c < parts ? c : c0);
             ml[y] = p.part_ml[k * np + pair];
             o[y] = p.part_o[(k * 64 + four) * np + pair];
-            if (c0 + y >= parts) ml[y] = float2{-__builtin_inff(), 0.0f}, o[y] = float4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (c >= parts) ml[y] = float2{-__builtin_inff(), 0.0f}, o[y] = float4{0.0f, 0.0f, 0.0f, 0.0f};
         }
         float top = mx;
 #pragma unroll
@@ -717,14 +734,17 @@ __global__ __launch_bounds__(256) void pg_merge_kernel(PagedParams p) {
         l *= w, acc.x *= w, acc.y *= w, acc.z *= w, acc.w *= w;
         mx = top;
 #pragma unroll
-        for (int y = 0; y < kBatch; ++y) {
-            const float v = weight(ml[y].x, mx);
-            l += v * ml[y].y;
-            acc.x += v * o[y].x;
-            acc.y += v * o[y].y;
-            acc.z += v * o[y].z;
-            acc.w += v * o[y].w;
-        }
+        for (int y = 0; y < kBatch; ++y) add(weight(ml[y].x, mx), ml[y], o[y]);
+    }
+    if constexpr (W > 1) {
+        accs[wave][lane] = acc, mls[wave][lane] = float2{mx, l};
+        __syncthreads();
+        if (wave > 0) return;
+#pragma unroll
+        for (int w = 1; w < W; ++w) mx = __builtin_fmaxf(mx, mls[w][lane].x);
+        l = 0.0f, acc = float4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < W; ++w) add(weight(mls[w][lane].x, mx), mls[w][lane], accs[w][lane]);
     }
     const int t = qb * p.nb + (pair >> 2);
     if (t >= n) return;
@@ -738,7 +758,7 @@ __global__ __launch_bounds__(256) void pg_merge_kernel(PagedParams p) {
 constexpr int kCus = 256;
 
 struct Plan {
-    int R;                       // row blocks of a workgroup; 0: pg_few_kernel
+    int G;                       // pg_few_kernel's waves of a run; 0: pg_fwd_kernel
     int nb, runs, least, begin;  // see PagedParams
     long long units, tiles, states; // most units; most places of the row; partial states
 };
@@ -746,14 +766,14 @@ struct Plan {
 Plan plan(long long B, long long T, int HK, int width, int longest) {
     Plan pl{};
     const long long hint = longest > 0 && longest < T ? longest : T;
-    pl.R = hint <= 8 ? 0 : hint <= 16 ? 2 : hint <= 32 ? 4 : 8;
-    pl.nb = hint <= 1 ? 1 : hint <= 2 ? 2 : hint <= 4 ? 4 : hint <= 8 ? 8 : 8 * pl.R;
+    pl.G = hint <= 8 ? 1 : hint <= 16 ? 2 : hint <= 32 ? 4 : 0;
+    pl.nb = hint <= 1 ? 1 : hint <= 2 ? 2 : hint <= 4 ? 4 : pl.G ? 8 * pl.G : 64;
     const long long most = (T + (pl.nb - 1) * B) / pl.nb;
     pl.units = most < T ? most : T;
-    pl.begin = B == 1 && pl.units == 1 ? 0 : pl.R ? 4 : 2;
-    pl.least = pl.R ? 4 : 1;
+    pl.begin = B == 1 && pl.units == 1 ? 0 : pl.G ? 2 : 4;
+    pl.least = pl.G ? 1 : 4;
     pl.tiles = pl.units * (width + 1ll + pl.begin);
-    const long long slots = pl.R == 0 ? 4 * kCus : kCus; // waves or workgroups that the chip holds at once
+    const long long slots = pl.G ? 4 * kCus / pl.G : kCus; // runs that the chip holds at once
     long long runs = slots / HK > 0 ? slots / HK : 1;
     const long long useful = pl.tiles / (pl.least + pl.begin) + 1; // (no more than can have tiles)
     pl.runs = (int)(runs < useful ? runs : useful);
@@ -794,13 +814,17 @@ extern "C" int mica_attention_paged(const void *q, long long shq, long long ldq,
     p.part_ml = (float2 *)((char *)workspace + pl.states * kGroup * pl.nb * kD * 4);
     hipStream_t st = (hipStream_t)stream;
     const long long workers = (long long)pl.runs * HK;
-    if (pl.R == 0) hipLaunchKernelGGL(pg_few_kernel, dim3((unsigned)((workers + 3) / 4)), dim3(256), 0, st, p);
-    else if (pl.R == 2) hipLaunchKernelGGL(pg_fwd_kernel<2>, dim3((unsigned)workers), dim3(kThreads), 0, st, p);
-    else if (pl.R == 4) hipLaunchKernelGGL(pg_fwd_kernel<4>, dim3((unsigned)workers), dim3(kThreads), 0, st, p);
+    const unsigned few = pl.G ? (unsigned)((workers * pl.G + 3) / 4) : 0;
+    if (pl.G == 1) hipLaunchKernelGGL(pg_few_kernel<1>, dim3(few), dim3(256), 0, st, p);
+    else if (pl.G == 2) hipLaunchKernelGGL(pg_few_kernel<2>, dim3(few), dim3(256), 0, st, p);
+    else if (pl.G == 4) hipLaunchKernelGGL(pg_few_kernel<4>, dim3(few), dim3(256), 0, st, p);
     else hipLaunchKernelGGL(pg_fwd_kernel<8>, dim3((unsigned)workers), dim3(kThreads), 0, st, p);
     if (const int rc = mica_err(hipGetLastError())) return rc;
     if (pl.states == 0) return 0;
-    hipLaunchKernelGGL(pg_merge_kernel, dim3((unsigned)((pl.runs - 1) * HK * pl.nb)), dim3(256), 0, st, p);
+    // (many parts a unit: four waves share them)
+    const unsigned joins = (unsigned)((pl.runs - 1) * HK * pl.nb);
+    if (pl.runs >= 8 * pl.units) hipLaunchKernelGGL(pg_merge_kernel<4>, dim3(joins * 4), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL(pg_merge_kernel<1>, dim3(joins), dim3(256), 0, st, p);
     return mica_err(hipGetLastError());
 }
 

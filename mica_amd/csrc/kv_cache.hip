@@ -212,6 +212,7 @@ struct ReadParams {
     Pages c;
     Ragged rows;
     uint16_t *k, *v;   // [T][HK][256]
+    int each, wgs;     // workgroups a sequence (0: one for each unit); of a head and side
 };
 
 __global__ __launch_bounds__(kThreads) void kv_read_kernel(ReadParams p) {
@@ -225,63 +226,65 @@ __global__ __launch_bounds__(kThreads) void kv_read_kernel(ReadParams p) {
         for (int j = 0; j < 4; ++j) *(u32x4 *)(out + row * ld + 8 * (sub + 8 * j)) = x[j];
     };
     const u32x4 zeros[4] = {};
+    // rows of no sequence, before the first and behind the last
+    const int before = p.rows.at(0), none = before + p.rows.T - p.rows.at(p.rows.B);
+    for (int i = id * kPage + token; i < none; i += p.wgs * kPage) store(i < before ? i : p.rows.T - none + (long long)i, zeros);
     // a sequence's units: the blocks that its rows lie in (places before the sequence's beginning too: they are zeros)
     auto units = [&](int b) {
         const int n = p.rows.rows(b), last = p.c.len(b) - 1;
         return n ? (last >> 5) - ((last - n + 1) >> 5) + 1 : 0;
     };
     int b, u;
-    if (!find_unit(p.rows.B, units, id, b, u)) { // rows of no sequence
-        const int before = p.rows.at(0), i = (id - b) * kPage + token, t = i < before ? i : p.rows.at(p.rows.B) + i - before;
-        if (i >= 0 && t < p.rows.T) store(t, zeros);
-        return;
-    }
+    if (p.each) b = id / p.each, u = id % p.each;
+    else if (!find_unit(p.rows.B, units, id, b, u)) return;
     b = __builtin_amdgcn_readfirstlane(b), u = __builtin_amdgcn_readfirstlane(u);
-    const int n = p.rows.rows(b), len = p.c.len(b), from = len - n;
-    const int block = (from >> 5) + u, at = block * kPage + token;
-    const bool live = at >= from && at < len;
-    const long long row = p.rows.at(b) + (long long)at - from;
-    if (block < 0) {
-        if (live) store(row, zeros);
-        return;
-    }
-    u32x4 x[4];
-    if (block < len / kPage) {
-        const int page = p.c.page(b, block);
-        const float s = page >= 0 ? p.c.scales[p.c.index(page, side, hk)] : __builtin_nanf("");
-        const int8_t *src = p.c.block(max(page, 0), side, hk);
-        if (side == 0) {
+    const int n = p.rows.rows(b), len = p.c.len(b), from = len - n, first = p.rows.at(b), slot = p.c.slot(b);
+    for (const int all = units(b); u < all; u += p.each ? p.each : all) {
+        const int block = (from >> 5) + u, at = block * kPage + token;
+        const bool live = at >= from && at < len;
+        const long long row = first + (long long)at - from;
+        if (block < 0) {
+            if (live) store(row, zeros);
+            continue;
+        }
+        u32x4 x[4];
+        if (block < len / kPage) {
+            const int page = p.c.page(b, block);
+            const float s = page >= 0 ? p.c.scales[p.c.index(page, side, hk)] : __builtin_nanf("");
+            const int8_t *src = p.c.block(max(page, 0), side, hk);
+            if (side == 0) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const u32x2 q = page >= 0 ? *(const u32x2 *)(src + (2 * j + (sub >> 2)) * 1024 + token * 32 + (sub & 3) * 8)
-                                          : u32x2{0u, 0u};
+                for (int j = 0; j < 4; ++j) {
+                    const u32x2 q = page >= 0 ? *(const u32x2 *)(src + (2 * j + (sub >> 2)) * 1024 + token * 32 + (sub & 3) * 8)
+                                              : u32x2{0u, 0u};
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t w = q[e >> 1] >> (16 * (e & 1));
-                    x[j][e] = pack_bf16x2((float)(int8_t)w * s, (float)(int8_t)(w >> 8) * s);
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t w = q[e >> 1] >> (16 * (e & 1));
+                        x[j][e] = pack_bf16x2((float)(int8_t)w * s, (float)(int8_t)(w >> 8) * s);
+                    }
                 }
+            } else {
+                u32x4 q[2] = {};
+                if (page >= 0) q[0] = ((const u32x4 *)(src + tid * 32))[0], q[1] = ((const u32x4 *)(src + tid * 32))[1];
+#pragma unroll
+                for (int w = 0; w < 8; ++w)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        tile[4 * page_four(w) + e][tid] = f32_to_bf16((float)(int8_t)(q[w >> 2][w & 3] >> (8 * e)) * s);
+                __syncthreads();
+#pragma unroll
+                for (int j = 0; j < 4; ++j) x[j] = *(const u32x4 *)&tile[token][8 * (sub + 8 * j)];
+                __syncthreads(); // the tile is free again
             }
         } else {
-            u32x4 q[2] = {};
-            if (page >= 0) q[0] = ((const u32x4 *)(src + tid * 32))[0], q[1] = ((const u32x4 *)(src + tid * 32))[1];
+            const uint16_t *rest = p.c.rest(max(slot, 0), side, hk);
+            const uint32_t nan = 0x7fc07fc0u;
 #pragma unroll
-            for (int w = 0; w < 8; ++w)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    tile[4 * page_four(w) + e][tid] = f32_to_bf16((float)(int8_t)(q[w >> 2][w & 3] >> (8 * e)) * s);
-            __syncthreads();
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x[j] = *(const u32x4 *)&tile[token][8 * (sub + 8 * j)];
+            for (int j = 0; j < 4; ++j)
+                x[j] = slot >= 0 && live ? *(const u32x4 *)(rest + token * kPagedDim + 8 * (sub + 8 * j)) : u32x4{nan, nan, nan, nan};
         }
-    } else {
-        const int slot = p.c.slot(b);
-        const uint16_t *rest = p.c.rest(max(slot, 0), side, hk);
-        const uint32_t nan = 0x7fc07fc0u;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            x[j] = slot >= 0 && live ? *(const u32x4 *)(rest + token * kPagedDim + 8 * (sub + 8 * j)) : u32x4{nan, nan, nan, nan};
+        if (live) store(row, x);
     }
-    if (live) store(row, x);
 }
 
 }  // namespace
@@ -324,7 +327,7 @@ extern "C" int mica_kv_append(const void *k, long long shk, long long ldk, const
 
 extern "C" int mica_kv_read(void *k, void *v, const int *starts, int B, int T, const void *data, const float *scales,
                             const void *recent, int pages, int n_slots, int HK, int head_dim, const int *table, long long ldt,
-                            int width, const int *lens, const int *slots, mica_stream_t stream) {
+                            int width, const int *lens, const int *slots, int longest, mica_stream_t stream) {
     if (B < 0 || T < 0) return MICA_MISS_SHAPE;
     if (T == 0) return 0;
     ReadParams p{};
@@ -335,8 +338,12 @@ extern "C" int mica_kv_read(void *k, void *v, const int *starts, int B, int T, c
     if (!mica_aligned16(k) || !mica_aligned16(v) || ((uintptr_t)starts & 3)) return MICA_MISS_ALIGN;
     p.rows = Ragged{starts, B, T};
     p.k = (uint16_t *)k; p.v = (uint16_t *)v;
-    // blocks that n rows lie in: at most (n + 62) / 32 and n; rows of no sequence 32 at a time
-    const long long most = ((long long)T + 62ll * B + 31) / 32, units = most < T ? most : T, wgs = units * HK * 2;
+    // blocks that n rows lie in: at most (n + 62) / 32 and n; each sequence's without the search as for an append
+    const long long most = ((long long)T + 62ll * B) / 32, units = B == 0 ? 1 : most < T ? most : T;
+    const long long hint = longest > 0 && longest < T ? longest : T, each = hint < 2 ? 1 : (hint + 62) / 32;
+    p.each = B > 0 && each * B <= 2 * units ? (int)each : 0;
+    const long long per = p.each ? each * B : units, wgs = per * HK * 2;
+    p.wgs = (int)(per < (1 << 30) ? per : 1);
     if (wgs >= (1 << 24)) return MICA_MISS_RANGE;
     hipLaunchKernelGGL(kv_read_kernel, dim3((unsigned)wgs), dim3(kThreads), 0, (hipStream_t)stream, p);
     return mica_err(hipGetLastError());

@@ -20,7 +20,7 @@ import torch
 
 from . import _lib
 from .attention import GROUP, HEAD_DIM, _counts, _hint, _out, _rows, _scale, _starts
-from .int8_kernels import _gpu_ok, _launched, _on, _stream
+from .int8_kernels import _gpu_ok, _launched, _native, _on, _stream
 
 PAGE = 32        # tokens of a block
 
@@ -88,6 +88,12 @@ def append_kv(cache: PagedKV, k, v, starts, lens, table, slots=None, longest: in
     lens[b] + i or pos[t] (int32 [T]); tables bf16 or fp32 [n_pos, dims / 2]; a row whose position lies outside them is not
     rotated.  Both in fp32 and rounded to bf16 once (``fused_kernels.head_norm_rope`` rounds each step as the model's bf16
     operations do; rows that it has treated go in without these)."""
+    w, offset, eps = (None, 0.0, 0.0) if norm is None else norm
+    cos, sin, pos = (None, None, None) if rope is None else rope if len(rope) == 3 else (*rope, None)
+    r = _lib.FAST.append_kv(*cache, k, v, starts, lens, table, slots, longest, cos, sin, pos, w, offset, eps)
+    if r is not None:
+        _native(r, "mica_kv_append")
+        return cache
     sk, sv = _rows(k, "k"), _rows(v, "v", k.device)
     if k.shape != v.shape:
         raise ValueError("k and v must have one shape")
@@ -96,13 +102,11 @@ def append_kv(cache: PagedKV, k, v, starts, lens, table, slots=None, longest: in
     T = k.shape[0]
     if k.shape[1] != HK:
         raise ValueError("k and v must have the cache's heads")
-    w, offset, eps, rot_dim, cos, sin, pos, code = None, 0.0, 0.0, 0, None, None, None, _lib.BF16
+    rot_dim, code = 0, _lib.BF16
     if norm is not None:
-        w, offset, eps = norm
         if w.dtype != torch.bfloat16 or w.device != dev or w.numel() != HEAD_DIM or not w.is_contiguous():
             raise ValueError("the norm weight must be a contiguous bf16 [256] tensor on the rows' device")
     if rope is not None:
-        cos, sin, pos = rope if len(rope) == 3 else (*rope, None)
         for t in (cos, sin):
             if (t.dtype not in (torch.bfloat16, torch.float32) or t.device != dev or t.dim() != 2 or not t.is_contiguous()
                     or t.shape != cos.shape or t.dtype != cos.dtype):
@@ -127,6 +131,9 @@ def read_kv(cache: PagedKV, rows: int, starts, lens, table, slots=None, longest:
     """Rows of the cache back in bf16 (mica_kv_read): (k, v), [rows, HK, 256] each, the rows of sequence b (starts[b] ..
     starts[b + 1] - 1) being its last tokens; zeros for those before its first and for rows of no sequence.  rows: how many there
     are in all (starts[B], which the host is not to wait for); the other arguments as in append_kv, lens the tokens now."""
+    r = _lib.FAST.read_kv(*cache, rows, starts, lens, table, slots, longest)
+    if r is not None:
+        return _native(r, "mica_kv_read")
     B, rows, longest = _starts(starts, cache[0].device), int(rows), _hint(longest)
     if not 0 <= rows < 2 ** 31:
         raise ValueError("rows must be a count of rows")
@@ -134,7 +141,7 @@ def read_kv(cache: PagedKV, rows: int, starts, lens, table, slots=None, longest:
     k, v = (torch.empty((rows, HK, HEAD_DIM), dtype=torch.bfloat16, device=dev) for _ in range(2))
     L = _lib.load()
     rc = _lib.check(_on(dev, lambda: L.mica_kv_read(k.data_ptr(), v.data_ptr(), starts.data_ptr(), B, rows, *args,
-                                                    _stream(dev))), "mica_kv_read")
+                                                    longest, _stream(dev))), "mica_kv_read")
     if rc:
         raise ValueError(f"read_kv: unsupported input ({_lib.status_name(rc)})")
     _launched()
@@ -150,6 +157,9 @@ def paged_attention(q, cache: PagedKV, starts, lens, table, slots=None, longest:
     as in append_kv.  longest (the longest sequence's rows, a hint), the result and out= as in ``attention.packed_attention``; a
     row before its sequence's first token has zeros."""
     scale = _scale(scale)
+    r = _lib.FAST.paged_attention(q, *cache, starts, lens, table, slots, longest, scale, out)
+    if r is not None:
+        return _native(r, "mica_attention_paged")
     sq = _rows(q, "q")
     B, longest = _starts(starts, q.device), _hint(longest)
     dev, HK, args = _cache(cache, B, lens, table, slots, q.device)

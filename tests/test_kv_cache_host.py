@@ -56,7 +56,7 @@ def test_append_refuses(kw, code):
 
 
 def read(**kw):
-    a = dict(k=A16, v=A16, starts=A16, B=2, T=50, **CACHE, stream=None)
+    a = dict(k=A16, v=A16, starts=A16, B=2, T=50, **CACHE, longest=0, stream=None)
     a.update(kw)
     return _lib.load().mica_kv_read(*a.values())
 
