@@ -74,6 +74,19 @@ struct Walk {
         }
         per = max((total + p.runs - 1) / p.runs, p.least + p.begin);
     }
+    // the place where unit qb of sequence b begins; called once
+    MICA_DEVICE int place(const PagedParams &p, int b, int qb) {
+        int before = 0;
+        for (int from = 0; from < b / 64 * 64; from += 64) {
+            if (from) take(p, from);
+            before += __builtin_amdgcn_readlane(sum, 63);
+        }
+        if (b >= 64) take(p, b / 64 * 64);
+        before += __builtin_amdgcn_readlane(sum - x, b % 64);
+        const int n = p.rows.rows(b), len = p.c.len(b);
+        for (int q = 0; q < qb; ++q) before += tiles(p, n, len, q) + p.begin;
+        return __builtin_amdgcn_readfirstlane(before);
+    }
     // the unit at place `at` (below total), and the place where it begins; called once
     MICA_DEVICE void find(const PagedParams &p, int at, int &b, int &qb, int &from) {
         int before = 0;
@@ -681,25 +694,32 @@ __global__ __launch_bounds__(kThreads, 2) void pg_fwd_kernel(PagedParams p) {
 }
 
 // The partial states of a divided unit joined: with M = max_c m_c, w_c = 2^(m_c - M), o = (sum w_c O_c) / (sum w_c l_c).  A
-// workgroup goes by the place where run r begins, and joins the unit there if it is the unit's first division; a thread has
-// four dims of one pair, or W waves share the parts of theirs.
-template <int W>
+// workgroup goes by the units, or, where there may be more of them than runs, by the place where run r begins, and joins the
+// unit there if it is the unit's first division; a thread has four dims of one pair, or W waves share the parts of theirs.
+template <int W, bool UNITS>
 __global__ __launch_bounds__(256) void pg_merge_kernel(PagedParams p) {
     __shared__ float4 accs[W > 1 ? 4 : 1][64];
     __shared__ float2 mls[W > 1 ? 4 : 1][64];
     const int np = kGroup * p.nb, blocks = np * W / 4; // workgroups that share a unit's 64 x np fours
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int x = (blockIdx.x % blocks * 4 + wave) / W * 64 + lane;
-    const int hk = blockIdx.x / blocks % p.c.HK, r = blockIdx.x / blocks / p.c.HK + 1;
+    const int hk = blockIdx.x / blocks % p.c.HK, y = blockIdx.x / blocks / p.c.HK;
     Walk all(p);
-    const int at = r * all.per;
-    if (at >= all.total) return;
     int b, qb, from;
-    all.find(p, at, b, qb, from);
+    if constexpr (UNITS) {
+        if (!find_unit(p.rows.B, [&](int i) { return (p.rows.rows(i) + p.nb - 1) / p.nb; }, y, b, qb)) return;
+        from = all.place(p, b, qb);
+    } else {
+        const int at = (y + 1) * all.per;
+        if (at >= all.total) return;
+        all.find(p, at, b, qb, from);
+        const int start = from + p.begin;
+        if (at <= start || start / all.per != y) return;
+    }
     const int start = from + p.begin, g0 = start / all.per; // the unit's first tile, and the run that has it
-    if (at <= start || g0 != r - 1) return;
     const int n = p.rows.rows(b), tiles = Walk::tiles(p, n, p.c.len(b), qb);
     const int parts = (start + tiles - 1) / all.per - g0 + 1;
+    if (parts < 2) return; // its worker wrote it
     const int pair = x % np, four = x / np;
     auto part = [&](int c) { // (a unit that begins within a run has the run's second place)
         return (2 * (long long)(g0 + c) + ((g0 + c) * all.per < from)) * p.c.HK + hk;
@@ -821,10 +841,12 @@ extern "C" int mica_attention_paged(const void *q, long long shq, long long ldq,
     else hipLaunchKernelGGL(pg_fwd_kernel<8>, dim3((unsigned)workers), dim3(kThreads), 0, st, p);
     if (const int rc = mica_err(hipGetLastError())) return rc;
     if (pl.states == 0) return 0;
-    // (many parts a unit: four waves share them)
-    const unsigned joins = (unsigned)((pl.runs - 1) * HK * pl.nb);
-    if (pl.runs >= 8 * pl.units) hipLaunchKernelGGL(pg_merge_kernel<4>, dim3(joins * 4), dim3(256), 0, st, p);
-    else hipLaunchKernelGGL(pg_merge_kernel<1>, dim3(joins), dim3(256), 0, st, p);
+    const bool units = pl.units < pl.runs;
+    const unsigned joins = (unsigned)((units ? pl.units : pl.runs - 1) * HK * pl.nb);
+    if (units && pl.runs >= 8 * pl.units) // many parts a unit: four waves share them
+        hipLaunchKernelGGL((pg_merge_kernel<4, true>), dim3(joins * 4), dim3(256), 0, st, p);
+    else if (units) hipLaunchKernelGGL((pg_merge_kernel<1, true>), dim3(joins), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((pg_merge_kernel<1, false>), dim3(joins), dim3(256), 0, st, p);
     return mica_err(hipGetLastError());
 }
 
