@@ -43,6 +43,40 @@ MICA_DEVICE void fill_rows(const PackedParams &p, int hk, int i0) {
     }
 }
 
+// The id-th block of all, the longest first (a block has as many tiles as its place in its sequence, and one): with one sequence
+// after the other the last ones keep a few CUs busy alone.  Up to 64 sequences, a lane each; a lane for each of 64 candidate
+// places.  False where there are fewer blocks (b is then their number).
+MICA_DEVICE bool longest_first(const Ragged &rows, int id, int &b, int &qb) {
+    const int lane = threadIdx.x & 63;
+    const int nb = lane < rows.B ? (rows.rows(lane) + kB - 1) / kB : 0;
+    int most = nb;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) most = max(most, __shfl_xor(most, m, 64));
+    most = __builtin_amdgcn_readfirstlane(most);
+    auto from = [&](int place) { // blocks at that place or later
+        int n = 0;
+        for (int i = 0; i < rows.B; ++i) n += max(__builtin_amdgcn_readlane(nb, i) - place, 0);
+        return n;
+    };
+    int step = 1, place = 0; // the last place from which on there are more than id blocks, by strides
+    while (step * 64 <= most) step *= 64;
+    for (;; step /= 64) {
+        const int n = from(place + lane * step);
+        const unsigned long long more = __builtin_amdgcn_ballot_w64(n > id);
+        if (!more) {
+            b = __builtin_amdgcn_readfirstlane(n);
+            return false;
+        }
+        place += (63 - __builtin_clzll(more)) * step;
+        if (step == 1) break;
+    }
+    const unsigned long long has = __builtin_amdgcn_ballot_w64(nb > place);
+    const int rank = __builtin_popcountll(has & ((1ull << lane) - 1));
+    b = __builtin_ctzll(__builtin_amdgcn_ballot_w64(nb > place && rank == id - from(place + 1)));
+    qb = place;
+    return true;
+}
+
 __global__ __launch_bounds__(kThreads, 2) void pk_fwd_kernel(PackedParams p) {
     constexpr int kSmem = kGroup * kB * kD * 2 > 2 * kStage ? kGroup * kB * kD * 2 : 2 * kStage; // the stages; the output, in the end
     __shared__ __attribute__((aligned(1024))) int8_t smem[kSmem + 16];
@@ -51,14 +85,16 @@ __global__ __launch_bounds__(kThreads, 2) void pk_fwd_kernel(PackedParams p) {
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
     const int hk = blockIdx.x % p.HK, id = blockIdx.x / p.HK;
-    int b, u;
-    if (!find_unit(p.rows.B, [&](int i) { return (p.rows.rows(i) + kB - 1) / kB; }, id, b, u)) {
+    int b, qb;
+    const bool any = p.rows.B <= 64 ? longest_first(p.rows, id, b, qb)
+                                    : find_unit(p.rows.B, [&](int i) { return (p.rows.rows(i) + kB - 1) / kB; }, id, b, qb);
+    if (!any) {
         if (p.fill) fill_rows(p, hk, (id - b) * kB);
         return;
     }
-    b = __builtin_amdgcn_readfirstlane(b), u = __builtin_amdgcn_readfirstlane(u);
+    b = __builtin_amdgcn_readfirstlane(b), qb = __builtin_amdgcn_readfirstlane(qb);
     const int first = p.rows.at(b), n = p.rows.rows(b);
-    const int qb = (n + kB - 1) / kB - 1 - u; // a sequence's longest blocks first
+    if (p.rows.B > 64) qb = (n + kB - 1) / kB - 1 - qb; // a sequence's longest first
     const int q0 = qb * kB;
 
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void *)smem;
