@@ -695,14 +695,15 @@ __global__ __launch_bounds__(kThreads, 2) void pg_fwd_kernel(PagedParams p) {
 
 // The partial states of a divided unit joined: with M = max_c m_c, w_c = 2^(m_c - M), o = (sum w_c O_c) / (sum w_c l_c).  A
 // workgroup goes by the units, or, where there may be more of them than runs, by the place where run r begins, and joins the
-// unit there if it is the unit's first division; a thread has four dims of one pair, or W waves share the parts of theirs.
-template <int W, bool UNITS>
+// unit there if it is the unit's first division; a thread has four dims of a pair, for K pairs, or W waves share the parts of
+// theirs.
+template <int W, int K, bool UNITS>
 __global__ __launch_bounds__(256) void pg_merge_kernel(PagedParams p) {
     __shared__ float4 accs[W > 1 ? 4 : 1][64];
     __shared__ float2 mls[W > 1 ? 4 : 1][64];
-    const int np = kGroup * p.nb, blocks = np * W / 4; // workgroups that share a unit's 64 x np fours
+    const int np = kGroup * p.nb, blocks = np * W / (4 * K); // workgroups that share a unit's 64 x np fours
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int x = (blockIdx.x % blocks * 4 + wave) / W * 64 + lane;
+    const int x0 = (blockIdx.x % blocks * 4 + wave) / W * (64 * K) + lane;
     const int hk = blockIdx.x / blocks % p.c.HK, y = blockIdx.x / blocks / p.c.HK;
     Walk all(p);
     int b, qb, from;
@@ -720,57 +721,68 @@ __global__ __launch_bounds__(256) void pg_merge_kernel(PagedParams p) {
     const int n = p.rows.rows(b), tiles = Walk::tiles(p, n, p.c.len(b), qb);
     const int parts = (start + tiles - 1) / all.per - g0 + 1;
     if (parts < 2) return; // its worker wrote it
-    const int pair = x % np, four = x / np;
     auto part = [&](int c) { // (a unit that begins within a run has the run's second place)
         return (2 * (long long)(g0 + c) + ((g0 + c) * all.per < from)) * p.c.HK + hk;
     };
-    float mx = -__builtin_inff(), l = 0.0f;
-    float4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    float mx[K], l[K];
+    float4 acc[K];
     // no part has a key that counts: weights 1 on zeros (a sum that is NaN or -1 stays so)
     auto weight = [](float m, float top) { return top == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - top); };
-    auto add = [&](float w, float2 ml, float4 o) {
-        l += w * ml.y;
-        acc.x += w * o.x;
-        acc.y += w * o.y;
-        acc.z += w * o.z;
-        acc.w += w * o.w;
+    auto add = [&](int k, float w, float2 ml, float4 o) {
+        l[k] += w * ml.y;
+        acc[k].x += w * o.x;
+        acc[k].y += w * o.y;
+        acc[k].z += w * o.z;
+        acc[k].w += w * o.w;
     };
-    constexpr int kBatch = 8; // parts whose loads are in flight together
+#pragma unroll
+    for (int k = 0; k < K; ++k) mx[k] = -__builtin_inff(), l[k] = 0.0f, acc[k] = float4{0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int kBatch = W > 1 ? 8 : K > 1 ? 2 : 4; // parts whose loads are in flight together
     for (int c0 = wave % W; c0 < parts; c0 += W * kBatch) {
-        float2 ml[kBatch];
-        float4 o[kBatch];
+        float2 ml[K][kBatch];
+        float4 o[K][kBatch];
 #pragma unroll
         for (int y = 0; y < kBatch; ++y) {
             const int c = c0 + y * W;
-            const long long k = part(c < parts ? c : c0);
-            ml[y] = p.part_ml[k * np + pair];
-            o[y] = p.part_o[(k * 64 + four) * np + pair];
-            if (c >= parts) ml[y] = float2{-__builtin_inff(), 0.0f}, o[y] = float4{0.0f, 0.0f, 0.0f, 0.0f};
+            const long long at = part(c < parts ? c : c0);
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const int x = x0 + k * 64;
+                ml[k][y] = p.part_ml[at * np + x % np];
+                o[k][y] = p.part_o[at * 64 * np + x];
+                if (c >= parts) ml[k][y] = float2{-__builtin_inff(), 0.0f}, o[k][y] = float4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
         }
-        float top = mx;
 #pragma unroll
-        for (int y = 0; y < kBatch; ++y) top = __builtin_fmaxf(top, ml[y].x);
-        const float w = weight(mx, top);
-        l *= w, acc.x *= w, acc.y *= w, acc.z *= w, acc.w *= w;
-        mx = top;
+        for (int k = 0; k < K; ++k) {
+            float top = mx[k];
 #pragma unroll
-        for (int y = 0; y < kBatch; ++y) add(weight(ml[y].x, mx), ml[y], o[y]);
+            for (int y = 0; y < kBatch; ++y) top = __builtin_fmaxf(top, ml[k][y].x);
+            const float w = weight(mx[k], top);
+            l[k] *= w, acc[k].x *= w, acc[k].y *= w, acc[k].z *= w, acc[k].w *= w;
+            mx[k] = top;
+#pragma unroll
+            for (int y = 0; y < kBatch; ++y) add(k, weight(ml[k][y].x, mx[k]), ml[k][y], o[k][y]);
+        }
     }
     if constexpr (W > 1) {
-        accs[wave][lane] = acc, mls[wave][lane] = float2{mx, l};
+        accs[wave][lane] = acc[0], mls[wave][lane] = float2{mx[0], l[0]};
         __syncthreads();
         if (wave > 0) return;
 #pragma unroll
-        for (int w = 1; w < W; ++w) mx = __builtin_fmaxf(mx, mls[w][lane].x);
-        l = 0.0f, acc = float4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int w = 1; w < W; ++w) mx[0] = __builtin_fmaxf(mx[0], mls[w][lane].x);
+        l[0] = 0.0f, acc[0] = float4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int w = 0; w < W; ++w) add(weight(mls[w][lane].x, mx), mls[w][lane], accs[w][lane]);
+        for (int w = 0; w < W; ++w) add(0, weight(mls[w][lane].x, mx[0]), mls[w][lane], accs[w][lane]);
     }
-    const int t = qb * p.nb + (pair >> 2);
-    if (t >= n) return;
-    const float inv = l < 0.0f ? 0.0f : 1.0f / l; // (a row that sees no key: the parts' -1)
-    const u32x2 w = {pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv)};
-    *(u32x2 *)(p.o + (hk * kGroup + (pair & 3)) * p.sho + (long long)(p.rows.at(b) + t) * p.ldo + four * 4) = w;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int x = x0 + k * 64, pair = x % np, four = x / np, t = qb * p.nb + (pair >> 2);
+        if (t >= n) continue;
+        const float inv = l[k] < 0.0f ? 0.0f : 1.0f / l[k]; // (a row that sees no key: the parts' -1)
+        const u32x2 w = {pack_bf16x2(acc[k].x * inv, acc[k].y * inv), pack_bf16x2(acc[k].z * inv, acc[k].w * inv)};
+        *(u32x2 *)(p.o + (hk * kGroup + (pair & 3)) * p.sho + (long long)(p.rows.at(b) + t) * p.ldo + four * 4) = w;
+    }
 }
 
 // ---- host side ----
@@ -843,10 +855,12 @@ extern "C" int mica_attention_paged(const void *q, long long shq, long long ldq,
     if (pl.states == 0) return 0;
     const bool units = pl.units < pl.runs;
     const unsigned joins = (unsigned)((units ? pl.units : pl.runs - 1) * HK * pl.nb);
-    if (units && pl.runs >= 8 * pl.units) // many parts a unit: four waves share them
-        hipLaunchKernelGGL((pg_merge_kernel<4, true>), dim3(joins * 4), dim3(256), 0, st, p);
-    else if (units) hipLaunchKernelGGL((pg_merge_kernel<1, true>), dim3(joins), dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((pg_merge_kernel<1, false>), dim3(joins), dim3(256), 0, st, p);
+    if (units && pl.nb <= 8 && pl.runs >= 8 * pl.units) // many parts a unit: four waves share them
+        hipLaunchKernelGGL((pg_merge_kernel<4, 1, true>), dim3(joins * 4), dim3(256), 0, st, p);
+    else if (units && pl.nb < 4) hipLaunchKernelGGL((pg_merge_kernel<1, 1, true>), dim3(joins), dim3(256), 0, st, p);
+    else if (units) hipLaunchKernelGGL((pg_merge_kernel<1, 4, true>), dim3(joins / 4), dim3(256), 0, st, p);
+    else if (pl.nb < 4) hipLaunchKernelGGL((pg_merge_kernel<1, 1, false>), dim3(joins), dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((pg_merge_kernel<1, 4, false>), dim3(joins / 4), dim3(256), 0, st, p);
     return mica_err(hipGetLastError());
 }
 
