@@ -6,7 +6,8 @@
 // Work split: a workgroup takes one key/value head and a block of 32 rows of one sequence; wave w takes query head 4 hk + w, so
 // that every tile of 32 keys brought into LDS serves four heads.  It computes S^T = K Q^T (32 keys x 32 rows,
 // v_mfma_f32_32x32x16_bf16), the online softmax of its rows (a lane holds 16 of a row's 32 scores, lane l ^ 32 the others) and
-// O^T += V^T P^T.  Blocks are found on the device from the sequences' starts, so that nothing is padded.
+// O^T += V^T P^T.  Blocks are found on the device from the sequences' starts, so that nothing is padded.  Where a few long
+// prompts do not fill the chip, a block's keys are divided over workgroups, whose partial states (fp32) pk_merge_kernel joins.
 //
 // Data movement: K and V tiles come by LDS DMA into two stages in turn, 16-byte chunks XOR-swizzled by row, rows past the
 // sequence's end as zeros (the buffer's range check); V is kept as it lies in memory and its V^T fragments are transposing
@@ -20,6 +21,7 @@ constexpr int kD = 256;             // head dim
 constexpr int kGroup = 4;           // query heads per key/value head, a wave each
 constexpr int kB = 32;              // rows of a block, keys of a tile
 constexpr int kThreads = 64 * kGroup;
+constexpr int kRows = kGroup * kB;  // (head, row) pairs of a block
 constexpr int kTile = kB * kD * 2;  // 16 KB of K or V
 constexpr int kStage = 2 * kTile;
 
@@ -31,6 +33,10 @@ struct PackedParams {
     Ragged rows;
     int HK, fill;                          // fill: rows of no sequence become zeros
     float scale_log2;                      // softmax scale x log2(e)
+    int chunk, chunks;                     // a block's tiles are divided into chunks of about `chunk`, at most `chunks` of them
+    float4 *part_o;                        // partial O: [block][chunk][HK][64 fours of dims][128 rows x heads]
+    float2 *part_ml;                       // partial (m, l): [block][chunk][HK][128]
+    MICA_DEVICE int parts(int tiles) const { return min((tiles + chunk - 1) / chunk, chunks); }
 };
 
 // zeros for rows i0 .. i0 + 31 of those that no sequence has (the rows before the first and behind the last sequence)
@@ -77,6 +83,22 @@ MICA_DEVICE bool longest_first(const Ragged &rows, int id, int &b, int &qb) {
     return true;
 }
 
+// The id-th block: its sequence and its place in it; false where there are fewer (b is then their number)
+MICA_DEVICE bool find_block(const Ragged &rows, int id, int &b, int &qb) {
+    bool any;
+    if (rows.B == 1) { // (no search for one prompt)
+        const int nb = (rows.rows(0) + kB - 1) / kB;
+        any = id < nb, b = any ? 0 : nb, qb = nb - 1 - id;
+    } else if (rows.B <= 64) {
+        any = longest_first(rows, id, b, qb);
+    } else {
+        any = find_unit(rows.B, [&](int i) { return (rows.rows(i) + kB - 1) / kB; }, id, b, qb);
+        if (any) qb = (rows.rows(b) + kB - 1) / kB - 1 - qb; // a sequence's longest first
+    }
+    b = __builtin_amdgcn_readfirstlane(b), qb = __builtin_amdgcn_readfirstlane(qb);
+    return any;
+}
+
 __global__ __launch_bounds__(kThreads, 2) void pk_fwd_kernel(PackedParams p) {
     constexpr int kSmem = kGroup * kB * kD * 2 > 2 * kStage ? kGroup * kB * kD * 2 : 2 * kStage; // the stages; the output, in the end
     __shared__ __attribute__((aligned(1024))) int8_t smem[kSmem + 16];
@@ -84,25 +106,23 @@ __global__ __launch_bounds__(kThreads, 2) void pk_fwd_kernel(PackedParams p) {
 
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, hi = lane >> 5;
-    const int hk = blockIdx.x % p.HK, id = blockIdx.x / p.HK;
+    const int hk = blockIdx.x % p.HK, chunk = blockIdx.x / p.HK % p.chunks, id = blockIdx.x / p.HK / p.chunks;
     int b, qb;
-    const bool any = p.rows.B <= 64 ? longest_first(p.rows, id, b, qb)
-                                    : find_unit(p.rows.B, [&](int i) { return (p.rows.rows(i) + kB - 1) / kB; }, id, b, qb);
-    if (!any) {
-        if (p.fill) fill_rows(p, hk, (id - b) * kB);
+    if (!find_block(p.rows, id, b, qb)) {
+        if (p.fill && chunk == 0) fill_rows(p, hk, (id - b) * kB);
         return;
     }
-    b = __builtin_amdgcn_readfirstlane(b), qb = __builtin_amdgcn_readfirstlane(qb);
-    const int first = p.rows.at(b), n = p.rows.rows(b);
-    if (p.rows.B > 64) qb = (n + kB - 1) / kB - 1 - qb; // a sequence's longest first
-    const int q0 = qb * kB;
+    const int first = p.rows.at(b), n = p.rows.rows(b), q0 = qb * kB;
+    const int parts = p.parts(qb + 1); // this workgroup's tiles, i0 .. i1 - 1 of the block's
+    if (chunk >= parts) return;
+    const int i0 = (int)((long long)(qb + 1) * chunk / parts), i1 = (int)((long long)(qb + 1) * (chunk + 1) / parts);
 
     const uint32_t lds0 = (uint32_t)(uintptr_t)(lds_void *)smem;
     const uint16_t *const kb = p.k + hk * p.shk + (long long)first * p.ldk;
     const uint16_t *const vb = p.v + hk * p.shv + (long long)first * p.ldv;
-    // DMA of tile i into stage st; past the block's last from a zero-sized buffer
+    // DMA of tile i into stage st; past the last from a zero-sized buffer
     auto issue = [&](int i, int st) {
-        const int rows = i <= qb ? min(n - i * kB, kB) : 0;
+        const int rows = i < i1 ? min(n - i * kB, kB) : 0;
         const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
             (void *)(kb + (long long)i * kB * p.ldk), 0, rows > 0 ? (int)((rows - 1) * p.ldk * 2) + kD * 2 : 0, kBufferFlags);
         const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
@@ -131,7 +151,7 @@ __global__ __launch_bounds__(kThreads, 2) void pk_fwd_kernel(PackedParams p) {
         for (int s = 0; s < kD / 16; ++s) qf[s] = __builtin_bit_cast(bf16x8, *(const u32x4 *)(qr + s * 16));
     }
     __builtin_amdgcn_sched_barrier(0);
-    issue(0, 0);
+    issue(i0, 0);
     if (tid == 0) *odd_tile = 0;
     wait_lgkmcnt0(); // seen by every wave after the first tile's barrier
     f32x16 O[kD / 32];
@@ -159,8 +179,8 @@ __global__ __launch_bounds__(kThreads, 2) void pk_fwd_kernel(PackedParams p) {
     };
     constexpr int kPf = 3; // operand fragments read ahead
 #pragma unroll 1
-    for (int i = 0; i <= qb; ++i) {
-        const int st = i & 1;
+    for (int i = i0; i < i1; ++i) {
+        const int st = (i - i0) & 1;
         // this wave's DMA of tile i landed; after the barrier every wave's has, and nobody reads tile i - 1 any more
         wait_vmcnt<0>();
         meet();
@@ -270,8 +290,21 @@ __global__ __launch_bounds__(kThreads, 2) void pk_fwd_kernel(PackedParams p) {
         __builtin_amdgcn_s_setprio(0);
     }
     wait_vmcnt<0>(); // the last (empty) loads have written before the stages are used again
+    const float ltot = half_swap_sum(lsum);
+    if (parts > 1) { // the state, left for pk_merge_kernel
+        const long long part = ((long long)id * p.chunks + chunk) * p.HK + hk;
+        const int row = wave * kB + l32;
+#pragma unroll
+        for (int dt = 0; dt < kD / 32; ++dt)
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4)
+                p.part_o[(part * 64 + (dt * 4 + r4) * 2 + hi) * kRows + row] =
+                    float4{O[dt][4 * r4], O[dt][4 * r4 + 1], O[dt][4 * r4 + 2], O[dt][4 * r4 + 3]};
+        if (hi == 0) p.part_ml[part * kRows + row] = float2{m, ltot};
+        return;
+    }
     // ---- normalise (a row whose scores are all -inf has no softmax: 0 / 0), stage in LDS, write 16-byte row pieces ----
-    const float inv = 1.0f / half_swap_sum(lsum);
+    const float inv = 1.0f / ltot;
     __syncthreads();
 #pragma unroll
     for (int dt = 0; dt < kD / 32; ++dt)
@@ -293,6 +326,96 @@ __global__ __launch_bounds__(kThreads, 2) void pk_fwd_kernel(PackedParams p) {
     }
 }
 
+// The partial states of a divided block joined: with M = max_c m_c, w_c = 2^(m_c - M), o = (sum w_c O_c) / (sum w_c l_c); a
+// thread has four dims of a row, for four rows.
+__global__ __launch_bounds__(256) void pk_merge_kernel(PackedParams p) {
+    constexpr int K = 4, kBlocks = 64 * kRows / (256 * K); // workgroups of a block and head
+    const int x0 = (blockIdx.x % kBlocks * 4 + (threadIdx.x >> 6)) * (64 * K) + (threadIdx.x & 63);
+    const int hk = blockIdx.x / kBlocks % p.HK, id = blockIdx.x / kBlocks / p.HK;
+    int b, qb;
+    if (!find_block(p.rows, id, b, qb)) return;
+    const int parts = p.parts(qb + 1);
+    if (parts < 2) return; // its workgroup wrote it
+    const int first = p.rows.at(b), n = p.rows.rows(b);
+    float mx[K], l[K];
+    float4 acc[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) mx[k] = -__builtin_inff(), l[k] = 0.0f, acc[k] = float4{0.0f, 0.0f, 0.0f, 0.0f};
+    // no part has a score above -inf: weights 1 on zeros
+    auto weight = [](float m, float top) { return top == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - top); };
+    constexpr int kBatch = 2; // parts whose loads are in flight together
+    for (int c0 = 0; c0 < parts; c0 += kBatch) {
+        float2 ml[K][kBatch];
+        float4 o[K][kBatch];
+#pragma unroll
+        for (int y = 0; y < kBatch; ++y) {
+            const long long at = ((long long)id * p.chunks + min(c0 + y, parts - 1)) * p.HK + hk;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const int x = x0 + k * 64;
+                ml[k][y] = p.part_ml[at * kRows + x % kRows];
+                o[k][y] = p.part_o[at * 64 * kRows + x];
+                if (c0 + y >= parts) ml[k][y] = float2{-__builtin_inff(), 0.0f}, o[k][y] = float4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            float top = mx[k];
+#pragma unroll
+            for (int y = 0; y < kBatch; ++y) top = __builtin_fmaxf(top, ml[k][y].x);
+            const float w = weight(mx[k], top);
+            l[k] *= w, acc[k].x *= w, acc[k].y *= w, acc[k].z *= w, acc[k].w *= w;
+            mx[k] = top;
+#pragma unroll
+            for (int y = 0; y < kBatch; ++y) {
+                const float v = weight(ml[k][y].x, top);
+                l[k] += v * ml[k][y].y;
+                acc[k].x += v * o[k][y].x;
+                acc[k].y += v * o[k][y].y;
+                acc[k].z += v * o[k][y].z;
+                acc[k].w += v * o[k][y].w;
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        const int x = x0 + k * 64, row = x % kRows, four = x / kRows, t = qb * kB + row % kB;
+        if (t >= n) continue;
+        const float inv = 1.0f / l[k];
+        const u32x2 w = {pack_bf16x2(acc[k].x * inv, acc[k].y * inv), pack_bf16x2(acc[k].z * inv, acc[k].w * inv)};
+        *(u32x2 *)(p.o + (long long)(hk * kGroup + row / kB) * p.sho + (long long)(first + t) * p.ldo + four * 4) = w;
+    }
+}
+
+// ---- host side ----
+
+constexpr int kCus = 256; // CUs of the chip
+
+struct Plan {
+    int chunk, chunks;
+    long long units, states; // blocks (of all sequences and of the rows of none), partial rows
+};
+
+Plan plan(long long B, long long T, long long HK, int longest) {
+    Plan pl{};
+    // blocks: at most (n + 31) / 32 and n of each sequence, and of the rows of none
+    const long long most = (T + 31 * B + 31) / 32;
+    pl.units = most < T ? most : T;
+    pl.chunk = 1 << 30, pl.chunks = 1;
+    const long long hint = longest > 0 && longest < T ? longest : T, nb = (hint + kB - 1) / kB;
+    // Too few blocks to fill the chip, and long ones: each is divided into up to three chunks, so that the longest does not
+    // run alone in the end.  Undivided / divided, us: 1 x 600 26.7 / 25.6, 1 x 1000 40.4 / 33.8, 1 x 1500 56.3 / 45.8, 1 x 2048
+    // 73.8 / 61.1, but 2 x 1000 42.2 / 46.9, 1 x 3000 112 / 117 (64 KB of state a wave, written and read).  Chunks of 16 / 24 / 32
+    // tiles: 1 x 1000 33.8 / 39.9 / 40.3, 1 x 2048 82.0 / 61.1 / 69.8.
+    if (pl.units * HK <= kCus && nb >= 24) {
+        pl.chunk = (int)((3 * nb / 8 + 7) / 8 * 8);
+        pl.chunks = (int)((nb + pl.chunk - 1) / pl.chunk);
+        pl.states = pl.units * pl.chunks * HK * kRows;
+    }
+    return pl;
+}
+long long state_bytes(const Plan &pl) { return pl.states * (kD * 4 + 8); }
+
 }  // namespace
 
 extern "C" int mica_attention_packed(const void *q, long long shq, long long ldq, const void *k, long long shk, long long ldk,
@@ -312,9 +435,9 @@ extern "C" int mica_attention_packed(const void *q, long long shq, long long ldq
     }
     if (!mica_aligned16(q) || !mica_aligned16(k) || !mica_aligned16(v) || !mica_aligned16(o) || ((uintptr_t)starts & 3))
         return MICA_MISS_ALIGN;
-    // blocks of all sequences and of the rows of none: at most (n + 31) / 32 and n of each
-    const long long most = ((long long)T + 31ll * B + 31) / 32, units = most < T ? most : T;
-    if (units * HK >= (1 << 24)) return MICA_MISS_RANGE; // (a grid of 2^32 work-items wraps round)
+    const Plan pl = plan(B, T, HK, longest);
+    if (pl.units * HK * pl.chunks >= (1 << 24)) return MICA_MISS_RANGE; // (a grid of 2^32 work-items wraps round)
+    if (pl.states && (!workspace || !mica_aligned16(workspace) || workspace_bytes < state_bytes(pl))) return MICA_MISS_ARG;
     PackedParams p{};
     p.q = (const uint16_t *)q; p.shq = shq; p.ldq = ldq;
     p.k = (const uint16_t *)k; p.shk = shk; p.ldk = ldk;
@@ -323,11 +446,18 @@ extern "C" int mica_attention_packed(const void *q, long long shq, long long ldq
     p.rows = Ragged{starts, B, T};
     p.HK = HK; p.fill = fill;
     p.scale_log2 = scale * 1.44269504088896341f;
-    hipLaunchKernelGGL(pk_fwd_kernel, dim3((unsigned)(units * HK)), dim3(kThreads), 0, (hipStream_t)stream, p);
+    p.chunk = pl.chunk, p.chunks = pl.chunks;
+    p.part_o = (float4 *)workspace;
+    p.part_ml = (float2 *)((char *)workspace + pl.states * kD * 4);
+    hipStream_t st = (hipStream_t)stream;
+    hipLaunchKernelGGL(pk_fwd_kernel, dim3((unsigned)(pl.units * HK * pl.chunks)), dim3(kThreads), 0, st, p);
+    if (const int rc = mica_err(hipGetLastError())) return rc;
+    if (pl.states == 0) return 0;
+    hipLaunchKernelGGL(pk_merge_kernel, dim3((unsigned)(pl.units * HK * (64 * kRows / 1024))), dim3(256), 0, st, p);
     return mica_err(hipGetLastError());
 }
 
 extern "C" long long mica_attention_packed_workspace_bytes(int B, int T, int HK, int longest) {
-    if (B < 0 || T < 0 || HK <= 0) return -1;
-    return 0;
+    if (B < 0 || T < 0 || HK <= 0 || HK > (1 << 20)) return -1;
+    return state_bytes(plan(B, T, HK, longest));
 }
