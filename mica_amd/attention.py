@@ -369,7 +369,9 @@ def _out(out, q):
     so = _rows(out, "out", q.device)
     if out.shape != q.shape:
         raise ValueError("out must have q's shape")
-    if any(n > 1 and st < HEAD_DIM for n, st in zip(out.shape[1::-1], so)):
+    (T, HQ), (sh, ld) = out.shape[:2], so
+    if (T > 1 and ld < HEAD_DIM) or (HQ > 1 and sh < HEAD_DIM) or (
+            T > 1 and HQ > 1 and ld < (HQ - 1) * sh + HEAD_DIM and sh < (T - 1) * ld + HEAD_DIM):
         raise ValueError("out's rows and heads must not overlap")
     return out, so, 0
 

@@ -695,7 +695,10 @@ struct Out {
     bool of(const Call &c, const Tensor &q, const Tensor *out) {
         if (out) {
             Rows r;
-            if (!r.of(c, *out) || out->sizes() != q.sizes() || (out->size(0) > 1 && r.ld < 256) || (out->size(1) > 1 && r.sh < 256))
+            if (!r.of(c, *out) || out->sizes() != q.sizes()) return false;
+            const int64_t T = out->size(0), HQ = out->size(1);
+            if ((T > 1 && r.ld < 256) || (HQ > 1 && r.sh < 256) ||
+                (T > 1 && HQ > 1 && r.ld < (HQ - 1) * r.sh + 256 && r.sh < (T - 1) * r.ld + 256))
                 return false;
             p = out->data_ptr(), sh = r.sh, ld = r.ld;
             return true;

@@ -189,8 +189,7 @@ struct Softmax {
     // Scores sc of a tile (score r of a lane is key k0 + 8 (r / 4) + 4 hi + r % 4) become weights, unscaled ones in the sum and
     // sv times them in sc; `masked`: keys past pos get none.  The reference moves only when the maximum exceeds it by more than
     // 8, and then O with it.
-    template <int NDT>
-    MICA_DEVICE void add(f32x16 &sc, f32x16 (&O)[NDT], float scale, float sv, bool masked, int k0, int pos, int hi) {
+    MICA_DEVICE void add(f32x16 &sc, f32x16 (&O)[kD / 32], float scale, float sv, bool masked, int k0, int pos, int hi) {
         if (masked) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) sc[r] = k0 + 8 * (r >> 2) + 4 * hi + (r & 3) <= pos ? sc[r] : -__builtin_inff();
@@ -204,7 +203,7 @@ struct Softmax {
         if (grow) m = mx;
         if (__builtin_amdgcn_ballot_w64(grow)) {
 #pragma unroll
-            for (int dt = 0; dt < NDT; ++dt) O[dt] *= alpha;
+            for (int dt = 0; dt < kD / 32; ++dt) O[dt] *= alpha;
             lsum *= alpha;
         }
         const float ref = m == -__builtin_inff() ? 0.0f : m; // a row that has seen nothing yet: exp2(-inf - 0) = 0
@@ -251,20 +250,19 @@ MICA_DEVICE uint32_t without_odd(uint32_t w) {
 MICA_DEVICE uint32_t odd_bits(uint32_t w) { return (w & 0x7f807f80u) + 0x00800080u; }
 
 // A worker's state of its unit, left for pg_merge_kernel: (m, l) with l = -1 for a row that sees no key
-template <int NDT>
-MICA_DEVICE void leave(const PagedParams &p, long long part, int pair, int dt0, int hi, bool blind, const f32x16 (&O)[NDT],
-                       float m, float l) {
+MICA_DEVICE void leave(const PagedParams &p, long long part, int pair, int hi, bool blind, const f32x16 (&O)[kD / 32], float m,
+                       float l) {
     const int np = kGroup * p.nb;
     if (pair >= np) return;
 #pragma unroll
-    for (int dt = 0; dt < NDT; ++dt)
+    for (int dt = 0; dt < kD / 32; ++dt)
 #pragma unroll
         for (int r4 = 0; r4 < 4; ++r4) {
             const f32x16 x = O[dt];
-            p.part_o[(part * 64 + ((dt0 + dt) * 4 + r4) * 2 + hi) * np + pair] =
+            p.part_o[(part * 64 + (dt * 4 + r4) * 2 + hi) * np + pair] =
                 blind ? float4{0.0f, 0.0f, 0.0f, 0.0f} : float4{x[4 * r4], x[4 * r4 + 1], x[4 * r4 + 2], x[4 * r4 + 3]};
         }
-    if (dt0 == 0 && hi == 0) p.part_ml[part * np + pair] = blind ? float2{-__builtin_inff(), -1.0f} : float2{m, l};
+    if (hi == 0) p.part_ml[part * np + pair] = blind ? float2{-__builtin_inff(), -1.0f} : float2{m, l};
 }
 
 // ---- few rows: up to 8 G of a sequence ----
@@ -341,9 +339,11 @@ __global__ __launch_bounds__(256, 1) void pg_few_kernel(PagedParams p) {
                 }
                 sm.add(sc, O, p.scale_log2 * sk, sv, (i + 1) * kBK - 1 > from + q0, i * kBK, pos, hi);
                 const bf16x8 h0 = weights(sc, 0), h1 = weights(sc, 1);
-                f32x16 lo;
+                f32x16 lo = {}; // what h0 and h1 leave
+                if constexpr (G == 1) {
 #pragma unroll
-                for (int r = 0; r < 16; ++r) lo[r] = sc[r] - round_bf16(sc[r]);
+                    for (int r = 0; r < 16; ++r) lo[r] = sc[r] - round_bf16(sc[r]);
+                }
                 const bf16x8 g0 = weights(lo, 0), g1 = weights(lo, 1);
 #pragma unroll
                 for (int x = 0; x < 8; ++x) {
@@ -420,7 +420,7 @@ __global__ __launch_bounds__(256, 1) void pg_few_kernel(PagedParams p) {
         }
         const float l = half_swap_sum(sm.lsum);
         if (!w.whole()) {
-            leave(p, (long long)w.part * p.c.HK + hk, pair, 0, hi, pos < 0, O, sm.m, l);
+            leave(p, (long long)w.part * p.c.HK + hk, pair, hi, pos < 0, O, sm.m, l);
         } else if (t < w.n && (pair >> 2) < p.nb) {
             // (a row whose scores are all -inf has no softmax: 0 / 0; one that sees no key: zeros)
             const float inv = 1.0f / l;
@@ -441,28 +441,24 @@ __global__ __launch_bounds__(256, 1) void pg_few_kernel(PagedParams p) {
 // ---- more rows ----
 // A workgroup of 8 waves shares each page, one workgroup a CU.  A page's 16 pieces come by LDS DMA, two of them by each wave,
 // three tiles ahead into a ring; when its two have landed a wave widens them to bf16, once for all waves, into one of two
-// stages, from which every operand is one contiguous 16-byte read a lane.  A wave holds 32 (row, head) pairs (R row blocks): it
-// computes S^T = K Q^T (32 keys x 32 pairs, v_mfma_f32_32x32x16_bf16), the online softmax of its pairs (a lane holds 16 of a
-// pair's 32 scores, lane l ^ 32 the others) and 256 / D dims of O^T += V^T P^T; with few rows D = 8 / R waves repeat a row
-// block's scores and divide its dims.
+// stages, from which every operand is one contiguous 16-byte read a lane.  A wave holds 32 (row, head) pairs, 64 rows a
+// workgroup: it computes S^T = K Q^T (32 keys x 32 pairs, v_mfma_f32_32x32x16_bf16), the online softmax of its pairs (a lane holds
+// 16 of a pair's 32 scores, lane l ^ 32 the others) and O^T += V^T P^T.
 constexpr int kWaves = 8, kThreads = 64 * kWaves;
 constexpr int kOwn = 16 / kWaves;       // pieces of a page a wave brings
 constexpr int kRing = 4;                // pages in the ring: one being widened, three on their way
 constexpr int kRaw = 2 * kPageBytes;
 
-template <int R>
 __global__ __launch_bounds__(kThreads, 2) void pg_fwd_kernel(PagedParams p) {
-    constexpr int D = kWaves / R;           // waves of a row block
-    constexpr int NDT = kD / 32 / D;        // 32-dim tiles of O a wave holds
+    constexpr int NDT = kD / 32;            // 32-dim tiles of O
     constexpr int kSmem = 2 * kStage + kRing * kRaw; // the stages and the ring; the output, in the end
-    static_assert(kSmem >= R * 32 * kD * 2, "the output is staged in their place");
+    static_assert(kSmem >= kWaves * 32 * kD * 2, "the output is staged in their place");
     // (one array: with several the compiler lets every operand read wait for all DMA in flight)
     __shared__ __attribute__((aligned(1024))) int8_t smem[kSmem + kWaves * 64 * 16 + 16];
     int *const index = (int *)(smem + kSmem) + (threadIdx.x >> 6) * 256; // this wave's: page and scales of 64 tiles, i at i % 64
     int *const odd_rest = (int *)(smem + kSmem + kWaves * 64 * 16);      // whether the rest holds a value that is not finite
 
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const int rb = wave / D, dt0 = (wave % D) * NDT;
     const int hk = blockIdx.x % p.c.HK, run = blockIdx.x / p.c.HK;
     if (p.fill) {
         const int none = p.rows.at(0) + p.rows.T - p.rows.at(p.rows.B);
@@ -506,7 +502,7 @@ __global__ __launch_bounds__(kThreads, 2) void pg_fwd_kernel(PagedParams p) {
         };
         // Q fragments (B operand of S^T): step 2 c + e takes dims 32 c + 16 hi + 8 e .. + 7, as a page's bytes lie; rows past the
         // last repeat it
-        const int t = q0 + rb * 8 + (l32 >> 2), pos = from + t; // this lane's pair: row t, head l % 4
+        const int t = q0 + wave * 8 + (l32 >> 2), pos = from + t; // this lane's pair: row t, head l % 4
         bf16x8 qf[kD / 16];
         {
             const uint16_t *qr = p.q + (hk * kGroup + (l32 & 3)) * p.shq + (long long)(w.first + min(t, w.n - 1)) * p.ldq + hi * 16;
@@ -557,9 +553,7 @@ __global__ __launch_bounds__(kThreads, 2) void pg_fwd_kernel(PagedParams p) {
         lds_void *none = (lds_void *)smem;
         __asm__ volatile("" : "+s"(none));
         auto kfrag = [none](uint32_t a, int s) { return __builtin_bit_cast(bf16x8, lds_read(a + s * 1024, none)); };
-        auto vfrag = [none](uint32_t a, int s, int dt) { // a: of the wave's first dims
-            return __builtin_bit_cast(bf16x8, lds_read(a + dt * 2048 + s * 1024, none));
-        };
+        auto vfrag = [none](uint32_t a, int s, int dt) { return __builtin_bit_cast(bf16x8, lds_read(a + dt * 2048 + s * 1024, none)); };
         f32x16 O[NDT];
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) O[dt] = f32x16{};
@@ -639,33 +633,32 @@ __global__ __launch_bounds__(kThreads, 2) void pg_fwd_kernel(PagedParams p) {
             }
             // ---- O^T += V^T P^T ----
             auto product = [&](uint32_t v) { // values at v
-                constexpr int kPv = kPf < 2 * NDT ? kPf : 2 * NDT;
                 __builtin_amdgcn_s_setprio(1);
-                bf16x8 vf[kPv];
+                bf16x8 vf[kPf];
 #pragma unroll
-                for (int x = 0; x < kPv; ++x) vf[x] = vfrag(v, x / NDT, x % NDT);
+                for (int x = 0; x < kPf; ++x) vf[x] = vfrag(v, x / NDT, x % NDT);
 #pragma unroll
                 for (int x = 0; x < 2 * NDT; ++x) {
-                    const bf16x8 a = vf[x % kPv];
-                    if (x + kPv < 2 * NDT) vf[x % kPv] = vfrag(v, (x + kPv) / NDT, (x + kPv) % NDT);
+                    const bf16x8 a = vf[x % kPf];
+                    if (x + kPf < 2 * NDT) vf[x % kPf] = vfrag(v, (x + kPf) / NDT, (x + kPf) % NDT);
                     __builtin_amdgcn_sched_barrier(0);
                     O[x % NDT] = mfma_bf16(a, pb[x / NDT], O[x % NDT]);
                 }
                 __builtin_amdgcn_s_setprio(0);
             };
-            product(at + kTile + dt0 * 2048);
+            product(at + kTile);
             if (odd) {
                 pb[0] = indicators(pb[0]), pb[1] = indicators(pb[1]);
 #pragma unroll 1
-                for (int x = 0; x < 2; ++x) product(base + 2 * kStage + x * kTile + dt0 * 2048);
+                for (int x = 0; x < 2; ++x) product(base + 2 * kStage + x * kTile);
             }
         }
         wait_vmcnt<0>(); // the last (empty) loads have written before the ring is used again or given up
         const float l = half_swap_sum(sm.lsum);
         __asm__ volatile("" : "+v"(tid));
-        const int ln = tid & 63, row = rb * 32 + (ln & 31), half = ln >> 5;
+        const int ln = tid & 63, row = wave * 32 + (ln & 31), half = ln >> 5;
         if (!w.whole()) {
-            leave(p, (long long)w.part * p.c.HK + hk, row, dt0, half, pos < 0, O, sm.m, l);
+            leave(p, (long long)w.part * p.c.HK + hk, row, half, pos < 0, O, sm.m, l);
         } else {
             // ---- normalise (a row whose scores are all -inf has no softmax: 0 / 0; one that sees no key: zeros), stage, write ----
             const float inv = 1.0f / l;
@@ -674,7 +667,7 @@ __global__ __launch_bounds__(kThreads, 2) void pg_fwd_kernel(PagedParams p) {
             for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
                 for (int r4 = 0; r4 < 4; ++r4) {
-                    const int d = (dt0 + dt) * 32 + 8 * r4 + 4 * half;
+                    const int d = dt * 32 + 8 * r4 + 4 * half;
                     const f32x16 x = O[dt];
                     u32x2 v = {pack_bf16x2(x[4 * r4] * inv, x[4 * r4 + 1] * inv), pack_bf16x2(x[4 * r4 + 2] * inv, x[4 * r4 + 3] * inv)};
                     if (pos < 0) v = u32x2{0u, 0u};
@@ -682,7 +675,7 @@ __global__ __launch_bounds__(kThreads, 2) void pg_fwd_kernel(PagedParams p) {
                 }
             __syncthreads();
 #pragma unroll 2
-            for (int x = tid; x < 32 * R * 32; x += kThreads) {
+            for (int x = tid; x < 32 * kWaves * 32; x += kThreads) {
                 const int rr = x >> 5, ch = x & 31, tt = q0 + (rr >> 2);
                 if (tt < w.n)
                     *(u32x4 *)(p.o + (long long)(hk * kGroup + (rr & 3)) * p.sho + (long long)(w.first + tt) * p.ldo + ch * 8) =
@@ -722,7 +715,8 @@ __global__ __launch_bounds__(256) void pg_merge_kernel(PagedParams p) {
     const int parts = (start + tiles - 1) / all.per - g0 + 1;
     if (parts < 2) return; // its worker wrote it
     auto part = [&](int c) { // (a unit that begins within a run has the run's second place)
-        return (2 * (long long)(g0 + c) + ((g0 + c) * all.per < from)) * p.c.HK + hk;
+        const int g = min(max(g0 + c, 0), p.runs - 1); // (starts that are no running sum may wrap places round)
+        return (2 * (long long)g + (g * all.per < from)) * p.c.HK + hk;
     };
     float mx[K], l[K];
     float4 acc[K];
@@ -809,7 +803,7 @@ Plan plan(long long B, long long T, int HK, int width, int longest) {
     long long runs = slots / HK > 0 ? slots / HK : 1;
     const long long useful = pl.tiles / (pl.least + pl.begin) + 1; // (no more than can have tiles)
     pl.runs = (int)(runs < useful ? runs : useful);
-    pl.states = pl.runs > 1 ? 2ll * pl.runs * HK : 0;
+    pl.states = B > 0 && pl.runs > 1 ? 2ll * pl.runs * HK : 0;
     return pl;
 }
 long long state_bytes(const Plan &pl) { return pl.states * kGroup * pl.nb * (kD * 4 + 8); }
@@ -850,7 +844,7 @@ extern "C" int mica_attention_paged(const void *q, long long shq, long long ldq,
     if (pl.G == 1) hipLaunchKernelGGL(pg_few_kernel<1>, dim3(few), dim3(256), 0, st, p);
     else if (pl.G == 2) hipLaunchKernelGGL(pg_few_kernel<2>, dim3(few), dim3(256), 0, st, p);
     else if (pl.G == 4) hipLaunchKernelGGL(pg_few_kernel<4>, dim3(few), dim3(256), 0, st, p);
-    else hipLaunchKernelGGL(pg_fwd_kernel<8>, dim3((unsigned)workers), dim3(kThreads), 0, st, p);
+    else hipLaunchKernelGGL(pg_fwd_kernel, dim3((unsigned)workers), dim3(kThreads), 0, st, p);
     if (const int rc = mica_err(hipGetLastError())) return rc;
     if (pl.states == 0) return 0;
     const bool units = pl.units < pl.runs;
@@ -866,6 +860,5 @@ extern "C" int mica_attention_paged(const void *q, long long shq, long long ldq,
 
 extern "C" long long mica_attention_paged_workspace_bytes(int B, int T, int HK, int width, int longest) {
     if (B < 0 || T < 0 || HK <= 0 || HK > (1 << 16) || width < 0 || width > (1 << 24)) return -1;
-    if (B == 0 || T == 0) return 0;
     return state_bytes(plan(B, T, HK, width, longest));
 }
