@@ -363,20 +363,22 @@ __global__ __launch_bounds__(256, 1) void pg_few_kernel(PagedParams p) {
             // The rest: keys from memory as operands, values by DMA into this wave's LDS (chunk c of row r at c ^ 4 (r % 4)),
             // from where they are read transposed; zeros past the last token.
             const int slot = __builtin_amdgcn_readfirstlane(p.c.slot(w.b)), have = slot < 0 ? 0 : w.len - whole * kBK;
-            const uint16_t *kr = p.c.rest(max(slot, 0), 0, hk);
-            const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc((void *)p.c.rest(max(slot, 0), 1, hk), 0,
-                                                                                 have * kD * 2, kBufferFlags);
+            auto source = [&](int side) {
+                return __builtin_amdgcn_make_buffer_rsrc((void *)p.c.rest(max(slot, 0), side, hk), 0, have * kD * 2, kBufferFlags);
+            };
+            const __amdgpu_buffer_rsrc_t kr = source(0), vr = source(1);
+            f32x16 sc = {};
+            u32x4 kf[kD / 16];
+#pragma unroll
+            for (int s = 0; s < kD / 16; ++s)
+                kf[s] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                      kr, l32 * (kD * 2) + hi * 32, (s >> 1) * 64 + (s & 1) * 16, 0));
 #pragma unroll
             for (int x = 0; x < 16; ++x)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_void *)(mine + x * 1024), 16,
                                                          (2 * x + hi) * (kD * 2) + ((l32 ^ (((2 * x + hi) & 3) << 2)) << 4), 0, 0, 0);
-            f32x16 sc = {};
 #pragma unroll
-            for (int s = 0; s < kD / 16; ++s) {
-                u32x4 a = {0u, 0u, 0u, 0u};
-                if (l32 < have) a = *(const u32x4 *)(kr + l32 * kD + (s >> 1) * 32 + hi * 16 + (s & 1) * 8);
-                sc = mfma_bf16(__builtin_bit_cast(bf16x8, a), qf[s], sc);
-            }
+            for (int s = 0; s < kD / 16; ++s) sc = mfma_bf16(__builtin_bit_cast(bf16x8, kf[s]), qf[s], sc);
             const float one = slot < 0 ? __builtin_nanf("") : 1.0f;
             sm.add(sc, O, p.scale_log2 * one, one, true, whole * kBK, pos, hi);
             bf16x8 pb[2] = {weights(sc, 0), weights(sc, 1)};
@@ -849,7 +851,10 @@ extern "C" int mica_attention_paged(const void *q, long long shq, long long ldq,
     if (pl.states == 0) return 0;
     const bool units = pl.units < pl.runs;
     const unsigned joins = (unsigned)((units ? pl.units : pl.runs - 1) * HK * pl.nb);
-    if (units && pl.nb <= 8 && pl.runs >= 8 * pl.units) // many parts a unit: four waves share them
+    // Many parts a unit, and few workgroups with four pairs a thread: four waves share the parts.  Without / with, us: 16 rows
+    // after 30000 tokens 77 / 39, 32 after 30000 70 / 51, 64 after 30000 80 / 68, 4 x 16 after 7000 45 / 37, but 8 x 16 57 / 58,
+    // 4 x 64 63 / 73.
+    if (units && pl.runs >= 8 * pl.units && (pl.nb <= 8 || joins < 4 * kCus / 2))
         hipLaunchKernelGGL((pg_merge_kernel<4, 1, true>), dim3(joins * 4), dim3(256), 0, st, p);
     else if (units && pl.nb < 4) hipLaunchKernelGGL((pg_merge_kernel<1, 1, true>), dim3(joins), dim3(256), 0, st, p);
     else if (units) hipLaunchKernelGGL((pg_merge_kernel<1, 4, true>), dim3(joins / 4), dim3(256), 0, st, p);
