@@ -268,8 +268,16 @@ MICA_DEVICE void leave(const PagedParams &p, long long part, int pair, int hi, b
 // ---- few rows: up to 8 G of a sequence ----
 // A wave takes tiles by itself: a page's pieces go from memory straight into the registers of the matrix cores' operands, 16
 // bytes a lane, each loaded for the next tile as soon as this one's has been widened, so that a wave has a page (16 KB) in
-// flight all the time.  Nothing is shared, there is no barrier, and the matrix cores' time (of which a single row uses an
-// eighth) is hidden behind the memory's.  The weights are taken as two bf16 summands: they cost products that are free here.
+// flight all the time.  Nothing is shared and there is no barrier.  G waves take a run together, 8 rows each.
+//
+// Bound: up to 4 rows by HBM (64 single rows over up to 8192 tokens: 112 us, 4.9 TB/s, a copy's rate); then by instruction issue,
+// about 800 for a page and wave, half of them to widen it, which all G waves repeat (64 x 8 rows 134 us, 16 177, 32 299).  Pages
+// through LDS instead, by DMA of each wave: 126 us for single rows, 190 for 16.  Two waves a SIMD, queries in LDS: 16 rows 187, 32
+// 268, and twice the partial states to join (8 x 16 rows over 7000 58 -> 69).
+//
+// Rounding: with one wave a run the weights are taken as two bf16 summands (hi and what it leaves), whose products are hidden
+// behind the memory (64 x 8 rows 131 -> 134 us); with more rows they are rounded to bf16 once (two summands: 32 x 32 rows over up
+// to 4096 97 -> 108 us).
 template <int G>
 __global__ __launch_bounds__(256, 1) void pg_few_kernel(PagedParams p) {
     __shared__ __attribute__((aligned(1024))) int8_t smem[4 * kTile]; // a wave's values of the rest
@@ -444,8 +452,12 @@ __global__ __launch_bounds__(256, 1) void pg_few_kernel(PagedParams p) {
 // A workgroup of 8 waves shares each page, one workgroup a CU.  A page's 16 pieces come by LDS DMA, two of them by each wave,
 // three tiles ahead into a ring; when its two have landed a wave widens them to bf16, once for all waves, into one of two
 // stages, from which every operand is one contiguous 16-byte read a lane.  A wave holds 32 (row, head) pairs, 64 rows a
-// workgroup: it computes S^T = K Q^T (32 keys x 32 pairs, v_mfma_f32_32x32x16_bf16), the online softmax of its pairs (a lane holds
-// 16 of a pair's 32 scores, lane l ^ 32 the others) and O^T += V^T P^T.
+// workgroup: it computes S^T = K Q^T (32 keys x 32 pairs, v_mfma_f32_32x32x16_bf16), the online softmax of its pairs (a lane
+// holds 16 of a pair's 32 scores, lane l ^ 32 the others) and O^T += V^T P^T.
+//
+// Bound: the matrix cores beside widening and softmax (2048 rows over 18001 tokens 540 us and 31 for the join, 1000 TFLOP/s; the
+// library's 8192^3 product reaches 1400).  Pages widened in registers by the waves that use them, before the ring: 1234 us; the
+// next page widened beside this one's PV, for one phase less: 636 against 605.
 constexpr int kWaves = 8, kThreads = 64 * kWaves;
 constexpr int kOwn = 16 / kWaves;       // pieces of a page a wave brings
 constexpr int kRing = 4;                // pages in the ring: one being widened, three on their way
@@ -691,7 +703,9 @@ __global__ __launch_bounds__(kThreads, 2) void pg_fwd_kernel(PagedParams p) {
 // The partial states of a divided unit joined: with M = max_c m_c, w_c = 2^(m_c - M), o = (sum w_c O_c) / (sum w_c l_c).  A
 // workgroup goes by the units, or, where there may be more of them than runs, by the place where run r begins, and joins the
 // unit there if it is the unit's first division; a thread has four dims of a pair, for K pairs, or W waves share the parts of
-// theirs.
+// theirs.  Bound: the partial states, read from the caches (2048 rows over 18001 tokens: about 100 MB, 31 us), or the launch,
+// 5 us.  By units where these are fewer than runs: 32 x up to 16 rows over up to 4096 65 -> 60 us; four pairs a thread: 8 x up to
+// 240 rows over 7152 186 -> 178.
 template <int W, int K, bool UNITS>
 __global__ __launch_bounds__(256) void pg_merge_kernel(PagedParams p) {
     __shared__ float4 accs[W > 1 ? 4 : 1][64];
@@ -794,11 +808,19 @@ struct Plan {
 Plan plan(long long B, long long T, int HK, int width, int longest) {
     Plan pl{};
     const long long hint = longest > 0 && longest < T ? longest : T;
+    // 8 rows a wave.  64 sequences of up to 8192 tokens, us with G = 1 / 2 / 4 / the workgroup kernel: 8 rows 134 / 169 / 274 / 306,
+    // 16 rows 177 (G = 2) / 284 / 321, 32 rows 299 (G = 4) / 331; 8 x 32 rows over 7000 82 / 91.
     pl.G = hint <= 8 ? 1 : hint <= 16 ? 2 : hint <= 32 ? 4 : 0;
+    // (a unit's rows are those of its partial states: single rows with nb = 1 / 2 / 4 / 8 112 / 114 / 120 / 128 us)
     pl.nb = hint <= 1 ? 1 : hint <= 2 ? 2 : hint <= 4 ? 4 : pl.G ? 8 * pl.G : 64;
     const long long most = (T + (pl.nb - 1) * B) / pl.nb;
     pl.units = most < T ? most : T;
+    // What a unit's beginning costs, in tiles: few rows with 0 / 1 / 2 / 4 64 x 1 over up to 8192 117 / 114 / 112 / 112 us, 32 x up to 16
+    // over up to 4096 64 / 60 / 58 / 58, and a run's one unit has none (1 x 500: 15.5 / 17.4 / 20.2 / 23.3); the workgroup kernel
+    // with 0 / 2 / 4 / 8 64 x 64 over up to 4096 256 / 232 / 215 / 216.
     pl.begin = B == 1 && pl.units == 1 ? 0 : pl.G ? 2 : 4;
+    // A run's fewest tiles: few rows 1 / 2 / 4, 1 x 500 15.5 / 18.5 / 21.2 us; the workgroup kernel 1 / 2 / 4 / 8, 64 rows over 2000
+    // 55 / 44 / 36 / 35 (and as many partial states fewer to join).
     pl.least = pl.G ? 1 : 4;
     pl.tiles = pl.units * (width + 1ll + pl.begin);
     const long long slots = pl.G ? 4 * kCus / pl.G : kCus; // runs that the chip holds at once

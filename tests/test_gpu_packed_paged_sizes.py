@@ -121,3 +121,19 @@ def test_starts_and_lengths_that_are_none(gpu):
                 read_kv(c.kv(), 600, st, lens, c.table, longest=hint)
     torch.cuda.synchronize()
     assert all(torch.equal(torch.nan_to_num(a.float()), torch.nan_to_num(b.float())) for a, b in zip(kept, c.kv()))
+
+
+@pytest.mark.parametrize("n", [1, 3, 12, 30, 60, 300, 1000])
+def test_results_in_the_queries_place(gpu, n):
+    """out= q itself, strided as the fused rows leave it: the same bits as beside it, k and v left alone."""
+    counts = [n, max(1, n // 3)]
+    q, k, v = heads(gpu, n, sum(counts), 2)
+    g = torch.Generator(device=gpu).manual_seed(n)
+    c = Cache(gpu, *[[torch.randn(n + 150, 2, D, generator=g, device=gpu).to(BF) for _ in counts] for _ in range(2)])
+    s, kept = starts_of(counts, gpu), (k.clone(), v.clone())
+    want = packed_attention(q, k, v, s, longest=n), paged_attention(q, c.kv(), s, c.lens, c.table, longest=n)
+    for f, w in ((lambda x: packed_attention(x, k, v, s, longest=n, out=x), want[0]), (lambda x: paged_attention(x, c.kv(), s, c.lens, c.table, longest=n, out=x), want[1])):
+        was = q.clone()
+        assert f(q) is q and torch.equal(q, w)
+        q.copy_(was)
+    assert torch.equal(k, kept[0]) and torch.equal(v, kept[1])
