@@ -13,10 +13,11 @@
 // sequence's end as zeros (the buffer's range check); V is kept as it lies in memory and its V^T fragments are transposing
 // reads (ds_read_b64_tr_b16: 16 lanes fetch 4 keys x 16 dims and each gets the 4 keys of one dim).
 //
-// Bound: the matrix cores beside the softmax, two waves a SIMD (10922 + 5461 tokens 1050 us, 1160 TFLOP/s, busy 67 % of the cycles;
-// the library's 8192^3 product reaches 1400); of shorter prompts the diagonal tiles and the last blocks (13 of up to 2047 tokens 190
-// us, 880 TFLOP/s), of a short one its tiles one after the other (77 tokens 9 us).  Rounding: the weights become bf16 for the
-// matrix cores, their sum does not, and the result is rounded once.
+// Bound: the matrix cores beside the softmax, two waves a SIMD (10922 + 5461 tokens 1033 to 1091 us, 1120 to 1180 TFLOP/s, busy 67 %
+// of the cycles; the library's 8192^3 product reaches 1400); of shorter prompts a block's queries and output as well, 16 us beside
+// 1.65 us a tile, which two workgroups a CU hide poorly (13 of up to 2047 tokens 191 to 199 us, 860 TFLOP/s); of a short one its
+// tiles one after the other (77 tokens 9 us).  Queries by whole rows through LDS: 198.5 -> 196.  Rounding: the weights become bf16
+// for the matrix cores, their sum does not, and the result is rounded once.
 #include "attn_common.h"
 #include "ragged.h"
 
