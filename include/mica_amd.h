@@ -476,8 +476,9 @@ int mica_kv_read(void *k, void *v, const int *starts, int B, int T, const void *
  * Attention of each sequence's last rows over the cache, HQ = 4 HK: row i of the n of sequence b is at position p = lens[b] - n
  * + i (its keys and values are in the cache already) and sees the tokens 0 .. p:
  *   o[t, h] = sum_{u <= p} softmax_u(scale q[t, h] . key_u[h / 4]) value_u[h / 4];   zeros where p < 0.
- * q / o, fill, scale, longest, workspace and values that are not finite as in mica_attention_packed.  The products are of int8
- * values, exact in bf16: a block's scales multiply its scores and weights in fp32, before the weights are rounded.
+ * q / o, fill, scale, longest (0: as if all sequences had as many rows), workspace and values that are not finite as in
+ * mica_attention_packed.  The products are of int8 values, exact in bf16: a block's scales multiply its scores and weights in
+ * fp32, before the weights are rounded.
  */
 int mica_attention_paged(const void *q, long long shq, long long ldq, void *o, long long sho, long long ldo, const int *starts,
                          int B, int T, int HQ, const void *data, const float *scales, const void *recent, int pages,

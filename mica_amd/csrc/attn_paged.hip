@@ -807,7 +807,9 @@ struct Plan {
 
 Plan plan(long long B, long long T, int HK, int width, int longest) {
     Plan pl{};
-    const long long hint = longest > 0 && longest < T ? longest : T;
+    // Unknown: as if all had as many rows (64 single tokens over up to 8192: 112 us, with T as the guess 305; 32 x up
+    // to 16 over up to 4096 59 / 106).
+    const long long guess = longest > 0 ? longest : B > 0 ? (T + B - 1) / B : T, hint = guess < T ? guess : T;
     // 8 rows a wave.  64 sequences of up to 8192 tokens, us with G = 1 / 2 / 4 / the workgroup kernel: 8 rows 134 / 169 / 274 / 306,
     // 16 rows 177 (G = 2) / 284 / 321, 32 rows 299 (G = 4) / 331; 8 x 32 rows over 7000 82 / 91.
     pl.G = hint <= 8 ? 1 : hint <= 16 ? 2 : hint <= 32 ? 4 : 0;

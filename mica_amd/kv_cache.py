@@ -154,8 +154,8 @@ def paged_attention(q, cache: PagedKV, starts, lens, table, slots=None, longest:
     row i of the n of sequence b is at position lens[b] - n + i and sees the tokens up to its own.
 
     q [T, HQ, 256]: a bf16 view with unit feature stride, positions applied, HQ = 4 HK.  lens: the tokens now; starts, table, slots
-    as in append_kv.  longest (the longest sequence's rows, a hint), the result and out= as in ``attention.packed_attention``; a
-    row before its sequence's first token has zeros."""
+    as in append_kv.  longest: the longest sequence's rows, a hint (None: as if all had as many).  The result and out= as in
+    ``attention.packed_attention``; a row before its sequence's first token has zeros."""
     scale = _scale(scale)
     r = _lib.FAST.paged_attention(q, *cache, starts, lens, table, slots, longest, scale, out)
     if r is not None:
