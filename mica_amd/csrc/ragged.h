@@ -24,7 +24,8 @@ MICA_DEVICE int wave_scan(int x) {
 
 // Sequence b has units(b) units of work.  The sequence and the unit at place `at` in the row of all sequences' units; false
 // where there are fewer (b is then their number).  All lanes of a wave call and get the same; a lane reads every 64th
-// sequence's lengths.
+// sequence's lengths.  (In two levels, a lane 1 / 64 of the sequences at first: 1000 prompts of up to 60 tokens 199 -> 179 us, 400
+// and 256 the same, 128 of 512 tokens 483 -> 491.)
 template <class F>
 MICA_DEVICE bool find_unit(int B, F units, int at, int &b, int &u) {
     int before = 0;
