@@ -437,7 +437,7 @@ long long mica_attention_packed_workspace_bytes(int B, int T, int HK, int longes
  * them.  A block with a value that is not finite has the scale NaN: all of it is NaN.
  *   data   int8 [pages][2][HK][8192]: keys [8 groups of 32 dims][32 tokens][32 dims]; values [256 dims][32 tokens, in fours
  *          in the order 0 4 2 6 1 5 3 7]
- *   scales fp32 [pages][2][HK]
+ *   scales fp32 [pages][2][HK]: of any sign, or 0, where another quantizer wrote the page; one that is not finite makes its block NaN
  *   recent bf16 [n_slots][2][HK][32][256]
  *   table  int32 [B][width], rows ldt apart: the page of block j of sequence b; pages may be shared
  *   lens   int32 [B]: the sequence's tokens (clamped to 0 .. 32 width + 31); slots int32 [B]: its slot, NULL: b

@@ -162,8 +162,8 @@ struct Index {
         base = from;
         page = i < whole ? p.c.page(b, i) : -1;
         // (a block without a page: NaN, for the rows that see it)
-        sk = page >= 0 ? p.c.scales[p.c.index(page, 0, hk)] : __builtin_nanf("");
-        sv = page >= 0 ? p.c.scales[p.c.index(page, 1, hk)] : __builtin_nanf("");
+        sk = p.c.scale(page, 0, hk);
+        sv = p.c.scale(page, 1, hk);
     }
     MICA_DEVICE int page_of(int i) const { return __builtin_amdgcn_readlane(page, i - base); }
     MICA_DEVICE float sk_of(int i) const { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sk), i - base)); }
@@ -187,17 +187,25 @@ struct Softmax {
     float m, lsum;
     MICA_DEVICE void clear() { m = -__builtin_inff(), lsum = 0.0f; }
     // Scores sc of a tile (score r of a lane is key k0 + 8 (r / 4) + 4 hi + r % 4) become weights, unscaled ones in the sum and
-    // sv times them in sc; `masked`: keys past pos get none.  The reference moves only when the maximum exceeds it by more than
+    // sv times them in sc; `masked`: keys past pos get none.  A scale (the softmax's times a block's) may be 0 or negative: then
+    // the least score is the largest product.  The reference moves only when the maximum exceeds it by more than
     // 8, and then O with it.
     MICA_DEVICE void add(f32x16 &sc, f32x16 (&O)[kD / 32], float scale, float sv, bool masked, int k0, int pos, int hi) {
+        const float none = scale < 0.0f ? __builtin_inff() : -__builtin_inff();
         if (masked) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sc[r] = k0 + 8 * (r >> 2) + 4 * hi + (r & 3) <= pos ? sc[r] : -__builtin_inff();
+            for (int r = 0; r < 16; ++r) sc[r] = k0 + 8 * (r >> 2) + 4 * hi + (r & 3) <= pos ? sc[r] : none;
         }
-        float mx = -__builtin_inff();
+        float mx = none;
+        if (scale < 0.0f) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) mx = __builtin_fmaxf(mx, sc[r]);
-        mx = half_swap_max(mx) * scale;
+            for (int r = 0; r < 16; ++r) mx = __builtin_fminf(mx, sc[r]);
+            mx = half_swap_max(-mx) * -scale;
+        } else {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) mx = __builtin_fmaxf(mx, sc[r]);
+            mx = half_swap_max(mx) * scale;
+        }
         const bool grow = mx > m + 8.0f;
         const float alpha = grow ? __builtin_amdgcn_exp2f(m - mx) : 1.0f;
         if (grow) m = mx;
@@ -209,7 +217,7 @@ struct Softmax {
         const float ref = m == -__builtin_inff() ? 0.0f : m; // a row that has seen nothing yet: exp2(-inf - 0) = 0
 #pragma unroll
         for (int r = 0; r < 16; ++r) sc[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[r], scale, -ref));
-        if (masked && !(scale < __builtin_inff())) { // (a scale of NaN makes NaN of -inf)
+        if (masked && !(scale > 0.0f && scale < __builtin_inff())) { // (a scale of 0 or NaN makes NaN of -inf)
 #pragma unroll
             for (int r = 0; r < 16; ++r) sc[r] = k0 + 8 * (r >> 2) + 4 * hi + (r & 3) <= pos ? sc[r] : 0.0f;
         }
@@ -493,7 +501,7 @@ __global__ __launch_bounds__(kThreads, 2) void pg_fwd_kernel(PagedParams p) {
         auto look_up = [&](int i) {
             const int j = i + (lane & 31), page = j < whole ? p.c.page(w.b, j) : -1;
             // (a block without a page: NaN, for the rows that see it)
-            const float x = page >= 0 ? p.c.scales[p.c.index(page, hi, hk)] : __builtin_nanf("");
+            const float x = p.c.scale(page, hi, hk);
             index[(j & 63) * 4] = page;
             index[(j & 63) * 4 + 1 + hi] = __float_as_int(x);
         };

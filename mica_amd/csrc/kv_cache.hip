@@ -257,7 +257,7 @@ __global__ __launch_bounds__(kThreads) void kv_read_kernel(ReadParams p) {
         u32x4 x[4];
         if (block < len / kPage) {
             const int page = p.c.page(b, block);
-            const float s = page >= 0 ? p.c.scales[p.c.index(page, side, hk)] : __builtin_nanf("");
+            const float s = p.c.scale(page, side, hk);
             const int8_t *src = p.c.block(max(page, 0), side, hk);
             if (side == 0) {
 #pragma unroll

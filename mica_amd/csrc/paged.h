@@ -44,6 +44,11 @@ struct Pages {
     }
     MICA_DEVICE long long index(int page, int side, int hk) const { return ((long long)page * 2 + side) * HK + hk; }
     MICA_DEVICE int8_t *block(int page, int side, int hk) const { return data + index(page, side, hk) * kPageBytes; }
+    // the scale of a block; NaN without a page, and for one that is not finite
+    MICA_DEVICE float scale(int page, int side, int hk) const {
+        const float s = page >= 0 ? scales[index(page, side, hk)] : __builtin_nanf("");
+        return __builtin_fabsf(s) < __builtin_inff() ? s : __builtin_nanf("");
+    }
     MICA_DEVICE uint16_t *rest(int slot, int side, int hk) const {
         return recent + index(slot, side, hk) * (kPage * kPagedDim);
     }

@@ -30,7 +30,8 @@ class PagedKV(NamedTuple):
     all contiguous; axis 1 is keys, values.
 
     Keys of a page lie as [8 groups of 32 dims][32 tokens][32 dims], values as [256 dims][32 tokens], the tokens in fours in
-    the order 0 4 2 6 1 5 3 7; a value is scale x int8.  A sequence of n tokens needs n // 32 pages and a slot."""
+    the order 0 4 2 6 1 5 3 7; a value is scale x int8, NaN where the scale is not finite (an append writes positive ones).  A
+    sequence of n tokens needs n // 32 pages and a slot."""
 
     data: torch.Tensor
     scales: torch.Tensor
