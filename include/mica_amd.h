@@ -437,7 +437,8 @@ long long mica_attention_packed_workspace_bytes(int B, int T, int HK, int longes
  * them.  A block with a value that is not finite has the scale NaN: all of it is NaN.
  *   data   int8 [pages][2][HK][8192]: keys [8 groups of 32 dims][32 tokens][32 dims]; values [256 dims][32 tokens, in fours
  *          in the order 0 4 2 6 1 5 3 7]
- *   scales fp32 [pages][2][HK]: of any sign, or 0, where another quantizer wrote the page; one that is not finite makes its block NaN
+ *   scales fp32 [pages][2][HK]: of any sign, or 0, where another quantizer wrote the page; one that is not finite makes its
+ *          block NaN
  *   recent bf16 [n_slots][2][HK][32][256]
  *   table  int32 [B][width], rows ldt apart: the page of block j of sequence b; pages may be shared
  *   lens   int32 [B]: the sequence's tokens (clamped to 0 .. 32 width + 31); slots int32 [B]: its slot, NULL: b
@@ -453,9 +454,9 @@ long long mica_attention_packed_workspace_bytes(int B, int T, int HK, int longes
  * is stored its head is normed, (x / sqrt(mean(x^2) + norm_eps)) (norm_offset + w), with norm_w (bf16 [256]; NULL: not), then
  * rotated over its first rot_dim dims (0: not; 16, 32, 64, 128 or 256): (x_i, x_{i + rot_dim / 2}) -> (x_i cos - x_{i +
  * rot_dim / 2} sin, x_{i + rot_dim / 2} cos + x_i sin) with cos_tab / sin_tab [n_pos][rot_dim / 2] (MICA_BF16 or MICA_FP32,
- * 16-byte aligned) at the row's position pos[t] (int32 [T]; NULL: lens[b] + i), not at all outside the tables.  Both in fp32,
- * rounded to bf16 once.  longest as in mica_attention_packed.  Two sequences of one call must not share a slot or a page that
- * the call writes.
+ * 16-byte aligned, n_pos at least 1) at the row's position pos[t] (int32 [T]; NULL: lens[b] + i), not at all outside the tables.
+ * Both in fp32, rounded to bf16 once.  longest as in mica_attention_packed.  Two sequences of one call must not share a slot or
+ * a page that the call writes.
  */
 int mica_kv_append(const void *k, long long shk, long long ldk, const void *v, long long shv, long long ldv, const int *starts,
                    int B, int T, void *data, float *scales, void *recent, int pages, int n_slots, int HK, int head_dim,

@@ -315,6 +315,7 @@ extern "C" int mica_kv_append(const void *k, long long shk, long long ldk, const
     if (!mica_aligned16(k) || !mica_aligned16(v) || !mica_aligned16(norm_w) || !mica_aligned16(cos_tab) ||
         !mica_aligned16(sin_tab) || ((uintptr_t)starts & 3) || ((uintptr_t)pos & 3))
         return MICA_MISS_ALIGN;
+    if (rot_dim && n_pos == 0) return MICA_MISS_ARG; // (a row outside the tables takes their first row's place, unused)
     p.rows = Ragged{starts, B, T};
     p.k = (const uint16_t *)k; p.shk = shk; p.ldk = ldk;
     p.v = (const uint16_t *)v; p.shv = shv; p.ldv = ldv;

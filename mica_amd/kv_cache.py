@@ -86,8 +86,8 @@ def append_kv(cache: PagedKV, k, v, starts, lens, table, slots=None, longest: in
 
     norm: (weight bf16 [256], offset, eps): each key head becomes (x / sqrt(mean(x^2) + eps)) (offset + weight).  rope: (cos,
     sin) or (cos, sin, pos): then its first 2 cos.shape[1] dims (16, 32, 64, 128 or 256) are rotated at the row's position,
-    lens[b] + i or pos[t] (int32 [T]); tables bf16 or fp32 [n_pos, dims / 2]; a row whose position lies outside them is not
-    rotated.  Both in fp32 and rounded to bf16 once (``fused_kernels.head_norm_rope`` rounds each step as the model's bf16
+    lens[b] + i or pos[t] (int32 [T]); tables bf16 or fp32 [n_pos, dims / 2], n_pos >= 1; a row whose position lies outside
+    them is not rotated.  Both in fp32 and rounded to bf16 once (``fused_kernels.head_norm_rope`` rounds each step as the model's bf16
     operations do; rows that it has treated go in without these)."""
     w, offset, eps = (None, 0.0, 0.0) if norm is None else norm
     cos, sin, pos = (None, None, None) if rope is None else rope if len(rope) == 3 else (*rope, None)

@@ -1,0 +1,9 @@
+"""Limits of the packed and paged operators' arguments that are found before any device call (CPU)."""
+import pytest
+from test_kv_cache_host import A16, ARG, append
+
+
+@pytest.mark.parametrize("more", [dict(), dict(dt=2), dict(pos=A16), dict(rot=256)])
+def test_append_refuses_empty_tables(more):
+    """Rotation with tables of no position: every row would be outside them, and no entry may be read."""
+    assert append(**{**dict(rot=64, cos=A16, sin=A16, n_pos=0), **more}) == ARG
