@@ -283,9 +283,9 @@ MICA_DEVICE void leave(const PagedParams &p, long long part, int pair, int hi, b
 // through LDS instead, by DMA of each wave: 126 us for single rows, 190 for 16.  Two waves a SIMD, queries in LDS: 16 rows 187, 32
 // 268, and twice the partial states to join (8 x 16 rows over 7000 58 -> 69).
 //
-// Rounding: with one wave a run the weights are taken as two bf16 summands (hi and what it leaves), whose products are hidden
-// behind the memory (64 x 8 rows 131 -> 134 us); with more rows they are rounded to bf16 once (two summands: 32 x 32 rows over up
-// to 4096 97 -> 108 us).
+// Rounding: with one wave a run the weights are taken as two bf16 summands (hi and what it leaves), of pages and of the rest (64 x 8
+// rows 131 -> 134 us, the rest's among them 137 -> 138.5); with more rows they are rounded to bf16 once (two summands: 32 x 32
+// rows over up to 4096 97 -> 108 us).
 template <int G>
 __global__ __launch_bounds__(256, 1) void pg_few_kernel(PagedParams p) {
     __shared__ __attribute__((aligned(1024))) int8_t smem[4 * kTile]; // a wave's values of the rest
@@ -318,6 +318,14 @@ __global__ __launch_bounds__(256, 1) void pg_few_kernel(PagedParams p) {
         Softmax sm;
         sm.clear();
         const int end = min(w.i1, whole); // pages; then the rest
+        auto left = [](const f32x16 &x) { // what the first summand of the weights leaves
+            f32x16 lo = {};
+            if constexpr (G == 1) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) lo[r] = x[r] - round_bf16(x[r]);
+            }
+            return lo;
+        };
         if (w.i0 < end) {
             Index ix;
             ix.load(p, w.b, hk, whole, w.i0);
@@ -355,11 +363,7 @@ __global__ __launch_bounds__(256, 1) void pg_few_kernel(PagedParams p) {
                 }
                 sm.add(sc, O, p.scale_log2 * sk, sv, (i + 1) * kBK - 1 > from + q0, i * kBK, pos, hi);
                 const bf16x8 h0 = weights(sc, 0), h1 = weights(sc, 1);
-                f32x16 lo = {}; // what h0 and h1 leave
-                if constexpr (G == 1) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) lo[r] = sc[r] - round_bf16(sc[r]);
-                }
+                const f32x16 lo = left(sc);
                 const bf16x8 g0 = weights(lo, 0), g1 = weights(lo, 1);
 #pragma unroll
                 for (int x = 0; x < 8; ++x) {
@@ -397,7 +401,9 @@ __global__ __launch_bounds__(256, 1) void pg_few_kernel(PagedParams p) {
             for (int s = 0; s < kD / 16; ++s) sc = mfma_bf16(__builtin_bit_cast(bf16x8, kf[s]), qf[s], sc);
             const float one = slot < 0 ? __builtin_nanf("") : 1.0f;
             sm.add(sc, O, p.scale_log2 * one, one, true, whole * kBK, pos, hi);
-            bf16x8 pb[2] = {weights(sc, 0), weights(sc, 1)};
+            const bf16x8 pb[2] = {weights(sc, 0), weights(sc, 1)};
+            const f32x16 lo = left(sc);
+            const bf16x8 gb[2] = {weights(lo, 0), weights(lo, 1)};
             wait_vmcnt<0>();
             __asm__ volatile("" ::: "memory");
             uint32_t odd = 0;
@@ -433,7 +439,11 @@ __global__ __launch_bounds__(256, 1) void pg_few_kernel(PagedParams p) {
                 __asm__ volatile("" ::: "memory");
             }
 #pragma unroll
-            for (int x = 0; x < 2 * (kD / 32); ++x) O[x >> 1] = mfma_bf16(vfrag(x & 1, x >> 1), pb[x & 1], O[x >> 1]);
+            for (int x = 0; x < 2 * (kD / 32); ++x) {
+                const bf16x8 a = vfrag(x & 1, x >> 1);
+                O[x >> 1] = mfma_bf16(a, pb[x & 1], O[x >> 1]);
+                if constexpr (G == 1) O[x >> 1] = mfma_bf16(a, gb[x & 1], O[x >> 1]);
+            }
             wait_lgkmcnt0();
         }
         const float l = half_swap_sum(sm.lsum);
