@@ -415,9 +415,9 @@ long long mica_attention_window_workspace_bytes(int B, int Sq, int Sk, int HK, i
  *   o[t, h] = sum_{u in seq(t), u <= t} softmax_u(scale q[t, h] . k[u, h / 4]) v[u, h / 4].
  * Rows of no sequence, before the first or behind the last, become zeros with fill != 0 and are left as they were without.
  * q / k / v / o: bf16, 16-byte aligned; head j of row t at ptr + j sh + t ld (elements, all % 8 and not negative; rows of k and
- * v at least 256 and less than 2^25 apart).  scale positive and finite.  fp32 softmax and sums, the weights rounded to bf16 for the
- * product with v; the softmax of scores that are all -inf is NaN; a key or value that is not finite reaches only the rows
- * that see it.  longest: the rows of the longest sequence, or 0 for T, where the host knows it: a hint for the division of the
+ * v at least 256 and less than 2^25 apart).  scale positive, and finite times log2(e).  fp32 softmax and sums, the weights
+ * rounded to bf16 for the product with v; the softmax of scores that are all -inf is NaN; a key or value that is not finite
+ * reaches only the rows that see it.  longest: the rows of the longest sequence, or 0 for T, where the host knows it: a hint for the division of the
  * work.  workspace: mica_attention_packed_workspace_bytes(B, T, HK, longest) bytes (0: none), 16-byte aligned, no
  * initialisation needed.  The reference pads a batch to a common width (prefill_engine.py:171-418).
  */

@@ -8,6 +8,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) void lds_void;
 
 constexpr int kBufferFlags = 0x00020000;   // raw buffer, 32-bit data format (gfx9)
+constexpr float kLog2e = 1.44269504088896341f;
 
 MICA_DEVICE f32x16 mfma_bf16(const bf16x8 &a, const bf16x8 &b, const f32x16 &c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);

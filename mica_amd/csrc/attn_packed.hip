@@ -429,7 +429,7 @@ extern "C" int mica_attention_packed(const void *q, long long shq, long long ldq
                                      const int *starts, int B, int T, int HQ, int HK, int head_dim, float scale, int fill,
                                      int longest, void *workspace, long long workspace_bytes, mica_stream_t stream) {
     if (head_dim != kD || HK <= 0 || HK > (1 << 20) || HQ != HK * kGroup || B < 0 || T < 0) return MICA_MISS_SHAPE;
-    if (!(scale > 0.0f) || !(scale < __builtin_inff())) return MICA_MISS_ARG;
+    if (!(scale > 0.0f) || !(scale * kLog2e < __builtin_inff())) return MICA_MISS_ARG;
     if (T == 0 || (B == 0 && !fill)) return 0;
     if (!q || !k || !v || !o || !starts) return MICA_MISS_ARG;
     if (T == 1) ldk = ldv = kD; // (never used; the range check of a tile counts on it)
@@ -451,7 +451,7 @@ extern "C" int mica_attention_packed(const void *q, long long shq, long long ldq
     p.o = (uint16_t *)o; p.sho = sho; p.ldo = ldo;
     p.rows = Ragged{starts, B, T};
     p.HK = HK; p.fill = fill;
-    p.scale_log2 = scale * 1.44269504088896341f;
+    p.scale_log2 = scale * kLog2e;
     p.chunk = pl.chunk, p.chunks = pl.chunks;
     p.part_o = (float4 *)workspace;
     p.part_ml = (float2 *)((char *)workspace + pl.states * kD * 4);

@@ -860,7 +860,7 @@ extern "C" int mica_attention_paged(const void *q, long long shq, long long ldq,
                                     long long ldt, int width, const int *lens, const int *slots, float scale, int fill,
                                     int longest, void *workspace, long long workspace_bytes, mica_stream_t stream) {
     if (B < 0 || T < 0) return MICA_MISS_SHAPE;
-    if (!(scale > 0.0f) || !(scale < __builtin_inff())) return MICA_MISS_ARG;
+    if (!(scale > 0.0f) || !(scale * kLog2e < __builtin_inff())) return MICA_MISS_ARG;
     if (T == 0 || (B == 0 && !fill)) return 0;
     PagedParams p{};
     if (const int rc = mica_paged_check(p.c, (void *)data, (void *)scales, (void *)recent, pages, n_slots, HK, head_dim, table,
@@ -878,7 +878,7 @@ extern "C" int mica_attention_paged(const void *q, long long shq, long long ldq,
     p.o = (uint16_t *)o; p.sho = sho; p.ldo = ldo;
     p.rows = Ragged{starts, B, T};
     p.fill = fill;
-    p.scale_log2 = scale * 1.44269504088896341f;
+    p.scale_log2 = scale * kLog2e;
     p.nb = pl.nb, p.runs = pl.runs, p.least = pl.least, p.begin = pl.begin;
     p.part_o = (float4 *)workspace;
     p.part_ml = (float2 *)((char *)workspace + pl.states * kGroup * pl.nb * kD * 4);
