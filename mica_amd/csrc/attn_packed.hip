@@ -410,10 +410,14 @@ Plan plan(long long B, long long T, long long HK, int longest) {
     pl.chunk = 1 << 30, pl.chunks = 1;
     const long long hint = longest > 0 && longest < T ? longest : T, nb = (hint + kB - 1) / kB;
     // Too few blocks to fill the chip, and long ones: each is divided into up to three chunks, so that the longest does not
-    // run alone in the end.  Undivided / divided, us: 1 x 600 26.7 / 25.6, 1 x 1000 40.4 / 33.8, 1 x 1500 56.3 / 45.8, 1 x 2048
-    // 73.8 / 61.1, but 2 x 1000 42.2 / 46.9, 1 x 3000 112 / 117 (64 KB of state a wave, written and read).  Chunks of 16 / 24 / 32
-    // tiles: 1 x 1000 33.8 / 39.9 / 40.3, 1 x 2048 82.0 / 61.1 / 69.8.
-    if (pl.units * HK <= kCus && nb >= 24) {
+    // run alone in the end, against 64 KB of state a wave, written and read.  Undivided / divided, us:
+    //   4 heads, 1 x 700 30 / 27, 1000 40 / 34, 1500 56 / 47, 2048 73.6 / 60.5, 2400 86 / 74, 2500 90 / 85, 2600 94 / 97, 3000 110 / 118:
+    //   as long as the divided blocks' workgroups are about two a CU (units x HK up to 320; 1 head, 10000 rows 328 / 249);
+    //   2 x 768 33.9 / 36.2, 900 38.5 / 40.6, 1000 41.7 / 47.1, 1500 61 / 75, but 1 head 5 x 1000 40 / 36, 6 x 1000 40.5 / 38.3, 6 x 1500
+    //   58 / 57, 8 x 1000 42 / 46, 3 heads 2 x 1000 40 / 38, 4 heads 1000 + 500 40.7 / 36.5, 1500 + 1125 59 / 64: where all rows and
+    //   heads are those of up to six of the longest sequence.
+    // Chunks of 16 / 24 / 32 tiles: 1 x 1000 33.8 / 39.9 / 40.3, 1 x 2048 82.0 / 61.1 / 69.8.
+    if (pl.units * HK <= kCus + kCus / 4 && T * HK <= 6 * hint && nb >= 24) {
         pl.chunk = (int)((3 * nb / 8 + 7) / 8 * 8);
         pl.chunks = (int)((nb + pl.chunk - 1) / pl.chunk);
         pl.states = pl.units * pl.chunks * HK * kRows;
