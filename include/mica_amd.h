@@ -417,9 +417,9 @@ long long mica_attention_window_workspace_bytes(int B, int Sq, int Sk, int HK, i
  * q / k / v / o: bf16, 16-byte aligned; head j of row t at ptr + j sh + t ld (elements, all % 8 and not negative; rows of k and
  * v at least 256 and less than 2^25 apart).  scale positive, and finite times log2(e).  fp32 softmax and sums, the weights
  * rounded to bf16 for the product with v; the softmax of scores that are all -inf is NaN; a key or value that is not finite
- * reaches only the rows that see it.  longest: the rows of the longest sequence, or 0 for T, where the host knows it: a hint for the division of the
- * work.  workspace: mica_attention_packed_workspace_bytes(B, T, HK, longest) bytes (0: none), 16-byte aligned, no
- * initialisation needed.  The reference pads a batch to a common width (prefill_engine.py:171-418).
+ * reaches only the rows that see it.  longest: the rows of the longest sequence where the host knows it, or 0 (as if all
+ * sequences had as many): a hint for the division of the work.  workspace: mica_attention_packed_workspace_bytes(B, T, HK,
+ * longest) bytes (0: none), 16-byte aligned, no initialisation needed.  The reference pads a batch to a common width (prefill_engine.py:171-418).
  */
 int mica_attention_packed(const void *q, long long shq, long long ldq, const void *k, long long shk, long long ldk,
                           const void *v, long long shv, long long ldv, void *o, long long sho, long long ldo,
@@ -477,9 +477,8 @@ int mica_kv_read(void *k, void *v, const int *starts, int B, int T, const void *
  * Attention of each sequence's last rows over the cache, HQ = 4 HK: row i of the n of sequence b is at position p = lens[b] - n
  * + i (its keys and values are in the cache already) and sees the tokens 0 .. p:
  *   o[t, h] = sum_{u <= p} softmax_u(scale q[t, h] . key_u[h / 4]) value_u[h / 4];   zeros where p < 0.
- * q / o, fill, scale, longest (0: as if all sequences had as many rows), workspace and values that are not finite as in
- * mica_attention_packed.  The products are of int8 values, exact in bf16: a block's scales multiply its scores and weights in
- * fp32, before the weights are rounded.
+ * q / o, fill, scale, longest, workspace and values that are not finite as in mica_attention_packed.  The products are of int8
+ * values, exact in bf16: a block's scales multiply its scores and weights in fp32, before the weights are rounded.
  */
 int mica_attention_paged(const void *q, long long shq, long long ldq, void *o, long long sho, long long ldo, const int *starts,
                          int B, int T, int HQ, const void *data, const float *scales, const void *recent, int pages,

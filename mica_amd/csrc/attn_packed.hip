@@ -408,7 +408,10 @@ Plan plan(long long B, long long T, long long HK, int longest) {
     const long long most = (T + 31 * B + 31) / 32;
     pl.units = most < T ? most : T;
     pl.chunk = 1 << 30, pl.chunks = 1;
-    const long long hint = longest > 0 && longest < T ? longest : T, nb = (hint + kB - 1) / kB;
+    // Unknown: as if all had as many rows (4 heads: 4 x 400 25.7 / 22.1 us with T as the guess / so, 5 x 300 26.3 / 19.0, 3 x 600
+    // 32.2 / 29.1; 1500 + 375 47.5 / 56.6, which the hint mends: 50).
+    const long long guess = longest > 0 ? longest : B > 0 ? (T + B - 1) / B : T, hint = guess < T ? guess : T;
+    const long long nb = (hint + kB - 1) / kB;
     // Too few blocks to fill the chip, and long ones: each is divided into up to three chunks, so that the longest does not
     // run alone in the end, against 64 KB of state a wave, written and read.  Undivided / divided, us:
     //   4 heads, 1 x 700 30 / 27, 1000 40 / 34, 1500 56 / 47, 2048 73.6 / 60.5, 2400 86 / 74, 2500 90 / 85, 2600 94 / 97, 3000 110 / 118:

@@ -29,3 +29,10 @@ def test_states_of_many_sequences_stay_small(T):
         for HK in (1, 2, 4):
             n = _lib.load().mica_attention_packed_workspace_bytes(B, T, HK, min(1500, T))
             assert 0 <= n <= 320 * 3 * 128 * 1032
+
+
+@pytest.mark.parametrize("B,T,HK,want", [(4, 1600, 4, False), (5, 1500, 4, False), (3, 1800, 4, False), (8, 1600, 4, False),
+                                         (10, 4000, 1, False), (1, 1000, 4, True), (1, 2048, 4, True), (4, 4000, 1, True)])
+def test_without_a_hint_as_if_all_had_as_many_rows(B, T, HK, want):
+    """A batch of short prompts asks for no division that none of its blocks would take."""
+    assert (_lib.load().mica_attention_packed_workspace_bytes(B, T, HK, 0) > 0) == want
