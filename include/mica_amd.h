@@ -416,10 +416,12 @@ long long mica_attention_window_workspace_bytes(int B, int Sq, int Sk, int HK, i
  * Rows of no sequence, before the first or behind the last, become zeros with fill != 0 and are left as they were without.
  * q / k / v / o: bf16, 16-byte aligned; head j of row t at ptr + j sh + t ld (elements, all % 8 and not negative; rows of k and
  * v at least 256 and less than 2^25 apart).  scale positive, and finite times log2(e).  fp32 softmax and sums, the weights
- * rounded to bf16 for the product with v; the softmax of scores that are all -inf is NaN; a key or value that is not finite
+ * rounded to bf16 for the product with v; they are up to 2^8 before they are normalised, so that the fp32 sums of a row of n keys
+ * hold values of v up to 2^120 / n; the softmax of scores that are all -inf is NaN; a key or value that is not finite
  * reaches only the rows that see it.  longest: the rows of the longest sequence where the host knows it, or 0 (as if all
- * sequences had as many): a hint for the division of the work.  workspace: mica_attention_packed_workspace_bytes(B, T, HK,
- * longest) bytes (0: none), 16-byte aligned, no initialisation needed.  The reference pads a batch to a common width (prefill_engine.py:171-418).
+ * sequences had as many): a hint for the division of the work, which goes by the whole call: a row's roundings may differ with
+ * the other sequences beside it.  workspace: mica_attention_packed_workspace_bytes(B, T, HK, longest) bytes (0: none), 16-byte
+ * aligned, no initialisation needed.  The reference pads a batch to a common width (prefill_engine.py:171-418).
  */
 int mica_attention_packed(const void *q, long long shq, long long ldq, const void *k, long long shk, long long ldk,
                           const void *v, long long shv, long long ldv, void *o, long long sho, long long ldo,

@@ -383,10 +383,10 @@ def packed_attention(q, k, v, starts, longest: int | None = None, scale: float |
     q [T, HQ, 256], k / v [T, HK, 256]: bf16 views with unit feature stride (e.g. of the fused QKV rows), positions applied,
     HQ = 4 HK.  starts: int32 [B + 1] on the device, not falling: rows starts[b] .. starts[b + 1] - 1 are sequence b's, and each
     attends to those up to itself; a sequence may be empty.  longest: the longest sequence's rows where the host knows it (a
-    hint, None: as if all had as many; it changes the division of the work and so roundings, not what is computed).  Strides of
-    whole 16 bytes, rows of k and v at least 256 elements apart.  Returns o [T, HQ, 256] bf16, zeros in rows of no sequence; with
-    out= (such a view) that, whose rows of no sequence are left as they were: rows and heads that do not overlap, in memory that
-    may be q's (each row and head in its own place) but not k's or v's."""
+    hint, None: as if all had as many; it changes the division of the work and so roundings, as the other sequences of the call
+    may, not what is computed).  Strides of whole 16 bytes, rows of k and v at least 256 elements apart.  Returns o [T, HQ, 256]
+    bf16, zeros in rows of no sequence; with out= (such a view) that, whose rows of no sequence are left as they were: rows and
+    heads that do not overlap, in memory that may be q's (each row and head in its own place) but not k's or v's."""
     scale = _scale(scale)
     r = _lib.FAST.packed_attention(q, k, v, starts, longest, scale, out)
     if r is not None:

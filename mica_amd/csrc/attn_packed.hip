@@ -13,11 +13,12 @@
 // sequence's end as zeros (the buffer's range check); V is kept as it lies in memory and its V^T fragments are transposing
 // reads (ds_read_b64_tr_b16: 16 lanes fetch 4 keys x 16 dims and each gets the 4 keys of one dim).
 //
-// Bound: the matrix cores beside the softmax, two waves a SIMD (10922 + 5461 tokens 1033 to 1091 us, 1120 to 1180 TFLOP/s, busy 67 %
+// Bound: the matrix cores beside the softmax, two waves a SIMD (10922 + 5461 tokens 1029 to 1094 us, 1115 to 1190 TFLOP/s, busy 68 %
 // of the cycles; the library's 8192^3 product reaches 1400); of shorter prompts a block's queries and output as well, 16 us beside
-// 1.65 us a tile, which two workgroups a CU hide poorly (13 of up to 2047 tokens 191 to 199 us, 860 TFLOP/s); of a short one its
-// tiles one after the other (77 tokens 9 us).  Queries by whole rows through LDS: 198.5 -> 196.  Rounding: the weights become bf16
-// for the matrix cores, their sum does not, and the result is rounded once.
+// 1.65 us a tile, which two workgroups a CU hide poorly (13 of up to 2047 tokens 188 to 205 us, 810 to 880 TFLOP/s); of a short one
+// its tiles one after the other (77 tokens 9 us).  The queries come straight from memory, a lane a row (by whole rows through LDS:
+// 198.5 -> 196 us, not kept).  Rounding: the weights become bf16 for the matrix cores, their sum does not, and the result is
+// rounded once.
 #include "attn_common.h"
 #include "ragged.h"
 
@@ -414,11 +415,11 @@ Plan plan(long long B, long long T, long long HK, int longest) {
     const long long nb = (hint + kB - 1) / kB;
     // Too few blocks to fill the chip, and long ones: each is divided into up to three chunks, so that the longest does not
     // run alone in the end, against 64 KB of state a wave, written and read.  Undivided / divided, us:
-    //   4 heads, 1 x 700 30 / 27, 1000 40 / 34, 1500 56 / 47, 2048 73.6 / 60.5, 2400 86 / 74, 2500 90 / 85, 2600 94 / 97, 3000 110 / 118:
-    //   as long as the divided blocks' workgroups are about two a CU (units x HK up to 320; 1 head, 10000 rows 328 / 249);
-    //   2 x 768 33.9 / 36.2, 900 38.5 / 40.6, 1000 41.7 / 47.1, 1500 61 / 75, but 1 head 5 x 1000 40 / 36, 6 x 1000 40.5 / 38.3, 6 x 1500
-    //   58 / 57, 8 x 1000 42 / 46, 3 heads 2 x 1000 40 / 38, 4 heads 1000 + 500 40.7 / 36.5, 1500 + 1125 59 / 64: where all rows and
-    //   heads are those of up to six of the longest sequence.
+    //   4 heads, 1 x 700 30 / 27, 1000 40 / 34, 1500 56 / 47, 2048 73.6 / 60.5, 2400 86 / 74, 2500 90 / 85, 2600 94 / 97, 3000
+    //   110 / 118: as long as the divided blocks' workgroups are about two a CU (units x HK up to 320; 1 head, 10000 rows 328 / 249);
+    //   2 x 768 33.9 / 36.2, 900 38.5 / 40.6, 1000 41.7 / 47.1, 1500 61 / 75, but 1 head 5 x 1000 40 / 36, 6 x 1000 40.5 / 38.3,
+    //   6 x 1500 58 / 57, 8 x 1000 42 / 46, 3 heads 2 x 1000 40 / 38, 4 heads 1000 + 500 40.7 / 36.5, 1500 + 1125 59 / 64: where all
+    //   rows and heads are those of up to six of the longest sequence.
     // Chunks of 16 / 24 / 32 tiles: 1 x 1000 33.8 / 39.9 / 40.3, 1 x 2048 82.0 / 61.1 / 69.8.
     if (pl.units * HK <= kCus + kCus / 4 && T * HK <= 6 * hint && nb >= 24) {
         pl.chunk = (int)((3 * nb / 8 + 7) / 8 * 8);

@@ -278,10 +278,11 @@ MICA_DEVICE void leave(const PagedParams &p, long long part, int pair, int hi, b
 // bytes a lane, each loaded for the next tile as soon as this one's has been widened, so that a wave has a page (16 KB) in
 // flight all the time.  Nothing is shared and there is no barrier.  G waves take a run together, 8 rows each.
 //
-// Bound: up to 4 rows by HBM (64 single rows over up to 8192 tokens: 112 us, 4.9 TB/s, a copy's rate); then by instruction issue,
-// about 800 for a page and wave, half of them to widen it, which all G waves repeat (64 x 8 rows 134 us, 16 177, 32 299).  Pages
-// through LDS instead, by DMA of each wave: 126 us for single rows, 190 for 16.  Two waves a SIMD, queries in LDS: 16 rows 187, 32
-// 268, and twice the partial states to join (8 x 16 rows over 7000 58 -> 69).
+// Bound: up to 4 rows by HBM (64 single rows over up to 8192 tokens: 112 us, 4.9 TB/s, a copy's rate; 114 where the sequences' last
+// blocks are not finished, whose tiles have nothing in flight beside them); then by instruction issue, about 800 for a page and
+// wave, half of them to widen it, which all G waves repeat (64 x 8 rows 134 to 144 us, 16 177 to 181, 32 290 to 302).  Pages through
+// LDS instead, by DMA of each wave: 126 us for single rows, 190 for 16.  Two waves a SIMD, queries in LDS: 16 rows 177 -> 187, 32 299
+// -> 268, and twice the partial states to join (8 x 16 rows over 7000 58 -> 69); not built for G = 4 alone.
 //
 // Rounding: with one wave a run the weights are taken as two bf16 summands (hi and what it leaves), of pages and of the rest (64 x 8
 // rows 131 -> 134 us, the rest's among them 137 -> 138.5); with more rows they are rounded to bf16 once (two summands: 32 x 32
@@ -473,7 +474,7 @@ __global__ __launch_bounds__(256, 1) void pg_few_kernel(PagedParams p) {
 // workgroup: it computes S^T = K Q^T (32 keys x 32 pairs, v_mfma_f32_32x32x16_bf16), the online softmax of its pairs (a lane
 // holds 16 of a pair's 32 scores, lane l ^ 32 the others) and O^T += V^T P^T.
 //
-// Bound: the matrix cores beside widening and softmax (2048 rows over 18001 tokens 540 us and 31 for the join, 1000 TFLOP/s; the
+// Bound: the matrix cores beside widening and softmax (2048 rows over 18001 tokens 530 to 560 us and 31 for the join, 1000 TFLOP/s; the
 // library's 8192^3 product reaches 1400).  Pages widened in registers by the waves that use them, before the ring: 1234 us; the
 // next page widened beside this one's PV, for one phase less: 636 against 605.
 constexpr int kWaves = 8, kThreads = 64 * kWaves;
@@ -829,7 +830,10 @@ Plan plan(long long B, long long T, int HK, int width, int longest) {
     // to 16 over up to 4096 59 / 106).
     const long long guess = longest > 0 ? longest : B > 0 ? (T + B - 1) / B : T, hint = guess < T ? guess : T;
     // 8 rows a wave.  64 sequences of up to 8192 tokens, us with G = 1 / 2 / 4 / the workgroup kernel: 8 rows 134 / 169 / 274 / 306,
-    // 16 rows 177 (G = 2) / 284 / 321, 32 rows 299 (G = 4) / 331; 8 x 32 rows over 7000 82 / 91.
+    // 16 rows 177 (G = 2) / 284 / 321, 32 rows 299 (G = 4) / 331; 8 x 32 rows over 7000 82 / 91.  All units of a call are as the longest
+    // sequence asks.  Where most have fewer rows, smaller units can be faster, which the longest does not tell: with G = 2 / 4, 32 x
+    // up to 32 rows over up to 4096 86 / 91, 64 x up to 32 over up to 8192 275 / 284, but 64 x up to 32 over 1000 80 / 75, 32 x 32
+    // over up to 4096 99 / 96; 2048 rows beside 63 single ones 545 in one call, 269 + 111 in two.
     pl.G = hint <= 8 ? 1 : hint <= 16 ? 2 : hint <= 32 ? 4 : 0;
     // (a unit's rows are those of its partial states: single rows with nb = 1 / 2 / 4 / 8 112 / 114 / 120 / 128 us)
     pl.nb = hint <= 1 ? 1 : hint <= 2 ? 2 : hint <= 4 ? 4 : pl.G ? 8 * pl.G : 64;

@@ -12,7 +12,7 @@
 //
 // Bound: append by HBM and, before it, the waves' phases (load, norm and rotation, the block's largest, store): 15 prompts of up to
 // 2047 tokens, 16 K rows of 4 heads, 31 us, 67 MB read and 34 written, 3.2 TB/s.  More waves a SIMD than the registers allow (5 / 6
-// / 8) spill: 52 -> 59 / 69 / 84 us with the read of the same rows.  Read by HBM: 40005 rows of 4 heads 38 to 44 us, 5.6 to 6.4 TB/s.
+// / 8) spill: 52 -> 59 / 69 / 84 us with the read of the same rows.  Read by HBM: 40005 rows of 4 heads 38 to 52 us, 4.7 to 6.4 TB/s.
 // Single tokens cost their launch: 64 x 1 appended 5 us, 320 rows read 5.
 //
 // Rounding: a bf16 value goes to the nearest of 255 steps of its block's scale once; read, scale x int8 goes to bf16 once.
